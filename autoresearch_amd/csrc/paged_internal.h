@@ -1,0 +1,38 @@
+// paged_internal.h -- launchers of the paged cache's operators (kern_paged.hip,
+// kern_pages.hip, kern_draw.hip). Arguments are checked by the C entries
+// (fgpt_paged.hip); all launches go to `s`.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/fgpt.h"
+
+namespace fgpt {
+
+// ---- attention
+// Where the attention's output goes: rows of fp32 or bf16, or the split operand
+// planes of the GEMM that follows (tile_at over n_head * head_dim columns).
+struct PagedOut {
+  void* y = nullptr;
+  int64_t ld = 0;            // elements
+  uint16_t* planes = nullptr;
+  int64_t plane = 0;
+};
+// Workspace of an attention launch: floats (0: none needed).
+int64_t paged_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c);
+void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c,
+                       const void* q, const PagedOut& out, float* work);
+
+// ---- append and page copies
+void launch_qk_append(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_append_cfg& c,
+                      const void* qkv, void* q_out);
+void launch_pages_copy(hipStream_t s, void* base, int32_t n_planes, int64_t plane_bytes,
+                       int64_t page_bytes, const int32_t* src, const int32_t* dst, int32_t n);
+
+// ---- draws
+constexpr int32_t DRAW_MAX_V = 1 << 18;
+int64_t draw_work_bytes(int32_t rows, int32_t V);
+void launch_draw_rows(hipStream_t s, const float* logits, int32_t rows, int32_t V, int64_t ld,
+                      const fg_draw_cfg& c, int32_t* ids, float* probs, void* work);
+
+}  // namespace fgpt

@@ -35,6 +35,8 @@ EXPORTS = (
     "fg_decode_greedy", "fg_sync", "fg_model_bytes", "fg_timing", "fg_timing_read",
     "fg_eval_bpb", "fg_rows_npy", "fg_decode_spec", "fg_spec_accept", "fg_spec_draft",
     "fg_sample", "fg_decode_sample", "fg_set_option", "fg_get_option", "fg_step_dev_noalloc",
+    "fg_qk_append", "fg_paged_attn_work", "fg_paged_attn", "fg_pages_copy", "fg_draw_rows_work",
+    "fg_draw_rows",
 )
 
 KERNEL_KINDS = {0: "gemm", 1: "gemv", 2: "attn_chunk", 3: "attn_decode", 4: "other",
@@ -77,6 +79,39 @@ class _SampleCfg(C.Structure):
     _fields_ = [("temp", C.c_float), ("topp", C.c_float), ("pres", C.c_float),
                 ("freq", C.c_float), ("rep", C.c_float), ("plen", C.c_float),
                 ("pwin", C.c_int32), ("nblock", C.c_int32), ("byte_space", C.c_int32)]
+
+
+FG_F32, FG_BF16 = 0, 1  # value types of the paged operators' rows and pages
+
+
+class _Pages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("n_kv_head", C.c_int32), ("head_dim", C.c_int32),
+                ("type", C.c_int32)]
+
+
+class _Ragged(C.Structure):
+    _fields_ = [("n_seq", C.c_int32), ("n_rows", C.c_int32), ("max_q", C.c_int32),
+                ("max_kv", C.c_int32), ("table_ld", C.c_int32), ("q_start", C.c_void_p),
+                ("kv_len", C.c_void_p), ("table", C.c_void_p)]
+
+
+class _AppendCfg(C.Structure):
+    _fields_ = [("n_head", C.c_int32), ("type", C.c_int32), ("norm", C.c_int32),
+                ("interleaved", C.c_int32), ("eps", C.c_float), ("rope_n", C.c_int32),
+                ("wq", C.c_void_p), ("wk", C.c_void_p), ("cos_buf", C.c_void_p),
+                ("sin_buf", C.c_void_p), ("qkv_ld", C.c_int64), ("q_ld", C.c_int64)]
+
+
+class _AttnCfg(C.Structure):
+    _fields_ = [("n_head", C.c_int32), ("type", C.c_int32), ("window", C.c_int32),
+                ("sinks", C.c_int32), ("scale", C.c_float), ("q_ld", C.c_int64),
+                ("out_ld", C.c_int64)]
+
+
+class _DrawCfg(C.Structure):
+    _fields_ = [("temp", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
+                ("min_p", C.c_void_p), ("u", C.c_void_p)]
 
 
 def sample_cfg(temp=0.0, topp=1.0, pres=0.0, freq=0.0, rep=1.0, plen=0.0, pwin=0, nblock=0,
@@ -136,6 +171,15 @@ def load_library(path: str = LIB_PATH):
         "fg_set_option": (i32, [_vp, i32, i32]),
         "fg_step_dev_noalloc": (i32, [_vp, _vp, _vp, _vp, _vp, _vp]),
         "fg_get_option": (i32, [_vp, i32, _i, C.c_char_p, i32]),
+        "fg_qk_append": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AppendCfg), _vp,
+                               _vp, _vp]),
+        "fg_paged_attn_work": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AttnCfg),
+                                     C.POINTER(i64)]),
+        "fg_paged_attn": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AttnCfg), _vp,
+                                _vp, _vp, i64, _vp]),
+        "fg_pages_copy": (i32, [_vp, i32, i64, i32, i64, _i, _i, i32, _vp]),
+        "fg_draw_rows_work": (i32, [i32, i32, C.POINTER(i64)]),
+        "fg_draw_rows": (i32, [_vp, i32, i32, i64, C.POINTER(_DrawCfg), _vp, _vp, _vp, i64, _vp]),
         "fg_timing_read": (i32, [_vp, i32, C.POINTER(i64), C.POINTER(C.c_double),
                                  C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     }
@@ -464,6 +508,83 @@ def spec_draft(ids, p: int, m: int, k: int):
     n = C.c_int32()
     _check(_LIB.fg_spec_draft(_ip(ids) if ids.size else None, p, m, k, _ip(d), C.byref(n)))
     return d[:n.value].tolist()
+
+
+# ------------------------------------------------------- paged caches
+#
+# The operators of include/fgpt.h on device pointers (ints; 0 = none), enqueued
+# on `stream` (an int, 0 = the null stream) without host synchronisation. The
+# descriptors only name the caller's buffers and may be kept with them.
+
+def pages(k: int, v: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int,
+          bf16: bool = False) -> _Pages:
+    """fg_pages: one layer's keys and values, [n_pages][n_kv_head][page_size][head_dim]."""
+    return _Pages(k, v, n_pages, page_size, n_kv_head, head_dim, FG_BF16 if bf16 else FG_F32)
+
+
+def ragged(q_start: int, kv_len: int, table: int, n_seq: int, n_rows: int, max_q: int, max_kv: int,
+           table_ld: int) -> _Ragged:
+    """fg_ragged: new tokens of n_seq sequences (device int32 arrays q_start
+    [n_seq+1], kv_len [n_seq], table [n_seq][table_ld]) and their bounds."""
+    return _Ragged(n_seq, n_rows, max_q, max_kv, table_ld, q_start, kv_len, table)
+
+
+def append_cfg(n_head: int, cos: int = 0, sin: int = 0, rope_n: int = 0, norm: bool = False,
+               eps: float = 1e-5, wq: int = 0, wk: int = 0, bf16: bool = False,
+               interleaved: bool = False, qkv_ld: int = 0, q_ld: int = 0) -> _AppendCfg:
+    """fg_append_cfg: head norms (weights wq, wk), rotation tables, row type."""
+    return _AppendCfg(n_head, FG_BF16 if bf16 else FG_F32, 1 if norm else 0,
+                      1 if interleaved else 0, eps, rope_n, wq, wk, cos, sin, qkv_ld, q_ld)
+
+
+def qk_append(pg: _Pages, batch: _Ragged, cfg: _AppendCfg, qkv: int, q_out: int, stream: int = 0):
+    """fg_qk_append: heads normed and rotated, q out, k and v into their slots."""
+    _check(load_library().fg_qk_append(pg, batch, cfg, qkv, q_out, stream))
+
+
+def attn_cfg(n_head: int, window: int = 0, sinks: int = 0, scale: float = 0.0, bf16: bool = False,
+             q_ld: int = 0, out_ld: int = 0) -> _AttnCfg:
+    """fg_attn_cfg: heads, sliding window and sinks (0: none), scale (0: 1/sqrt(head_dim))."""
+    return _AttnCfg(n_head, FG_BF16 if bf16 else FG_F32, window, sinks, scale, q_ld, out_ld)
+
+
+def paged_attn_work(pg: _Pages, batch: _Ragged, cfg: _AttnCfg) -> int:
+    """Bytes of device memory that paged_attn needs as its workspace."""
+    n = C.c_int64()
+    _check(load_library().fg_paged_attn_work(pg, batch, cfg, C.byref(n)))
+    return n.value
+
+
+def paged_attn(pg: _Pages, batch: _Ragged, cfg: _AttnCfg, q: int, out: int, work: int = 0,
+               work_bytes: int = 0, stream: int = 0):
+    """fg_paged_attn: the batch's new tokens over their sequences' pages."""
+    _check(load_library().fg_paged_attn(pg, batch, cfg, q, out, work, work_bytes, stream))
+
+
+def pages_copy(base: int, n_planes: int, plane_bytes: int, n_pages: int, page_bytes: int, src, dst,
+               stream: int = 0):
+    """fg_pages_copy: pages src[i] -> dst[i] (host lists) in every plane."""
+    src, dst = _i32(src).reshape(-1), _i32(dst).reshape(-1)
+    if src.size != dst.size:
+        raise ValueError("src and dst must hold one page each per copy")
+    _check(load_library().fg_pages_copy(base, n_planes, plane_bytes, n_pages, page_bytes, _ip(src),
+                                        _ip(dst), src.size, stream))
+
+
+def draw_rows_work(rows: int, V: int) -> int:
+    """Bytes of device memory that draw_rows needs as its workspace."""
+    n = C.c_int64()
+    _check(load_library().fg_draw_rows_work(rows, V, C.byref(n)))
+    return n.value
+
+
+def draw_rows(logits: int, rows: int, V: int, ld: int, u: int, ids: int, probs: int = 0, *,
+              temp: int = 0, top_k: int = 0, top_p: int = 0, min_p: int = 0, work: int = 0,
+              work_bytes: int = 0, stream: int = 0):
+    """fg_draw_rows: an id a row from the uniform numbers u, under per-row
+    settings (device arrays, 0 = off)."""
+    _check(load_library().fg_draw_rows(logits, rows, V, ld, _DrawCfg(temp, top_k, top_p, min_p, u),
+                                       ids, probs, work, work_bytes, stream))
 
 
 # ------------------------------------------------------- reference-shaped API

@@ -359,6 +359,133 @@ int32_t fg_timing_read(fg_model *m, int32_t kind, int64_t *launches, double *ms,
  * (gpu_shim.cpp:172-186). */
 int32_t fg_model_bytes(const fg_model *m, int64_t *weight_bytes, int64_t *work_bytes);
 
+/* ------------------------------------------------------------ paged caches
+ *
+ * Operators over a cache kept in pages, for callers that serve sequences of
+ * their own lengths (no counterpart in the reference, whose caches are one
+ * array of equally long sequences). They take device pointers of any
+ * allocation, run on `stream` (a hipStream_t of any device; NULL = the null
+ * stream of the current device) without host synchronisation or allocation,
+ * may be captured into a graph, and keep nothing between calls: calls on
+ * different streams and threads need only workspaces of their own.
+ * Pointers are 16-byte aligned. What the arguments say of sizes is checked on
+ * the host; device arrays are bounds-checked by the kernels, as each says.
+ *
+ * fg_pages: one layer's keys and values, each [n_pages][n_kv_head][page_size]
+ * [head_dim] (a head's positions of a page are consecutive rows). head_dim 64
+ * or 128; page_size a power of two, 16..256. */
+enum { FG_F32 = 0, FG_BF16 = 1 };
+typedef struct fg_pages {
+  void *k, *v;
+  int32_t n_pages, page_size, n_kv_head, head_dim;
+  int32_t type; /* FG_F32 or FG_BF16 */
+} fg_pages;
+
+/* A batch of new tokens: rows q_start[s] .. q_start[s+1]-1 of the row arrays
+ * are the last tokens of sequence s, whose cache holds kv_len[s] positions with
+ * them: row r sits at position kv_len[s] - (q_start[s+1] - r). Position p is
+ * slot p % page_size of page table[s * table_ld + p / page_size]. q_start[0]
+ * is 0 and q_start does not fall; a sequence may have no new token; rows from
+ * q_start[n_seq] on (padding up to n_rows) are neither read nor written.
+ * max_q and max_kv bound the new tokens and positions of every sequence (they
+ * size the launch, so a captured call serves any lengths within them);
+ * max_kv <= table_ld * page_size. Table entries of positions that no row sees
+ * are not read (pages behind a sliding window may be gone). */
+typedef struct fg_ragged {
+  int32_t n_seq, n_rows, max_q, max_kv, table_ld;
+  const int32_t *q_start; /* device [n_seq + 1] */
+  const int32_t *kv_len;  /* device [n_seq]     */
+  const int32_t *table;   /* device [n_seq][table_ld] */
+} fg_ragged;
+
+/* The heads of the batch's QKV rows normed, rotated and put away, in one pass:
+ * qkv holds rows of (n_head + 2 n_kv_head) * head_dim values (q heads, k heads,
+ * v heads). With norm, each q and k head x becomes x / sqrt(mean(x^2) + eps)
+ * times wq / wk (fp32 [head_dim], nullable = ones). With rope tables cos / sin
+ * (fp32 [rope_n][head_dim/2], nullable together = no rotation; rope_n >=
+ * max_kv) the halves (x1, x2) of a q or k head at position p become (x1 c + x2 s, x2 c -
+ * x1 s) (rope_4d, src/lib/fortran_rope.f90:25-52). q goes to q_out rows of
+ * n_head * head_dim in the type of qkv, k and v to their slots, rounded to the
+ * pages' type. All arithmetic is fp32. interleaved: a head's values come in
+ * pairs (d, d + head_dim/2), as the engine keeps its QKV weights' rows; q_out
+ * and the pages are in head order either way. A row at a position below 0 or
+ * not below max_kv is left alone; one whose page is not in [0, n_pages)
+ * gets its q, and its k and v go nowhere. Two rows on one slot (a page that two
+ * sequences share) leave either's values. */
+typedef struct fg_append_cfg {
+  int32_t n_head;
+  int32_t type;        /* of qkv and q_out: FG_F32 or FG_BF16 */
+  int32_t norm, interleaved;
+  float eps;
+  int32_t rope_n;
+  const float *wq, *wk;
+  const float *cos_buf, *sin_buf;
+  int64_t qkv_ld, q_ld; /* elements between rows; 0 = packed */
+} fg_append_cfg;
+int32_t fg_qk_append(const fg_pages *pages, const fg_ragged *batch, const fg_append_cfg *cfg,
+                     const void *qkv, void *q_out, void *stream);
+
+/* Attention of the batch's new tokens over the paged cache (their own keys and
+ * values appended before): out = softmax(scale q.k) v over the keys at
+ * positions j <= p of the row's sequence and, with window > 0, only those with
+ * j > p - window or j < sinks. Query head h reads key head h / (n_head /
+ * n_kv_head). A row that sees no key gives zeros. q and out are rows of n_head *
+ * head_dim values, both fp32 or (with bf16 pages) both bf16; sums, maxima and
+ * softmax are fp32. fp32 rows come out as exact as fp32 products give them
+ * (operands in three bf16 terms); bf16 ones take one term of each, the
+ * probabilities rounded to bf16. A sequence whose table names a page outside
+ * [0, n_pages) for a position in use gives NaN rows. A NaN or infinity in a key
+ * or value that no row sees changes nothing; a value row that is not finite
+ * may reach earlier tokens of the same chunk.
+ * work: fg_paged_attn_work bytes of device memory (NULL when that is 0),
+ * written and read within the call; two calls that may run at once, replays of
+ * captured ones included, need one each. */
+typedef struct fg_attn_cfg {
+  int32_t n_head;
+  int32_t type;        /* of q and out */
+  int32_t window, sinks; /* window 0: every earlier key */
+  float scale;         /* 0: 1/sqrt(head_dim) */
+  int64_t q_ld, out_ld; /* elements between rows; 0 = packed */
+} fg_attn_cfg;
+int32_t fg_paged_attn_work(const fg_pages *pages, const fg_ragged *batch, const fg_attn_cfg *cfg,
+                           int64_t *bytes);
+int32_t fg_paged_attn(const fg_pages *pages, const fg_ragged *batch, const fg_attn_cfg *cfg,
+                      const void *q, void *out, void *work, int64_t work_bytes, void *stream);
+
+/* Page src[i] copied to page dst[i] in each of n_planes arrays of n_pages pages
+ * (plane_bytes apart; a cache's layers, keys and values), i < n. src and dst
+ * are host arrays, read before the call returns; no page may be named twice in
+ * dst nor stand in both. page_bytes a multiple of 16. */
+int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t n_pages,
+                      int64_t page_bytes, const int32_t *src, const int32_t *dst, int32_t n,
+                      void *stream);
+
+/* One id a row of logits [rows][ld] (V <= 262144 used) from given uniform
+ * numbers. With e_i = exp((x_i - max x) / temp): of the ids, the top_k largest
+ * are kept (ties: the lowest id first); of those, in descending order, each one
+ * while the mass before it is below top_p of their mass; of those, the ones
+ * with e_i >= min_p. The id drawn is the first kept one, in id order, whose
+ * cumulative mass exceeds u times the kept mass. Settings are per row
+ * (device arrays, each nullable = off; temp: 1): temp <= 0 takes the first
+ * largest id; top_k <= 0, top_p >= 1 and min_p <= 0 are off; a top_p <= 0 or
+ * min_p > 1 keeps the largest id alone; u below 0 counts as 0, 1 or more as the last
+ * mass; NaN settings are off (a NaN u counts as 0). NaN and -inf logits are
+ * never drawn; a row of nothing else gives id -1. +inf ones share the
+ * mass. probs (nullable): the drawn id's share of the kept mass. Masses are
+ * exact sums of 64-bit integers (e_i in steps of 2^-44): ids do not
+ * depend on the order of any sum. work: fg_draw_rows_work bytes, as for
+ * fg_paged_attn. */
+typedef struct fg_draw_cfg {
+  const float *temp;    /* device [rows] */
+  const int32_t *top_k;
+  const float *top_p, *min_p;
+  const float *u;       /* required */
+} fg_draw_cfg;
+int32_t fg_draw_rows_work(int32_t rows, int32_t V, int64_t *bytes);
+int32_t fg_draw_rows(const float *logits, int32_t rows, int32_t V, int64_t ld,
+                     const fg_draw_cfg *cfg, int32_t *ids, float *probs, void *work,
+                     int64_t work_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,162 @@
+"""Refusals of the paged cache's operators, on the CPU: arguments are checked
+before anything asks for a device, and nothing runs without one."""
+import ctypes as C
+
+import pytest
+
+from autoresearch_amd import engine
+
+P = 1 << 20  # a 16-byte aligned address that nothing reads
+
+
+def no_gpu():
+    import torch
+    return not torch.cuda.is_available()
+
+
+def pages(**kw):
+    a = dict(k=P, v=P, n_pages=8, page_size=16, n_kv_head=2, head_dim=64, bf16=False)
+    a.update(kw)
+    t = a.pop("type", None)
+    s = engine.pages(**a)
+    if t is not None:
+        s.type = t
+    return s
+
+
+def batch(**kw):
+    a = dict(q_start=P, kv_len=P, table=P, n_seq=2, n_rows=4, max_q=2, max_kv=32, table_ld=2)
+    a.update(kw)
+    return engine.ragged(**a)
+
+
+def attn(pg=None, bt=None, q=P, out=P, work=0, work_bytes=0, n_head=4, **kw):
+    t = kw.pop("type", None)
+    cfg = engine.attn_cfg(n_head, **kw)
+    if t is not None:
+        cfg.type = t
+    engine.paged_attn(pg or pages(), bt or batch(), cfg, q, out, work, work_bytes)
+
+
+def append(pg=None, bt=None, qkv=P, q=P, n_head=4, **kw):
+    engine.qk_append(pg or pages(), bt or batch(), engine.append_cfg(n_head, **kw), qkv, q)
+
+
+def refused(match, f, *a, **kw):
+    with pytest.raises(engine.FgptError, match=match) as e:
+        f(*a, **kw)
+    assert e.value.code == -1
+
+
+BAD_PAGES = [("NULL", dict(k=0)), ("NULL", dict(v=0)), ("head_dim", dict(head_dim=96)),
+             ("page_size", dict(page_size=8)), ("page_size", dict(page_size=48)),
+             ("page_size", dict(page_size=512)), ("n_pages", dict(n_pages=0)),
+             ("n_pages", dict(n_kv_head=0)), ("type", dict(type=5)), ("aligned", dict(k=P + 8)),
+             ("n_kv_head", dict(n_kv_head=2000))]
+BAD_BATCH = [("NULL", dict(q_start=0)), ("NULL", dict(kv_len=0)), ("NULL", dict(table=0)),
+             ("n_seq", dict(n_seq=0)), ("n_rows", dict(n_rows=-1)), ("max_q", dict(max_q=-1)),
+             ("max_kv", dict(max_kv=-1)), ("table_ld", dict(table_ld=0)), ("beyond", dict(max_kv=33)),
+             ("above 2\\^30", dict(n_rows=(1 << 30)))]
+
+
+@pytest.mark.parametrize("match,kw", BAD_PAGES)
+def test_bad_pages(match, kw):
+    refused(match, attn, pages(**kw))
+    refused(match, append, pages(**kw))
+
+
+@pytest.mark.parametrize("match,kw", BAD_BATCH)
+def test_bad_batch(match, kw):
+    refused(match, attn, bt=batch(**kw))
+    refused(match, append, bt=batch(**kw))
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("multiple of n_kv_head", dict(n_head=3)), ("multiple of n_kv_head", dict(n_head=0)),
+    ("bf16 rows need bf16 pages", dict(bf16=True)), ("row type", dict(type=9)),
+    ("window", dict(window=-1)), ("window", dict(sinks=-1)), ("scale", dict(scale=-1.0)),
+    ("scale", dict(scale=float("nan"))), ("scale", dict(scale=float("inf"))),
+    ("q_ld", dict(q_ld=255)), ("q_ld", dict(q_ld=258)), ("out_ld", dict(out_ld=128)),
+    ("NULL", dict(q=0)), ("NULL", dict(out=0)), ("aligned", dict(q=P + 4)), ("aligned", dict(out=P + 8))])
+def test_bad_attention(match, kw):
+    refused(match, attn, **kw)
+
+
+def test_attention_workspace():
+    bt = batch(max_kv=4096, table_ld=256)
+    need = engine.paged_attn_work(pages(), bt, engine.attn_cfg(4))
+    assert need > 0
+    refused("work", attn, bt=bt)
+    refused("work", attn, bt=bt, work=P, work_bytes=need - 1)
+    refused("aligned", attn, bt=bt, work=P + 4, work_bytes=need)
+    assert engine.paged_attn_work(pages(), batch(n_rows=0, max_q=0), engine.attn_cfg(4)) == 0
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("go together", dict(cos=P)), ("rope_n", dict(cos=P, sin=P, rope_n=31)),
+    ("aligned", dict(cos=P + 4, sin=P, rope_n=32)), ("eps", dict(norm=True, eps=-1.0)),
+    ("eps", dict(norm=True, eps=float("nan"))), ("qkv_ld", dict(qkv_ld=511)), ("q_ld", dict(q_ld=254)),
+    ("NULL", dict(qkv=0)), ("NULL", dict(q=0)), ("aligned", dict(qkv=P + 8)),
+    ("multiple of n_kv_head", dict(n_head=5))])
+def test_bad_append(match, kw):
+    refused(match, append, **kw)
+
+
+def copy(src=(0,), dst=(1,), base=P, planes=2, plane_bytes=256, n_pages=4, page_bytes=64):
+    engine.pages_copy(base, planes, plane_bytes, n_pages, page_bytes, list(src), list(dst))
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("outside", dict(src=[4])), ("outside", dict(dst=[-1])), ("outside", dict(src=[-1])),
+    ("named before", dict(src=[0, 2], dst=[1, 1])), ("also written", dict(src=[0, 1], dst=[1, 2])),
+    ("named before", dict(src=[0, 2], dst=[1, 0])), ("also written", dict(src=[1], dst=[1])),
+    ("n_planes", dict(planes=0)), ("n_planes", dict(planes=70000)), ("page_bytes", dict(page_bytes=24)),
+    ("page_bytes", dict(page_bytes=0)), ("plane_bytes", dict(plane_bytes=192)),
+    ("plane_bytes", dict(plane_bytes=264)), ("NULL", dict(base=0)), ("aligned", dict(base=P + 4))])
+def test_bad_copy(match, kw):
+    refused(match, copy, **kw)
+
+
+def test_copy_lists_of_unlike_length():
+    with pytest.raises(ValueError):
+        copy(src=[0, 1], dst=[2])
+
+
+def draw(logits=P, rows=2, V=100, ld=100, u=P, ids=P, **kw):
+    engine.draw_rows(logits, rows, V, ld, u, ids, work=P, work_bytes=1 << 40, **kw)
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("rows", dict(rows=-1)), ("V 0", dict(V=0)), ("V 262145", dict(V=262145, ld=262145)), ("ld", dict(ld=99)),
+    ("NULL", dict(logits=0)), ("NULL", dict(u=0)), ("NULL", dict(ids=0))])
+def test_bad_draw(match, kw):
+    refused(match, draw, **kw)
+
+
+def test_null_structs():
+    lib = engine.load_library()
+    n = C.c_int64()
+    assert lib.fg_paged_attn(None, None, None, P, P, None, 0, None) == -1
+    assert lib.fg_paged_attn(pages(), batch(), None, P, P, None, 0, None) == -1
+    assert lib.fg_qk_append(pages(), None, None, P, P, None) == -1
+    assert lib.fg_qk_append(pages(), batch(), None, P, P, None) == -1
+    assert lib.fg_draw_rows(P, 1, 5, 5, None, P, None, None, 0, None) == -1
+    assert lib.fg_paged_attn_work(pages(), batch(), engine.attn_cfg(4), None) == -1
+    assert lib.fg_draw_rows_work(1, 5, None) == -1
+    assert lib.fg_pages_copy(P, 1, 0, 4, 16, None, None, 1, None) == -1
+    assert lib.fg_draw_rows_work(1, 5, C.byref(n)) == 0
+
+
+@pytest.mark.skipif(not no_gpu(), reason="a GPU is visible")
+def test_no_device_fails_loudly():
+    for f in (lambda: attn(work=P, work_bytes=1 << 40), append, copy, draw):
+        with pytest.raises(engine.FgptError) as e:
+            f()
+        assert e.value.code == -7
+
+
+def test_nothing_to_do_needs_no_device():
+    attn(bt=batch(n_rows=0))
+    append(bt=batch(n_rows=0))
+    copy(src=[], dst=[])
+    draw(rows=0)
