@@ -14,6 +14,7 @@
 #include <condition_variable>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <system_error>
 #include <thread>
@@ -23,6 +24,7 @@
 
 #include "../../include/fgpt.h"
 #include "fgpt_internal.h"
+#include "paged_internal.h"
 
 using namespace fgpt;
 
@@ -2311,4 +2313,457 @@ extern "C" int32_t fg_model_bytes(const fg_model* m, int64_t* weight_bytes, int6
     *work_bytes = n;
   }
   return FG_OK;
+}
+
+// ------------------------------------------------------------ paged cache
+struct fg_paged {
+  fg_model* m = nullptr;
+  fg_pool* pool = nullptr;
+  int n_pages = 0, page_size = 0, max_seq = 0, window = 0, sinks = 0;
+  bool kv16 = false;
+  char* kv = nullptr;         // [2 (k, v)][L][n_pages][KH][page_size][hd]
+  int64_t plane_bytes = 0, page_bytes = 0;
+  float* last = nullptr;      // [max_seq][D], then [max_seq][H*hd]: last tokens' rows
+  char* meta = nullptr;       // a step's ids, lengths, tables and settings
+  char* h_meta = nullptr;     // pinned: the same, as the host writes them
+  int64_t meta_bytes = 0;
+  char* work = nullptr;       // the attention's or the draw's workspace
+  int64_t work_bytes = 0;
+};
+
+namespace {
+
+fg_pages paged_layer(const fg_paged* pc, int l) {
+  const Dims& d = pc->m->d;
+  fg_pages p;
+  p.k = pc->kv + l * pc->plane_bytes;
+  p.v = pc->kv + (d.L + l) * pc->plane_bytes;
+  p.n_pages = pc->n_pages;
+  p.page_size = pc->page_size;
+  p.n_kv_head = d.KH;
+  p.head_dim = d.hd;
+  p.type = pc->kv16 ? FG_BF16 : FG_F32;
+  return p;
+}
+
+// *p of at least `need` bytes; what it held is lost.
+int32_t grow(fg_model* m, char** p, int64_t* have, int64_t need) {
+  if (need <= *have) return FG_OK;
+  RCCHK(quiesce(m));
+  if (*p) HIPCHK(hipFree(*p));
+  *p = nullptr;
+  *have = 0;
+  HIPCHK(hipMalloc((void**)p, (size_t)need));
+  *have = need;
+  return FG_OK;
+}
+
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// The pass of fg_paged_step: rows token rows of the batch b (device arrays) at
+// m->ws.ids; logits of the n sequences' last rows to m->ws.logits. Where there
+// are more rows than sequences, the last layer goes on with the last tokens
+// alone from its attention on (batch one: one new token a sequence, whose row is
+// last_rows[i]).
+void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, const fg_ragged& b,
+                  const fg_ragged& one, const int32_t* last_rows, int64_t pairs, int64_t keys) {
+  const Dims& d = m->d;
+  Work& ws = m->ws;
+  int rows = b.n_rows;
+  const int n = one.n_rows;
+  bool gm = use_gemm(d, rows);
+  int64_t prow = tile_rows(rows);
+  float* x = ws.x;
+  const float* q = ws.q;
+  auto W = [&](const bf16_t* p) { return gm ? m->wt + (p - m->w.base) : p; };
+  const double ekv = pc->kv16 ? 2 : 4;
+  timed(m, s, FG_K_OTHER, 0, (double)rows * d.D * (gm ? 10 : 6), [&] {
+    launch_embed_norm(s, d, m->w.wte, ids, rows, x, gm ? ws.xs : nullptr, prow * d.D,
+                      gm ? ws.ssq : nullptr);
+  });
+  int nt = 1;  // partial sums of squares per row of the residual
+  const fg_append_cfg ap = {d.H, FG_F32, 0, 1, 0.f, m->rope_n, nullptr, nullptr, m->d_cos, m->d_sin, 0, 0};
+  const fg_attn_cfg at = {d.H, FG_F32, pc->window, pc->sinks, 0.f, 0, 0};
+  for (int l = 0; l < d.L; ++l) {
+    const fg_pages pg = paged_layer(pc, l);
+    GemvArgs a = base_args(m, ws);
+    a.M = rows;
+    a.T = rows;
+    // q, k, v = rmsnorm(x) Wqkv^T into h (fc's place), then rotated: q out, k and
+    // v into their pages
+    a.x = x; a.xs = ws.xs; a.xs_plane = prow * d.D; a.ssq_in = ws.ssq; a.ssq_n = nt;
+    a.w = W(m->w.qkv(l)); a.N = d.nqkv(); a.K = d.D; a.norm = 1; a.y = ws.h;
+    linear(m, s, GV_STORE, a, nullptr, gm);
+    timed(m, s, FG_K_OTHER, 0, rows * (4.0 * (d.nqkv() + d.qd()) + 2 * ekv * d.kvd()), [&] {
+      launch_qk_append(s, pg, b, ap, ws.h, ws.q);
+    });
+    const bool cut = l == d.L - 1 && rows > n;
+    if (cut) {  // go on with the last token of each sequence
+      float* lx = pc->last;
+      float* lq = pc->last + (int64_t)pc->max_seq * d.D;
+      timed(m, s, FG_K_OTHER, 0, 8.0 * n * (d.D + d.qd()), [&] {
+        launch_take_rows(s, last_rows, n, x, lx, d.D, ws.q, lq, d.qd());
+      });
+      x = lx;
+      q = lq;
+      rows = a.M = a.T = n;
+      gm = use_gemm(d, rows);
+      prow = tile_rows(rows);
+    }
+    PagedOut out;
+    out.y = ws.ao;
+    out.ld = d.qd();
+    if (gm) {
+      out.planes = ws.aos;
+      out.plane = prow * d.qd();
+    }
+    const double seen = cut ? keys : pairs;
+    timed(m, s, b.max_q > 1 && !cut ? FG_K_ATTN_CHUNK : FG_K_ATTN_DECODE, 4.0 * d.hd * d.H * seen,
+          8.0 * rows * d.qd() + 2 * ekv * keys * d.kvd(), [&] {
+            launch_paged_attn(s, pg, cut ? one : b, at, q, out, (float*)pc->work);
+          });
+    // x += attn_out Wproj^T; h = relu(rmsnorm(x) Wfc^T)^2; x += h Wproj2^T
+    a.x = ws.ao; a.xs = ws.aos; a.xs_plane = prow * d.qd(); a.ssq_n = 0;
+    a.w = W(m->w.proj(l)); a.N = d.D; a.K = d.qd(); a.norm = 0; a.y = x;
+    a.ys = ws.xs; a.ys_plane = prow * d.D; a.ssq_out = ws.ssq;
+    linear(m, s, GV_RESID, a, nullptr, gm);
+    nt = gemm_ssq_parts(rows, d.D, d.qd());
+    a.x = x; a.xs = ws.xs; a.xs_plane = prow * d.D; a.ssq_in = ws.ssq; a.ssq_n = nt;
+    a.w = W(m->w.fc(l)); a.N = d.dff; a.K = d.D; a.norm = 1; a.y = ws.h;
+    a.ys = ws.hs; a.ys_plane = prow * d.dff; a.ssq_out = nullptr;
+    linear(m, s, GV_RELU2, a, nullptr, gm);
+    a.x = ws.h; a.xs = ws.hs; a.xs_plane = prow * d.dff; a.ssq_n = 0;
+    a.w = W(m->w.proj2(l)); a.N = d.D; a.K = d.dff; a.norm = 0; a.y = x;
+    a.ys = ws.xs; a.ys_plane = prow * d.D; a.ssq_out = ws.ssq;
+    linear(m, s, GV_RESID, a, nullptr, gm);
+    nt = gemm_ssq_parts(rows, d.D, d.dff);
+  }
+  GemvArgs a = base_args(m, ws);
+  a.M = a.T = rows;
+  a.x = x; a.xs = ws.xs; a.xs_plane = prow * d.D; a.ssq_in = ws.ssq; a.ssq_n = nt;
+  a.w = W(m->w.lm); a.N = d.V; a.K = d.D; a.norm = 1; a.y = ws.logits;
+  linear(m, s, GV_STORE, a, nullptr, gm);
+}
+
+int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const int32_t* counts,
+                   const int32_t* ids, const fg_draw_cfg* draw, float* logits, int32_t* next_ids) {
+  const Dims& d = m->d;
+  // what the batch needs, before anything changes
+  std::vector<uint8_t> named((size_t)pc->max_seq, 0);
+  std::vector<int32_t> len((size_t)n);
+  std::map<int32_t, int> shared;  // copies that a shared last page still takes
+  int64_t rows = 0, need = 0, pairs = 0, keys = 0;
+  int max_q = 0, max_kv = 0;
+  for (int i = 0; i < n; ++i) {
+    if (seqs[i] < 0 || seqs[i] >= pc->max_seq)
+      return seterr(FG_EARG, "sequence %d outside [0, %d)", seqs[i], pc->max_seq);
+    if (named[seqs[i]]) return seterr(FG_EARG, "sequence %d is named twice", seqs[i]);
+    named[seqs[i]] = 1;
+    if (counts[i] < 1) return seterr(FG_EARG, "counts must be >= 1");
+    int32_t pages = 0;
+    RCCHK(fg_pool_need(pc->pool, seqs[i], counts[i], &pages));
+    RCCHK(fg_pool_len(pc->pool, seqs[i], &len[i]));
+    // (the last holder of a shared page keeps it: of k sequences that go on from
+    // one all but one take a copy where nobody else holds it)
+    int32_t holders = 0;
+    const int32_t page = pool_last_page(pc->pool, seqs[i], &holders);
+    if (len[i] % pc->page_size && holders > 1) {
+      auto it = shared.emplace(page, holders - 1).first;
+      if (it->second-- <= 0) --pages;
+    }
+    len[i] += counts[i];
+    need += pages;
+    rows += counts[i];
+    pairs += (int64_t)counts[i] * (len[i] - counts[i]) + (int64_t)counts[i] * (counts[i] + 1) / 2;
+    keys += len[i];
+    max_q = std::max(max_q, counts[i]);
+    max_kv = std::max(max_kv, len[i]);
+  }
+  if (rows > (1ll << 30) / std::max(d.V, d.dff)) return seterr(FG_EARG, "%lld tokens: too many", (long long)rows);
+  RCCHK(check_ids(m, ids, rows));
+  RCCHK(check_rope(m, max_kv));
+  int32_t nfree = 0;
+  RCCHK(fg_pool_free(pc->pool, &nfree));
+  if (need > nfree)
+    return seterr(FG_EFULL, "page pool full: %lld pages needed, %d free", (long long)need, nfree);
+  RCCHK(ensure_work(m, rows));
+  // the step's arrays on the device, one copy for all of them
+  const int ld = (max_kv + pc->page_size - 1) / pc->page_size;
+  int64_t at = 0;
+  auto place = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up16(bytes);
+    return o;
+  };
+  const int64_t o_ids = place(rows * 4), o_start = place((n + 1) * 4ll), o_one = place((n + 1) * 4ll),
+                o_len = place(n * 4ll), o_last = place(n * 4ll), o_table = place((int64_t)n * ld * 4);
+  const int64_t o_set = place(5 * up16(n * 4ll));
+  if (at > pc->meta_bytes) {
+    if (pc->h_meta) HIPCHK(hipHostFree(pc->h_meta));
+    pc->h_meta = nullptr;
+    const int64_t want = at + at / 2;
+    RCCHK(grow(m, &pc->meta, &pc->meta_bytes, want));
+    if (hipHostMalloc((void**)&pc->h_meta, (size_t)want, hipHostMallocDefault) != hipSuccess) {
+      pc->h_meta = nullptr;
+      pc->meta_bytes = 0;
+      (void)hipGetLastError();
+      (void)hipFree(pc->meta);
+      pc->meta = nullptr;
+      return seterr(FG_EHIP, "no %lld bytes of pinned host memory", (long long)want);
+    }
+  }
+  fg_ragged b = {n, (int32_t)rows, max_q, max_kv, ld, (int32_t*)(pc->meta + o_start),
+                 (int32_t*)(pc->meta + o_len), (int32_t*)(pc->meta + o_table)};
+  fg_ragged one = b;
+  one.n_rows = n;
+  one.max_q = 1;
+  one.q_start = (int32_t*)(pc->meta + o_one);
+  const fg_attn_cfg cfg = {d.H, FG_F32, pc->window, pc->sinks, 0.f, 0, 0};
+  int64_t wb = 4 * std::max(paged_attn_floats(paged_layer(pc, 0), b, cfg),
+                            paged_attn_floats(paged_layer(pc, 0), one, cfg));
+  wb = std::max(wb, draw_work_bytes(n, d.V));
+  RCCHK(grow(m, &pc->work, &pc->work_bytes, wb));
+
+  // from here on the sequences have their new tokens' pages
+  std::vector<int32_t> src, dst;
+  src.reserve((size_t)n);
+  dst.reserve((size_t)n);
+  auto H = [&](int64_t o) { return (int32_t*)(pc->h_meta + o); };
+  int done = 0;
+  hipStream_t s = m->stream;
+  auto copies = [&] {  // what the shared last pages held, into the sequences' own
+    if (src.empty()) return;
+    timed(m, s, FG_K_OTHER, 0, 4.0 * d.L * pc->page_bytes * src.size(), [&] {
+      launch_pages_copy(s, pc->kv, 2 * d.L, pc->plane_bytes, pc->page_bytes, src.data(), dst.data(),
+                        (int32_t)src.size());
+    });
+  };
+  auto undo = [&](int32_t rc) {  // the new tokens' positions go again
+    (void)hipStreamSynchronize(s);
+    for (int i = 0; i < done; ++i) (void)fg_pool_trim(pc->pool, seqs[i], len[i] - counts[i]);
+    return rc;
+  };
+  memcpy(H(o_ids), ids, (size_t)rows * 4);
+  int32_t r = 0;
+  for (int i = 0; i < n; ++i) {
+    int32_t a = -1, c = -1;
+    const int32_t rc = fg_pool_extend(pc->pool, seqs[i], counts[i], &a, &c);
+    if (rc != FG_OK) {
+      copies();
+      return undo(rc);
+    }
+    ++done;
+    if (a >= 0) {
+      src.push_back(a);
+      dst.push_back(c);
+    }
+    H(o_start)[i] = r;
+    H(o_one)[i] = i;
+    r += counts[i];
+    H(o_last)[i] = r - 1;
+    H(o_len)[i] = len[i];
+    int32_t* row = H(o_table) + (int64_t)i * ld;
+    int32_t held = 0;
+    (void)fg_pool_table(pc->pool, seqs[i], row, ld, &held);
+    std::fill(row + held, row + ld, -1);
+  }
+  H(o_start)[n] = r;
+  H(o_one)[n] = n;
+  fg_draw_cfg dc = {};
+  if (draw) {
+    const int64_t col = up16(n * 4ll);
+    auto put = [&](int k, const void* p) -> const void* {
+      if (!p) return nullptr;
+      memcpy(pc->h_meta + o_set + k * col, p, (size_t)n * 4);
+      return pc->meta + o_set + k * col;
+    };
+    dc.temp = (const float*)put(0, draw->temp);
+    dc.top_k = (const int32_t*)put(1, draw->top_k);
+    dc.top_p = (const float*)put(2, draw->top_p);
+    dc.min_p = (const float*)put(3, draw->min_p);
+    dc.u = (const float*)put(4, draw->u);
+  }
+  auto run = [&]() -> int32_t {
+    copies();
+    HIPCHK(hipMemcpyAsync(pc->meta, pc->h_meta, (size_t)at, hipMemcpyHostToDevice, s));
+    paged_layers(m, pc, s, (int32_t*)(pc->meta + o_ids), b, one, (int32_t*)(pc->meta + o_last), pairs, keys);
+    if (next_ids) {
+      timed(m, s, FG_K_OTHER, 0, 4.0 * n * d.V, [&] {
+        if (draw)
+          launch_draw_rows(s, m->ws.logits, n, d.V, d.V, dc, m->ws.amax, nullptr, pc->work);
+        else
+          launch_argmax(s, m->ws.logits, n, d.V, m->ws.amax);
+      });
+    }
+    HIPCHK(hipGetLastError());
+    if (next_ids) HIPCHK(hipMemcpyAsync(next_ids, m->ws.amax, (size_t)n * 4, hipMemcpyDeviceToHost, s));
+    if (logits) RCCHK(copy_out(m, logits, m->ws.logits, (size_t)n * d.V * 4, s));
+    HIPCHK(hipStreamSynchronize(s));
+    return FG_OK;
+  };
+  const int32_t rc = run();
+  if (rc != FG_OK) return undo(rc);
+  if (pc->window > 0)
+    for (int i = 0; i < n; ++i) RCCHK(fg_pool_slide(pc->pool, seqs[i], pc->window, pc->sinks));
+  return FG_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t fg_paged_create(fg_model* m, int32_t n_pages, int32_t page_size, int32_t max_seq,
+                                   int32_t flags, int32_t window, int32_t sinks, fg_paged** out) {
+  if (!m || !out) return seterr(FG_EARG, "NULL argument");
+  *out = nullptr;
+  if (flags & ~FG_KV_BF16) return seterr(FG_EARG, "unknown cache flags 0x%x", flags);
+  if (window < 0 || sinks < 0 || window > (1 << 30) || sinks > (1 << 30))
+    return seterr(FG_EARG, "window and sinks must be in 0..2^30");
+  GUARD(m);
+  const Dims& d = m->d;
+  fg_pool* pool = nullptr;
+  RCCHK(fg_pool_create(n_pages, page_size, max_seq, &pool));
+  fg_paged* pc = new (std::nothrow) fg_paged();
+  if (!pc) {
+    (void)fg_pool_destroy(pool);
+    return seterr(FG_EARG, "out of host memory");
+  }
+  pc->m = m;
+  pc->pool = pool;
+  pc->n_pages = n_pages;
+  pc->page_size = page_size;
+  pc->max_seq = max_seq;
+  pc->window = window;
+  pc->sinks = sinks;
+  pc->kv16 = (flags & FG_KV_BF16) != 0;
+  pc->page_bytes = (int64_t)d.kvd() * page_size * (pc->kv16 ? 2 : 4);
+  pc->plane_bytes = n_pages * pc->page_bytes;
+  const size_t bytes = (size_t)(2 * d.L * pc->plane_bytes);
+  const size_t last = (size_t)max_seq * (d.D + d.qd()) * 4;
+  hipError_t e = hipMalloc((void**)&pc->kv, bytes);
+  if (e == hipSuccess) e = hipMalloc((void**)&pc->last, last);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->kv, 0, bytes, m->stream);
+  if (e == hipSuccess) e = hipMemsetAsync(pc->last, 0, last, m->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(m->stream);
+  if (e != hipSuccess) {
+    (void)hipStreamSynchronize(m->stream);
+    if (pc->kv) (void)hipFree(pc->kv);
+    if (pc->last) (void)hipFree(pc->last);
+    (void)fg_pool_destroy(pool);
+    delete pc;
+    return seterr(FG_EHIP, "paged cache allocation (%zu bytes): %s", bytes, hipGetErrorString(e));
+  }
+  *out = pc;
+  return FG_OK;
+}
+
+extern "C" int32_t fg_paged_destroy(fg_paged* pc) {
+  if (!pc) return FG_OK;
+  (void)hipSetDevice(pc->m->device);
+  (void)hipStreamSynchronize(pc->m->stream);
+  void* ptrs[] = {pc->kv, pc->last, pc->meta, pc->work};
+  for (void* p : ptrs)
+    if (p) (void)hipFree(p);
+  if (pc->h_meta) (void)hipHostFree(pc->h_meta);
+  (void)fg_pool_destroy(pc->pool);
+  delete pc;
+  return FG_OK;
+}
+
+extern "C" int32_t fg_paged_len(const fg_paged* pc, int32_t seq, int32_t* len) {
+  if (!pc) return seterr(FG_EARG, "NULL argument");
+  return fg_pool_len(pc->pool, seq, len);
+}
+
+extern "C" int32_t fg_paged_free(const fg_paged* pc, int32_t* n_pages) {
+  if (!pc) return seterr(FG_EARG, "NULL argument");
+  return fg_pool_free(pc->pool, n_pages);
+}
+
+extern "C" int32_t fg_paged_fork(fg_paged* pc, int32_t from, int32_t to, int32_t len) {
+  if (!pc) return seterr(FG_EARG, "NULL argument");
+  GUARD(pc->m);
+  return fg_pool_fork(pc->pool, from, to, len);
+}
+
+extern "C" int32_t fg_paged_trim(fg_paged* pc, int32_t seq, int32_t len) {
+  if (!pc) return seterr(FG_EARG, "NULL argument");
+  GUARD(pc->m);
+  return fg_pool_trim(pc->pool, seq, len);
+}
+
+extern "C" int32_t fg_paged_compact(fg_paged* pc, int32_t* moved) {
+  if (!pc) return seterr(FG_EARG, "NULL argument");
+  fg_model* m = pc->m;
+  GUARD(m);
+  try {
+    std::vector<int32_t> src((size_t)pc->n_pages), dst((size_t)pc->n_pages);
+    int32_t n = 0;
+    RCCHK(fg_pool_compact(pc->pool, src.data(), dst.data(), pc->n_pages, &n));
+    if (n > 0) {
+      hipStream_t s = m->stream;
+      timed(m, s, FG_K_OTHER, 0, 4.0 * m->d.L * pc->page_bytes * n, [&] {
+        launch_pages_copy(s, pc->kv, 2 * m->d.L, pc->plane_bytes, pc->page_bytes, src.data(), dst.data(), n);
+      });
+      HIPCHK(hipGetLastError());
+      HIPCHK(hipStreamSynchronize(s));
+    }
+    if (moved) *moved = n;
+  } catch (const std::exception& e) {
+    return seterr(FG_EARG, "paged cache: %s", e.what());
+  }
+  return FG_OK;
+}
+
+extern "C" int32_t fg_paged_read(fg_paged* pc, int32_t seq, float* k_out, float* v_out) {
+  if (!pc) return seterr(FG_EARG, "NULL argument");
+  fg_model* m = pc->m;
+  GUARD(m);
+  const Dims& d = m->d;
+  int32_t len = 0, n = 0;
+  RCCHK(fg_pool_len(pc->pool, seq, &len));
+  try {
+    RCCHK(fg_pool_table(pc->pool, seq, nullptr, 0, &n));
+    std::vector<int32_t> pages((size_t)n);
+    RCCHK(fg_pool_table(pc->pool, seq, pages.data(), n, &n));
+    HIPCHK(hipStreamSynchronize(m->stream));
+    std::vector<char> page((size_t)pc->page_bytes);
+    float* outs[2] = {k_out, v_out};
+    for (int t = 0; t < 2; ++t)
+      for (int l = 0; outs[t] && l < d.L; ++l)
+        for (int i = 0; i < n; ++i) {
+          const char* src = pc->kv + (t * d.L + l) * pc->plane_bytes + pages[i] * pc->page_bytes;
+          if (pages[i] >= 0)
+            HIPCHK(hipMemcpy(page.data(), src, (size_t)pc->page_bytes, hipMemcpyDeviceToHost));
+          for (int h = 0; h < d.KH; ++h)
+            for (int p = i * pc->page_size; p < std::min<int>(len, (i + 1) * pc->page_size); ++p)
+              for (int e = 0; e < d.hd; ++e) {
+                const size_t at = ((size_t)h * pc->page_size + p % pc->page_size) * d.hd + e;
+                float v = 0.f;
+                if (pages[i] >= 0 && pc->kv16) {
+                  const uint32_t u = (uint32_t)((const uint16_t*)page.data())[at] << 16;
+                  memcpy(&v, &u, 4);
+                } else if (pages[i] >= 0) {
+                  v = ((const float*)page.data())[at];
+                }
+                outs[t][((size_t)l * len + p) * d.kvd() + h * d.hd + e] = v;
+              }
+        }
+  } catch (const std::exception& e) {
+    return seterr(FG_EARG, "paged cache: %s", e.what());
+  }
+  return FG_OK;
+}
+
+extern "C" int32_t fg_paged_step(fg_model* m, fg_paged* pc, int32_t n, const int32_t* seqs,
+                                 const int32_t* counts, const int32_t* ids, const fg_draw_cfg* draw,
+                                 float* logits, int32_t* next_ids) {
+  if (!m || !pc || pc->m != m || !seqs || !counts || !ids) return seterr(FG_EARG, "bad argument");
+  if (n < 1) return seterr(FG_EARG, "n must be >= 1");
+  if (draw && (!draw->u || !next_ids)) return seterr(FG_EARG, "a draw needs u and next_ids");
+  if (draw && m->d.V > DRAW_MAX_V) return seterr(FG_EARG, "draws up to %d ids", DRAW_MAX_V);
+  GUARD(m);
+  try {
+    return paged_pass(m, pc, n, seqs, counts, ids, draw, logits, next_ids);
+  } catch (const std::exception& e) {
+    return seterr(FG_EARG, "paged step: %s", e.what());
+  }
 }

@@ -180,6 +180,15 @@ __global__ __launch_bounds__(256) void k_pages_copy(CopyArgs a) {
     if (at + k * 4096 < a.page_bytes) *(u32x4v_t*)(d + at + k * 4096) = v[k];
 }
 
+__global__ __launch_bounds__(256) void k_take_rows(const int32_t* __restrict__ rows,
+                                                   const float* __restrict__ x, float* __restrict__ xo,
+                                                   int nx, const float* __restrict__ q,
+                                                   float* __restrict__ qo, int nq) {
+  const int64_t from = rows[blockIdx.x], to = blockIdx.x;
+  for (int k = threadIdx.x; k < nx; k += 256) xo[to * nx + k] = x[from * nx + k];
+  for (int k = threadIdx.x; k < nq; k += 256) qo[to * nq + k] = q[from * nq + k];
+}
+
 template <int HD>
 void append_hd(hipStream_t s, const AppendArgs& a) {
   const dim3 grid((unsigned)a.b.n_rows), block(256);
@@ -204,6 +213,11 @@ void launch_qk_append(hipStream_t s, const fg_pages& pg, const fg_ragged& b, con
     append_hd<128>(s, a);
   else
     append_hd<64>(s, a);
+}
+
+void launch_take_rows(hipStream_t s, const int32_t* rows, int n, const float* x, float* xo, int nx,
+                      const float* q, float* qo, int nq) {
+  FG_LAUNCH(k_take_rows, dim3((unsigned)n), dim3(256), 0, s, rows, x, xo, nx, q, qo, nq);
 }
 
 void launch_pages_copy(hipStream_t s, void* base, int32_t n_planes, int64_t plane_bytes,

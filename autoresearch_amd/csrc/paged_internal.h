@@ -29,6 +29,14 @@ void launch_qk_append(hipStream_t s, const fg_pages& pg, const fg_ragged& b, con
 void launch_pages_copy(hipStream_t s, void* base, int32_t n_planes, int64_t plane_bytes,
                        int64_t page_bytes, const int32_t* src, const int32_t* dst, int32_t n);
 
+// xo[i] = x[rows[i]] (nx floats a row), qo likewise of q (nq), i < n.
+void launch_take_rows(hipStream_t s, const int32_t* rows, int n, const float* x, float* xo, int nx,
+                      const float* q, float* qo, int nq);
+
+// ---- pages
+// The last page of a pool's sequence (-1: none) and how many sequences hold it.
+int32_t pool_last_page(const fg_pool* p, int32_t seq, int32_t* holders);
+
 // ---- draws
 constexpr int32_t DRAW_MAX_V = 1 << 18;
 int64_t draw_work_bytes(int32_t rows, int32_t V);

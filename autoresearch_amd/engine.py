@@ -37,6 +37,11 @@ EXPORTS = (
     "fg_sample", "fg_decode_sample", "fg_set_option", "fg_get_option", "fg_step_dev_noalloc",
     "fg_qk_append", "fg_paged_attn_work", "fg_paged_attn", "fg_pages_copy", "fg_draw_rows_work",
     "fg_draw_rows",
+    "fg_pool_create", "fg_pool_destroy", "fg_pool_len", "fg_pool_free", "fg_pool_table",
+    "fg_pool_need", "fg_pool_extend", "fg_pool_fork", "fg_pool_trim", "fg_pool_slide",
+    "fg_pool_compact",
+    "fg_paged_create", "fg_paged_destroy", "fg_paged_len", "fg_paged_free", "fg_paged_fork",
+    "fg_paged_trim", "fg_paged_compact", "fg_paged_read", "fg_paged_step",
 )
 
 KERNEL_KINDS = {0: "gemm", 1: "gemv", 2: "attn_chunk", 3: "attn_decode", 4: "other",
@@ -180,6 +185,26 @@ def load_library(path: str = LIB_PATH):
         "fg_pages_copy": (i32, [_vp, i32, i64, i32, i64, _i, _i, i32, _vp]),
         "fg_draw_rows_work": (i32, [i32, i32, C.POINTER(i64)]),
         "fg_draw_rows": (i32, [_vp, i32, i32, i64, C.POINTER(_DrawCfg), _vp, _vp, _vp, i64, _vp]),
+        "fg_pool_create": (i32, [i32, i32, i32, C.POINTER(_vp)]),
+        "fg_pool_destroy": (i32, [_vp]),
+        "fg_pool_len": (i32, [_vp, i32, _i]),
+        "fg_pool_free": (i32, [_vp, _i]),
+        "fg_pool_table": (i32, [_vp, i32, _i, i32, _i]),
+        "fg_pool_need": (i32, [_vp, i32, i32, _i]),
+        "fg_pool_extend": (i32, [_vp, i32, i32, _i, _i]),
+        "fg_pool_fork": (i32, [_vp, i32, i32, i32]),
+        "fg_pool_trim": (i32, [_vp, i32, i32]),
+        "fg_pool_slide": (i32, [_vp, i32, i32, i32]),
+        "fg_pool_compact": (i32, [_vp, _i, _i, i32, _i]),
+        "fg_paged_create": (i32, [_vp, i32, i32, i32, i32, i32, i32, C.POINTER(_vp)]),
+        "fg_paged_destroy": (i32, [_vp]),
+        "fg_paged_len": (i32, [_vp, i32, _i]),
+        "fg_paged_free": (i32, [_vp, _i]),
+        "fg_paged_fork": (i32, [_vp, i32, i32, i32]),
+        "fg_paged_trim": (i32, [_vp, i32, i32]),
+        "fg_paged_compact": (i32, [_vp, _i]),
+        "fg_paged_read": (i32, [_vp, i32, _f, _f]),
+        "fg_paged_step": (i32, [_vp, _vp, i32, _i, _i, _i, C.POINTER(_DrawCfg), _f, _i]),
         "fg_timing_read": (i32, [_vp, i32, C.POINTER(i64), C.POINTER(C.c_double),
                                  C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     }
@@ -384,6 +409,10 @@ class Model:
     def kv(self, B: int, maxT: int, bf16: bool = False) -> "KV":
         return KV(self, B, maxT, bf16)
 
+    def paged(self, n_pages: int, page_size: int = 64, max_seq: int = 64, bf16: bool = False,
+              window: int = 0, sinks: int = 0) -> "Paged":
+        return Paged(self, n_pages, page_size, max_seq, bf16, window, sinks)
+
 
 class KV:
     """A KV cache of B sequences x maxT positions resident in HBM."""
@@ -473,6 +502,158 @@ class KV:
         `prompt` (its first len-1 ids already cached, B = 1). Returns the
         n_gen ids and the generator state after them."""
         return _decode_sample(self, prompt, n_gen, seed, cfg)
+
+
+class Paged:
+    """fg_paged: a model's KV cache in pages, for sequences of their own lengths
+    (numbered 0..max_seq-1, empty until a step names them)."""
+
+    def __init__(self, m: Model, n_pages: int, page_size: int = 64, max_seq: int = 64,
+                 bf16: bool = False, window: int = 0, sinks: int = 0):
+        self.m, self.n_pages, self.page_size, self.max_seq = m, n_pages, page_size, max_seq
+        self._h = _vp()
+        _check(_LIB.fg_paged_create(m.handle, n_pages, page_size, max_seq, FG_KV_BF16 if bf16 else 0,
+                                    window, sinks, C.byref(self._h)))
+
+    def close(self):
+        if self._h:
+            _LIB.fg_paged_destroy(self._h)
+            self._h = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def len(self, seq: int) -> int:
+        v = C.c_int32()
+        _check(_LIB.fg_paged_len(self._h, seq, C.byref(v)))
+        return v.value
+
+    @property
+    def free(self) -> int:
+        """Free pages."""
+        v = C.c_int32()
+        _check(_LIB.fg_paged_free(self._h, C.byref(v)))
+        return v.value
+
+    def fork(self, src: int, dst: int, length: int | None = None):
+        """The empty sequence dst shares the first `length` positions of src (all of them)."""
+        _check(_LIB.fg_paged_fork(self._h, src, dst, self.len(src) if length is None else length))
+
+    def trim(self, seq: int, length: int = 0):
+        """Drops the positions from `length` on; 0 ends the sequence."""
+        _check(_LIB.fg_paged_trim(self._h, seq, length))
+
+    def compact(self) -> int:
+        """Moves the pages in use to the lowest places; how many moved."""
+        v = C.c_int32()
+        _check(_LIB.fg_paged_compact(self._h, C.byref(v)))
+        return v.value
+
+    def read(self, seq: int):
+        """Keys and values of a sequence, fp32 [n_layer, len, n_kv_head * head_dim]."""
+        d = self.m.d
+        shape = (d.n_layer, self.len(seq), d.n_kv_head * d.head_dim)
+        k, v = np.empty(shape, np.float32), np.empty(shape, np.float32)
+        _check(_LIB.fg_paged_read(self._h, seq, _fp(k), _fp(v)))
+        return k, v
+
+    def step(self, batch: dict, want_logits: bool = True, u=None, temp=None, top_k=None, top_p=None,
+             min_p=None):
+        """fg_paged_step over {sequence: its new ids}: (logits [n, V] or None,
+        next ids [n]) of each sequence's last token, in the dict's order. With u
+        (a uniform number a sequence) the ids are drawn under the given
+        settings (a value a sequence, or one for all), else they are the argmax."""
+        seqs = _i32(list(batch))
+        parts = [_i32(v).reshape(-1) for v in batch.values()]
+        n = seqs.size
+        counts = _i32([p.size for p in parts])
+        ids = np.concatenate(parts) if n else _i32([])
+        draw, keep = None, []
+        if u is not None:
+            def col(a, t):
+                if a is None:
+                    return None
+                keep.append(np.ascontiguousarray(np.broadcast_to(np.asarray(a, t), (n,))))
+                return keep[-1].ctypes.data
+            draw = _DrawCfg(col(temp, np.float32), col(top_k, np.int32), col(top_p, np.float32),
+                            col(min_p, np.float32), col(u, np.float32))
+        elif any(a is not None for a in (temp, top_k, top_p, min_p)):
+            raise ValueError("settings of a draw without u")
+        lg = np.empty((n, self.m.d.vocab), np.float32) if want_logits else None
+        nxt = np.empty(n, np.int32)
+        _check(_LIB.fg_paged_step(self.m.handle, self._h, n, _ip(seqs), _ip(counts), _ip(ids), draw,
+                                  _fp(lg), _ip(nxt)))
+        return lg, nxt
+
+
+class Pool:
+    """fg_pool: which pages the sequences of a paged cache hold (host only), for
+    callers of the operators on pages of their own."""
+
+    def __init__(self, n_pages: int, page_size: int, max_seq: int):
+        self.n_pages, self.page_size, self.max_seq = n_pages, page_size, max_seq
+        self._h = _vp()
+        _check(load_library().fg_pool_create(n_pages, page_size, max_seq, C.byref(self._h)))
+
+    def close(self):
+        if self._h:
+            _LIB.fg_pool_destroy(self._h)
+            self._h = _vp()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def len(self, seq: int) -> int:
+        v = C.c_int32()
+        _check(_LIB.fg_pool_len(self._h, seq, C.byref(v)))
+        return v.value
+
+    @property
+    def free(self) -> int:
+        v = C.c_int32()
+        _check(_LIB.fg_pool_free(self._h, C.byref(v)))
+        return v.value
+
+    def table(self, seq: int) -> np.ndarray:
+        """The sequence's pages in order; -1 where slide gave one back."""
+        n = C.c_int32()
+        _check(_LIB.fg_pool_table(self._h, seq, None, 0, C.byref(n)))
+        out = np.empty(n.value, np.int32)
+        _check(_LIB.fg_pool_table(self._h, seq, _ip(out), n.value, C.byref(n)))
+        return out
+
+    def need(self, seq: int, n: int) -> int:
+        v = C.c_int32()
+        _check(_LIB.fg_pool_need(self._h, seq, n, C.byref(v)))
+        return v.value
+
+    def extend(self, seq: int, n: int):
+        """Room for n more tokens: None, or the page copy (src, dst) to make first."""
+        a, b = C.c_int32(), C.c_int32()
+        _check(_LIB.fg_pool_extend(self._h, seq, n, C.byref(a), C.byref(b)))
+        return None if a.value < 0 else (a.value, b.value)
+
+    def fork(self, src: int, dst: int, length: int):
+        _check(_LIB.fg_pool_fork(self._h, src, dst, length))
+
+    def trim(self, seq: int, length: int = 0):
+        _check(_LIB.fg_pool_trim(self._h, seq, length))
+
+    def slide(self, seq: int, window: int, sinks: int = 0):
+        _check(_LIB.fg_pool_slide(self._h, seq, window, sinks))
+
+    def compact(self):
+        """(src, dst) of the page copies to make."""
+        n = C.c_int32()
+        src, dst = np.empty(self.n_pages, np.int32), np.empty(self.n_pages, np.int32)
+        _check(_LIB.fg_pool_compact(self._h, _ip(src), _ip(dst), self.n_pages, C.byref(n)))
+        return src[:n.value], dst[:n.value]
 
 
 def _decode_sample(kv, prompt, n_gen, seed, cfg):

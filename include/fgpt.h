@@ -486,6 +486,69 @@ int32_t fg_draw_rows(const float *logits, int32_t rows, int32_t V, int64_t ld,
                      const fg_draw_cfg *cfg, int32_t *ids, float *probs, void *work,
                      int64_t work_bytes, void *stream);
 
+/* The bookkeeping of a cache's pages, for callers of the operators above (host
+ * only: needs no device, moves no data; calls on one pool must not overlap).
+ * A pool hands the pages 0..n_pages-1 to max_seq sequences, lowest free page
+ * first. Sequences may share pages: a page is free again when its last holder
+ * lets go of it. A call that fails changes nothing. */
+typedef struct fg_pool fg_pool;
+int32_t fg_pool_create(int32_t n_pages, int32_t page_size, int32_t max_seq, fg_pool **out);
+int32_t fg_pool_destroy(fg_pool *pool);
+/* Positions of sequence seq; free pages of the pool. */
+int32_t fg_pool_len(const fg_pool *pool, int32_t seq, int32_t *len);
+int32_t fg_pool_free(const fg_pool *pool, int32_t *n);
+/* The sequence's pages in order (its row of a page table; -1 where
+ * fg_pool_slide gave one back): *n of them, copied to pages unless NULL. */
+int32_t fg_pool_table(const fg_pool *pool, int32_t seq, int32_t *pages, int32_t cap, int32_t *n);
+/* The free pages that n more tokens of the sequence would take. */
+int32_t fg_pool_need(const fg_pool *pool, int32_t seq, int32_t n, int32_t *pages);
+/* Room for n more tokens (FG_EFULL when the pool has not enough). A partly
+ * filled last page that another sequence shares is replaced by one of its own:
+ * *src and *dst then name the copy that the caller makes before it appends
+ * (fg_pages_copy), else they are -1. */
+int32_t fg_pool_extend(fg_pool *pool, int32_t seq, int32_t n, int32_t *src, int32_t *dst);
+/* The empty sequence `to` shares the first len positions of `from`. */
+int32_t fg_pool_fork(fg_pool *pool, int32_t from, int32_t to, int32_t len);
+/* Drops the positions from len on (0: ends the sequence). */
+int32_t fg_pool_trim(fg_pool *pool, int32_t seq, int32_t len);
+/* Gives back the pages that no later token sees under a sliding window and the
+ * first `sinks` positions. Shortening or forking the sequence to where those
+ * pages would be seen again is refused from then on. */
+int32_t fg_pool_slide(fg_pool *pool, int32_t seq, int32_t window, int32_t sinks);
+/* Moves pages so that those in use are the lowest: *n copies src -> dst (no page
+ * is in both) that the caller makes before anything reads the new tables.
+ * FG_EARG, with *n set and nothing moved, when cap is smaller. */
+int32_t fg_pool_compact(fg_pool *pool, int32_t *src, int32_t *dst, int32_t cap, int32_t *n);
+
+/* A model's paged KV cache: up to max_seq sequences of their own lengths in
+ * n_pages pages of page_size positions for every layer, fp32 or (FG_KV_BF16)
+ * bf16. window > 0: each token sees the last `window` positions and the first
+ * `sinks`, and pages behind both are given back after each step. The model must
+ * outlive it; its calls count as the model's (FG_EBUSY). */
+typedef struct fg_paged fg_paged;
+int32_t fg_paged_create(fg_model *m, int32_t n_pages, int32_t page_size, int32_t max_seq,
+                        int32_t flags, int32_t window, int32_t sinks, fg_paged **out);
+int32_t fg_paged_destroy(fg_paged *pc);
+int32_t fg_paged_len(const fg_paged *pc, int32_t seq, int32_t *len);
+int32_t fg_paged_free(const fg_paged *pc, int32_t *n_pages);
+/* fg_pool_fork and fg_pool_trim on the cache's sequences. */
+int32_t fg_paged_fork(fg_paged *pc, int32_t from, int32_t to, int32_t len);
+int32_t fg_paged_trim(fg_paged *pc, int32_t seq, int32_t len);
+/* fg_pool_compact with its copies; *moved (nullable): pages moved. */
+int32_t fg_paged_compact(fg_paged *pc, int32_t *moved);
+/* Keys and values of a sequence, fp32 [n_layer][len][n_kv_head * head_dim]
+ * (each nullable); zeros where a page was given back. */
+int32_t fg_paged_read(fg_paged *pc, int32_t seq, float *k_out, float *v_out);
+/* One pass over a ragged batch: counts[i] >= 1 new tokens of sequence seqs[i]
+ * (distinct), i < n, their ids one sequence after another. Prompts, prompt
+ * chunks and single tokens may be mixed. logits (n*V, nullable): of each
+ * sequence's last token. next_ids (n, nullable): drawn from those with the
+ * settings of draw (fg_draw_cfg of host arrays [n]), or their argmax when draw
+ * is NULL. FG_EFULL, with nothing done, when the pages do not suffice. */
+int32_t fg_paged_step(fg_model *m, fg_paged *pc, int32_t n, const int32_t *seqs,
+                      const int32_t *counts, const int32_t *ids, const fg_draw_cfg *draw,
+                      float *logits, int32_t *next_ids);
+
 #ifdef __cplusplus
 }
 #endif
