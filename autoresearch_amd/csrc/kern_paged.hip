@@ -505,6 +505,353 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
   store_row4<QF>(p, t.row0 + rr / p.G, (kvh * p.G + rr % p.G) * HD + d, a);
 }
 
+// ------------------------------------------------------------ many rows
+// For chunks of new tokens: 128 RB flattened rows a tile, 32 RB to each of four
+// wavefronts, which all go through the same keys, 64 a step (two 32-key tiles of
+// the list). v_mfma_f32_32x32x16_bf16 with S^T = K Q^T and O^T = V^T P^T: lane
+// 32 g + c holds query row c of its wavefront. The key rows of a 32-key tile are
+// taken with bits 2 and 3 of their number swapped, so that a lane's scores 8 s ..
+// 8 s + 7 are keys 16 s + 8 g .., which are its K slots of the second product:
+// probabilities never leave their registers. V^T's operand is read from the
+// row-major value rows by the LDS's transposing reads (ds_read_b64_tr_b16).
+//
+// bf16 pages go memory -> LDS by DMA into two buffers, the next step's rows
+// landing while this one's are used; fp32 ones through registers, cut into
+// three bf16 terms once for the whole workgroup, into one buffer.
+// An operand read from LDS (1 KB) feeds one MFMA of 32 clocks for each query
+// block and term product: at one of both the LDS, 128 bytes a clock, would be
+// busy all the time, hence RB = 2 where operands have one term.
+constexpr int SK = 64;
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+
+template <int HD, bool QF, bool KF>
+struct Many {
+  static constexpr int RB = QF ? 1 : 2;  // query blocks of 32 rows a wavefront
+  static constexpr int RT = 128 * RB;    // rows of a tile
+  static constexpr int NA = KF ? 3 : 1, NB = QF ? 3 : 1;
+  static constexpr int ROW = 2 * HD;           // bytes of a K or V row in LDS
+  static constexpr int PLANE = SK * ROW;
+  static constexpr int STAGE = 2 * NA * PLANE;  // K planes, V planes
+  static constexpr int NST = KF ? 1 : 2;
+  static constexpr int LDS = NST * STAGE;
+};
+
+// key held by operand row i of a 32-key tile (bits 2 and 3 swapped)
+__device__ __forceinline__ int tile_key(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
+// 16-byte slot of chunk c of row r: 16 rows read at one chunk lie in different
+// banks (K), four rows read over 64 bytes too (V, the transposing reads)
+template <int HD>
+__device__ __forceinline__ int kslot(int r, int c) { return HD == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7); }
+template <int HD>
+__device__ __forceinline__ int vslot(int r, int c) {
+  return HD == 128 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2);
+}
+
+__device__ __forceinline__ float swap_max(float v) {
+  const uint32_t u = bits(v);
+  const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+}
+__device__ __forceinline__ float swap_sum(float v) {
+  const uint32_t u = bits(v);
+  const auto w = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float(w[0]) + __uint_as_float(w[1]);
+}
+
+template <int NA, int NB>
+__device__ __forceinline__ f32x16_t mma32(const bf16x8_t (&a)[NA], const bf16x8_t (&b)[NB], f32x16_t c) {
+#pragma unroll
+  for (int o = 2; o >= 0; --o)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (o - i >= 0 && o - i < NB) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[o - i], c, 0, 0, 0);
+  return c;
+}
+
+template <int HD, bool QF, bool KF>
+__global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
+  typedef Many<HD, QF, KF> C;
+  constexpr int RB = C::RB, NS = HD / 16, ND = HD / 32, NA = C::NA, ROW = C::ROW, PLANE = C::PLANE;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % p.KH, rest = blockIdx.x / p.KH;
+  const int id = p.ntile - 1 - rest % p.ntile, z = rest / p.ntile;  // longest tiles first
+  RowTile t;
+  if (!find_tile<C::RT>(p, id, t)) return;
+  const KeyTiles kt = key_tiles(t);
+  const int v0 = z * p.cpt, v1 = min(kt.n, v0 + p.cpt);
+  if (z > 0 && v0 >= kt.n) return;
+  const int nstep = (v1 - v0 + 1) / 2;
+
+  bool bad = false;
+  const int P = 1 << p.pshift;
+  const int32_t* tab = p.table + (int64_t)t.seq * p.table_ld;
+  auto base_of = [&](int v) { return v < kt.na ? 32 * v : kt.from + 32 * (v - kt.na); };
+  // the 16-key blocks of a step as in k_paged_few: where a block's rows lie,
+  // its first key, the row read in the place of an unseen one
+  struct Block {
+    int64_t off;
+    int e, sub;
+  };
+  auto block_of = [&](int st, int b4) {
+    const int v = min(v0 + 2 * st + (b4 >> 1), v1 - 1), kb = b4 & 1;
+    Block k;
+    k.e = base_of(v) + 16 * kb;
+    if (k.e >= t.sa && (k.e >= t.hi || k.e + 16 <= t.lo)) k.e += 16 - 32 * kb;
+    const int pg = tab[k.e >> p.pshift];
+    const bool ok = (uint32_t)pg < (uint32_t)p.n_pages;
+    bad |= !ok;
+    k.off = (((int64_t)(ok ? pg : 0) * p.KH + kvh) * P + (k.e & (P - 1))) * HD;
+    k.sub = k.e < t.sa ? 0 : max(0, t.lo - k.e);
+    return k;
+  };
+  auto row_of = [&](const Block& k, int x) {
+    const int j = k.e + x;
+    return j < t.sa || (j >= t.lo && j < t.hi) ? x : k.sub;
+  };
+
+  // ---- staging
+  // bf16: rows of one 1 KB DMA group (RPG of them) lie in one block; this
+  // wavefront fills groups wv, wv + 4, ..
+  constexpr int RPG = 1024 / ROW, GPP = PLANE / 1024;  // rows a group, groups a plane
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_off(lds));
+  auto fill = [&](int st, int buf) {
+#pragma unroll
+    for (int q = 0; q < GPP / 4; ++q) {
+      const int grp = wv + 4 * q, r = grp * RPG + lane / (ROW / 16), slot = lane % (ROW / 16);
+      const Block b = block_of(st, grp * RPG / 16);
+      const int64_t at = b.off + row_of(b, r & 15) * HD;
+      const uint32_t to = lds0 + buf * C::STAGE + grp * 1024;
+      dma16((const uint16_t*)p.k + at + kslot<HD>(r, slot) * 8, to);
+      dma16((const uint16_t*)p.v + at + vslot<HD>(r, slot) * 8, to + PLANE);
+    }
+  };
+  // fp32: this thread's 8-value chunks of both planes' rows, loaded a step ahead
+  constexpr int CH = HD / 8, RPT = 256 / CH, NT = SK / RPT;  // chunks a row, rows at once, rounds
+  float4 raw[KF ? NT : 1][4];
+  auto fetch = [&](int st) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int r = i * RPT + tid / CH;
+      const int b4 = __builtin_amdgcn_readfirstlane(r / 16);  // (a wavefront's rows lie in one block)
+      const Block b = block_of(st, b4);
+      const int64_t at = b.off + row_of(b, r & 15) * HD + (tid % CH) * 8;
+      const float* kp = (const float*)p.k + at;
+      const float* vp = (const float*)p.v + at;
+      raw[i][0] = *(const float4*)kp;
+      raw[i][1] = *(const float4*)(kp + 4);
+      raw[i][2] = *(const float4*)vp;
+      raw[i][3] = *(const float4*)(vp + 4);
+    }
+  };
+  auto put = [&] {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int r = i * RPT + tid / CH;
+#pragma unroll
+      for (int kvi = 0; kvi < 2; ++kvi) {
+        const float4 a = raw[i][2 * kvi], b = raw[i][2 * kvi + 1];
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        bf16x8_t w[3];
+        split3(x, w);
+        const int slot = kvi ? vslot<HD>(r, tid % CH) : kslot<HD>(r, tid % CH);
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          *(bf16x8_t*)(lds + (3 * kvi + k) * PLANE + r * ROW + slot * 16) = w[k];
+      }
+    }
+  };
+
+  // ---- this lane's query rows
+  const int w0 = 32 * RB * wv;  // the wavefront's first row of the tile
+  const bool active = w0 < t.rows;
+  int klim[RB], klo[RB];
+  Terms<QF> q[RB][NS];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int fr = t.r0 + min(w0 + 32 * b + c, t.rows - 1), tok = fr / p.G, h = kvh * p.G + fr % p.G;
+    klim[b] = t.pos0 + tok + 1;
+    klo[b] = p.window > 0 ? klim[b] - p.window : 0;
+    const int64_t at = (int64_t)(t.row0 + tok) * p.q_ld + h * HD + 8 * g;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if constexpr (QF) {
+        const float* qp = (const float*)p.q + at + 16 * s;
+        const float4 x0 = *(const float4*)qp, x1 = *(const float4*)(qp + 4);
+        const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+        q[b][s].set(x);
+      } else {
+        q[b][s].t[0] = __builtin_bit_cast(bf16x8_t, *(const u32x4v_t*)((const uint16_t*)p.q + at + 16 * s));
+      }
+    }
+  }
+  // positions of the wavefront's first and last row: which tiles need no mask
+  const int wlast = t.r0 + min(w0 + 32 * RB, t.rows) - 1;
+  const int wp0 = t.pos0 + (t.r0 + min(w0, t.rows - 1)) / p.G, wp1 = t.pos0 + wlast / p.G;
+
+  f32x16_t o[RB][ND];
+  float m_run[RB], l_run[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    m_run[b] = -FLT_MAX;
+    l_run[b] = 0.f;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[b][i][r] = 0.f;
+  }
+
+  if (nstep > 0) {
+    if constexpr (KF) fetch(0);
+    else fill(0, 0);
+  }
+  for (int st = 0; st < nstep; ++st) {
+    if constexpr (KF) {
+      if (st > 0) __syncthreads();  // (every wavefront is done with the last step)
+      put();
+      __syncthreads();
+      if (st + 1 < nstep) fetch(st + 1);
+    } else {
+      stage_sync<0>();  // this step has landed, and nobody reads the other buffer
+      if (st + 1 < nstep) fill(st + 1, (st + 1) & 1);
+    }
+    if (!active) continue;
+    const uint8_t* S = lds + (KF ? 0 : (st & 1) * C::STAGE);
+    const int b0 = base_of(v0 + 2 * st);
+    const bool two = v0 + 2 * st + 1 < v1;
+    const int b1 = two ? base_of(v0 + 2 * st + 1) : 0x3fffffff;  // (no such keys: all masked)
+    if (b0 > wp1 && b1 > wp1) continue;  // (behind the wavefront's rows)
+
+    f32x16_t sc[RB][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[b][kb][r] = 0.f;
+      const int row = 32 * kb + tile_key(c);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int at = row * ROW + kslot<HD>(row, 2 * s + g) * 16;
+        bf16x8_t a[NA];
+#pragma unroll
+        for (int k = 0; k < NA; ++k) a[k] = *(const bf16x8_t*)(S + k * PLANE + at);
+#pragma unroll
+        for (int b = 0; b < RB; ++b) sc[b][kb] = mma32(a, q[b][s].t, sc[b][kb]);
+      }
+    }
+    // masks, where some row does not see the whole of a tile
+    const int far = max(b0, b1) + 31;
+    const bool masked = far > wp0 || (p.window > 0 && min(b0, b1) <= wp1 - p.window);
+    if (masked) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int j = (kb ? b1 : b0) + 16 * (r >> 3) + 8 * g + (r & 7);
+            const bool seen = j < klim[b] && (j >= klo[b] || j < p.sinks);
+            sc[b][kb][r] = seen ? sc[b][kb][r] : -INFINITY;
+          }
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[b][kb][r]);
+      mx = swap_max(mx) * p.cs;
+      if (__any(mx > m_run[b] + 8.f)) {  // (as in k_paged_few)
+        const float m_new = fmaxf(m_run[b], mx);
+        const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_new);
+        l_run[b] *= alpha;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[b][i][r] *= alpha;
+        m_run[b] = m_new;
+      }
+      float ps = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][kb][r], p.cs, -m_run[b]));
+          sc[b][kb][r] = e;
+          ps += e;
+        }
+      l_run[b] += ps;
+    }
+    // O^T += V^T P^T, 16 keys at a time
+    const uint32_t vb = lds_off(S) + NA * PLANE;
+#pragma unroll
+    for (int s4 = 0; s4 < 4; ++s4) {
+      Terms<QF> pt[RB];
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = sc[b][s4 >> 1][8 * (s4 & 1) + e];
+        pt[b].set(x);
+      }
+      // rows 16 s4 + 8 g + lane % 16 / 4 (+ 4), dims 32 i + 16 (lane / 16 % 2) + 4 (lane % 4)
+      const int row = 16 * s4 + 8 * g + ((lane >> 2) & 3);
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const int ch = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+        bf16x8_t a[NA];
+#pragma unroll
+        for (int k = 0; k < NA; ++k) {
+          s16x4_t h[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const uint32_t at = vb + k * PLANE + (row + 4 * u) * ROW + vslot<HD>(row + 4 * u, ch) * 16 +
+                                8 * (lane & 1);
+            h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4_t*)(uintptr_t)at);
+          }
+          a[k] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+#pragma unroll
+        for (int b = 0; b < RB; ++b) o[b][i] = mma32(a, pt[b].t, o[b][i]);
+      }
+    }
+  }
+  if (!active) return;
+
+  bad = __any(bad);
+  const bool whole = kt.n <= p.cpt;
+  float* P0 = p.part + ((int64_t)(id * p.KH + kvh) * p.nsplit + z) * part_floats<HD>(C::RT);
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int r = w0 + 32 * b + c;
+    float l = swap_sum(l_run[b]);
+    if (bad) l = NAN;
+    if (r >= t.rows) continue;
+    const float f = whole ? inv_sum(l) : 1.f;
+    const int rr = t.r0 + r;
+    const int64_t row = t.row0 + rr / p.G;
+    const int col = (kvh * p.G + rr % p.G) * HD;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = o[b][i][4 * r4 + e] * f;
+        const int d = 32 * i + 8 * r4 + 4 * g;
+        if (whole) store_row4<QF>(p, row, col + d, v);
+        else *(float4*)(P0 + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    if (!whole && g == 0) *(float2*)(P0 + C::RT * HD + 2 * r) = make_float2(m_run[b], l);
+  }
+}
+
 // ------------------------------------------------------------ host side
 
 // (a constant, not the current device's: a workspace asked for with one device
@@ -512,6 +859,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
 constexpr int64_t CUS = 256;
 
 struct Plan {
+  bool many;
   int rt;      // rows of a tile
   int ntile, nsplit, cpt;
   int64_t floats;
@@ -521,8 +869,9 @@ struct Plan {
 // alone (lengths may differ under a captured launch).
 Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
   Plan pl;
-  pl.rt = DR;
   const int64_t G = c.n_head / pg.n_kv_head;
+  pl.many = b.max_q * G > 32;
+  pl.rt = !pl.many ? DR : c.type == FG_F32 ? Many<128, true, true>::RT : Many<128, false, false>::RT;
   const int64_t per_seq = (b.max_q * G + pl.rt - 1) / pl.rt;
   pl.ntile = (int)std::min<int64_t>(per_seq * b.n_seq, b.n_rows * G / pl.rt + b.n_seq);
   int64_t keys = b.max_kv;
@@ -553,14 +902,29 @@ void launch_few(hipStream_t s, const PagedArgs& a) {
               dim3(256), 0, s, a);
 }
 
+template <int HD, bool QF, bool KF>
+void launch_many(hipStream_t s, const PagedArgs& a) {
+  typedef Many<HD, QF, KF> C;
+  static std::atomic<uint64_t> lds_set{0};
+  raise_lds_once((const void*)k_paged_many<HD, QF, KF>, C::LDS, &lds_set);
+  FG_LAUNCH((k_paged_many<HD, QF, KF>), dim3((unsigned)(a.ntile * a.KH * a.nsplit)), dim3(256), C::LDS,
+            s, a);
+  if (a.nsplit > 1)
+    FG_LAUNCH((k_paged_merge<HD, QF, C::RT>), dim3((unsigned)(a.ntile * a.KH * (C::RT * HD / 1024))),
+              dim3(256), 0, s, a);
+}
+
+template <int HD, bool QF, bool KF>
+void launch_t(hipStream_t s, const PagedArgs& a, bool many) {
+  if (many) launch_many<HD, QF, KF>(s, a);
+  else launch_few<HD, QF, KF>(s, a);
+}
+
 template <int HD>
-void launch_hd(hipStream_t s, const PagedArgs& a, bool qf, bool kf) {
-  if (kf)
-    launch_few<HD, true, true>(s, a);
-  else if (qf)
-    launch_few<HD, true, false>(s, a);
-  else
-    launch_few<HD, false, false>(s, a);
+void launch_hd(hipStream_t s, const PagedArgs& a, bool many, bool qf, bool kf) {
+  if (kf) launch_t<HD, true, true>(s, a, many);
+  else if (qf) launch_t<HD, true, false>(s, a, many);
+  else launch_t<HD, false, false>(s, a, many);
 }
 
 }  // namespace
@@ -599,9 +963,9 @@ void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, co
   a.cpt = pl.cpt;
   a.part = work;
   if (pg.head_dim == 128)
-    launch_hd<128>(s, a, c.type == FG_F32, pg.type == FG_F32);
+    launch_hd<128>(s, a, pl.many, c.type == FG_F32, pg.type == FG_F32);
   else
-    launch_hd<64>(s, a, c.type == FG_F32, pg.type == FG_F32);
+    launch_hd<64>(s, a, pl.many, c.type == FG_F32, pg.type == FG_F32);
 }
 
 }  // namespace fgpt
