@@ -1,19 +1,24 @@
 // kern_draw.hip -- one id a row under temperature, top-k, top-p and min-p from
 // given uniform numbers (fg_draw_rows of include/fgpt.h).
 //
-// No sort: each of the three filters keeps a prefix of the row in descending
-// order (ties by ascending id), so all of them together are one threshold: the
-// ids whose key is above K, and the first `ties` ids of key K. K is found by
-// histograms over the digits of the key (11, 11 and 10 bits): one pass over the
-// row for the first digit of all ids, one each for the digits below within the
-// bin where top_k's count or top_p's mass is reached. A last pass sums the kept
-// mass by chunks of 64 ids, in id order, and the draw scans those.
+// No sort: each of the three filters keeps a prefix of the row in its order
+// (descending logits, ties by ascending id), so top-k and top-p are a cut, the
+// last id kept, and min-p is a bound on the masses. Where the cut lies is found
+// from one histogram of counts and masses over bins of equal width in
+// (max - x) / temp: the bin in which top_k's count or top_p's mass is reached,
+// then the place within it by comparing its few ids with each other (a bin of
+// more than LIST ids, as rows of many equal logits have, goes by digits
+// instead). The kept mass is then summed by chunks of 64 ids, in id order, and
+// the draw scans those.
 //
 // Masses are integers, e_i = exp((x_i - max) / temp) in steps of 2^-44 (sums of
 // up to 2^18 of them fit 64 bits), so every sum is exact in any order: atomics
 // may add them as they come, and an id next to a border of the cumulative mass
 // comes out the same in every run. 32-bit sums would misplace about n 2^-24 of
 // the draws of a row with n likely ids.
+//
+// A workgroup a row. Up to 8192 ids the row stays in registers and the time is
+// that of the chain of block-wide steps; past that it is the exponentials'.
 #include "fgpt_internal.h"
 #include "kern_common.h"
 #include "paged_internal.h"
@@ -23,9 +28,14 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int DT = 1024, DW = DT / 64;   // threads, wavefronts
-constexpr int BINS = 2048;               // of the widest digit
+constexpr int DT = 1024, DW = DT / 64;  // threads, wavefronts
+constexpr int PER = 8;                  // ids a thread holds in registers
+constexpr int BINS = 2 * DT;
+constexpr float BIN_UNITS = 64.f;       // bins per unit of (max - x) / temp: 32 units in all
+constexpr int LIST = 512;               // ids of one bin that are compared with each other
+constexpr int TAB = 1024;
 constexpr int MAX_CHUNKS = DRAW_MAX_V / 64;
+constexpr int ID_BITS = 18;             // DRAW_MAX_V ids
 
 struct DrawArgs {
   const float* x;
@@ -42,195 +52,241 @@ __device__ __forceinline__ uint32_t key_of(float x) {
   return u ^ ((u >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-// e^y in steps of 2^-44 for y <= 0: y = (n ln 2)/32 + r, |r| <= ln2 / 64, as
-// 2^(n/32) (tab[j] = 2^(j/32)) times r's Taylor sum to degree 5 (the next term
-// is below 2.3e-15). The addition of 2^52 rounds to an integer.
-__device__ __forceinline__ u64 mass_of(double y, const double* tab) {
-  if (!(y > -31.0)) return 0;  // (below half a step)
-  const double n = rint(y * 46.166241308446828384);  // 32 / ln 2
-  const double r = fma(-n, 0.021660849392498290, y);  // ln 2 / 32
-  double s = fma(r, 1.0 / 120, 1.0 / 24);
-  s = fma(r, s, 1.0 / 6);
-  s = fma(r, s, 0.5);
-  s = fma(r, s, 1.0);
-  s = fma(r, s, 1.0);
-  const int k = (int)n;
-  const double e = ldexp(s * tab[k & 31], 44 + (k >> 5));
-  return (u64)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+// v of the lane that DPP control CTRL names, 0 where that is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_or_0(u64 v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xF, false);
+  return ((u64)hi << 32) | lo;
 }
+// Inclusive sums by lane: within rows of 16 lanes by row shifts, then the last
+// lane of a row to the next row, of the first half to the second.
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+  v += dpp_or_0<0x111, 0xF>(v);
+  v += dpp_or_0<0x112, 0xF>(v);
+  v += dpp_or_0<0x114, 0xF>(v);
+  v += dpp_or_0<0x118, 0xF>(v);
+  v += dpp_or_0<0x142, 0xA>(v);  // row_bcast15 into rows 1 and 3
+  v += dpp_or_0<0x143, 0xC>(v);  // row_bcast31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ u64 lane_value(u64 v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return ((u64)hi << 32) | lo;
+}
+
+// The place of an id in the row's order: ascending (max key - key, id).
+typedef u64 place_t;
+
+struct Shared {
+  unsigned int cnt[BINS];
+  u64 mass[BINS];
+  double tab[TAB];  // 2^(j / TAB)
+  place_t list_at[LIST];
+  u64 list_mass[LIST];
+  u64 red[2][DW];
+  float redf[DW];
+  int redi[DW];
+  u64 found[4];
+  int n_list;
+};
 
 struct Row {  // what a row's threads share
   const float* x;
   int V;
-  float m;       // largest logit (may be +inf)
-  uint32_t km;   // its key
-  double inv_t;
+  float m;      // largest logit (may be +inf)
+  uint32_t km;  // its key
+  double unit;  // TAB / (ln 2 temp)
+  float bin;    // BIN_UNITS / temp
   const double* tab;
-  __device__ __forceinline__ bool drawable(float v) const { return v > -INFINITY; }  // (no NaN)
-  __device__ __forceinline__ uint32_t down(float v) const { return km - key_of(v); }  // 0 at the top
+  // exp((v - m) / temp) in steps of 2^-44: with y = (v - m) unit = n + f, |f| <=
+  // 1/2, 2^(n / TAB) from the table times 2^(f / TAB), f's Taylor sum to degree 3
+  // (the next term is below 6e-16). The addition of 2^52 rounds to an integer.
   __device__ __forceinline__ u64 mass(float v) const {
     if (v == m) return 1ull << 44;
-    return mass_of(((double)v - (double)m) * inv_t, tab);
+    const double y = ((double)v - (double)m) * unit;
+    if (!(y > -45.0 * TAB)) return 0;
+    const double n = rint(y), f = y - n;
+    constexpr double L = 0.69314718055994530942 / TAB;
+    double s = fma(f, L * L * L / 6, L * L / 2);
+    s = fma(f, s, L);
+    s = fma(f, s, 1.0);
+    const int k = (int)n;
+    const double e = ldexp(s * tab[k & (TAB - 1)], 44 + (k >> 10));
+    return (u64)__double_as_longlong(e + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+  }
+  __device__ __forceinline__ int bin_of(float v) const {  // does not fall as v falls
+    const float b = (m - v) * bin;
+    return v == m ? 0 : b < (float)(BINS - 1) ? (int)b : BINS - 1;  // (NaN: the last)
+  }
+  __device__ __forceinline__ place_t place(float v, int i) const {
+    return ((place_t)(km - key_of(v)) << ID_BITS) | (uint32_t)i;
   }
 };
 
-__device__ __forceinline__ u64 wave_scan(u64 v) {  // inclusive, by lane
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ bool drawable(float v) { return v > -INFINITY; }  // (false for NaN)
+
+// f(v, i) for this thread's ids; HELD: from registers.
+template <bool HELD, class F>
+__device__ __forceinline__ void each(const Row& row, const float (&held)[PER], F&& f) {
+  if constexpr (HELD) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 u = __shfl_up(v, o, 64);
-    if (lane >= o) v += u;
-  }
-  return v;
-}
-
-// Sum of the values of the threads before this one, and of all; red: [DW].
-__device__ u64 block_scan(u64 v, u64* red, u64* total) {
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const u64 in = wave_scan(v);
-  __syncthreads();
-  if (lane == 63) red[wv] = in;
-  __syncthreads();
-  u64 before = 0, all = 0;
-  for (int k = 0; k < DW; ++k) {
-    const u64 r = red[k];
-    before += k < wv ? r : 0;
-    all += r;
-  }
-  *total = all;
-  return before + in - v;
-}
-
-struct Hist {
-  unsigned int cnt[BINS];
-  u64 mass[BINS];
-};
-
-// Histogram of the digit (down >> shift) & mask over the ids whose digits above
-// it are `prefix` (counts, and masses if wanted).
-__device__ void fill(const Row& row, Hist& h, uint32_t prefix, int shift, int width, bool masses) {
-  for (int i = threadIdx.x; i < BINS; i += DT) {
-    h.cnt[i] = 0;
-    h.mass[i] = 0;
-  }
-  __syncthreads();
-  const uint32_t mask = (1u << width) - 1;
-  for (int i = threadIdx.x; i < row.V; i += DT) {
-    const float v = row.x[i];
-    if (!row.drawable(v)) continue;
-    const uint32_t d = row.down(v);
-    if ((u64)d >> (shift + width) != prefix) continue;
-    const uint32_t b = (d >> shift) & mask;
-    atomicAdd(&h.cnt[b], 1u);
-    if (masses) atomicAdd(&h.mass[b], row.mass(v));
-  }
-  __syncthreads();
-}
-
-// The first bin (from the top of the order) with which the counts (or masses)
-// before it and its own reach `want` - that is before < want <= before + own;
-// *before gets what lies above it. -1: all together stay below.
-__device__ int find(const Hist& h, bool masses, u64 want, u64* before, u64* shared, u64* total) {
-  const int i = 2 * threadIdx.x;
-  const u64 a = masses ? h.mass[i] : h.cnt[i], b = masses ? h.mass[i + 1] : h.cnt[i + 1];
-  u64 all;
-  const u64 pre = block_scan(a + b, shared, &all);
-  *total = all;
-  if (threadIdx.x == 0) shared[DW] = (u64)-1;
-  __syncthreads();
-  if (pre < want && want <= pre + a) {
-    shared[DW] = i;
-    shared[DW + 1] = pre;
-  } else if (pre + a < want && want <= pre + a + b) {
-    shared[DW] = i + 1;
-    shared[DW + 1] = pre + a;
-  }
-  __syncthreads();
-  const int bin = (int)shared[DW];
-  *before = shared[DW + 1];
-  __syncthreads();
-  return bin;
-}
-
-struct Cut {      // the kept ids: down < d, and the first `ties` ids of down == d
-  uint32_t d;
-  uint32_t ties;
-};
-
-// The cut at which the counts (masses) of the order reach `want` >= 1, given
-// the histogram of the first digit; false where all of it stays below.
-// before_mass (of counts): the mass above the cut, if asked for.
-__device__ bool cut_at(const Row& row, Hist& h, bool masses, u64 want, Cut* cut, u64* shared) {
-  u64 before, total, above = 0;
-  int b = find(h, masses, want, &before, shared, &total);
-  if (b < 0) return false;
-  uint32_t prefix = b;
-  above = before;
-#pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    const int shift = k == 0 ? 10 : 0, width = k == 0 ? 11 : 10;
-    fill(row, h, prefix, shift, width, masses);
-    b = find(h, masses, want - above, &before, shared, &total);
-    above += before;
-    prefix = (prefix << width) | (uint32_t)b;
-  }
-  cut->d = prefix;
-  const u64 left = want - above;  // of the last digit's bin, all of one key
-  if (masses) {
-    const u64 each = h.mass[b] / h.cnt[b];
-    cut->ties = (uint32_t)((left + each - 1) / each);
+    for (int k = 0; k < PER; ++k) {
+      const int i = k * DT + (int)threadIdx.x;
+      if (i < row.V) f(held[k], i);
+    }
   } else {
-    cut->ties = (uint32_t)left;
+    for (int i0 = threadIdx.x; i0 < row.V; i0 += PER * DT) {
+      float v[PER];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) v[k] = i0 + k * DT < row.V ? row.x[i0 + k * DT] : -INFINITY;
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (i0 + k * DT < row.V) f(v[k], i0 + k * DT);
+    }
   }
-  return true;
 }
 
+// Sums of the threads' a and b before this one, and of all threads.
+__device__ void block_scan2(Shared& s, u64& a, u64& b, u64& all_a, u64& all_b) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const u64 ia = wave_scan(a), ib = wave_scan(b);
+  if (lane == 63) {
+    s.red[0][wv] = ia;
+    s.red[1][wv] = ib;
+  }
+  __syncthreads();
+  const u64 wa = wave_scan(lane < DW ? s.red[0][lane] : 0), wb = wave_scan(lane < DW ? s.red[1][lane] : 0);
+  a = ia - a + (wv ? lane_value(wa, wv - 1) : 0);
+  b = ib - b + (wv ? lane_value(wb, wv - 1) : 0);
+  all_a = lane_value(wa, 63);
+  all_b = lane_value(wb, 63);
+}
+
+// Where, in the row's order, the counts (or masses) first reach `want` >= 1:
+// the place of that id, within the bin `b` before which `before` lies. mass_to
+// gets the bin's mass up to and with it.
+template <bool HELD>
+__device__ place_t place_at(Shared& s, const Row& row, const float (&held)[PER], bool masses, u64 want,
+                            int b, u64 before, u64* mass_to) {
+  const int tid = threadIdx.x;
+  const u64 left = want - before;
+  const unsigned n = s.cnt[b];
+  __syncthreads();  // (found and cnt are read)
+  if (n <= LIST) {
+    if (tid == 0) s.n_list = 0;
+    __syncthreads();
+    each<HELD>(row, held, [&](float v, int i) {
+      if (!drawable(v) || row.bin_of(v) != b) return;
+      const int at = atomicAdd(&s.n_list, 1);
+      s.list_at[at] = row.place(v, i);
+      s.list_mass[at] = row.mass(v);
+    });
+    __syncthreads();
+    if (tid < (int)n) {
+      const place_t mine = s.list_at[tid];
+      const u64 w = s.list_mass[tid];
+      u64 rank = 0, mass = 0;
+#pragma unroll 4
+      for (unsigned k = 0; k < n; ++k) {
+        const bool first = s.list_at[k] < mine;
+        rank += first ? 1 : 0;
+        mass += first ? s.list_mass[k] : 0;
+      }
+      if (masses ? mass < left && left <= mass + w : rank == left - 1) {
+        s.found[0] = mine;
+        s.found[1] = mass + w;
+      }
+    }
+    __syncthreads();
+    *mass_to = s.found[1];
+    return s.found[0];
+  }
+  // by the digits of the places: 11, 11 and 10 bits of the key, 9 and 9 of the id
+  constexpr int widths[5] = {11, 11, 10, 9, 9};
+  place_t prefix = 0;
+  u64 above_c = 0, above_m = 0;
+  int shift = 32 + ID_BITS;
+#pragma unroll 1
+  for (int k = 0; k < 5; ++k) {
+    const int width = widths[k];
+    shift -= width;
+    s.cnt[2 * tid] = s.cnt[2 * tid + 1] = 0;
+    s.mass[2 * tid] = s.mass[2 * tid + 1] = 0;
+    __syncthreads();
+    each<HELD>(row, held, [&](float v, int i) {
+      if (!drawable(v) || row.bin_of(v) != b) return;
+      const place_t p = row.place(v, i);
+      if (k > 0 && (p >> (shift + width)) != prefix) return;
+      const int d = (int)((p >> shift) & ((1u << width) - 1));
+      atomicAdd(&s.cnt[d], 1u);
+      atomicAdd(&s.mass[d], row.mass(v));
+    });
+    __syncthreads();
+    const u64 c0 = s.cnt[2 * tid], m0 = s.mass[2 * tid];
+    u64 pc = c0 + s.cnt[2 * tid + 1], pm = m0 + s.mass[2 * tid + 1], tc, tm;
+    const u64 c1 = pc - c0, m1 = pm - m0;
+    block_scan2(s, pc, pm, tc, tm);
+    const u64 at0 = masses ? above_m + pm : above_c + pc, w0 = masses ? m0 : c0, w1 = masses ? m1 : c1;
+    const bool h0 = at0 < left && left <= at0 + w0, h1 = at0 + w0 < left && left <= at0 + w0 + w1;
+    if (h0 || h1) {
+      s.found[0] = 2 * tid + (h1 ? 1 : 0);
+      s.found[1] = above_m + pm + (h1 ? m0 : 0);
+      s.found[2] = above_c + pc + (h1 ? c0 : 0);
+      s.found[3] = h1 ? m1 : m0;
+    }
+    __syncthreads();
+    prefix = (prefix << width) | s.found[0];
+    above_m = s.found[1];
+    above_c = s.found[2];
+  }
+  *mass_to = above_m + s.found[3];
+  return prefix;
+}
+
+template <bool HELD>
 __global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
-  __shared__ Hist h;
-  __shared__ u64 shared[DW + 2];
-  __shared__ double tab[32];
-  __shared__ float redf[DW];
-  __shared__ int redi[DW];
-  extern __shared__ __attribute__((aligned(16))) u64 chunk_mass[];  // [chunks], then their ties
+  __shared__ Shared s;
+  extern __shared__ __attribute__((aligned(16))) u64 chunk_mass[];  // [chunks]
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, r = blockIdx.x;
   const int chunks = (a.V + 63) / 64;
-  unsigned int* chunk_ties = (unsigned int*)(chunk_mass + chunks);
-  if (tid < 32) tab[tid] = exp2(tid / 32.0);
   Row row;
   row.x = a.x + (int64_t)r * a.ld;
   row.V = a.V;
-  row.tab = tab;
+  row.tab = s.tab;
+  float held[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) held[k] = HELD && k * DT + tid < a.V ? row.x[k * DT + tid] : -INFINITY;
+  s.tab[tid] = exp2(tid / (double)TAB);
+  s.cnt[2 * tid] = s.cnt[2 * tid + 1] = 0;
+  s.mass[2 * tid] = s.mass[2 * tid + 1] = 0;
 
   // the largest logit and its first id
   float m = -INFINITY;
   int at = 0x7fffffff;
-  for (int i = tid; i < a.V; i += DT) {
-    const float v = row.x[i];
+  each<HELD>(row, held, [&](float v, int i) {
     if (v > m) {
       m = v;
       at = i;
     }
-  }
+  });
+  const float wm = wave_max(m);
+  at = m == wm ? at : 0x7fffffff;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor(m, o, 64);
-    const int a2 = __shfl_xor(at, o, 64);
-    if (m2 > m || (m2 == m && a2 < at)) {
-      m = m2;
-      at = a2;
-    }
-  }
+  for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
   if (lane == 0) {
-    redf[wv] = m;
-    redi[wv] = at;
+    s.redf[wv] = wm;
+    s.redi[wv] = at;
   }
   __syncthreads();
-  m = redf[0];
-  at = redi[0];
+  m = s.redf[0];
+  at = s.redi[0];
+#pragma unroll
   for (int k = 1; k < DW; ++k)
-    if (redf[k] > m || (redf[k] == m && redi[k] < at)) {
-      m = redf[k];
-      at = redi[k];
+    if (s.redf[k] > m || (s.redf[k] == m && s.redi[k] < at)) {
+      m = s.redf[k];
+      at = s.redi[k];
     }
   const float temp = a.c.temp ? a.c.temp[r] : 1.f;
   if (at == 0x7fffffff || temp <= 0.f) {
@@ -240,125 +296,115 @@ __global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
     }
     return;
   }
+  const float t = temp != temp ? 1.f : temp;
   row.m = m;
   row.km = key_of(m);
-  row.inv_t = temp != temp ? 1.0 : 1.0 / (double)temp;
+  row.unit = TAB * 1.44269504088896340736 / (double)t;
+  row.bin = BIN_UNITS / t;
   const int top_k = a.c.top_k ? a.c.top_k[r] : 0;
   const float top_p = a.c.top_p ? a.c.top_p[r] : 1.f, min_p = a.c.min_p ? a.c.min_p[r] : 0.f;
-
-  Cut cut{0xFFFFFFFFu, 0xFFFFFFFFu};  // everything
   const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
-  if (by_k) {
-    fill(row, h, 0, 21, 11, false);
-    cut_at(row, h, false, (u64)top_k, &cut, shared);
-  }
-  if (by_p) {
-    // the mass that top_k leaves, by id order of the ties as below
-    u64 mass = 0, n = 0, all, ties;
-    for (int i = tid; i < a.V; i += DT) {
-      const float v = row.x[i];
-      if (!row.drawable(v)) continue;
-      const uint32_t d = row.down(v);
-      if (d < cut.d || !by_k) mass += row.mass(v);
-      if (by_k && d == cut.d) ++n;
-    }
-    block_scan(mass, shared, &all);
+
+  place_t cut = ~0ull;  // the last id kept
+  if (by_k || by_p) {
+    each<HELD>(row, held, [&](float v, int) {
+      if (!drawable(v)) return;
+      const int b = row.bin_of(v);
+      atomicAdd(&s.cnt[b], 1u);
+      if (by_p) atomicAdd(&s.mass[b], row.mass(v));
+    });
     __syncthreads();
-    block_scan(n, shared, &ties);
-    __syncthreads();
-    if (by_k) {
-      const u64 t = ties < cut.ties ? ties : cut.ties;
-      // (a key's float: the inverse of key_of)
-      const uint32_t k = row.km - cut.d;
-      all += t * row.mass(__uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k));
+    const u64 c0 = s.cnt[2 * tid], m0 = s.mass[2 * tid];
+    u64 pc = c0 + s.cnt[2 * tid + 1], pm = m0 + s.mass[2 * tid + 1], all_c, all;
+    const u64 c1 = pc - c0, m1 = pm - m0;
+    block_scan2(s, pc, pm, all_c, all);
+    // (place_at by digits uses the bins again: the masses before them stay in pm, m0, m1)
+    auto find = [&](u64 want, u64 before, u64 w0, u64 w1) {
+      if (before < want && want <= before + w0) {
+        s.found[0] = 2 * tid;
+        s.found[1] = before;
+        s.found[2] = pm;
+        s.found[3] = s.cnt[2 * tid];
+      } else if (before + w0 < want && want <= before + w0 + w1) {
+        s.found[0] = 2 * tid + 1;
+        s.found[1] = before + w0;
+        s.found[2] = pm + m0;
+      }
+      __syncthreads();
+    };
+    if (by_k && (u64)top_k < all_c) {
+      find(top_k, pc, c0, c1);
+      const u64 above = s.found[2], before = s.found[1];
+      u64 to;
+      cut = place_at<HELD>(s, row, held, false, top_k, (int)s.found[0], before, &to);
+      all = above + to;  // the mass that top_k leaves
+      __syncthreads();
+      s.cnt[2 * tid] = c0;
+      s.cnt[2 * tid + 1] = c1;
+      __syncthreads();
     }
-    const double want = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)all);
-    fill(row, h, 0, 21, 11, true);
-    Cut c2;
-    if (cut_at(row, h, true, want < 1.0 ? 1ull : (u64)want, &c2, shared) &&
-        (c2.d < cut.d || (c2.d == cut.d && c2.ties < cut.ties)))
-      cut = c2;
+    if (by_p) {
+      const double w = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)all);
+      const u64 want = w < 1.0 ? 1ull : (u64)w;
+      find(want, pm, m0, m1);
+      u64 to;
+      const place_t c2 = place_at<HELD>(s, row, held, true, want, (int)s.found[0], s.found[1], &to);
+      cut = c2 < cut ? c2 : cut;
+    }
   }
-  const u64 floor_mass =
+  const u64 least =
       min_p > 0.f ? (min_p >= 1.f ? 1ull << 44 : (u64)ceil((double)min_p * 17592186044416.0)) : 0;
 
-  // kept mass and ties of each chunk of 64 ids
-  auto kept = [&](float v, uint32_t d, u64* w) {  // above the cut, or one of its ties
-    if (!row.drawable(v) || d > cut.d) return false;
-    *w = row.mass(v);
-    return *w >= floor_mass;
+  // kept mass of each chunk of 64 ids (a wavefront's ids of one k)
+  auto kept = [&](float v, int i) -> u64 {
+    if (!drawable(v) || row.place(v, i) > cut) return 0;
+    const u64 w = row.mass(v);
+    return w >= least ? w : 0;
   };
-  __syncthreads();
-  for (int c = wv; c < chunks; c += DW) {
-    const int i = 64 * c + lane;
-    const float v = i < a.V ? row.x[i] : -INFINITY;
-    u64 w = 0;
-    const uint32_t d = row.drawable(v) ? row.down(v) : 0;
-    const bool k = kept(v, d, &w);
-    const uint64_t tie = __ballot(k && d == cut.d);
-    const u64 s = wave_scan(k && d != cut.d ? w : 0);
-    if (lane == 63) {
-      chunk_mass[c] = s;
-      chunk_ties[c] = __popcll(tie);
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int c = k * DW + wv;
+      if (c >= chunks) break;
+      const u64 sum = wave_scan(kept(held[k], k * DT + tid));
+      if (lane == 63) chunk_mass[c] = sum;
     }
-  }
-  __syncthreads();
-  // the tied ids' own mass, and which of them stay: the first cut.ties
-  u64 tie_mass = 0;
-  {
-    const uint32_t k = row.km - cut.d;
-    if (cut.ties != 0xFFFFFFFFu && cut.d <= row.km)
-      tie_mass = row.mass(__uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k));
-  }
-  const int per = (chunks + DT - 1) / DT, c0 = tid * per;
-  u64 nt = 0, all, total;
-  for (int q = 0; q < per; ++q)
-    if (c0 + q < chunks) nt += chunk_ties[c0 + q];
-  u64 tb = block_scan(nt, shared, &all);
-  __syncthreads();
-  u64 mine = 0;
-  for (int q = 0; q < per; ++q)
-    if (c0 + q < chunks) {
-      const u64 n = chunk_ties[c0 + q];
-      const u64 stay = tb >= cut.ties ? 0 : (n < cut.ties - tb ? n : cut.ties - tb);
-      mine += chunk_mass[c0 + q] + stay * tie_mass;
-      tb += n;
-    }
-  u64 before = block_scan(mine, shared, &total);
-  const float u = a.c.u[r];
-  double want = (double)(u > 0.f ? (u < 1.f ? u : 1.f) : 0.f) * (double)total;
-  u64 target = (u64)want;
-  if (target >= total) target = total - 1;
-  __syncthreads();
-  if (mine > 0 && before <= target && target < before + mine) {  // one thread
-    tb -= nt;
-    for (int q = 0; q < per && c0 + q < chunks; ++q) {
-      const u64 n = chunk_ties[c0 + q];
-      const u64 stay = tb >= cut.ties ? 0 : (n < cut.ties - tb ? n : cut.ties - tb);
-      const u64 w = chunk_mass[c0 + q] + stay * tie_mass;
-      if (target < before + w) {
-        shared[DW] = c0 + q;
-        shared[DW + 1] = target - before;
-        shared[0] = stay;
-        break;
+  } else {
+    for (int c0 = wv; c0 < chunks; c0 += PER * DW) {
+      float v[PER];
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int i = 64 * (c0 + k * DW) + lane;
+        v[k] = i < a.V ? row.x[i] : -INFINITY;
       }
-      before += w;
-      tb += n;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int c = c0 + k * DW;
+        if (c >= chunks) break;
+        const u64 w = kept(v[k], 64 * c + lane);
+        const u64 sum = __any(w != 0) ? wave_scan(w) : 0;
+        if (lane == 63) chunk_mass[c] = sum;
+      }
     }
   }
   __syncthreads();
+  // the first wavefront finds the chunk, then the id
   if (wv != 0) return;
-  const int c = (int)shared[DW], i = 64 * c + lane;
-  const u64 stay = shared[0];
-  const float v = i < a.V ? row.x[i] : -INFINITY;
-  u64 w = 0;
-  const uint32_t d = row.drawable(v) ? row.down(v) : 0;
-  bool k = kept(v, d, &w);
-  const uint64_t tie = __ballot(k && d == cut.d);
-  if (d == cut.d && __popcll(tie & ((1ull << lane) - 1)) >= stay) k = false;
-  const u64 s = wave_scan(k ? w : 0);
-  const uint64_t hit = __ballot(k && s > shared[DW + 1]);
-  if (lane == __builtin_ctzll(hit)) {
+  const int per = (chunks + 63) / 64, q0 = lane * per;
+  u64 mine = 0;
+  for (int q = 0; q < per; ++q) mine += q0 + q < chunks ? chunk_mass[q0 + q] : 0;
+  const u64 upto = wave_scan(mine), total = lane_value(upto, 63);
+  const float u = a.c.u[r];
+  u64 target = (u64)((double)(u > 0.f ? (u < 1.f ? u : 1.f) : 0.f) * (double)total);
+  if (target >= total) target = total - 1;
+  const int l = __builtin_ctzll(__ballot(upto > target));
+  u64 before = lane_value(upto - mine, l);
+  int c = l * per;
+  while (before + chunk_mass[c] <= target) before += chunk_mass[c++];
+  const int i = 64 * c + lane;
+  const u64 w = kept(i < a.V ? row.x[i] : -INFINITY, i);
+  const u64 sum = before + wave_scan(w);
+  if (lane == __builtin_ctzll(__ballot(sum > target))) {
     a.ids[r] = i;
     if (a.probs) a.probs[r] = (float)((double)w / (double)total);
   }
@@ -371,10 +417,14 @@ int64_t draw_work_bytes(int32_t, int32_t) { return 0; }
 void launch_draw_rows(hipStream_t s, const float* logits, int32_t rows, int32_t V, int64_t ld,
                       const fg_draw_cfg& c, int32_t* ids, float* probs, void*) {
   const DrawArgs a{logits, V, ld, c, ids, probs};
-  const unsigned lds = (unsigned)((V + 63) / 64 * 12 + 16);
-  static std::atomic<uint64_t> lds_set{0};
-  raise_lds_once((const void*)k_draw_rows, MAX_CHUNKS * 12 + 16, &lds_set);
-  FG_LAUNCH(k_draw_rows, dim3((unsigned)rows), dim3(DT), lds, s, a);
+  const unsigned lds = (unsigned)((V + 63) / 64 * 8);
+  if (V <= PER * DT) {
+    FG_LAUNCH((k_draw_rows<true>), dim3((unsigned)rows), dim3(DT), lds, s, a);
+  } else {
+    static std::atomic<uint64_t> lds_set{0};
+    raise_lds_once((const void*)k_draw_rows<false>, MAX_CHUNKS * 8, &lds_set);
+    FG_LAUNCH((k_draw_rows<false>), dim3((unsigned)rows), dim3(DT), lds, s, a);
+  }
 }
 
 }  // namespace fgpt
