@@ -92,6 +92,8 @@ int32_t check_pages(const fg_pages* p) {
         "page_size %d is not a power of two in 16..256", p->page_size);
   CHECK(p->n_pages >= 1 && p->n_kv_head >= 1, "pages: n_pages and n_kv_head must be >= 1");
   CHECK(p->n_kv_head <= 1024, "n_kv_head %d above 1024", p->n_kv_head);
+  CHECK((int64_t)p->n_pages * p->n_kv_head * p->page_size < (int64_t)1 << 32,
+        "pages: %d x %d heads x %d rows above 2^32", p->n_pages, p->n_kv_head, p->page_size);
   CHECK(p->type == FG_F32 || p->type == FG_BF16, "pages: unknown type %d", p->type);
   CHECK(aligned(p->k) && aligned(p->v), "pages are not 16-byte aligned");
   return FG_OK;

@@ -10,6 +10,7 @@
 #include <float.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "fgpt_internal.h"
 #include "kern_common.h"
@@ -123,6 +124,51 @@ __device__ __forceinline__ KeyTiles key_tiles(const RowTile& t) {
   return k;
 }
 
+__device__ __forceinline__ int tile_base(const RowTile& t, const KeyTiles& k, int v) {
+  return v < k.na ? 32 * v : k.from + 32 * (v - k.na);
+}
+
+// A tile's 16-key blocks, where their rows lie: pages hold 16 rows or a
+// multiple, so a block lies in one. A wavefront looks up 64 blocks ahead, one a
+// lane (PageList), and takes them by lane reads: the table's entries then cost
+// no wait in the loop, and a block ten scalar instructions.
+// Only rows that some query sees are read: in the place of another one the
+// block's first such row, in the place of a block without any the tile's other
+// block (its page may be gone, its memory hold anything).
+struct PageList {
+  uint32_t row;  // (page, key head)'s first row of the block, in rows of the pool
+  uint32_t vis;  // which of its 16 rows are seen, and (above) the first that is
+};
+struct PageAsk {
+  int e, page;  // first key, the table's entry
+};
+__device__ __forceinline__ PageAsk page_ask(const PagedArgs& p, const RowTile& t, const KeyTiles& kt,
+                                            const int32_t* tab, int v, int kb) {
+  PageAsk a;
+  a.e = tile_base(t, kt, v) + 16 * kb;
+  if (a.e >= t.sa && (a.e >= t.hi || a.e + 16 <= t.lo)) a.e += 16 - 32 * kb;
+  a.page = tab[a.e >> p.pshift];
+  return a;
+}
+__device__ __forceinline__ PageList page_place(const PagedArgs& p, const RowTile& t, int kvh,
+                                               const PageAsk& a, bool& bad) {
+  auto upto = [&](int j) { return (1u << max(0, min(j - a.e, 16))) - 1; };  // rows below key j
+  const bool ok = (uint32_t)a.page < (uint32_t)p.n_pages;
+  bad |= !ok;
+  PageList l;
+  l.row = (((uint32_t)(ok ? a.page : 0) * p.KH + kvh) << p.pshift) + (a.e & ((1 << p.pshift) - 1));
+  const uint32_t seen = upto(t.sa) | (upto(t.hi) & ~upto(t.lo));
+  l.vis = seen | ((uint32_t)__builtin_ctz(seen | 0x10000u) << 16);
+  return l;
+}
+// The row of a block to read for its row x.
+__device__ __forceinline__ int page_row(uint32_t vis, int x) {
+  return (vis >> x) & 1 ? x : (int)(vis >> 16);
+}
+__device__ __forceinline__ uint32_t lane_u32(uint32_t v, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+
 __device__ __forceinline__ uint32_t bits(float f) { return __float_as_uint(f); }
 
 // x as the sum of three bf16 terms: its leading 8 significant bits, the next 8,
@@ -163,67 +209,88 @@ __device__ __forceinline__ f32x4_t mma16(const bf16x8_t& a, const bf16x8_t& b, c
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// c += a . b over the term products that matter: all of those whose terms'
-// places add up to 2 at most (the others are below 2^-24 of the product),
-// smallest first.
-template <int NA, int NB>
-__device__ __forceinline__ f32x4_t mma_terms(const bf16x8_t (&a)[NA], const bf16x8_t (&b)[NB], f32x4_t c) {
+// c += a . b over b's terms, smallest first.
+template <bool QF>
+__device__ __forceinline__ f32x4_t mma_terms(const bf16x8_t& a, const Terms<QF>& b, f32x4_t c) {
 #pragma unroll
-  for (int o = 2; o >= 0; --o)
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-      if (o - i >= 0 && o - i < NB) c = mma16(a[i], b[o - i], c);
+  for (int i = Terms<QF>::N - 1; i >= 0; --i) c = mma16(a, b.t[i], c);
   return c;
 }
 
 // One 32-key tile's pieces of the K and V rows, as a lane (row c = lane % 16,
-// group g = lane / 16) loads them, and the operands made of them. K step s of
-// S^T = K Q^T covers head dims 32 s + KD g + .. of the lane's key; row c of
-// O^T's i-th block stands for head dim vdim(c, i): both are chosen so that a
-// lane's pieces are whole 16-byte (8 for head dim 64) loads of adjacent lanes.
-template <int HD, bool KF>
+// group g = lane / 16) loads them, the lane's query operand and the two
+// products. Which head dims a K slot of S^T = K Q^T and row c of O^T's i-th
+// block (vdim) stand for is chosen so that a lane's pieces are whole 16-byte (8
+// for head dim 64) loads of adjacent lanes.
+template <int HD, bool QF, bool KF>
 struct KvTile;
-template <int HD>
-struct KvTile<HD, true> {
-  static constexpr int NS = HD / 32, VD = HD / 16, N = 3;
+// fp32 pages: v_mfma_f32_16x16x4_f32, whose operands are single values (K slot g
+// of step (j, e) is head dim 16 j + 4 g + e; of the second product, key 4 g + r):
+// exact products without cutting K and V into terms, which costs a wavefront
+// more clocks than these MFMAs take, and registers (cut: one token after 300
+// positions 13.4 us, so 5.6).
+template <int HD, bool QF>
+struct KvTile<HD, QF, true> {
+  static constexpr int NJ = HD / 16, VD = HD / 16;
   typedef float elem;
   static __device__ __forceinline__ int vdim(int c, int i) { return 64 * (i / 4) + 4 * c + i % 4; }
-  static __device__ __forceinline__ int qdim(int s, int g, int half) { return 32 * s + 16 * half + 4 * g; }
-  float4 k[2][NS][2], v[8][VD / 4];
+  float4 q[NJ], k[2][NJ], v[8][VD / 4];
+  static __device__ __forceinline__ float at(const float4& f, int e) {
+    return e == 0 ? f.x : e == 1 ? f.y : e == 2 ? f.z : f.w;
+  }
+  __device__ __forceinline__ void load_q(const void* base, int64_t row, int g) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) q[j] = *(const float4*)((const float*)base + row + 16 * j + 4 * g);
+  }
   __device__ __forceinline__ void load_k(int kb, const float* row, int g) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) k[kb][s][h] = *(const float4*)(row + qdim(s, g, h));
+    for (int j = 0; j < NJ; ++j) k[kb][j] = *(const float4*)(row + 16 * j + 4 * g);
   }
   __device__ __forceinline__ void load_v(int e, const float* row, int c) {
 #pragma unroll
     for (int i = 0; i < VD / 4; ++i) v[e][i] = *(const float4*)(row + 64 * i + 4 * c);
   }
-  __device__ __forceinline__ void kop(int kb, int s, bf16x8_t (&t)[3]) const {
-    const float4 a = k[kb][s][0], b = k[kb][s][1];
-    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    split3(x, t);
-  }
-  __device__ __forceinline__ void vop(int i, bf16x8_t (&t)[3]) const {
-    float x[8];
+  __device__ __forceinline__ f32x4_t scores(int kb) const {
+    f32x4_t s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float4 w = v[e][i / 4];
-      x[e] = i % 4 == 0 ? w.x : i % 4 == 1 ? w.y : i % 4 == 2 ? w.z : w.w;
-    }
-    split3(x, t);
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s = __builtin_amdgcn_mfma_f32_16x16x4f32(at(k[kb][j], e), at(q[j], e), s, 0, 0, 0);
+    return s;
+  }
+  __device__ __forceinline__ void add_values(const float (&p)[8], f32x4_t (&o)[VD]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < VD; ++i)
+        o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(at(v[e][i / 4], i % 4), p[e], o[i], 0, 0, 0);
   }
 };
-template <int HD>
-struct KvTile<HD, false> {
-  static constexpr int NS = HD / 32, VD = HD / 16, N = 1;
+// bf16 pages: v_mfma_f32_16x16x32_bf16, K and V exact in one term, fp32 q and
+// probabilities in three.
+template <int HD, bool QF>
+struct KvTile<HD, QF, false> {
+  static constexpr int NS = HD / 32, VD = HD / 16;
   typedef uint16_t elem;
   static __device__ __forceinline__ int vdim(int c, int i) { return VD * c + i; }
-  static __device__ __forceinline__ int qdim(int s, int g, int half) { return 32 * s + 8 * g + 4 * half; }
   typedef uint32_t vrow_t __attribute__((ext_vector_type(VD / 2)));
+  Terms<QF> q[NS];
   u32x4v_t k[2][NS];
   vrow_t v[8];
+  __device__ __forceinline__ void load_q(const void* base, int64_t row, int g) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if constexpr (QF) {
+        const float* qp = (const float*)base + row + 32 * s + 8 * g;
+        const float4 a = *(const float4*)qp, b = *(const float4*)(qp + 4);
+        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        q[s].set(x);
+      } else {
+        q[s].t[0] = __builtin_bit_cast(bf16x8_t, *(const u32x4v_t*)((const uint16_t*)base + row + 32 * s + 8 * g));
+      }
+    }
+  }
   __device__ __forceinline__ void load_k(int kb, const uint16_t* row, int g) {
 #pragma unroll
     for (int s = 0; s < NS; ++s) k[kb][s] = *(const u32x4v_t*)(row + 32 * s + 8 * g);
@@ -231,16 +298,24 @@ struct KvTile<HD, false> {
   __device__ __forceinline__ void load_v(int e, const uint16_t* row, int c) {
     v[e] = *(const vrow_t*)(row + VD * c);
   }
-  __device__ __forceinline__ void kop(int kb, int s, bf16x8_t (&t)[1]) const {
-    t[0] = __builtin_bit_cast(bf16x8_t, k[kb][s]);
-  }
-  __device__ __forceinline__ void vop(int i, bf16x8_t (&t)[1]) const {
-    u32x4v_t w;
+  __device__ __forceinline__ f32x4_t scores(int kb) const {
+    f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w[e] = __builtin_amdgcn_perm(v[2 * e + 1][i / 2], v[2 * e][i / 2],
-                                   i & 1 ? 0x07060302u : 0x05040100u);
-    t[0] = __builtin_bit_cast(bf16x8_t, w);
+    for (int s = 0; s < NS; ++s) sc = mma_terms(__builtin_bit_cast(bf16x8_t, k[kb][s]), q[s], sc);
+    return sc;
+  }
+  __device__ __forceinline__ void add_values(const float (&p)[8], f32x4_t (&o)[VD]) const {
+    Terms<QF> pt;
+    pt.set(p);
+#pragma unroll
+    for (int i = 0; i < VD; ++i) {
+      u32x4v_t w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = __builtin_amdgcn_perm(v[2 * e + 1][i / 2], v[2 * e][i / 2],
+                                     i & 1 ? 0x07060302u : 0x05040100u);
+      o[i] = mma_terms(__builtin_bit_cast(bf16x8_t, w), pt, o[i]);
+    }
   }
 };
 
@@ -272,7 +347,7 @@ __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.0f
 // slots of its operand of O^T = V^T P^T. Pages hold 16 rows or a multiple, so
 // a block's page is one scalar load.
 // Bound by the cache's bytes: every visible key and value is read once.
-constexpr int DR = 16, RWV = 8;
+constexpr int DR = 16, RWV = 4;
 
 template <int HD>
 constexpr int few_lds() { return RWV * DR * (HD + 4) * 4; }
@@ -280,10 +355,10 @@ template <int HD>
 constexpr int64_t part_floats(int rows) { return (int64_t)rows * (HD + 2); }
 
 template <int HD, bool QF, bool KF>
-__global__ __launch_bounds__(64 * RWV) void k_paged_few(PagedArgs p) {
-  typedef KvTile<HD, KF> Tile;
+__global__ __launch_bounds__(64 * RWV, 2) void k_paged_few(PagedArgs p) {
+  typedef KvTile<HD, QF, KF> Tile;
   typedef typename Tile::elem E;
-  constexpr int NS = Tile::NS, VD = Tile::VD, OST = HD + 4;
+  constexpr int VD = Tile::VD, OST = HD + 4;
   extern __shared__ __attribute__((aligned(16))) float xo[];  // [RWV][DR][OST]
   __shared__ float ml[RWV][DR][2];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -303,89 +378,53 @@ __global__ __launch_bounds__(64 * RWV) void k_paged_few(PagedArgs p) {
 
   Tile kv;
   bool bad = false;
-  const int P = 1 << p.pshift;
   const int32_t* tab = p.table + (int64_t)t.seq * p.table_ld;
-  auto base_of = [&](int v) { return v < kt.na ? 32 * v : kt.from + 32 * (v - kt.na); };
-  // A 16-key block of a tile: where its rows lie, and which row to read in the
-  // place of one that no query sees (its page is only known to be there where
-  // some query sees a key of the block; a block without one reads the other).
-  struct Block {
-    int64_t off;  // element offset of its first row
-    int e, sub;   // first key, substitute row
+  const int vw = v0 + wv;  // this wavefront's tiles: vw, vw + RWV, ..
+  auto ask = [&](int it) {
+    return page_ask(p, t, kt, tab, min(vw + RWV * (it + lane / 2), v1 - 1), lane & 1);
   };
-  auto block_of = [&](int v, int kb) {
-    Block k;
-    k.e = base_of(v) + 16 * kb;
-    if (k.e >= t.sa && (k.e >= t.hi || k.e + 16 <= t.lo)) k.e += 16 - 32 * kb;
-    const int pg = tab[k.e >> p.pshift];
-    const bool ok = (uint32_t)pg < (uint32_t)p.n_pages;
-    bad |= !ok;
-    k.off = (((int64_t)(ok ? pg : 0) * p.KH + kvh) * P + (k.e & (P - 1))) * HD;
-    k.sub = k.e < t.sa ? 0 : max(0, t.lo - k.e);
-    return k;
-  };
-  auto row_of = [&](const Block& k, int x) {
-    const int j = k.e + x;
-    return j < t.sa || (j >= t.lo && j < t.hi) ? x : k.sub;
-  };
-  auto load_k = [&](const Block (&bl)[2]) {
+  PageList pl = {};
+  PageAsk next = {};
+  // tile `it` of this wavefront
+  auto load_k = [&](int it) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-      kv.load_k(kb, (const E*)p.k + bl[kb].off + row_of(bl[kb], c) * HD, g);
-  };
-  auto load_v = [&](const Block (&bl)[2]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      kv.load_v(e, (const E*)p.v + bl[e >> 2].off + row_of(bl[e >> 2], 4 * g + (e & 3)) * HD, c);
-  };
-  int v = v0 + wv;
-  if (v < v1) {
-    const Block bl[2] = {block_of(v, 0), block_of(v, 1)};
-    load_k(bl);
-    load_v(bl);
-  }
-  Terms<QF> q[NS];
-  {
-    const int64_t at = (int64_t)(t.row0 + tok) * p.q_ld + h * HD;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      if constexpr (QF) {
-        const float* qp = (const float*)p.q + at;
-        const float4 a = *(const float4*)(qp + Tile::qdim(s, g, 0));
-        const float4 b = *(const float4*)(qp + Tile::qdim(s, g, 1));
-        const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        q[s].set(x);
-      } else {  // (bf16 pages: a step's eight dims are consecutive)
-        q[s].t[0] = __builtin_bit_cast(
-            bf16x8_t, *(const u32x4v_t*)((const uint16_t*)p.q + at + Tile::qdim(s, g, 0)));
-      }
+    for (int kb = 0; kb < 2; ++kb) {
+      const int l = 2 * (it & 31) + kb;
+      const E* base = (const E*)p.k + (uint64_t)lane_u32(pl.row, l) * HD;
+      kv.load_k(kb, base + page_row(lane_u32(pl.vis, l), c) * HD, g);
     }
+  };
+  auto load_v = [&](int it) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int l = 2 * (it & 31) + kb;
+      const E* base = (const E*)p.v + (uint64_t)lane_u32(pl.row, l) * HD;
+      const uint32_t vis = lane_u32(pl.vis, l);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) kv.load_v(4 * kb + r, base + page_row(vis, 4 * g + r) * HD, c);
+    }
+  };
+  if (vw < v1) {
+    pl = page_place(p, t, kvh, ask(0), bad);
+    load_k(0);
+    load_v(0);
+    next = ask(32);
   }
+  kv.load_q(p.q, (int64_t)(t.row0 + tok) * p.q_ld + h * HD, g);
   f32x4_t o[VD];
 #pragma unroll
   for (int i = 0; i < VD; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m_run = -FLT_MAX, l_run = 0.f;  // log2 domain; l_run: this lane's keys
 
-  for (; v < v1; v += RWV) {
+  for (int it = 0, v = vw; v < v1; ++it, v += RWV) {
     const bool more = v + RWV < v1;
-    Block nb[2] = {};
-    if (more) {
-      nb[0] = block_of(v + RWV, 0);
-      nb[1] = block_of(v + RWV, 1);
+    const int b = tile_base(t, kt, v);
+    if (more && (it & 31) == 31) {
+      pl = page_place(p, t, kvh, next, bad);
+      next = ask(it + 33);
     }
-    const int b = base_of(v);
-    f32x4_t sc[2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      sc[kb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        bf16x8_t a[Tile::N];
-        kv.kop(kb, s, a);
-        sc[kb] = mma_terms(a, q[s].t, sc[kb]);
-      }
-    }
-    if (more) load_k(nb);
+    f32x4_t sc[2] = {kv.scores(0), kv.scores(1)};
+    if (more) load_k(it + 1);
     float mx = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -414,15 +453,8 @@ __global__ __launch_bounds__(64 * RWV) void k_paged_few(PagedArgs p) {
       pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e >> 2][e & 3], p.cs, -m_run));
       l_run += pv[e];
     }
-    Terms<QF> pt;
-    pt.set(pv);
-#pragma unroll
-    for (int i = 0; i < VD; ++i) {
-      bf16x8_t a[Tile::N];
-      kv.vop(i, a);
-      o[i] = mma_terms(a, pt.t, o[i]);
-    }
-    if (more) load_v(nb);
+    kv.add_values(pv, o);
+    if (more) load_v(it + 1);
   }
 
   l_run += __shfl_xor(l_run, 16, 64);
@@ -440,63 +472,86 @@ __global__ __launch_bounds__(64 * RWV) void k_paged_few(PagedArgs p) {
     ml[wv][c][1] = l_run;
   }
   __syncthreads();
-  const int r = tid / (HD / 4), d = 4 * (tid % (HD / 4));
-  if (r >= t.rows) return;
-  float m = -FLT_MAX, l = 0.f;
+  // a thread per row and four head dims, the wavefronts' sums in their order
+  for (int w = tid; w < t.rows * (HD / 4); w += 64 * RWV) {
+    const int r = w / (HD / 4), d = 4 * (w % (HD / 4));
+    float m = -FLT_MAX, l = 0.f;
 #pragma unroll
-  for (int k = 0; k < RWV; ++k) m = fmaxf(m, ml[k][r][0]);
-  float a[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < RWV; ++k) m = fmaxf(m, ml[k][r][0]);
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int k = 0; k < RWV; ++k) {
-    const float w = exp2f(ml[k][r][0] - m);
-    const float4 x = *(const float4*)(xo + (k * DR + r) * OST + d);
-    l += w * ml[k][r][1];
-    a[0] += w * x.x;
-    a[1] += w * x.y;
-    a[2] += w * x.z;
-    a[3] += w * x.w;
+    for (int k = 0; k < RWV; ++k) {
+      const float f = exp2f(ml[k][r][0] - m);
+      const float4 x = *(const float4*)(xo + (k * DR + r) * OST + d);
+      l += f * ml[k][r][1];
+      a[0] += f * x.x;
+      a[1] += f * x.y;
+      a[2] += f * x.z;
+      a[3] += f * x.w;
+    }
+    if (kt.n > p.cpt) {  // several parts: left for k_paged_merge
+      float* P0 = p.part + ((int64_t)(id * p.KH + kvh) * p.nsplit + z) * part_floats<HD>(DR);
+      *(float4*)(P0 + r * HD + d) = make_float4(a[0], a[1], a[2], a[3]);
+      if (d == 0) *(float2*)(P0 + DR * HD + 2 * r) = make_float2(m, l);
+      continue;
+    }
+    const float inv = inv_sum(l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] *= inv;
+    const int rr = t.r0 + r;
+    store_row4<QF>(p, t.row0 + rr / p.G, (kvh * p.G + rr % p.G) * HD + d, a);
   }
-  if (kt.n > p.cpt) {  // several parts: left for k_paged_merge
-    float* P0 = p.part + ((int64_t)(id * p.KH + kvh) * p.nsplit + z) * part_floats<HD>(DR);
-    *(float4*)(P0 + r * HD + d) = make_float4(a[0], a[1], a[2], a[3]);
-    if (d == 0) *(float2*)(P0 + DR * HD + 2 * r) = make_float2(m, l);
-    return;
-  }
-  const float inv = inv_sum(l);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) a[e] *= inv;
-  const int rr = t.r0 + r;
-  store_row4<QF>(p, t.row0 + rr / p.G, (kvh * p.G + rr % p.G) * HD + d, a);
 }
 
-// The parts of a row tile's keys joined in order: one workgroup an item, a
-// thread per row and four head dims.
+// The parts of a row tile's keys joined in order: a thread per row and four
+// head dims. Up to 8 parts take one round trip, issued before the lengths that
+// say how many there are have come (the others' memory is there, unused).
 template <int HD, bool QF, int RT>
 __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
   constexpr int PER = 1024 / HD;  // rows a workgroup takes
+  constexpr int64_t PF = part_floats<HD>(RT);
   const int sub = blockIdx.x % (RT / PER), item = blockIdx.x / (RT / PER);
   const int kvh = item % p.KH, id = item / p.KH;
+  const int r = sub * PER + threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
+  const float* P0 = p.part + (int64_t)item * p.nsplit * PF;
+  float2 s[8];
+  float4 x[8];
+  auto load = [&](int k0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k0 + k < p.nsplit) {
+        s[k] = *(const float2*)(P0 + (k0 + k) * PF + RT * HD + 2 * r);
+        x[k] = *(const float4*)(P0 + (k0 + k) * PF + r * HD + d);
+      }
+  };
+  load(0);
   RowTile t;
   if (!find_tile<RT>(p, id, t)) return;
   const KeyTiles kt = key_tiles(t);
-  if (kt.n <= p.cpt) return;  // written by the attention kernel itself
-  const int r = sub * PER + threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
-  if (r >= t.rows) return;
+  if (kt.n <= p.cpt || r >= t.rows) return;  // (written by the attention kernel itself)
   const int n = (kt.n + p.cpt - 1) / p.cpt;
-  const float* P0 = p.part + (int64_t)(id * p.KH + kvh) * p.nsplit * part_floats<HD>(RT);
   float m = -FLT_MAX, l = 0.f;
-  for (int k = 0; k < n; ++k) m = fmaxf(m, P0[k * part_floats<HD>(RT) + RT * HD + 2 * r]);
   float a[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < n; ++k) {
-    const float* P = P0 + k * part_floats<HD>(RT);
-    const float2 s = *(const float2*)(P + RT * HD + 2 * r);
-    const float4 x = *(const float4*)(P + r * HD + d);
-    const float w = exp2f(s.x - m);
-    l += w * s.y;
-    a[0] += w * x.x;
-    a[1] += w * x.y;
-    a[2] += w * x.z;
-    a[3] += w * x.w;
+  for (int k0 = 0; k0 < n; k0 += 8) {
+    if (k0 > 0) load(k0);
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = k0 + k < n ? fmaxf(top, s[k].x) : top;
+    const float f = exp2f(m - top);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] *= f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k >= n) break;
+      const float w = exp2f(s[k].x - m);
+      l += w * s[k].y;
+      a[0] += w * x[k].x;
+      a[1] += w * x[k].y;
+      a[2] += w * x[k].z;
+      a[3] += w * x[k].w;
+    }
   }
   const float inv = inv_sum(l);
 #pragma unroll
@@ -528,7 +583,7 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 template <int HD, bool QF, bool KF>
 struct Many {
-  static constexpr int RB = QF ? 1 : 2;  // query blocks of 32 rows a wavefront
+  static constexpr int RB = 1;  // query blocks of 32 rows a wavefront
   static constexpr int RT = 128 * RB;    // rows of a tile
   static constexpr int NA = KF ? 3 : 1, NB = QF ? 3 : 1;
   static constexpr int ROW = 2 * HD;           // bytes of a K or V row in LDS
@@ -571,7 +626,7 @@ __device__ __forceinline__ f32x16_t mma32(const bf16x8_t (&a)[NA], const bf16x8_
 }
 
 template <int HD, bool QF, bool KF>
-__global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
+__global__ __launch_bounds__(256, KF ? 1 : 2) void k_paged_many(PagedArgs p) {
   typedef Many<HD, QF, KF> C;
   constexpr int RB = C::RB, NS = HD / 16, ND = HD / 32, NA = C::NA, ROW = C::ROW, PLANE = C::PLANE;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -587,31 +642,13 @@ __global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
   const int nstep = (v1 - v0 + 1) / 2;
 
   bool bad = false;
-  const int P = 1 << p.pshift;
   const int32_t* tab = p.table + (int64_t)t.seq * p.table_ld;
-  auto base_of = [&](int v) { return v < kt.na ? 32 * v : kt.from + 32 * (v - kt.na); };
-  // the 16-key blocks of a step as in k_paged_few: where a block's rows lie,
-  // its first key, the row read in the place of an unseen one
-  struct Block {
-    int64_t off;
-    int e, sub;
+  // block b4 of step st is lane 4 (st % 16) + b4 of the step's list
+  auto ask = [&](int st) {
+    return page_ask(p, t, kt, tab, min(v0 + 2 * st + lane / 2, v1 - 1), lane & 1);
   };
-  auto block_of = [&](int st, int b4) {
-    const int v = min(v0 + 2 * st + (b4 >> 1), v1 - 1), kb = b4 & 1;
-    Block k;
-    k.e = base_of(v) + 16 * kb;
-    if (k.e >= t.sa && (k.e >= t.hi || k.e + 16 <= t.lo)) k.e += 16 - 32 * kb;
-    const int pg = tab[k.e >> p.pshift];
-    const bool ok = (uint32_t)pg < (uint32_t)p.n_pages;
-    bad |= !ok;
-    k.off = (((int64_t)(ok ? pg : 0) * p.KH + kvh) * P + (k.e & (P - 1))) * HD;
-    k.sub = k.e < t.sa ? 0 : max(0, t.lo - k.e);
-    return k;
-  };
-  auto row_of = [&](const Block& k, int x) {
-    const int j = k.e + x;
-    return j < t.sa || (j >= t.lo && j < t.hi) ? x : k.sub;
-  };
+  PageList pl = {};
+  PageAsk next = {};
 
   // ---- staging
   // bf16: rows of one 1 KB DMA group (RPG of them) lie in one block; this
@@ -622,8 +659,8 @@ __global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
 #pragma unroll
     for (int q = 0; q < GPP / 4; ++q) {
       const int grp = wv + 4 * q, r = grp * RPG + lane / (ROW / 16), slot = lane % (ROW / 16);
-      const Block b = block_of(st, grp * RPG / 16);
-      const int64_t at = b.off + row_of(b, r & 15) * HD;
+      const int l = 4 * (st & 15) + grp * RPG / 16;
+      const uint64_t at = (uint64_t)lane_u32(pl.row, l) * HD + page_row(lane_u32(pl.vis, l), r & 15) * HD;
       const uint32_t to = lds0 + buf * C::STAGE + grp * 1024;
       dma16((const uint16_t*)p.k + at + kslot<HD>(r, slot) * 8, to);
       dma16((const uint16_t*)p.v + at + vslot<HD>(r, slot) * 8, to + PLANE);
@@ -637,8 +674,9 @@ __global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
     for (int i = 0; i < NT; ++i) {
       const int r = i * RPT + tid / CH;
       const int b4 = __builtin_amdgcn_readfirstlane(r / 16);  // (a wavefront's rows lie in one block)
-      const Block b = block_of(st, b4);
-      const int64_t at = b.off + row_of(b, r & 15) * HD + (tid % CH) * 8;
+      const int l = 4 * (st & 15) + b4;
+      const uint64_t at = (uint64_t)lane_u32(pl.row, l) * HD + page_row(lane_u32(pl.vis, l), r & 15) * HD +
+                          (tid % CH) * 8;
       const float* kp = (const float*)p.k + at;
       const float* vp = (const float*)p.v + at;
       raw[i][0] = *(const float4*)kp;
@@ -705,10 +743,16 @@ __global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
   }
 
   if (nstep > 0) {
+    pl = page_place(p, t, kvh, ask(0), bad);
     if constexpr (KF) fetch(0);
     else fill(0, 0);
+    next = ask(16);
   }
   for (int st = 0; st < nstep; ++st) {
+    if (st + 1 < nstep && (st & 15) == 15) {
+      pl = page_place(p, t, kvh, next, bad);
+      next = ask(st + 17);
+    }
     if constexpr (KF) {
       if (st > 0) __syncthreads();  // (every wavefront is done with the last step)
       put();
@@ -720,9 +764,9 @@ __global__ __launch_bounds__(256) void k_paged_many(PagedArgs p) {
     }
     if (!active) continue;
     const uint8_t* S = lds + (KF ? 0 : (st & 1) * C::STAGE);
-    const int b0 = base_of(v0 + 2 * st);
+    const int b0 = tile_base(t, kt, v0 + 2 * st);
     const bool two = v0 + 2 * st + 1 < v1;
-    const int b1 = two ? base_of(v0 + 2 * st + 1) : 0x3fffffff;  // (no such keys: all masked)
+    const int b1 = two ? tile_base(t, kt, v0 + 2 * st + 1) : 0x3fffffff;  // (no such keys: all masked)
     if (b0 > wp1 && b1 > wp1) continue;  // (behind the wavefront's rows)
 
     f32x16_t sc[RB][2];
@@ -870,7 +914,8 @@ struct Plan {
 Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
   Plan pl;
   const int64_t G = c.n_head / pg.n_kv_head;
-  pl.many = b.max_q * G > 32;
+  static const int eTH = getenv("PG_TH") ? atoi(getenv("PG_TH")) : 32;
+  pl.many = b.max_q * G > eTH;
   pl.rt = !pl.many ? DR : c.type == FG_F32 ? Many<128, true, true>::RT : Many<128, false, false>::RT;
   const int64_t per_seq = (b.max_q * G + pl.rt - 1) / pl.rt;
   pl.ntile = (int)std::min<int64_t>(per_seq * b.n_seq, b.n_rows * G / pl.rt + b.n_seq);
@@ -881,8 +926,10 @@ Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
   // parts: enough workgroups for two a CU, each with a round of its
   // wavefronts' tiles at least
   const int64_t items = (int64_t)pl.ntile * pg.n_kv_head;
-  const int64_t want = (2 * CUS + items - 1) / items;
-  const int64_t most = (nkt + RWV - 1) / RWV;
+  static const int eSP = getenv("PG_SP") ? atoi(getenv("PG_SP")) : 4, eMT = getenv("PG_MT") ? atoi(getenv("PG_MT")) : 2;
+  const int64_t want = ((pl.many ? eSP : 4) * CUS / 4 + items - 1) / items;
+  const int64_t least = pl.many ? 4 * eMT : RWV;
+  const int64_t most = (nkt + least - 1) / least;
   const int64_t ns = std::max<int64_t>(1, std::min(want, most));
   pl.cpt = (int)((nkt + ns - 1) / ns + RWV - 1) / RWV * RWV;
   pl.nsplit = (int)((nkt + pl.cpt - 1) / pl.cpt);
