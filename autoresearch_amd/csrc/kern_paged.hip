@@ -10,7 +10,7 @@
 #include <float.h>
 
 #include <algorithm>
-#include <cstdlib>
+#include <type_traits>
 
 #include "fgpt_internal.h"
 #include "kern_common.h"
@@ -101,9 +101,10 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& p, int id, RowTile& t
   t.r0 = tile * RT;
   t.rows = min(RT, nq * p.G - t.r0);
   if (t.rows <= 0) return false;
-  t.row0 = p.q_start[t.seq];
-  t.kv = max(0, min(p.kv_len[t.seq], p.max_kv));
-  t.pos0 = t.kv - (p.q_start[t.seq + 1] - t.row0);
+  // (said to be uniform, or the compiler keeps masks and places per lane)
+  t.row0 = __builtin_amdgcn_readfirstlane(p.q_start[t.seq]);
+  t.kv = __builtin_amdgcn_readfirstlane(max(0, min(p.kv_len[t.seq], p.max_kv)));
+  t.pos0 = t.kv - (__builtin_amdgcn_readfirstlane(p.q_start[t.seq + 1]) - t.row0);
   const int pf = t.pos0 + t.r0 / p.G, pl = t.pos0 + (t.r0 + t.rows - 1) / p.G;
   t.hi = max(0, min(pl + 1, t.kv));
   t.lo = p.window > 0 ? max(0, min(pf - p.window + 1, t.hi)) : 0;
@@ -561,9 +562,8 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
 }
 
 // ------------------------------------------------------------ many rows
-// For chunks of new tokens: 128 RB flattened rows a tile, 32 RB to each of four
-// wavefronts, which all go through the same keys, 64 a step (two 32-key tiles of
-// the list). v_mfma_f32_32x32x16_bf16 with S^T = K Q^T and O^T = V^T P^T: lane
+// For chunks of new tokens: 128 flattened rows a tile, 32 to each of four
+// wavefronts, which all go through the same keys, a 32-key tile a step. v_mfma_f32_32x32x16_bf16 with S^T = K Q^T and O^T = V^T P^T: lane
 // 32 g + c holds query row c of its wavefront. The key rows of a 32-key tile are
 // taken with bits 2 and 3 of their number swapped, so that a lane's scores 8 s ..
 // 8 s + 7 are keys 16 s + 8 g .., which are its K slots of the second product:
@@ -573,24 +573,21 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
 // bf16 pages go memory -> LDS by DMA into two buffers, the next step's rows
 // landing while this one's are used; fp32 ones through registers, cut into
 // three bf16 terms once for the whole workgroup, into one buffer.
-// An operand read from LDS (1 KB) feeds one MFMA of 32 clocks for each query
-// block and term product: at one of both the LDS, 128 bytes a clock, would be
-// busy all the time, hence RB = 2 where operands have one term.
-constexpr int SK = 64;
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
 template <int HD, bool QF, bool KF>
 struct Many {
-  static constexpr int RB = 1;  // query blocks of 32 rows a wavefront
-  static constexpr int RT = 128 * RB;    // rows of a tile
-  static constexpr int NA = KF ? 3 : 1, NB = QF ? 3 : 1;
+  static constexpr int RT = 128;  // rows of a tile, 32 a wavefront
+  static constexpr int NA = KF ? 3 : 1;
+  static constexpr int KB = 1;        // 32-key tiles a step
+  static constexpr int SK = 32 * KB;
   static constexpr int ROW = 2 * HD;           // bytes of a K or V row in LDS
   static constexpr int PLANE = SK * ROW;
   static constexpr int STAGE = 2 * NA * PLANE;  // K planes, V planes
-  static constexpr int NST = KF ? 1 : 2;
-  static constexpr int LDS = NST * STAGE;
+  static constexpr int LDS = (KF ? 1 : 2) * STAGE;
+  static constexpr int WAVES = QF ? 2 : 3;  // a SIMD
 };
 
 // key held by operand row i of a 32-key tile (bits 2 and 3 swapped)
@@ -615,20 +612,30 @@ __device__ __forceinline__ float swap_sum(float v) {
   return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
 
-template <int NA, int NB>
-__device__ __forceinline__ f32x16_t mma32(const bf16x8_t (&a)[NA], const bf16x8_t (&b)[NB], f32x16_t c) {
+template <int NA, bool QF>
+__device__ __forceinline__ f32x16_t mma32(const bf16x8_t (&a)[NA], const Terms<QF>& b, f32x16_t c) {
 #pragma unroll
   for (int o = 2; o >= 0; --o)
 #pragma unroll
     for (int i = 0; i < NA; ++i)
-      if (o - i >= 0 && o - i < NB) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[o - i], c, 0, 0, 0);
+      if (o - i >= 0 && o - i < Terms<QF>::N)
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b.t[o - i], c, 0, 0, 0);
   return c;
 }
 
+template <class T>
+__device__ __forceinline__ T lds_at(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(uintptr_t)at;
+}
+__device__ __forceinline__ s16x4_t lds_tr(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(uintptr_t)at);
+}
+
 template <int HD, bool QF, bool KF>
-__global__ __launch_bounds__(256, KF ? 1 : 2) void k_paged_many(PagedArgs p) {
+__global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(PagedArgs p) {
   typedef Many<HD, QF, KF> C;
-  constexpr int RB = C::RB, NS = HD / 16, ND = HD / 32, NA = C::NA, ROW = C::ROW, PLANE = C::PLANE;
+  constexpr int NS = HD / 16, ND = HD / 32, NA = C::NA, KB = C::KB, SK = C::SK, ROW = C::ROW,
+                PLANE = C::PLANE, PER = 64 / (2 * KB);  // steps whose blocks a list holds
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -639,53 +646,60 @@ __global__ __launch_bounds__(256, KF ? 1 : 2) void k_paged_many(PagedArgs p) {
   const KeyTiles kt = key_tiles(t);
   const int v0 = z * p.cpt, v1 = min(kt.n, v0 + p.cpt);
   if (z > 0 && v0 >= kt.n) return;
-  const int nstep = (v1 - v0 + 1) / 2;
+  const int nstep = (v1 - v0 + KB - 1) / KB;
 
   bool bad = false;
   const int32_t* tab = p.table + (int64_t)t.seq * p.table_ld;
-  // block b4 of step st is lane 4 (st % 16) + b4 of the step's list
-  auto ask = [&](int st) {
-    return page_ask(p, t, kt, tab, min(v0 + 2 * st + lane / 2, v1 - 1), lane & 1);
+  // block b of step st is lane 2 KB (st % PER) + b of the step's list
+  auto ask = [&](int st) __attribute__((always_inline)) {
+    return page_ask(p, t, kt, tab, min(v0 + KB * st + lane / 2, v1 - 1), lane & 1);
   };
-  PageList pl = {};
+  PageList pl = {};  // of the step that is fetched next
   PageAsk next = {};
+  auto turn = [&](int st) __attribute__((always_inline)) {  // pl for step st, in order
+    if (st % PER == 0 && st > 0) {
+      pl = page_place(p, t, kvh, next, bad);
+      next = ask(st + PER);
+    }
+  };
 
   // ---- staging
   // bf16: rows of one 1 KB DMA group (RPG of them) lie in one block; this
   // wavefront fills groups wv, wv + 4, ..
   constexpr int RPG = 1024 / ROW, GPP = PLANE / 1024;  // rows a group, groups a plane
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_off(lds));
-  auto fill = [&](int st, int buf) {
+  auto fill = [&](int st, uint32_t to) __attribute__((always_inline)) {
+    turn(st);
 #pragma unroll
     for (int q = 0; q < GPP / 4; ++q) {
       const int grp = wv + 4 * q, r = grp * RPG + lane / (ROW / 16), slot = lane % (ROW / 16);
-      const int l = 4 * (st & 15) + grp * RPG / 16;
-      const uint64_t at = (uint64_t)lane_u32(pl.row, l) * HD + page_row(lane_u32(pl.vis, l), r & 15) * HD;
-      const uint32_t to = lds0 + buf * C::STAGE + grp * 1024;
-      dma16((const uint16_t*)p.k + at + kslot<HD>(r, slot) * 8, to);
-      dma16((const uint16_t*)p.v + at + vslot<HD>(r, slot) * 8, to + PLANE);
+      const int at = 2 * KB * (st % PER) + grp * RPG / 16;
+      const uint64_t row = (uint64_t)lane_u32(pl.row, at) * HD;
+      const int x = page_row(lane_u32(pl.vis, at), r & 15) * HD;
+      dma16((const uint16_t*)p.k + row + (x + kslot<HD>(r, slot) * 8), lds0 + to + grp * 1024);
+      dma16((const uint16_t*)p.v + row + (x + vslot<HD>(r, slot) * 8), lds0 + to + PLANE + grp * 1024);
     }
   };
   // fp32: this thread's 8-value chunks of both planes' rows, loaded a step ahead
   constexpr int CH = HD / 8, RPT = 256 / CH, NT = SK / RPT;  // chunks a row, rows at once, rounds
   float4 raw[KF ? NT : 1][4];
-  auto fetch = [&](int st) {
+  auto fetch = [&](int st) __attribute__((always_inline)) {
+    turn(st);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int r = i * RPT + tid / CH;
-      const int b4 = __builtin_amdgcn_readfirstlane(r / 16);  // (a wavefront's rows lie in one block)
-      const int l = 4 * (st & 15) + b4;
-      const uint64_t at = (uint64_t)lane_u32(pl.row, l) * HD + page_row(lane_u32(pl.vis, l), r & 15) * HD +
-                          (tid % CH) * 8;
-      const float* kp = (const float*)p.k + at;
-      const float* vp = (const float*)p.v + at;
+      const int at = 2 * KB * (st % PER) + __builtin_amdgcn_readfirstlane(r / 16);  // (a wavefront's rows lie in one block)
+      const int off = page_row(lane_u32(pl.vis, at), r & 15) * HD + (tid % CH) * 8;
+      const uint64_t row = (uint64_t)lane_u32(pl.row, at) * HD;
+      const float* kp = (const float*)p.k + row + off;
+      const float* vp = (const float*)p.v + row + off;
       raw[i][0] = *(const float4*)kp;
       raw[i][1] = *(const float4*)(kp + 4);
       raw[i][2] = *(const float4*)vp;
       raw[i][3] = *(const float4*)(vp + 4);
     }
   };
-  auto put = [&] {
+  auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int r = i * RPT + tid / CH;
@@ -703,16 +717,13 @@ __global__ __launch_bounds__(256, KF ? 1 : 2) void k_paged_many(PagedArgs p) {
     }
   };
 
-  // ---- this lane's query rows
-  const int w0 = 32 * RB * wv;  // the wavefront's first row of the tile
+  // ---- this lane's query row
+  const int w0 = 32 * wv;  // the wavefront's first row of the tile
   const bool active = w0 < t.rows;
-  int klim[RB], klo[RB];
-  Terms<QF> q[RB][NS];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int fr = t.r0 + min(w0 + 32 * b + c, t.rows - 1), tok = fr / p.G, h = kvh * p.G + fr % p.G;
-    klim[b] = t.pos0 + tok + 1;
-    klo[b] = p.window > 0 ? klim[b] - p.window : 0;
+  const int fr = t.r0 + min(w0 + c, t.rows - 1), tok = fr / p.G, h = kvh * p.G + fr % p.G;
+  const int klim = t.pos0 + tok + 1, klo = p.window > 0 ? klim - p.window : 0;
+  Terms<QF> q[NS];
+  {
     const int64_t at = (int64_t)(t.row0 + tok) * p.q_ld + h * HD + 8 * g;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
@@ -720,39 +731,130 @@ __global__ __launch_bounds__(256, KF ? 1 : 2) void k_paged_many(PagedArgs p) {
         const float* qp = (const float*)p.q + at + 16 * s;
         const float4 x0 = *(const float4*)qp, x1 = *(const float4*)(qp + 4);
         const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-        q[b][s].set(x);
+        q[s].set(x);
       } else {
-        q[b][s].t[0] = __builtin_bit_cast(bf16x8_t, *(const u32x4v_t*)((const uint16_t*)p.q + at + 16 * s));
+        q[s].t[0] = __builtin_bit_cast(bf16x8_t, *(const u32x4v_t*)((const uint16_t*)p.q + at + 16 * s));
       }
     }
   }
   // positions of the wavefront's first and last row: which tiles need no mask
-  const int wlast = t.r0 + min(w0 + 32 * RB, t.rows) - 1;
-  const int wp0 = t.pos0 + (t.r0 + min(w0, t.rows - 1)) / p.G, wp1 = t.pos0 + wlast / p.G;
+  const int wp0 = t.pos0 + (t.r0 + min(w0, t.rows - 1)) / p.G;
+  const int wp1 = t.pos0 + (t.r0 + min(w0 + 32, t.rows) - 1) / p.G;
 
-  f32x16_t o[RB][ND];
-  float m_run[RB], l_run[RB];
+  // ---- operand places in LDS (of buffer 0; a step's buffer and rows are
+  // added as constants). K: row tile_key(c), chunk 2 s + g. V: row 8 g + r3 of
+  // each 16, dims 32 i + 16 (lane / 16 % 2) + 4 (lane % 4).
+  uint32_t ka[NS], va[ND];
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    m_run[b] = -FLT_MAX;
-    l_run[b] = 0.f;
+  for (int s = 0; s < NS; ++s) ka[s] = lds0 + tile_key(c) * ROW + kslot<HD>(tile_key(c), 2 * s + g) * 16;
+  const int vr = 8 * g + ((lane >> 2) & 3);
 #pragma unroll
-    for (int i = 0; i < ND; ++i)
+  for (int i = 0; i < ND; ++i)
+    va[i] = lds0 + NA * PLANE + vr * ROW +
+            vslot<HD>(vr, 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) * 16 + 8 * (lane & 1);
+
+  f32x16_t o[ND];
+  float m_run = -FLT_MAX, l_run = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[b][i][r] = 0.f;
-  }
+  for (int i = 0; i < ND; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+
+  // S^T of the step's keys in K buffer `to`
+  auto scores = [&](uint32_t to, f32x16_t (&sc)[KB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[kb][r] = 0.f;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        bf16x8_t a[NA];
+#pragma unroll
+        for (int k = 0; k < NA; ++k) a[k] = lds_at<bf16x8_t>(ka[s] + to + k * PLANE + kb * 32 * ROW);
+        sc[kb] = mma32(a, q[s], sc[kb]);
+      }
+    }
+  };
+  // masks where some row does not see the whole of step st's tiles, and moves
+  // the running maximum (only past a score 2^8 above it, as in k_paged_few)
+  auto settle = [&](int st, f32x16_t (&sc)[KB]) __attribute__((always_inline)) {
+    int b[KB], low = 0x7fffffff, top = 0;  // first keys of the tiles
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const int v = v0 + KB * st + kb;
+      b[kb] = v < v1 ? tile_base(t, kt, v) : 0x3fffffff;  // (no such keys: all masked)
+      low = min(low, b[kb]);
+      top = max(top, b[kb]);
+    }
+    if (top + 31 > wp0 || (p.window > 0 && low <= wp1 - p.window)) {
+      asm volatile("");  // (a branch: most steps are seen whole, and the selects are not few)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {  // (of this lane's keys first + 0 .. 7 and 16 .. 23)
+        const int first = b[kb] + 8 * g;
+        const int end = klim - first, from = klo - first, sink = p.sinks - first;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int x = 16 * (r >> 3) + (r & 7);
+          const bool seen = x < end && (x >= from || x < sink);
+          sc[kb][r] = seen ? sc[kb][r] : -INFINITY;
+        }
+      }
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kb][r]);
+    mx = swap_max(mx) * p.cs;
+    if (__any(mx > m_run + 8.f)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+      m_run = m_new;
+    }
+  };
+  // the probabilities' operands of the four 16-key steps, and their sum
+  auto weigh = [&](const f32x16_t (&sc)[KB], Terms<QF> (&pt)[2 * KB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s4 = 0; s4 < 2 * KB; ++s4) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s4 >> 1][8 * (s4 & 1) + e], p.cs, -m_run));
+      pt[s4].set(x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) l_run += x[e];
+    }
+  };
+  // O^T += V^T P^T from V buffer `to`
+  auto add_values = [&](uint32_t to, const Terms<QF> (&pt)[2 * KB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s4 = 0; s4 < 2 * KB; ++s4)
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        bf16x8_t a[NA];
+#pragma unroll
+        for (int k = 0; k < NA; ++k)
+          a[k] = __builtin_bit_cast(
+              bf16x8_t, __builtin_shufflevector(lds_tr(va[i] + to + k * PLANE + 16 * s4 * ROW),
+                                                lds_tr(va[i] + to + k * PLANE + (16 * s4 + 4) * ROW), 0, 1, 2,
+                                                3, 4, 5, 6, 7));
+        o[i] = mma32(a, pt[s4], o[i]);
+      }
+  };
 
   if (nstep > 0) {
     pl = page_place(p, t, kvh, ask(0), bad);
     if constexpr (KF) fetch(0);
     else fill(0, 0);
-    next = ask(16);
+    next = ask(PER);
   }
-  for (int st = 0; st < nstep; ++st) {
-    if (st + 1 < nstep && (st & 15) == 15) {
-      pl = page_place(p, t, kvh, next, bad);
-      next = ask(st + 17);
-    }
+  auto step = [&](auto buf, int st) __attribute__((always_inline)) {
+    constexpr uint32_t here = decltype(buf)::value * C::STAGE;
     if constexpr (KF) {
       if (st > 0) __syncthreads();  // (every wavefront is done with the last step)
       put();
@@ -760,140 +862,42 @@ __global__ __launch_bounds__(256, KF ? 1 : 2) void k_paged_many(PagedArgs p) {
       if (st + 1 < nstep) fetch(st + 1);
     } else {
       stage_sync<0>();  // this step has landed, and nobody reads the other buffer
-      if (st + 1 < nstep) fill(st + 1, (st + 1) & 1);
+      if (st + 1 < nstep) fill(st + 1, C::STAGE - here);
     }
-    if (!active) continue;
-    const uint8_t* S = lds + (KF ? 0 : (st & 1) * C::STAGE);
-    const int b0 = tile_base(t, kt, v0 + 2 * st);
-    const bool two = v0 + 2 * st + 1 < v1;
-    const int b1 = two ? tile_base(t, kt, v0 + 2 * st + 1) : 0x3fffffff;  // (no such keys: all masked)
-    if (b0 > wp1 && b1 > wp1) continue;  // (behind the wavefront's rows)
-
-    f32x16_t sc[RB][2];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[b][kb][r] = 0.f;
-      const int row = 32 * kb + tile_key(c);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int at = row * ROW + kslot<HD>(row, 2 * s + g) * 16;
-        bf16x8_t a[NA];
-#pragma unroll
-        for (int k = 0; k < NA; ++k) a[k] = *(const bf16x8_t*)(S + k * PLANE + at);
-#pragma unroll
-        for (int b = 0; b < RB; ++b) sc[b][kb] = mma32(a, q[b][s].t, sc[b][kb]);
-      }
-    }
-    // masks, where some row does not see the whole of a tile
-    const int far = max(b0, b1) + 31;
-    const bool masked = far > wp0 || (p.window > 0 && min(b0, b1) <= wp1 - p.window);
-    if (masked) {
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int j = (kb ? b1 : b0) + 16 * (r >> 3) + 8 * g + (r & 7);
-            const bool seen = j < klim[b] && (j >= klo[b] || j < p.sinks);
-            sc[b][kb][r] = seen ? sc[b][kb][r] : -INFINITY;
-          }
-    }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      float mx = -INFINITY;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[b][kb][r]);
-      mx = swap_max(mx) * p.cs;
-      if (__any(mx > m_run[b] + 8.f)) {  // (as in k_paged_few)
-        const float m_new = fmaxf(m_run[b], mx);
-        const float alpha = __builtin_amdgcn_exp2f(m_run[b] - m_new);
-        l_run[b] *= alpha;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[b][i][r] *= alpha;
-        m_run[b] = m_new;
-      }
-      float ps = 0.f;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][kb][r], p.cs, -m_run[b]));
-          sc[b][kb][r] = e;
-          ps += e;
-        }
-      l_run[b] += ps;
-    }
-    // O^T += V^T P^T, 16 keys at a time
-    const uint32_t vb = lds_off(S) + NA * PLANE;
-#pragma unroll
-    for (int s4 = 0; s4 < 4; ++s4) {
-      Terms<QF> pt[RB];
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = sc[b][s4 >> 1][8 * (s4 & 1) + e];
-        pt[b].set(x);
-      }
-      // rows 16 s4 + 8 g + lane % 16 / 4 (+ 4), dims 32 i + 16 (lane / 16 % 2) + 4 (lane % 4)
-      const int row = 16 * s4 + 8 * g + ((lane >> 2) & 3);
-#pragma unroll
-      for (int i = 0; i < ND; ++i) {
-        const int ch = 4 * i + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-        bf16x8_t a[NA];
-#pragma unroll
-        for (int k = 0; k < NA; ++k) {
-          s16x4_t h[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const uint32_t at = vb + k * PLANE + (row + 4 * u) * ROW + vslot<HD>(row + 4 * u, ch) * 16 +
-                                8 * (lane & 1);
-            h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4_t*)(uintptr_t)at);
-          }
-          a[k] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        }
-#pragma unroll
-        for (int b = 0; b < RB; ++b) o[b][i] = mma32(a, pt[b].t, o[b][i]);
-      }
-    }
+    if (!active || tile_base(t, kt, v0 + KB * st) > wp1) return;  // (behind the wavefront's rows)
+    f32x16_t sc[KB];
+    scores(here, sc);
+    settle(st, sc);
+    Terms<QF> pt[2 * KB];
+    weigh(sc, pt);
+    add_values(here, pt);
+  };
+  for (int st = 0; st < nstep; st += 2) {
+    step(std::integral_constant<int, 0>(), st);
+    if (st + 1 < nstep) step(std::integral_constant<int, KF ? 0 : 1>(), st + 1);
   }
   if (!active) return;
 
-  bad = __any(bad);
   const bool whole = kt.n <= p.cpt;
   float* P0 = p.part + ((int64_t)(id * p.KH + kvh) * p.nsplit + z) * part_floats<HD>(C::RT);
+  const int r = w0 + c;
+  float l = swap_sum(l_run);
+  if (__any(bad)) l = NAN;
+  if (r >= t.rows) return;
+  const float f = whole ? inv_sum(l) : 1.f;
+  const int64_t row = t.row0 + tok;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int r = w0 + 32 * b + c;
-    float l = swap_sum(l_run[b]);
-    if (bad) l = NAN;
-    if (r >= t.rows) continue;
-    const float f = whole ? inv_sum(l) : 1.f;
-    const int rr = t.r0 + r;
-    const int64_t row = t.row0 + rr / p.G;
-    const int col = (kvh * p.G + rr % p.G) * HD;
+  for (int i = 0; i < ND; ++i)
 #pragma unroll
-    for (int i = 0; i < ND; ++i)
+    for (int r4 = 0; r4 < 4; ++r4) {
+      float v[4];
 #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = o[b][i][4 * r4 + e] * f;
-        const int d = 32 * i + 8 * r4 + 4 * g;
-        if (whole) store_row4<QF>(p, row, col + d, v);
-        else *(float4*)(P0 + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
-      }
-    if (!whole && g == 0) *(float2*)(P0 + C::RT * HD + 2 * r) = make_float2(m_run[b], l);
-  }
+      for (int e = 0; e < 4; ++e) v[e] = o[i][4 * r4 + e] * f;
+      const int d = 32 * i + 8 * r4 + 4 * g;
+      if (whole) store_row4<QF>(p, row, h * HD + d, v);
+      else *(float4*)(P0 + r * HD + d) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+  if (!whole && g == 0) *(float2*)(P0 + C::RT * HD + 2 * r) = make_float2(m_run, l);
 }
 
 // ------------------------------------------------------------ host side
@@ -911,28 +915,41 @@ struct Plan {
 
 // The tiles of a launch and the parts its keys are cut into, from the bounds
 // alone (lengths may differ under a captured launch).
+//
+// Which kernel: 16-row tiles keep a wavefront a 32-key tile, and read the keys
+// once for each tile; 128-row tiles read them once for eight of those, and
+// have four times the MFMA rate where there are enough of them. The latter take
+// over past 32 rows a sequence from MANY_WORK (16-row tile, 32-key tile) pairs
+// on. us, 16 rows -> 128: fp32 rows and pages, 64 tokens after 936 (768 pairs)
+// 15.0 -> 21.8, 8 x 96 after 1404, 6 heads (13.5k) 90 -> 53, 500 tokens (3k) 18.6
+// -> 25.5, 2048 (49k) 118 -> 74; bf16, 32 heads on 4, 8 x 8 rows after 1490
+// (6k) 17.4 -> 17.3, 256 after 7744 (128k) 145 -> 54. At 32 rows, 32 sequences
+// of a 2048-key window on 32 heads (17k) 36 -> 42.
+// Parts: as many as fill the CUs once with 16-row tiles (of at least a tile a
+// wavefront; more only add partial results: 64 sequences of ~1000 as one part
+// 44.5, two 49), twice with 128-row ones (mixed chunks and tokens of 9
+// sequences, 32 heads on 4, one part a CU 78, two 68).
+constexpr int64_t MANY_WORK = 6000;
 Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
   Plan pl;
   const int64_t G = c.n_head / pg.n_kv_head;
-  static const int eTH = getenv("PG_TH") ? atoi(getenv("PG_TH")) : 32;
-  pl.many = b.max_q * G > eTH;
-  pl.rt = !pl.many ? DR : c.type == FG_F32 ? Many<128, true, true>::RT : Many<128, false, false>::RT;
-  const int64_t per_seq = (b.max_q * G + pl.rt - 1) / pl.rt;
-  pl.ntile = (int)std::min<int64_t>(per_seq * b.n_seq, b.n_rows * G / pl.rt + b.n_seq);
-  int64_t keys = b.max_kv;
-  if (c.window > 0)  // (a tile's tokens see this many at most, and the tiles at both ends)
-    keys = std::min<int64_t>(keys, (int64_t)c.window + pl.rt / G + 1 + c.sinks + 96);
-  const int64_t nkt = (keys + 31) / 32;
-  // parts: enough workgroups for two a CU, each with a round of its
-  // wavefronts' tiles at least
-  const int64_t items = (int64_t)pl.ntile * pg.n_kv_head;
-  static const int eSP = getenv("PG_SP") ? atoi(getenv("PG_SP")) : 4, eMT = getenv("PG_MT") ? atoi(getenv("PG_MT")) : 2;
-  const int64_t want = ((pl.many ? eSP : 4) * CUS / 4 + items - 1) / items;
-  const int64_t least = pl.many ? 4 * eMT : RWV;
-  const int64_t most = (nkt + least - 1) / least;
-  const int64_t ns = std::max<int64_t>(1, std::min(want, most));
+  auto tiles = [&](int64_t rt) {
+    return std::min((b.max_q * G + rt - 1) / rt * b.n_seq, b.n_rows * G / rt + b.n_seq);
+  };
+  auto key_tiles_most = [&](int64_t rt) {
+    int64_t keys = b.max_kv;
+    if (c.window > 0)  // (a tile's tokens see this many at most, and the tiles at both ends)
+      keys = std::min<int64_t>(keys, (int64_t)c.window + rt / G + 1 + c.sinks + 96);
+    return (keys + 31) / 32;
+  };
+  pl.many = b.max_q * G > 32 && tiles(DR) * pg.n_kv_head * key_tiles_most(DR) > MANY_WORK;
+  pl.rt = pl.many ? Many<128, true, true>::RT : DR;
+  pl.ntile = (int)tiles(pl.rt);
+  const int64_t nkt = key_tiles_most(pl.rt), items = (int64_t)pl.ntile * pg.n_kv_head;
+  const int64_t want = pl.many ? (2 * CUS + items - 1) / items : CUS / items;
+  const int64_t ns = std::max<int64_t>(1, std::min(want, (nkt + RWV - 1) / RWV));
   pl.cpt = (int)((nkt + ns - 1) / ns + RWV - 1) / RWV * RWV;
-  pl.nsplit = (int)((nkt + pl.cpt - 1) / pl.cpt);
+  pl.nsplit = (int)std::max<int64_t>(1, (nkt + pl.cpt - 1) / pl.cpt);
   pl.floats = pl.nsplit > 1 ? items * pl.nsplit * pl.rt * (pg.head_dim + 2) : 0;
   return pl;
 }
