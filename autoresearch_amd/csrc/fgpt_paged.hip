@@ -106,6 +106,9 @@ int32_t check_batch(const fg_ragged* b, const fg_pages* p) {
   CHECK(b->max_kv >= 0 && b->table_ld >= 1, "batch: max_kv must be >= 0, table_ld >= 1");
   CHECK((int64_t)b->max_kv <= (int64_t)b->table_ld * p->page_size,
         "batch: max_kv %d beyond table_ld %d pages of %d", b->max_kv, b->table_ld, p->page_size);
+  // (launches of at most 2^23 workgroups)
+  CHECK((int64_t)b->n_seq * p->n_kv_head <= 1 << 22 && b->n_rows <= 1 << 23,
+        "batch: n_seq %d x %d heads above 2^22, or n_rows %d above 2^23", b->n_seq, p->n_kv_head, b->n_rows);
   CHECK(b->max_kv <= (1 << 30), "batch: max_kv %d above 2^30", b->max_kv);
   return FG_OK;
 }
@@ -114,8 +117,8 @@ int32_t check_heads(int32_t n_head, const fg_pages* p, int32_t type, const fg_ra
   CHECK(n_head >= 1 && n_head <= 1024 && n_head % p->n_kv_head == 0,
         "n_head %d is not a multiple of n_kv_head %d up to 1024", n_head, p->n_kv_head);
   CHECK(type == FG_F32 || type == FG_BF16, "unknown row type %d", type);
-  CHECK((int64_t)b->n_rows * n_head < ((int64_t)1 << 30), "batch: n_rows %d x %d heads above 2^30",
-        b->n_rows, n_head);
+  CHECK((int64_t)b->n_rows * n_head <= 1 << 26, "batch: n_rows %d x %d heads above 2^26", b->n_rows,
+        n_head);
   return FG_OK;
 }
 
@@ -243,6 +246,7 @@ extern "C" int32_t fg_draw_rows(const float* logits, int32_t rows, int32_t V, in
                                 int64_t work_bytes, void* stream) {
   CHECK(rows >= 0, "rows must be >= 0");
   CHECK(V >= 1 && V <= DRAW_MAX_V, "V %d outside 1..%d", V, DRAW_MAX_V);
+  CHECK(rows <= 1 << 21, "rows %d above 2^21", rows);
   CHECK(ld >= V && ld < ((int64_t)1 << 40), "ld %lld below V %d", (long long)ld, V);
   CHECK(cfg, "cfg is NULL");
   if (rows == 0) return FG_OK;

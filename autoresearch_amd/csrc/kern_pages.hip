@@ -11,10 +11,16 @@ namespace {
 typedef uint32_t u32x4v_t __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------ append
-// One workgroup a token row; LPH lanes a head, each with VEC dims of the
-// head's first half and the same of its second, so that a rotation pair lies in
-// one lane and every access is a 16-byte one. The mean square of a head is a
-// sum over its LPH lanes. Bound by bytes: the row once in, once out.
+// A thread keeps to one token row and LPH-th of a head: VEC dims of the head's
+// first half and the same of its second, so that a rotation pair lies in one
+// lane, every access is a 16-byte one and its cos and sin are read once; it goes
+// through the row's heads, HU of them in flight at a time. The mean square of a
+// head is a sum over its LPH lanes. A workgroup takes RW rows: four from 2048
+// rows on, where the head weights that a thread reads serve more heads (12k
+// rows of 40 bf16 heads of 128 with weights, 271 MB: 118 us with one row, 62 with
+// four; 11k of 24 heads of 64 without 25, 15), one below that (1024 rows of the
+// former shape 7.0 us, with four rows 8.6).
+// Bound by bytes: the row once in, once out.
 struct AppendArgs {
   fg_pages pg;
   fg_ragged b;
@@ -27,19 +33,31 @@ struct AppendArgs {
 template <int HD, bool F>
 struct RowIO {
   static constexpr int VEC = F ? 4 : 8, LPH = HD / 2 / VEC;
-  typedef float vals_t[VEC];
-  static __device__ __forceinline__ void load(const void* base, int64_t i, vals_t& v) {
+  static __device__ __forceinline__ uint4 load(const void* base, int64_t i) {  // VEC values
+    return *(const uint4*)((const char*)base + i * (F ? 4 : 2));
+  }
+  static __device__ __forceinline__ void values(const uint4& w, float (&v)[VEC]) {
     if constexpr (F) {
-      const float4 x = *(const float4*)((const float*)base + i);
-      v[0] = x.x;
-      v[1] = x.y;
-      v[2] = x.z;
-      v[3] = x.w;
+      v[0] = __uint_as_float(w.x);
+      v[1] = __uint_as_float(w.y);
+      v[2] = __uint_as_float(w.z);
+      v[3] = __uint_as_float(w.w);
     } else {
-      unpack8(*(const uint4*)((const uint16_t*)base + i), v);
+      unpack8(w, v);
     }
   }
 };
+
+// Sum over aligned groups of N lanes (4, 8 or 16), in each of them: quad
+// permutes, then half-row and row mirrors, which pair groups of equal values.
+template <int N>
+__device__ __forceinline__ float group_sum(float v) {
+  v += dpp_f<0xB1>(v);
+  v += dpp_f<0x4E>(v);
+  if constexpr (N >= 8) v += dpp_f<0x141>(v);
+  if constexpr (N >= 16) v += dpp_f<0x140>(v);
+  return v;
+}
 
 template <int VEC, bool F>
 __device__ __forceinline__ void store_vals(void* base, int64_t i, const float (&v)[VEC]) {
@@ -59,27 +77,39 @@ __device__ __forceinline__ void store_vals(void* base, int64_t i, const float (&
   }
 }
 
-template <int HD, bool QF, bool KF>
+template <int HD, bool QF, bool KF, int RW>
 __global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
   typedef RowIO<HD, QF> IO;
-  constexpr int VEC = IO::VEC, LPH = IO::LPH;
-  const int row = blockIdx.x, lane = threadIdx.x & 63;
-  // the row's sequence: the number of sequences that end at or before it
-  int seq = 0;
-  for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-    const bool before = s0 + lane < a.b.n_seq && a.b.q_start[s0 + lane + 1] <= row;
-    seq += __popcll(__ballot(before));
+  constexpr int VEC = IO::VEC, LPH = IO::LPH, HPT = 256 / (LPH * RW), HU = 4;  // heads at once
+  static_assert(RW <= 4, "a wavefront finds a row");
+  __shared__ int at[4][2];  // the rows' sequences and positions
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int r0 = blockIdx.x * RW;
+  if (wv < RW) {
+    // the row's sequence: the number of sequences that end at or before it
+    const int row = r0 + wv;
+    int seq = 0;
+    for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
+      const bool before = s0 + lane < a.b.n_seq && a.b.q_start[s0 + lane + 1] <= row;
+      seq += __popcll(__ballot(before));
+    }
+    if (lane == 0) {
+      const bool real = row < a.b.n_rows && seq < a.b.n_seq;  // (else padding behind the last sequence)
+      at[wv][0] = seq;
+      at[wv][1] = real ? a.b.kv_len[seq] - (a.b.q_start[seq + 1] - row) : -1;
+    }
   }
-  seq = __builtin_amdgcn_readfirstlane(seq);
-  if (seq >= a.b.n_seq) return;  // padding behind the last sequence
-  const int pos = a.b.kv_len[seq] - (a.b.q_start[seq + 1] - row);
+  __syncthreads();
+  const int slot = threadIdx.x / LPH % RW, seq = at[slot][0], pos = at[slot][1];
+  // (a whole group of LPH lanes has one row: the sums stay within it)
   if (pos < 0 || pos >= a.b.max_kv) return;
+  const int64_t row = r0 + slot;
   const int P = 1 << a.pshift;
   const int page = a.b.table[(int64_t)seq * a.b.table_ld + (pos >> a.pshift)];
   const bool kept = (uint32_t)page < (uint32_t)a.pg.n_pages;
   const int H = a.c.n_head, KH = a.pg.n_kv_head, nh = H + 2 * KH;
-  const int sub = threadIdx.x % LPH, d = sub * VEC;  // dims d.. and HD/2 + d..
-  const int64_t in0 = (int64_t)row * a.c.qkv_ld, q0 = (int64_t)row * a.c.q_ld;
+  const int d = threadIdx.x % LPH * VEC;  // dims d.. and HD/2 + d..
+  const int64_t in0 = row * a.c.qkv_ld, q0 = row * a.c.q_ld;
   float cs[VEC], sn[VEC];
   if (a.c.cos_buf) {
 #pragma unroll
@@ -93,61 +123,76 @@ __global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) cs[k] = 1.f, sn[k] = 0.f;
   }
-  // (whole groups of LPH lanes leave the loop together: the sums stay within them)
-  for (int h = threadIdx.x / LPH; h < nh; h += 256 / LPH) {
-    float x1[VEC], x2[VEC];
-    const int64_t at = in0 + (int64_t)h * HD;
-    if (a.c.interleaved) {
-      float u[VEC], w[VEC];
-      IO::load(a.qkv, at + 2 * d, u);
-      IO::load(a.qkv, at + 2 * d + VEC, w);
+  float wq[2 * VEC], wk[2 * VEC];
 #pragma unroll
-      for (int k = 0; k < VEC / 2; ++k) {
-        x1[k] = u[2 * k];
-        x2[k] = u[2 * k + 1];
-        x1[VEC / 2 + k] = w[2 * k];
-        x2[VEC / 2 + k] = w[2 * k + 1];
+  for (int k = 0; k < 2 * VEC; ++k) {
+    const int e = k < VEC ? d + k : HD / 2 + d + k - VEC;
+    wq[k] = a.c.norm && a.c.wq ? a.c.wq[e] : 1.f;
+    wk[k] = a.c.norm && a.c.wk ? a.c.wk[e] : 1.f;
+  }
+  // the two loads of a head: its halves' dims, or (interleaved) the pairs of d ..
+  // and d + VEC/2 ..
+  const int64_t l1 = a.c.interleaved ? 2 * d : d, l2 = a.c.interleaved ? 2 * d + VEC : HD / 2 + d;
+  for (int h0 = threadIdx.x / (LPH * RW); h0 < nh; h0 += HU * HPT) {
+    uint4 w1[HU], w2[HU];
+#pragma unroll
+    for (int u = 0; u < HU; ++u)
+      if (h0 + u * HPT < nh) {
+        const int64_t i = in0 + (int64_t)(h0 + u * HPT) * HD;
+        w1[u] = IO::load(a.qkv, i + l1);
+        w2[u] = IO::load(a.qkv, i + l2);
       }
-    } else {
-      IO::load(a.qkv, at + d, x1);
-      IO::load(a.qkv, at + HD / 2 + d, x2);
-    }
-    if (h < H + KH) {
-      if (a.c.norm) {
-        float ss = 0.f;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) ss += x1[k] * x1[k] + x2[k] * x2[k];
+    for (int u = 0; u < HU; ++u) {
+      const int h = h0 + u * HPT;
+      if (h >= nh) break;
+      float x1[VEC], x2[VEC];
+      if (a.c.interleaved) {
+        float s[VEC], t[VEC];
+        IO::values(w1[u], s);
+        IO::values(w2[u], t);
 #pragma unroll
-        for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor(ss, o, 64);
-        const float r = 1.0f / sqrtf(ss * (1.0f / HD) + a.c.eps);
-        const float* w = h < H ? a.c.wq : a.c.wk;
+        for (int k = 0; k < VEC / 2; ++k) {
+          x1[k] = s[2 * k];
+          x2[k] = s[2 * k + 1];
+          x1[VEC / 2 + k] = t[2 * k];
+          x2[VEC / 2 + k] = t[2 * k + 1];
+        }
+      } else {
+        IO::values(w1[u], x1);
+        IO::values(w2[u], x2);
+      }
+      if (h < H + KH) {
+        if (a.c.norm) {
+          float ss = 0.f;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          x1[k] *= r;
-          x2[k] *= r;
-          if (w) {
-            x1[k] *= w[d + k];
-            x2[k] *= w[HD / 2 + d + k];
+          for (int k = 0; k < VEC; ++k) ss += x1[k] * x1[k] + x2[k] * x2[k];
+          ss = group_sum<LPH>(ss);
+          const float r = __builtin_amdgcn_rsqf(ss * (1.0f / HD) + a.c.eps);  // (off by an ulp at most)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) {
+            x1[k] *= r * (h < H ? wq[k] : wk[k]);
+            x2[k] *= r * (h < H ? wq[VEC + k] : wk[VEC + k]);
           }
         }
-      }
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        const float u = x1[k], w = x2[k];
-        x1[k] = u * cs[k] + w * sn[k];
-        x2[k] = w * cs[k] - u * sn[k];
+        for (int k = 0; k < VEC; ++k) {
+          const float s = x1[k], t = x2[k];
+          x1[k] = s * cs[k] + t * sn[k];
+          x2[k] = t * cs[k] - s * sn[k];
+        }
       }
-    }
-    if (h < H) {
-      store_vals<VEC, QF>(a.q, q0 + (int64_t)h * HD + d, x1);
-      store_vals<VEC, QF>(a.q, q0 + (int64_t)h * HD + HD / 2 + d, x2);
-    } else if (kept) {
-      const bool key = h < H + KH;
-      const int kvh = h - H - (key ? 0 : KH);
-      void* base = key ? a.pg.k : a.pg.v;
-      const int64_t o = (((int64_t)page * KH + kvh) * P + (pos & (P - 1))) * HD + d;
-      store_vals<VEC, KF>(base, o, x1);
-      store_vals<VEC, KF>(base, o + HD / 2, x2);
+      if (h < H) {
+        store_vals<VEC, QF>(a.q, q0 + (int64_t)h * HD + d, x1);
+        store_vals<VEC, QF>(a.q, q0 + (int64_t)h * HD + HD / 2 + d, x2);
+      } else if (kept) {
+        const bool key = h < H + KH;
+        const int kvh = h - H - (key ? 0 : KH);
+        void* base = key ? a.pg.k : a.pg.v;
+        const int64_t o = (((int64_t)page * KH + kvh) * P + (pos & (P - 1))) * HD + d;
+        store_vals<VEC, KF>(base, o, x1);
+        store_vals<VEC, KF>(base, o + HD / 2, x2);
+      }
     }
   }
 }
@@ -189,17 +234,20 @@ __global__ __launch_bounds__(256) void k_take_rows(const int32_t* __restrict__ r
   for (int k = threadIdx.x; k < nq; k += 256) qo[to * nq + k] = q[from * nq + k];
 }
 
+template <int HD, bool QF, bool KF>
+void append_t(hipStream_t s, const AppendArgs& a) {
+  if (a.b.n_rows >= 2048)
+    FG_LAUNCH((k_qk_append<HD, QF, KF, 4>), dim3((unsigned)((a.b.n_rows + 3) / 4)), dim3(256), 0, s, a);
+  else
+    FG_LAUNCH((k_qk_append<HD, QF, KF, 1>), dim3((unsigned)a.b.n_rows), dim3(256), 0, s, a);
+}
+
 template <int HD>
 void append_hd(hipStream_t s, const AppendArgs& a) {
-  const dim3 grid((unsigned)a.b.n_rows), block(256);
-  if (a.pg.type == FG_F32 && a.c.type == FG_F32)
-    FG_LAUNCH((k_qk_append<HD, true, true>), grid, block, 0, s, a);
-  else if (a.c.type == FG_F32)
-    FG_LAUNCH((k_qk_append<HD, true, false>), grid, block, 0, s, a);
-  else if (a.pg.type == FG_F32)
-    FG_LAUNCH((k_qk_append<HD, false, true>), grid, block, 0, s, a);
-  else
-    FG_LAUNCH((k_qk_append<HD, false, false>), grid, block, 0, s, a);
+  if (a.pg.type == FG_F32 && a.c.type == FG_F32) append_t<HD, true, true>(s, a);
+  else if (a.c.type == FG_F32) append_t<HD, true, false>(s, a);
+  else if (a.pg.type == FG_F32) append_t<HD, false, true>(s, a);
+  else append_t<HD, false, false>(s, a);
 }
 
 }  // namespace
@@ -228,8 +276,10 @@ void launch_pages_copy(hipStream_t s, void* base, int32_t n_planes, int64_t plan
   a.page_bytes = page_bytes;
   a.n_planes = n_planes;
   a.chunks = (int)((page_bytes + COPY_CHUNK - 1) / COPY_CHUNK);
-  for (int32_t i0 = 0; i0 < n; i0 += COPY_LIST) {
-    const int m = n - i0 < COPY_LIST ? n - i0 : COPY_LIST;
+  // (a launch of at most 2^22 workgroups)
+  const int most = a.chunks > (1 << 22) / COPY_LIST ? (1 << 22) / a.chunks : COPY_LIST;
+  for (int32_t i0 = 0; i0 < n; i0 += most) {
+    const int m = n - i0 < most ? n - i0 : most;
     for (int i = 0; i < m; ++i) {
       a.src[i] = src[i0 + i];
       a.dst[i] = dst[i0 + i];

@@ -235,9 +235,21 @@ def tables(n, hd):
 @pytest.mark.parametrize("types", ["f32", "f32_kv16", "bf16", "bf16_kv32"])
 @pytest.mark.parametrize("shape,page", [("mha128", 16), ("gqa4_64", 64), ("gqa5", 256)])
 def test_append(shape, page, types, norm, interleaved):
+    check_append([(70, 70), (1, 1), (300, 17), (20, 0), (2, 3), (128, 1), (0, 0)] + [(9, 1)] * 70, shape,
+                 page, types, norm, interleaved)
+
+
+@pytest.mark.parametrize("norm", [None, "weights"])
+@pytest.mark.parametrize("types", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", ["mha128", "gqa4_64"])
+def test_append_many_rows(shape, types, norm):
+    """From 2048 rows on, four a workgroup (some of them of different sequences)."""
+    check_append([(901, 901), (2, 3), (1200, 1147), (30, 1), (31, 1), (1, 1)], shape, 32, types, norm, False)
+
+
+def check_append(seqs, shape, page, types, norm, interleaved):
     H, KH, hd = SHAPES[shape]
     qt, kt = {**TYPES, "bf16_kv32": (BF16, F32)}[types]
-    seqs = [(70, 70), (1, 1), (300, 17), (20, 0), (2, 3), (128, 1), (0, 0)] + [(9, 1)] * 70
     b = R.Batch(seqs, H, KH, hd, page, qt, kt, seed=11, pad=5)
     cos, sin = tables(b.max_kv, hd)
     w = [1 + 0.3 * b.normal(hd) for _ in range(2)] if norm == "weights" else [None, None]
@@ -250,26 +262,21 @@ def test_append(shape, page, types, norm, interleaved):
     engine.qk_append(pages_of(b), ragged_of(b), cfg, qkv.data_ptr(), out.data_ptr())
     torch.cuda.synchronize()
     q, k, v, where = R.append_rows(b, qkv, cos, sin, norm is not None, 1e-5, *w, interleaved=interleaved)
+    real = torch.tensor([p >= 0 for _, p in where], device="cuda")
+    pg = torch.tensor([int(b.table_np[s, p // page]) for s, p in where if p >= 0], device="cuda")
+    slot = torch.tensor([p % page for _, p in where if p >= 0], device="cuda")
     # fp32: a rotation adds two products of rounded factors (the norm's sum of hd
     # squares, root and quotient: hd / 2 + 4 halves of 2^-23 of x in all); bf16 adds one rounding
     for got, want, h0, dt in ((out.reshape(b.rows, H, hd), q, 0, qt), (b.k, k, H, kt), (b.v, v, H + KH, kt)):
         size = want.abs().amax(-1, keepdim=True) * 2
         tol = (hd / 2 + 8) * 2.0 ** -24 * size + (2.0 ** -8 * want.abs() if dt == BF16 else 0)
         if h0 == 0:
-            for r, (s, p) in enumerate(where):
-                if p < 0:
-                    assert (got[r] == 7.0).all()
-                else:
-                    assert ((got[r].double() - want[r]).abs() <= tol[r]).all()
+            assert ((got.double() - want).abs() <= tol)[real].all() and (got[~real] == 7.0).all()
             continue
-        seen = torch.zeros(b.n_pages, page, dtype=torch.bool)
-        for r, (s, p) in enumerate(where):
-            if p < 0:
-                continue
-            pg, slot = int(b.table_np[s, p // page]), p % page
-            seen[pg, slot] = True
-            assert ((got[pg, :, slot].double() - want[r]).abs() <= tol[r]).all()
-        assert torch.isnan(got.transpose(1, 2)[~seen.cuda()]).all()  # nothing else was written
+        assert ((got[pg, :, slot].double() - want[real]).abs() <= tol[real]).all()
+        unseen = torch.ones(b.n_pages, page, dtype=torch.bool, device="cuda")
+        unseen[pg, slot] = False
+        assert torch.isnan(got.transpose(1, 2)[unseen]).all()  # nothing else was written
 
 
 def test_append_without_rotation_and_bad_pages():

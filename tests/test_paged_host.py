@@ -56,7 +56,8 @@ BAD_PAGES = [("NULL", dict(k=0)), ("NULL", dict(v=0)), ("head_dim", dict(head_di
 BAD_BATCH = [("NULL", dict(q_start=0)), ("NULL", dict(kv_len=0)), ("NULL", dict(table=0)),
              ("n_seq", dict(n_seq=0)), ("n_rows", dict(n_rows=-1)), ("max_q", dict(max_q=-1)),
              ("max_kv", dict(max_kv=-1)), ("table_ld", dict(table_ld=0)), ("beyond", dict(max_kv=33)),
-             ("above 2\\^30", dict(n_rows=(1 << 30)))]
+             ("above 2\\^23", dict(n_rows=(1 << 23) + 1)), ("above 2\\^26", dict(n_rows=(1 << 23))),
+             ("above 2\\^22", dict(n_seq=(1 << 22)))]
 
 
 @pytest.mark.parametrize("match,kw", BAD_PAGES)
@@ -67,8 +68,8 @@ def test_bad_pages(match, kw):
 
 @pytest.mark.parametrize("match,kw", BAD_BATCH)
 def test_bad_batch(match, kw):
-    refused(match, attn, bt=batch(**kw))
-    refused(match, append, bt=batch(**kw))
+    refused(match, attn, bt=batch(**kw), n_head=16)
+    refused(match, append, bt=batch(**kw), n_head=16)
 
 
 @pytest.mark.parametrize("match,kw", [
@@ -127,7 +128,7 @@ def draw(logits=P, rows=2, V=100, ld=100, u=P, ids=P, **kw):
 
 
 @pytest.mark.parametrize("match,kw", [
-    ("rows", dict(rows=-1)), ("V 0", dict(V=0)), ("V 262145", dict(V=262145, ld=262145)), ("ld", dict(ld=99)),
+    ("rows", dict(rows=-1)), ("above 2\\^21", dict(rows=(1 << 21) + 1)), ("V 0", dict(V=0)), ("V 262145", dict(V=262145, ld=262145)), ("ld", dict(ld=99)),
     ("NULL", dict(logits=0)), ("NULL", dict(u=0)), ("NULL", dict(ids=0))])
 def test_bad_draw(match, kw):
     refused(match, draw, **kw)
