@@ -19,6 +19,8 @@
 //
 // A workgroup a row. Up to 8192 ids the row stays in registers and the time is
 // that of the chain of block-wide steps; past that it is the exponentials'.
+#include <algorithm>
+
 #include "fgpt_internal.h"
 #include "kern_common.h"
 #include "paged_internal.h"
@@ -84,7 +86,8 @@ struct Shared {
   u64 mass[BINS];
   double tab[TAB];  // 2^(j / TAB)
   place_t list_at[LIST];
-  u64 list_mass[LIST];
+  u64 list_mass[LIST], list_sum[LIST];
+  unsigned int list_rank[LIST];
   u64 red[2][DW];
   float redf[DW];
   int redi[DW];
@@ -127,23 +130,22 @@ struct Row {  // what a row's threads share
 
 __device__ __forceinline__ bool drawable(float v) { return v > -INFINITY; }  // (false for NaN)
 
-// f(v, i) for this thread's ids; HELD: from registers.
-template <bool HELD, class F>
-__device__ __forceinline__ void each(const Row& row, const float (&held)[PER], F&& f) {
+// f(v, i) for this thread's ids of [lo, hi) (lo a multiple of 64); HELD: of the
+// whole row, from registers. Past the end it sees -inf, which is never drawn.
+template <bool HELD, class F, int AHEAD = HELD ? PER : 16>
+__device__ __forceinline__ void each(const Row& row, const float (&held)[PER], int lo, int hi, F&& f) {
   if constexpr (HELD) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = k * DT + (int)threadIdx.x;
-      if (i < row.V) f(held[k], i);
+      f(held[k], k * DT + (int)threadIdx.x);
     }
   } else {
-    for (int i0 = threadIdx.x; i0 < row.V; i0 += PER * DT) {
-      float v[PER];
+    for (int i0 = lo + (int)threadIdx.x; i0 < hi; i0 += AHEAD * DT) {
+      float v[AHEAD];
 #pragma unroll
-      for (int k = 0; k < PER; ++k) v[k] = i0 + k * DT < row.V ? row.x[i0 + k * DT] : -INFINITY;
+      for (int k = 0; k < AHEAD; ++k) v[k] = i0 + k * DT < hi ? row.x[i0 + k * DT] : -INFINITY;
 #pragma unroll
-      for (int k = 0; k < PER; ++k)
-        if (i0 + k * DT < row.V) f(v[k], i0 + k * DT);
+      for (int k = 0; k < AHEAD; ++k) f(v[k], i0 + k * DT);
     }
   }
 }
@@ -164,6 +166,55 @@ __device__ void block_scan2(Shared& s, u64& a, u64& b, u64& all_a, u64& all_b) {
   all_b = lane_value(wb, 63);
 }
 
+// For entry tid of the n in the list: how many come before it in the row's order,
+// and their mass. Each entry is compared with all others, by as many threads as
+// there are for one (their shares meet in LDS).
+__device__ __forceinline__ void rank_in_list(Shared& s, unsigned n, u64& rank, u64& mass) {
+  const int tid = threadIdx.x;
+  rank = mass = 0;
+  if (n <= 64) {  // (not worth the meeting)
+    if (tid < (int)n) {
+      const place_t mine = s.list_at[tid];
+#pragma unroll 4
+      for (unsigned k = 0; k < n; ++k) {
+        const bool first = s.list_at[k] < mine;
+        rank += first ? 1 : 0;
+        mass += first ? s.list_mass[k] : 0;
+      }
+    }
+    return;
+  }
+  int n2 = 128;
+  while (n2 < (int)n) n2 <<= 1;
+  const int e = tid & (n2 - 1), part = tid / n2, parts = DT / n2;
+  if (tid < LIST) {
+    s.list_rank[tid] = 0;
+    s.list_sum[tid] = 0;
+  }
+  __syncthreads();
+  if (e < (int)n) {
+    const place_t mine = s.list_at[e];
+    unsigned r = 0;
+    u64 w = 0;
+#pragma unroll 8
+    for (unsigned k = part; k < n; k += parts) {
+      const bool first = s.list_at[k] < mine;
+      r += first ? 1 : 0;
+      w += first ? s.list_mass[k] : 0;
+    }
+    if (parts == 1) {
+      s.list_rank[e] = r;
+      s.list_sum[e] = w;
+    } else if (r) {
+      atomicAdd(&s.list_rank[e], r);
+      atomicAdd(&s.list_sum[e], w);
+    }
+  }
+  __syncthreads();
+  rank = tid < (int)n ? s.list_rank[tid] : 0;
+  mass = tid < (int)n ? s.list_sum[tid] : 0;
+}
+
 // Where, in the row's order, the counts (or masses) first reach `want` >= 1:
 // the place of that id, within the bin `b` before which `before` lies. mass_to
 // gets the bin's mass up to and with it.
@@ -177,27 +228,21 @@ __device__ place_t place_at(Shared& s, const Row& row, const float (&held)[PER],
   if (n <= LIST) {
     if (tid == 0) s.n_list = 0;
     __syncthreads();
-    each<HELD>(row, held, [&](float v, int i) {
-      if (!drawable(v) || row.bin_of(v) != b) return;
+    const float near = (float)b, far = b < BINS - 1 ? (float)(b + 1) : NAN;
+    each<HELD>(row, held, 0, row.V, [&](float v, int i) {
+      const float t = (row.m - v) * row.bin;
+      if (t < near || t >= far) return;  // (most ids; what is left is looked at again)
+      if (row.bin_of(v) != b || !drawable(v)) return;
       const int at = atomicAdd(&s.n_list, 1);
       s.list_at[at] = row.place(v, i);
       s.list_mass[at] = row.mass(v);
     });
     __syncthreads();
-    if (tid < (int)n) {
-      const place_t mine = s.list_at[tid];
-      const u64 w = s.list_mass[tid];
-      u64 rank = 0, mass = 0;
-#pragma unroll 4
-      for (unsigned k = 0; k < n; ++k) {
-        const bool first = s.list_at[k] < mine;
-        rank += first ? 1 : 0;
-        mass += first ? s.list_mass[k] : 0;
-      }
-      if (masses ? mass < left && left <= mass + w : rank == left - 1) {
-        s.found[0] = mine;
-        s.found[1] = mass + w;
-      }
+    u64 rank, mass;
+    rank_in_list(s, n, rank, mass);
+    if (tid < (int)n && (masses ? mass < left && left <= mass + s.list_mass[tid] : rank == left - 1)) {
+      s.found[0] = s.list_at[tid];
+      s.found[1] = mass + s.list_mass[tid];
     }
     __syncthreads();
     *mass_to = s.found[1];
@@ -215,7 +260,7 @@ __device__ place_t place_at(Shared& s, const Row& row, const float (&held)[PER],
     s.cnt[2 * tid] = s.cnt[2 * tid + 1] = 0;
     s.mass[2 * tid] = s.mass[2 * tid + 1] = 0;
     __syncthreads();
-    each<HELD>(row, held, [&](float v, int i) {
+    each<HELD>(row, held, 0, row.V, [&](float v, int i) {
       if (!drawable(v) || row.bin_of(v) != b) return;
       const place_t p = row.place(v, i);
       if (k > 0 && (p >> (shift + width)) != prefix) return;
@@ -245,32 +290,11 @@ __device__ place_t place_at(Shared& s, const Row& row, const float (&held)[PER],
   return prefix;
 }
 
-template <bool HELD>
-__global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
-  __shared__ Shared s;
-  extern __shared__ __attribute__((aligned(16))) u64 chunk_mass[];  // [chunks]
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, r = blockIdx.x;
-  const int chunks = (a.V + 63) / 64;
-  Row row;
-  row.x = a.x + (int64_t)r * a.ld;
-  row.V = a.V;
-  row.tab = s.tab;
-  float held[PER];
-#pragma unroll
-  for (int k = 0; k < PER; ++k) held[k] = HELD && k * DT + tid < a.V ? row.x[k * DT + tid] : -INFINITY;
-  s.tab[tid] = exp2(tid / (double)TAB);
-  s.cnt[2 * tid] = s.cnt[2 * tid + 1] = 0;
-  s.mass[2 * tid] = s.mass[2 * tid + 1] = 0;
+// ------------------------------------------------------------ the steps of a draw
 
-  // the largest logit and its first id
-  float m = -INFINITY;
-  int at = 0x7fffffff;
-  each<HELD>(row, held, [&](float v, int i) {
-    if (v > m) {
-      m = v;
-      at = i;
-    }
-  });
+// The largest of the threads' m and its first place (0x7fffffff: none).
+__device__ __forceinline__ void block_top(Shared& s, float& m, int& at) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const float wm = wave_max(m);
   at = m == wm ? at : 0x7fffffff;
 #pragma unroll
@@ -288,121 +312,194 @@ __global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
       m = s.redf[k];
       at = s.redi[k];
     }
-  const float temp = a.c.temp ? a.c.temp[r] : 1.f;
-  if (at == 0x7fffffff || temp <= 0.f) {
-    if (tid == 0) {
-      a.ids[r] = at == 0x7fffffff ? -1 : at;
-      if (a.probs) a.probs[r] = at == 0x7fffffff ? 0.f : 1.f;
+}
+
+template <bool HELD>
+__device__ __forceinline__ void top_of(const Row& row, const float (&held)[PER], int lo, int hi, float& m,
+                                       int& at) {
+  m = -INFINITY;
+  at = 0x7fffffff;
+  each<HELD>(row, held, lo, hi, [&](float v, int i) {
+    if (v > m) {
+      m = v;
+      at = i;
     }
-    return;
-  }
+  });
+}
+
+struct Settings {
+  float temp;
+  int top_k;
+  float top_p;
+  bool by_k, by_p;
+  u64 least;  // mass of an id that min_p keeps
+};
+
+__device__ __forceinline__ Settings settings_of(const DrawArgs& a, int r) {
+  Settings c;
+  c.temp = a.c.temp ? a.c.temp[r] : 1.f;
+  c.top_k = a.c.top_k ? a.c.top_k[r] : 0;
+  c.top_p = a.c.top_p ? a.c.top_p[r] : 1.f;
+  const float min_p = a.c.min_p ? a.c.min_p[r] : 0.f;
+  c.by_k = c.top_k > 0 && c.top_k < a.V;
+  c.by_p = c.top_p < 1.f;
+  c.least = min_p > 0.f ? (min_p >= 1.f ? 1ull << 44 : (u64)ceil((double)min_p * 17592186044416.0)) : 0;
+  return c;
+}
+
+// The row's units once its largest logit is known.
+__device__ __forceinline__ void scale_by(Row& row, float m, float temp) {
   const float t = temp != temp ? 1.f : temp;
   row.m = m;
   row.km = key_of(m);
   row.unit = TAB * 1.44269504088896340736 / (double)t;
   row.bin = BIN_UNITS / t;
-  const int top_k = a.c.top_k ? a.c.top_k[r] : 0;
-  const float top_p = a.c.top_p ? a.c.top_p[r] : 1.f, min_p = a.c.min_p ? a.c.min_p[r] : 0.f;
-  const bool by_k = top_k > 0 && top_k < a.V, by_p = top_p < 1.f;
+}
 
-  place_t cut = ~0ull;  // the last id kept
-  if (by_k || by_p) {
-    each<HELD>(row, held, [&](float v, int) {
-      if (!drawable(v)) return;
-      const int b = row.bin_of(v);
-      atomicAdd(&s.cnt[b], 1u);
-      if (by_p) atomicAdd(&s.mass[b], row.mass(v));
-    });
+// A row without a draw: nothing to draw from (id -1), or temp <= 0.
+__device__ __forceinline__ bool no_draw(const DrawArgs& a, int r, int at, float temp) {
+  if (at != 0x7fffffff && !(temp <= 0.f)) return false;
+  if (threadIdx.x == 0) {
+    a.ids[r] = at == 0x7fffffff ? -1 : at;
+    if (a.probs) a.probs[r] = at == 0x7fffffff ? 0.f : 1.f;
+  }
+  return true;
+}
+
+__device__ __forceinline__ void clear_bins(Shared& s) {
+  s.cnt[2 * threadIdx.x] = s.cnt[2 * threadIdx.x + 1] = 0;
+  s.mass[2 * threadIdx.x] = s.mass[2 * threadIdx.x + 1] = 0;
+}
+
+// Counts and (for top_p) masses of the ids of [lo, hi) by bin, into cleared bins.
+template <bool HELD>
+__device__ __forceinline__ void fill_bins(Shared& s, const Row& row, const float (&held)[PER], int lo, int hi,
+                                          bool by_p) {
+  each<HELD>(row, held, lo, hi, [&](float v, int) {
+    if (!drawable(v)) return;
+    const int b = row.bin_of(v);
+    atomicAdd(&s.cnt[b], 1u);
+    if (by_p) atomicAdd(&s.mass[b], row.mass(v));
+  });
+}
+
+// The mass at which top_p of `all` is reached.
+__device__ __forceinline__ u64 want_of(float top_p, u64 all) {
+  const double w = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)all);
+  return w < 1.0 ? 1ull : (u64)w;
+}
+
+// The last id that top_k and top_p keep, from the row's bins.
+template <bool HELD>
+__device__ place_t cut_of(Shared& s, const Row& row, const float (&held)[PER], const Settings& c) {
+  const int tid = threadIdx.x;
+  place_t cut = ~0ull;
+  const u64 c0 = s.cnt[2 * tid], m0 = s.mass[2 * tid];
+  u64 pc = c0 + s.cnt[2 * tid + 1], pm = m0 + s.mass[2 * tid + 1], all_c, all;
+  const u64 c1 = pc - c0, m1 = pm - m0;
+  block_scan2(s, pc, pm, all_c, all);
+  // (place_at by digits uses the bins again: the masses before them stay in pm, m0, m1)
+  auto find = [&](u64 want, u64 before, u64 w0, u64 w1) {
+    if (before < want && want <= before + w0) {
+      s.found[0] = 2 * tid;
+      s.found[1] = before;
+      s.found[2] = pm;
+    } else if (before + w0 < want && want <= before + w0 + w1) {
+      s.found[0] = 2 * tid + 1;
+      s.found[1] = before + w0;
+      s.found[2] = pm + m0;
+    }
     __syncthreads();
-    const u64 c0 = s.cnt[2 * tid], m0 = s.mass[2 * tid];
-    u64 pc = c0 + s.cnt[2 * tid + 1], pm = m0 + s.mass[2 * tid + 1], all_c, all;
-    const u64 c1 = pc - c0, m1 = pm - m0;
-    block_scan2(s, pc, pm, all_c, all);
-    // (place_at by digits uses the bins again: the masses before them stay in pm, m0, m1)
-    auto find = [&](u64 want, u64 before, u64 w0, u64 w1) {
-      if (before < want && want <= before + w0) {
-        s.found[0] = 2 * tid;
-        s.found[1] = before;
-        s.found[2] = pm;
-        s.found[3] = s.cnt[2 * tid];
-      } else if (before + w0 < want && want <= before + w0 + w1) {
-        s.found[0] = 2 * tid + 1;
-        s.found[1] = before + w0;
-        s.found[2] = pm + m0;
-      }
-      __syncthreads();
-    };
-    if (by_k && (u64)top_k < all_c) {
-      find(top_k, pc, c0, c1);
-      const u64 above = s.found[2], before = s.found[1];
-      u64 to;
-      cut = place_at<HELD>(s, row, held, false, top_k, (int)s.found[0], before, &to);
-      all = above + to;  // the mass that top_k leaves
-      __syncthreads();
-      s.cnt[2 * tid] = c0;
-      s.cnt[2 * tid + 1] = c1;
-      __syncthreads();
-    }
-    if (by_p) {
-      const double w = ceil((double)(top_p > 0.f ? top_p : 0.f) * (double)all);
-      const u64 want = w < 1.0 ? 1ull : (u64)w;
-      find(want, pm, m0, m1);
-      u64 to;
-      const place_t c2 = place_at<HELD>(s, row, held, true, want, (int)s.found[0], s.found[1], &to);
-      cut = c2 < cut ? c2 : cut;
-    }
-  }
-  const u64 least =
-      min_p > 0.f ? (min_p >= 1.f ? 1ull << 44 : (u64)ceil((double)min_p * 17592186044416.0)) : 0;
-
-  // kept mass of each chunk of 64 ids (a wavefront's ids of one k)
-  auto kept = [&](float v, int i) -> u64 {
-    if (!drawable(v) || row.place(v, i) > cut) return 0;
-    const u64 w = row.mass(v);
-    return w >= least ? w : 0;
   };
-  if constexpr (HELD) {
+  if (c.by_k && (u64)c.top_k < all_c) {
+    find(c.top_k, pc, c0, c1);
+    const u64 above = s.found[2], before = s.found[1];
+    u64 to;
+    cut = place_at<HELD>(s, row, held, false, c.top_k, (int)s.found[0], before, &to);
+    all = above + to;  // the mass that top_k leaves
+    __syncthreads();
+    s.cnt[2 * tid] = c0;
+    s.cnt[2 * tid + 1] = c1;
+    __syncthreads();
+  }
+  if (c.by_p) {
+    const u64 want = want_of(c.top_p, all);
+    find(want, pm, m0, m1);
+    u64 to;
+    const place_t c2 = place_at<HELD>(s, row, held, true, want, (int)s.found[0], s.found[1], &to);
+    cut = c2 < cut ? c2 : cut;
+  }
+  return cut;
+}
+
+// Mass of id i if it is kept.
+__device__ __forceinline__ u64 kept(const Row& row, place_t cut, u64 least, float v, int i) {
+  if (!drawable(v) || row.place(v, i) > cut) return 0;
+  const u64 w = row.mass(v);
+  return w >= least ? w : 0;
+}
+
+// Kept mass of the chunks of 64 ids in [c_lo, c_hi); returns this lane's share
+// of their sum (in lane 63).
+__device__ __forceinline__ u64 chunk_masses(const Row& row, place_t cut, u64 least, int c_lo, int c_hi,
+                                            u64* chunk_mass) {
+  constexpr int AHEAD = 16;
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  u64 all = 0;
+  for (int c0 = c_lo + wv; c0 < c_hi; c0 += AHEAD * DW) {
+    float v[AHEAD];
 #pragma unroll
-    for (int k = 0; k < PER; ++k) {
-      const int c = k * DW + wv;
-      if (c >= chunks) break;
-      const u64 sum = wave_scan(kept(held[k], k * DT + tid));
-      if (lane == 63) chunk_mass[c] = sum;
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = 64 * (c0 + k * DW) + lane;
+      v[k] = c0 + k * DW < c_hi && i < row.V ? row.x[i] : -INFINITY;
     }
-  } else {
-    for (int c0 = wv; c0 < chunks; c0 += PER * DW) {
-      float v[PER];
 #pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const int i = 64 * (c0 + k * DW) + lane;
-        v[k] = i < a.V ? row.x[i] : -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < PER; ++k) {
-        const int c = c0 + k * DW;
-        if (c >= chunks) break;
-        const u64 w = kept(v[k], 64 * c + lane);
-        const u64 sum = __any(w != 0) ? wave_scan(w) : 0;
-        if (lane == 63) chunk_mass[c] = sum;
-      }
+    for (int k = 0; k < AHEAD; ++k) {
+      const int c = c0 + k * DW;
+      if (c >= c_hi) break;
+      const u64 w = kept(row, cut, least, v[k], 64 * c + lane);
+      const u64 sum = __any(w != 0) ? wave_scan(w) : 0;
+      if (lane == 63) chunk_mass[c] = sum;
+      all += sum;
     }
   }
-  __syncthreads();
-  // the first wavefront finds the chunk, then the id
-  if (wv != 0) return;
-  const int per = (chunks + 63) / 64, q0 = lane * per;
-  u64 mine = 0;
-  for (int q = 0; q < per; ++q) mine += q0 + q < chunks ? chunk_mass[q0 + q] : 0;
-  const u64 upto = wave_scan(mine), total = lane_value(upto, 63);
+  return all;
+}
+
+// The uniform number's place in a kept mass.
+__device__ __forceinline__ u64 target_of(const DrawArgs& a, int r, u64 total) {
   const float u = a.c.u[r];
-  u64 target = (u64)((double)(u > 0.f ? (u < 1.f ? u : 1.f) : 0.f) * (double)total);
-  if (target >= total) target = total - 1;
+  const u64 t = (u64)((double)(u > 0.f ? (u < 1.f ? u : 1.f) : 0.f) * (double)total);
+  return t < total ? t : total - 1;
+}
+
+// The draw, by one wavefront: the chunk of [c_lo, c_hi) that holds `target` of
+// the kept mass (`before` of it lies in front of c_lo; WHOLE: nothing does, and
+// target and total come from the chunks), then the id.
+template <bool WHOLE>
+__device__ __forceinline__ void pick(const DrawArgs& a, int r, const Row& row, place_t cut, u64 least,
+                                     const u64* chunk_mass, int c_lo, int c_hi, u64 before, u64 target,
+                                     u64 total) {
+  const int lane = threadIdx.x & 63;
+  const int per = (c_hi - c_lo + 63) / 64, q0 = c_lo + lane * per;
+  u64 mine = 0;
+#pragma unroll 8
+  for (int q = 0; q < per; ++q) mine += q0 + q < c_hi ? chunk_mass[q0 + q] : 0;
+  const u64 upto = before + wave_scan(mine);
+  if constexpr (WHOLE) {
+    total = lane_value(upto, 63);
+    target = target_of(a, r, total);
+  }
   const int l = __builtin_ctzll(__ballot(upto > target));
-  u64 before = lane_value(upto - mine, l);
-  int c = l * per;
-  while (before + chunk_mass[c] <= target) before += chunk_mass[c++];
-  const int i = 64 * c + lane;
-  const u64 w = kept(i < a.V ? row.x[i] : -INFINITY, i);
+  before = lane_value(upto - mine, l);
+  // that lane's chunks, a lane each (64 at most)
+  const int cl = c_lo + l * per + lane;
+  const u64 cm = lane < per && cl < c_hi ? chunk_mass[cl] : 0;
+  const u64 cu = before + wave_scan(cm);
+  const int lc = __builtin_ctzll(__ballot(cu > target));
+  before = lane_value(cu - cm, lc);
+  const int i = 64 * (c_lo + l * per + lc) + lane;
+  const u64 w = kept(row, cut, least, i < a.V ? row.x[i] : -INFINITY, i);
   const u64 sum = before + wave_scan(w);
   if (lane == __builtin_ctzll(__ballot(sum > target))) {
     a.ids[r] = i;
@@ -410,21 +507,393 @@ __global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
   }
 }
 
+// ------------------------------------------------------------ a workgroup a row
+template <bool HELD>
+__global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
+  __shared__ Shared s;
+  extern __shared__ __attribute__((aligned(16))) u64 chunk_mass[];  // [chunks]
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, r = blockIdx.x;
+  const int chunks = (a.V + 63) / 64;
+  Row row;
+  row.x = a.x + (int64_t)r * a.ld;
+  row.V = a.V;
+  row.tab = s.tab;
+  float held[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) held[k] = HELD && k * DT + tid < a.V ? row.x[k * DT + tid] : -INFINITY;
+  s.tab[tid] = exp2(tid / (double)TAB);
+  clear_bins(s);
+  float m;
+  int at;
+  top_of<HELD>(row, held, 0, a.V, m, at);
+  block_top(s, m, at);
+  const Settings c = settings_of(a, r);
+  if (no_draw(a, r, at, c.temp)) return;
+  scale_by(row, m, c.temp);
+  place_t cut = ~0ull;
+  if (c.by_k || c.by_p) {
+    fill_bins<HELD>(s, row, held, 0, a.V, c.by_p);
+    __syncthreads();
+    cut = cut_of<HELD>(s, row, held, c);
+  }
+  if constexpr (HELD) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int ch = k * DW + wv;
+      if (ch >= chunks) break;
+      const u64 sum = wave_scan(kept(row, cut, c.least, held[k], k * DT + tid));
+      if (lane == 63) chunk_mass[ch] = sum;
+    }
+  } else {
+    chunk_masses(row, cut, c.least, 0, chunks, chunk_mass);
+  }
+  __syncthreads();
+  if (wv != 0) return;
+  pick<true>(a, r, row, cut, c.least, chunk_mass, 0, chunks, 0, 0, 0);
+}
+
+// ------------------------------------------------------------ rows in slices
+// Few rows of a large vocabulary leave most CUs without a row, and the
+// exponentials of a whole row (one an id for the masses of the bins, one more
+// for the chunks) to one of them. There the two passes that take them, and the
+// maximum's, run on n_slice workgroups a row, in launches of their own, and the
+// cut between them on one.
+// 48 rows of 131073 ids, top-p: 165 us with a workgroup a row, 83 so (the maximum 8, the bins 13, which
+// of them 8, their ids 10, the cut 24, the chunks 18, the draw 5).
+struct Found {  // of a row's bins
+  u64 count_before, mass_before, p_before, all;  // ahead of top_k's bin, of top_p's first; of the row
+  int bk, p1, p2;    // top_k's bin, top_p's first and last (BINS: none)
+  unsigned int n, listed;  // their ids, and how many of those the list has so far
+};
+struct SliceArgs {
+  DrawArgs a;
+  int n_slice, len;  // slices of a row (64 at most), ids of one (a multiple of 64)
+  double* tab;       // [TAB]
+  place_t* cut;      // [rows]
+  Found* found;      // [rows]
+  u64* mass;         // [rows][n_slice][BINS]
+  u64* chunk_mass;   // [rows][chunks]
+  u64* slice_mass;   // [rows][n_slice]: kept
+  unsigned int* cnt; // as mass
+  float* top;        // [rows][n_slice]
+  int32_t* top_at;
+  int32_t* list;     // [rows][LIST]: the ids that may be the cut
+};
+
+// A row as the later launches see it: its largest logit from its slices' (at:
+// its first place, 0x7fffffff for none).
+__device__ __forceinline__ Row slice_row(const SliceArgs& p, int r, const double* tab, const Settings& c,
+                                         int& at) {
+  const int lane = threadIdx.x & 63;
+  float m = lane < p.n_slice ? p.top[r * p.n_slice + lane] : -INFINITY;
+  at = lane < p.n_slice ? p.top_at[r * p.n_slice + lane] : 0x7fffffff;
+  const float wm = wave_max(m);
+  at = m == wm ? at : 0x7fffffff;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
+  Row row;
+  row.x = p.a.x + (int64_t)r * p.a.ld;
+  row.V = p.a.V;
+  row.tab = tab;
+  scale_by(row, wm, c.temp);
+  return row;
+}
+
+__global__ __launch_bounds__(DT) void k_draw_top(SliceArgs p) {
+  __shared__ Shared s;
+  const int r = blockIdx.x / p.n_slice, k = blockIdx.x % p.n_slice, lo = k * p.len;
+  Row row;
+  row.x = p.a.x + (int64_t)r * p.a.ld;
+  row.V = p.a.V;
+  const float held[PER] = {};
+  float m;
+  int at;
+  top_of<false>(row, held, lo, min(p.a.V, lo + p.len), m, at);
+  block_top(s, m, at);
+  if (threadIdx.x == 0) {
+    p.top[blockIdx.x] = m;
+    p.top_at[blockIdx.x] = at;
+  }
+  if (blockIdx.x == 0) p.tab[threadIdx.x] = exp2(threadIdx.x / (double)TAB);
+}
+
+__global__ __launch_bounds__(DT) void k_draw_bins(SliceArgs p) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, r = blockIdx.x / p.n_slice, k = blockIdx.x % p.n_slice, lo = k * p.len;
+  const Settings c = settings_of(p.a, r);
+  if (!(c.by_k || c.by_p) || c.temp <= 0.f) return;
+  s.tab[tid] = p.tab[tid];
+  clear_bins(s);
+  int at;
+  const Row row = slice_row(p, r, s.tab, c, at);
+  if (at == 0x7fffffff) return;
+  __syncthreads();
+  const float held[PER] = {};
+  fill_bins<false>(s, row, held, lo, min(p.a.V, lo + p.len), c.by_p);
+  __syncthreads();
+  const int64_t to = (int64_t)blockIdx.x * BINS + 2 * tid;
+  *(uint2*)(p.cnt + to) = make_uint2(s.cnt[2 * tid], s.cnt[2 * tid + 1]);
+  p.mass[to] = s.mass[2 * tid];
+  p.mass[to + 1] = s.mass[2 * tid + 1];
+}
+
+// The row's bins, from its slices'.
+__device__ __forceinline__ void sum_bins(const SliceArgs& p, int r, Shared& s) {
+  const int tid = threadIdx.x;
+  uint2 n = make_uint2(0, 0);
+  ulonglong2 w = make_ulonglong2(0, 0);
+#pragma unroll 8
+  for (int k = 0; k < p.n_slice; ++k) {
+    const int64_t from = (int64_t)(r * p.n_slice + k) * BINS + 2 * tid;
+    const uint2 x = *(const uint2*)(p.cnt + from);
+    const ulonglong2 y = *(const ulonglong2*)(p.mass + from);
+    n.x += x.x;
+    n.y += x.y;
+    w.x += y.x;
+    w.y += y.y;
+  }
+  s.cnt[2 * tid] = n.x;
+  s.cnt[2 * tid + 1] = n.y;
+  s.mass[2 * tid] = w.x;
+  s.mass[2 * tid + 1] = w.y;
+}
+
+// Which bins of the row can hold its cut: top_k's, and the ones that top_p's can
+// be in for any mass that top_k may leave (the ids above its bin, with none or
+// all of the bin's). Their ids are gathered by the slices; where they are more
+// than LIST, k_draw_cut goes over the row itself.
+__global__ __launch_bounds__(DT) void k_draw_find(SliceArgs p) {
+  __shared__ Shared s;
+  __shared__ u64 at[3][4];  // bin, counts before, mass before, mass with it
+  __shared__ unsigned int sum;
+  const int tid = threadIdx.x, r = blockIdx.x;
+  const Settings c = settings_of(p.a, r);
+  if (!(c.by_k || c.by_p) || c.temp <= 0.f) return;
+  sum_bins(p, r, s);
+  if (tid == 0) {
+    at[0][0] = BINS;  // (top_k takes all)
+    sum = 0;
+  }
+  __syncthreads();
+  const u64 cc[2] = {s.cnt[2 * tid], s.cnt[2 * tid + 1]}, mm[2] = {s.mass[2 * tid], s.mass[2 * tid + 1]};
+  u64 pc = cc[0] + cc[1], pm = mm[0] + mm[1], all_c, all;
+  block_scan2(s, pc, pm, all_c, all);
+  auto mark = [&](int k, bool masses, u64 want) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const u64 c0 = pc + (j ? cc[0] : 0), m0 = pm + (j ? mm[0] : 0);
+      const u64 b = masses ? m0 : c0, w = masses ? mm[j] : cc[j];
+      if (b < want && want <= b + w) {
+        at[k][0] = 2 * tid + j;
+        at[k][1] = c0;
+        at[k][2] = m0;
+        at[k][3] = m0 + mm[j];
+      }
+    }
+  };
+  const bool cut_k = c.by_k && (u64)c.top_k < all_c;
+  if (cut_k) mark(0, false, c.top_k);
+  __syncthreads();
+  const u64 low = cut_k ? at[0][2] : all, high = cut_k ? at[0][3] : all;
+  if (c.by_p) {
+    mark(1, true, want_of(c.top_p, low));
+    mark(2, true, want_of(c.top_p, high));
+  } else if (tid == 0) {
+    at[1][0] = BINS;
+    at[2][0] = 0;
+  }
+  __syncthreads();
+  const int bk = (int)at[0][0], p1 = (int)at[1][0], p2 = (int)at[2][0];
+  unsigned n = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int b = 2 * tid + j;
+    n += b == bk || (b >= p1 && b <= p2) ? (unsigned)cc[j] : 0;
+  }
+  if (n) atomicAdd(&sum, n);
+  __syncthreads();
+  if (tid == 0) {
+    Found f;
+    f.bk = bk;
+    f.p1 = p1;
+    f.p2 = p2;
+    f.count_before = cut_k ? at[0][1] : 0;
+    f.mass_before = cut_k ? at[0][2] : 0;
+    f.p_before = c.by_p ? at[1][2] : 0;
+    f.all = all;
+    f.n = sum;
+    f.listed = 0;
+    p.found[r] = f;
+  }
+}
+
+__global__ __launch_bounds__(DT) void k_draw_gather(SliceArgs p) {
+  const int r = blockIdx.x / p.n_slice, k = blockIdx.x % p.n_slice, lo = k * p.len;
+  const Settings c = settings_of(p.a, r);
+  if (!(c.by_k || c.by_p) || c.temp <= 0.f) return;
+  int at;
+  const Row row = slice_row(p, r, nullptr, c, at);
+  if (at == 0x7fffffff) return;
+  Found* f = p.found + r;
+  if (f->n > LIST) return;
+  const int bk = f->bk, p1 = f->p1, p2 = f->p2;
+  const float held[PER] = {};
+  each<false>(row, held, lo, min(p.a.V, lo + p.len), [&](float v, int i) {
+    if (!drawable(v)) return;
+    const int b = row.bin_of(v);
+    if (b == bk || (b >= p1 && b <= p2)) p.list[(int64_t)r * LIST + atomicAdd(&f->listed, 1u)] = i;
+  });
+}
+
+__global__ __launch_bounds__(DT) void k_draw_cut(SliceArgs p) {
+  __shared__ Shared s;
+  const int tid = threadIdx.x, r = blockIdx.x;
+  const Settings c = settings_of(p.a, r);
+  s.tab[tid] = p.tab[tid];
+  int at;
+  const Row row = slice_row(p, r, s.tab, c, at);
+  if (no_draw(p.a, r, at, c.temp)) return;
+  place_t cut = ~0ull;
+  if (c.by_k || c.by_p) {
+    const Found f = p.found[r];
+    if (f.n > LIST) {
+      sum_bins(p, r, s);
+      __syncthreads();
+      const float held[PER] = {};
+      cut = cut_of<false>(s, row, held, c);
+    } else {
+      __syncthreads();  // (tab)
+      int bin = -1;
+      place_t mine = 0;
+      u64 w = 0;
+      if (tid < (int)f.n) {
+        const int i = p.list[(int64_t)r * LIST + tid];
+        const float v = row.x[i];
+        bin = row.bin_of(v);
+        mine = row.place(v, i);
+        w = row.mass(v);
+        s.list_at[tid] = mine;
+      }
+      u64 all = f.all, rank, mass;
+      if (f.bk < BINS) {  // (of the list, the ids in front of its bin are not counted)
+        if (tid < (int)f.n) s.list_mass[tid] = bin == f.bk ? w : 0;
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        if (tid < (int)f.n && bin < f.bk) atomicAdd(&s.n_list, 1);
+        rank_in_list(s, f.n, rank, mass);
+        if (bin == f.bk && rank - s.n_list == (u64)c.top_k - f.count_before - 1) {
+          s.found[0] = mine;
+          s.found[1] = f.mass_before + mass + w;
+        }
+        __syncthreads();
+        cut = s.found[0];
+        all = s.found[1];
+      }
+      if (c.by_p) {
+        __syncthreads();
+        const bool in = bin >= f.p1 && bin <= f.p2;
+        if (tid < (int)f.n) s.list_mass[tid] = in ? w : 0;
+        __syncthreads();
+        rank_in_list(s, f.n, rank, mass);
+        const u64 left = want_of(c.top_p, all) - f.p_before;
+        if (in && mass < left && left <= mass + w) s.found[0] = mine;
+        __syncthreads();
+        cut = s.found[0] < cut ? s.found[0] : cut;
+      }
+    }
+  }
+  if (tid == 0) p.cut[r] = cut;
+}
+
+__global__ __launch_bounds__(DT) void k_draw_chunks(SliceArgs p) {
+  __shared__ double tab[TAB];
+  __shared__ u64 red[DW];
+  const int r = blockIdx.x / p.n_slice, k = blockIdx.x % p.n_slice;
+  const Settings c = settings_of(p.a, r);
+  tab[threadIdx.x] = p.tab[threadIdx.x];
+  int at;
+  const Row row = slice_row(p, r, tab, c, at);
+  if (at == 0x7fffffff || c.temp <= 0.f) return;
+  __syncthreads();
+  const int chunks = (p.a.V + 63) / 64, c0 = k * (p.len / 64);
+  const u64 sum = chunk_masses(row, p.cut[r], c.least, c0, min(chunks, c0 + p.len / 64),
+                               p.chunk_mass + (int64_t)r * chunks);
+  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    u64 t = 0;
+#pragma unroll
+    for (int w = 0; w < DW; ++w) t += red[w];
+    p.slice_mass[blockIdx.x] = t;
+  }
+}
+
+__global__ __launch_bounds__(64) void k_draw_pick(SliceArgs p) {
+  const int r = blockIdx.x, lane = threadIdx.x;
+  const Settings c = settings_of(p.a, r);
+  int at;
+  const Row row = slice_row(p, r, p.tab, c, at);
+  if (at == 0x7fffffff || c.temp <= 0.f) return;
+  const u64 mine = lane < p.n_slice ? p.slice_mass[r * p.n_slice + lane] : 0;
+  const u64 upto = wave_scan(mine), total = lane_value(upto, 63), target = target_of(p.a, r, total);
+  const int k = __builtin_ctzll(__ballot(upto > target));
+  const int chunks = (p.a.V + 63) / 64, c0 = k * (p.len / 64);
+  pick<false>(p.a, r, row, p.cut[r], c.least, p.chunk_mass + (int64_t)r * chunks, c0,
+              min(chunks, c0 + p.len / 64), lane_value(upto - mine, k), target, total);
+}
+
+// Slices of a row: as many of 8192 ids as its vocabulary has, while all rows
+// together have two a CU at most.
+int slices_of(int32_t rows, int32_t V) {
+  return V <= PER * DT ? 1 : std::max(1, std::min((V + PER * DT - 1) / (PER * DT), 512 / rows));
+}
+
 }  // namespace
 
-int64_t draw_work_bytes(int32_t, int32_t) { return 0; }
+int64_t draw_work_bytes(int32_t rows, int32_t V) {
+  const int64_t n = rows > 0 ? slices_of(rows, V) : 1;
+  if (n == 1) return 0;
+  return TAB * 8 + rows * (8 + (int64_t)sizeof(Found) + LIST * 4 + n * 16 + n * BINS * 12 + ((V + 63) / 64 + 1) * 8);
+}
 
 void launch_draw_rows(hipStream_t s, const float* logits, int32_t rows, int32_t V, int64_t ld,
-                      const fg_draw_cfg& c, int32_t* ids, float* probs, void*) {
+                      const fg_draw_cfg& c, int32_t* ids, float* probs, void* work) {
   const DrawArgs a{logits, V, ld, c, ids, probs};
-  const unsigned lds = (unsigned)((V + 63) / 64 * 8);
+  const int n = slices_of(rows, V), chunks = (V + 63) / 64;
+  const unsigned lds = (unsigned)chunks * 8;
   if (V <= PER * DT) {
     FG_LAUNCH((k_draw_rows<true>), dim3((unsigned)rows), dim3(DT), lds, s, a);
-  } else {
+    return;
+  }
+  if (n == 1) {
     static std::atomic<uint64_t> lds_set{0};
     raise_lds_once((const void*)k_draw_rows<false>, MAX_CHUNKS * 8, &lds_set);
     FG_LAUNCH((k_draw_rows<false>), dim3((unsigned)rows), dim3(DT), lds, s, a);
+    return;
   }
+  SliceArgs p;
+  p.a = a;
+  p.n_slice = n;
+  p.len = (chunks + n - 1) / n * 64;
+  const int64_t rn = (int64_t)rows * n;
+  p.tab = (double*)work;
+  p.mass = (u64*)(p.tab + TAB);
+  p.chunk_mass = p.mass + rn * BINS;
+  p.slice_mass = p.chunk_mass + (int64_t)rows * chunks;
+  p.cut = (place_t*)(p.slice_mass + rn);
+  p.found = (Found*)(p.cut + rows);
+  p.cnt = (unsigned int*)(p.found + rows);
+  p.list = (int32_t*)(p.cnt + rn * BINS);
+  p.top = (float*)(p.list + (int64_t)rows * LIST);
+  p.top_at = (int32_t*)(p.top + rn);
+  const dim3 all((unsigned)rn), one((unsigned)rows);
+  FG_LAUNCH(k_draw_top, all, dim3(DT), 0, s, p);
+  FG_LAUNCH(k_draw_bins, all, dim3(DT), 0, s, p);
+  FG_LAUNCH(k_draw_find, one, dim3(DT), 0, s, p);
+  FG_LAUNCH(k_draw_gather, all, dim3(DT), 0, s, p);
+  FG_LAUNCH(k_draw_cut, one, dim3(DT), 0, s, p);
+  FG_LAUNCH(k_draw_chunks, all, dim3(DT), 0, s, p);
+  FG_LAUNCH(k_draw_pick, one, dim3(64), 0, s, p);
 }
 
 }  // namespace fgpt

@@ -1,6 +1,8 @@
 // kern_pages.hip -- what fills and moves the pages of a paged KV cache:
 // k_qk_append (head norms, rotation, q out, k and v into their slots) and
 // k_pages_copy (include/fgpt.h: fg_qk_append, fg_pages_copy).
+#include <algorithm>
+
 #include "fgpt_internal.h"
 #include "kern_common.h"
 #include "paged_internal.h"
@@ -198,19 +200,23 @@ __global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
 }
 
 // ------------------------------------------------------------ page copies
-// The list travels in the kernel's arguments (COPY_LIST pairs a launch), so the
-// caller's arrays are free when the call returns and a captured launch holds
-// its own list. A workgroup copies 16 KB of one page: four 16-byte loads a
-// thread in flight before the first store. Bound by bytes.
-constexpr int COPY_LIST = 440, COPY_CHUNK = 16384;
+// The list travels in the kernel's arguments (COPY_LIST pairs a launch, or 16
+// where there are no more: less to write and to read), so the caller's arrays
+// are free when the call returns and a captured launch holds its own list. A
+// workgroup copies 16 KB of one page: four 16-byte loads a thread in flight
+// before the first store. Bound by bytes: 701 pages of 40 planes, 1.84 GB moved,
+// 368 us, 5.0 TB/s (a copy of 1 GB: 5.1).
+constexpr int COPY_LIST = 440, COPY_FEW = 16, COPY_CHUNK = 16384;
+template <int N>
 struct CopyArgs {
   char* base;
   int64_t plane_bytes, page_bytes;
-  int n_planes, chunks;  // chunks of a page
-  int32_t src[COPY_LIST], dst[COPY_LIST];
+  int chunks;  // of a page
+  int32_t src[N], dst[N];
 };
 
-__global__ __launch_bounds__(256) void k_pages_copy(CopyArgs a) {
+template <int N>
+__global__ __launch_bounds__(256) void k_pages_copy(CopyArgs<N> a) {
   const int chunk = blockIdx.x % a.chunks, i = blockIdx.x / a.chunks;
   const int64_t at = (int64_t)chunk * COPY_CHUNK + threadIdx.x * 16;
   char* plane = a.base + blockIdx.y * a.plane_bytes;
@@ -223,6 +229,21 @@ __global__ __launch_bounds__(256) void k_pages_copy(CopyArgs a) {
 #pragma unroll
   for (int k = 0; k < 4; ++k)
     if (at + k * 4096 < a.page_bytes) *(u32x4v_t*)(d + at + k * 4096) = v[k];
+}
+
+template <int N>
+void copy_list(hipStream_t s, char* base, int32_t n_planes, int64_t plane_bytes, int64_t page_bytes,
+               const int32_t* src, const int32_t* dst, int n) {
+  CopyArgs<N> a;
+  a.base = base;
+  a.plane_bytes = plane_bytes;
+  a.page_bytes = page_bytes;
+  a.chunks = (int)((page_bytes + COPY_CHUNK - 1) / COPY_CHUNK);
+  for (int i = 0; i < n; ++i) {
+    a.src[i] = src[i];
+    a.dst[i] = dst[i];
+  }
+  FG_LAUNCH((k_pages_copy<N>), dim3((unsigned)(n * a.chunks), (unsigned)n_planes), dim3(256), 0, s, a);
 }
 
 __global__ __launch_bounds__(256) void k_take_rows(const int32_t* __restrict__ rows,
@@ -270,21 +291,15 @@ void launch_take_rows(hipStream_t s, const int32_t* rows, int n, const float* x,
 
 void launch_pages_copy(hipStream_t s, void* base, int32_t n_planes, int64_t plane_bytes,
                        int64_t page_bytes, const int32_t* src, const int32_t* dst, int32_t n) {
-  CopyArgs a;
-  a.base = (char*)base;
-  a.plane_bytes = plane_bytes;
-  a.page_bytes = page_bytes;
-  a.n_planes = n_planes;
-  a.chunks = (int)((page_bytes + COPY_CHUNK - 1) / COPY_CHUNK);
-  // (a launch of at most 2^22 workgroups)
-  const int most = a.chunks > (1 << 22) / COPY_LIST ? (1 << 22) / a.chunks : COPY_LIST;
-  for (int32_t i0 = 0; i0 < n; i0 += most) {
-    const int m = n - i0 < most ? n - i0 : most;
-    for (int i = 0; i < m; ++i) {
-      a.src[i] = src[i0 + i];
-      a.dst[i] = dst[i0 + i];
-    }
-    FG_LAUNCH(k_pages_copy, dim3((unsigned)(m * a.chunks), (unsigned)n_planes), dim3(256), 0, s, a);
+  // (a launch of at most 2^22 workgroups a plane)
+  const int64_t chunks = (page_bytes + COPY_CHUNK - 1) / COPY_CHUNK;
+  const int32_t most = (int32_t)std::min<int64_t>(COPY_LIST, (1 << 22) / chunks);
+  for (int32_t i = 0; i < n; i += most) {
+    const int32_t m = std::min(most, n - i);
+    if (m <= COPY_FEW)
+      copy_list<COPY_FEW>(s, (char*)base, n_planes, plane_bytes, page_bytes, src + i, dst + i, m);
+    else
+      copy_list<COPY_LIST>(s, (char*)base, n_planes, plane_bytes, page_bytes, src + i, dst + i, m);
   }
 }
 

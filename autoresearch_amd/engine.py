@@ -182,7 +182,7 @@ def load_library(path: str = LIB_PATH):
                                      C.POINTER(i64)]),
         "fg_paged_attn": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AttnCfg), _vp,
                                 _vp, _vp, i64, _vp]),
-        "fg_pages_copy": (i32, [_vp, i32, i64, i32, i64, _i, _i, i32, _vp]),
+        "fg_pages_copy": (i32, [_vp, i32, i64, i32, i64, _vp, _vp, i32, _vp]),
         "fg_draw_rows_work": (i32, [i32, i32, C.POINTER(i64)]),
         "fg_draw_rows": (i32, [_vp, i32, i32, i64, C.POINTER(_DrawCfg), _vp, _vp, _vp, i64, _vp]),
         "fg_pool_create": (i32, [i32, i32, i32, C.POINTER(_vp)]),
@@ -748,8 +748,8 @@ def pages_copy(base: int, n_planes: int, plane_bytes: int, n_pages: int, page_by
     src, dst = _i32(src).reshape(-1), _i32(dst).reshape(-1)
     if src.size != dst.size:
         raise ValueError("src and dst must hold one page each per copy")
-    _check(load_library().fg_pages_copy(base, n_planes, plane_bytes, n_pages, page_bytes, _ip(src),
-                                        _ip(dst), src.size, stream))
+    _check(load_library().fg_pages_copy(base, n_planes, plane_bytes, n_pages, page_bytes,
+                                        src.ctypes.data, dst.ctypes.data, src.size, stream))
 
 
 def draw_rows_work(rows: int, V: int) -> int:

@@ -375,6 +375,14 @@ def test_draw(V, rows, kind):
         check_draw(x, run_draw(x, *s[:4], u=s[4]), *s)
 
 
+def test_draw_many_rows_of_many_ids():
+    """More rows than the slices are for: a workgroup a row past 8192 ids."""
+    rng = np.random.default_rng(4)
+    x = rng.normal(0, 2.5, (600, 9001)).astype(np.float32)
+    s = settings(rng, 600, 9001)
+    check_draw(x, run_draw(x, *s[:4], u=s[4]), *s)
+
+
 def test_draw_edges():
     """NaN, infinities and -0 among the logits; settings and u at and past their ends."""
     V = 300
