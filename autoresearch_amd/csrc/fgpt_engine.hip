@@ -2617,6 +2617,9 @@ extern "C" int32_t fg_paged_create(fg_model* m, int32_t n_pages, int32_t page_si
   if (flags & ~FG_KV_BF16) return seterr(FG_EARG, "unknown cache flags 0x%x", flags);
   if (window < 0 || sinks < 0 || window > (1 << 30) || sinks > (1 << 30))
     return seterr(FG_EARG, "window and sinks must be in 0..2^30");
+  // (the attention numbers a layer's rows with 32 bits)
+  if ((int64_t)n_pages * page_size * m->d.KH >= (int64_t)1 << 32)
+    return seterr(FG_EARG, "%d pages x %d positions x %d heads: 2^32 rows or more", n_pages, page_size, m->d.KH);
   GUARD(m);
   const Dims& d = m->d;
   fg_pool* pool = nullptr;

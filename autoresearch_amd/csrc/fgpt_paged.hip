@@ -38,8 +38,8 @@ int32_t err(int32_t code, const char* fmt, ...) {
 
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// Makes the stream's device the current one for the call (NULL: the current
-// device stays) and puts the caller's back afterwards.
+// Makes the stream's device the current one for the call (NULL and the runtime's
+// own streams are the current device's) and puts the caller's back afterwards.
 class OnStream {
  public:
   int32_t enter(void* stream) {
@@ -51,7 +51,8 @@ class OnStream {
     int cur = 0, dev = 0;
     hipError_t e = hipGetDevice(&cur);
     dev = cur;
-    if (e == hipSuccess && stream) e = hipStreamGetDevice((hipStream_t)stream, &dev);
+    const bool own = stream && stream != (void*)hipStreamLegacy && stream != (void*)hipStreamPerThread;
+    if (e == hipSuccess && own) e = hipStreamGetDevice((hipStream_t)stream, &dev);
     if (e == hipSuccess && dev != cur) {
       e = hipSetDevice(dev);
       if (e == hipSuccess) back_ = cur;

@@ -558,8 +558,9 @@ __global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
 // for the chunks) to one of them. There the two passes that take them, and the
 // maximum's, run on n_slice workgroups a row, in launches of their own, and the
 // cut between them on one.
-// 48 rows of 131073 ids, top-p: 165 us with a workgroup a row, 83 so (the maximum 8, the bins 13, which
-// of them 8, their ids 10, the cut 24, the chunks 18, the draw 5).
+// 48 rows of 131073 ids, top-p: 165 us with a workgroup a row, 83 so (the
+// maximum 8, the bins 13, which of them 8, their ids 10, the cut 24, the chunks
+// 18, the draw 5).
 struct Found {  // of a row's bins
   u64 count_before, mass_before, p_before, all;  // ahead of top_k's bin, of top_p's first; of the row
   int bk, p1, p2;    // top_k's bin, top_p's first and last (BINS: none)
@@ -669,6 +670,7 @@ __global__ __launch_bounds__(DT) void k_draw_find(SliceArgs p) {
   const int tid = threadIdx.x, r = blockIdx.x;
   const Settings c = settings_of(p.a, r);
   if (!(c.by_k || c.by_p) || c.temp <= 0.f) return;
+  // (a row with nothing to draw has no bins: what comes of them is not used)
   sum_bins(p, r, s);
   if (tid == 0) {
     at[0][0] = BINS;  // (top_k takes all)

@@ -433,10 +433,11 @@ int32_t fg_qk_append(const fg_pages *pages, const fg_ragged *batch, const fg_app
  * head_dim values, both fp32 or (with bf16 pages) both bf16; sums, maxima and
  * softmax are fp32. fp32 rows come out as exact as fp32 products give them
  * (operands in three bf16 terms); bf16 ones take one term of each, the
- * probabilities rounded to bf16. A sequence whose table names a page outside
- * [0, n_pages) for a position in use gives NaN rows. A NaN or infinity in a key
- * or value that no row sees changes nothing; a value row that is not finite
- * may reach earlier tokens of the same chunk.
+ * probabilities rounded to bf16. Rows that see a position whose table entry is
+ * outside [0, n_pages) are NaN, with other rows of the same call and sequence at
+ * most. A NaN or infinity in a key or value that no row of the sequence sees
+ * changes nothing; one that later tokens of a chunk see may reach its earlier
+ * ones. out may be q, with one row distance.
  * work: fg_paged_attn_work bytes of device memory (NULL when that is 0),
  * written and read within the call; two calls that may run at once, replays of
  * captured ones included, need one each. */

@@ -222,6 +222,61 @@ def test_repeats_are_equal():
     assert torch.equal(one, run_attn(b, q)) and torch.equal(one, run_attn(b, q, stream=s.cuda_stream))
 
 
+def test_two_streams_at_once():
+    """Calls on two streams with a workspace each, queued behind each other's work."""
+    bs = [R.Batch([(4000, 1), (900, 30)], 10, 2, 128, 32, F32, BF16, seed=21),
+          R.Batch([(64 + 50 * i, 1) for i in range(40)], 6, 6, 128, 16, F32, F32, seed=22)]
+    qs = []
+    for b in bs:
+        b.fill()
+        qs.append(b.normal(b.rows, b.H * b.hd))
+    alone = [run_attn(b, q) for b, q in zip(bs, qs)]
+    outs, keep = [], []
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for b, q in zip(bs, qs):
+        cfg = engine.attn_cfg(b.H)
+        n = engine.paged_attn_work(pages_of(b), ragged_of(b), cfg)
+        keep.append((cfg, n, torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")))
+        outs.append([torch.zeros(b.rows, b.H * b.hd, device="cuda") for _ in range(6)])
+    torch.cuda.synchronize()
+    for i in range(6):
+        for k, b in enumerate(bs):
+            cfg, n, work = keep[k]
+            engine.paged_attn(pages_of(b), ragged_of(b), cfg, qs[k].data_ptr(), outs[k][i].data_ptr(),
+                              work.data_ptr(), n, streams[k].cuda_stream)
+    torch.cuda.synchronize()
+    for a, o in zip(alone, outs):
+        assert all(torch.equal(a, x) for x in o)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_out_in_place(types):
+    qt, kt = TYPES[types]
+    b = R.Batch([(3000, 2), (200, 90)], 10, 2, 128, 32, qt, kt, seed=23)
+    b.fill()
+    q = b.normal(b.rows, 1280, dtype=qt)
+    want = run_attn(b, q)
+    assert torch.equal(run_attn(b, q, out=q), want)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+def test_large_batches(shape, types):
+    """Rows and keys enough for the 128-row tiles whole (no parts), part tiles
+    and wavefronts without rows among them."""
+    H, KH, hd = SHAPES[shape]
+    qt, kt = TYPES[types]
+    G = H // KH
+    b = R.Batch([(700, 700), (650, 1), (900, 300), (33, 33), (500, max(1, 100 // G)), (1, 1)], H, KH, hd, 64,
+                qt, kt, seed=24, pad=7)
+    for w, s in ((0, 0), (150, 5)):
+        b.k.fill_(NAN)
+        b.v.fill_(NAN)
+        b.fill(w, s, drop_pages=False)
+        q = b.normal(b.rows, H * hd, dtype=qt)
+        check_attn(b, q, run_attn(b, q, w, s), w, s)
+
+
 # ------------------------------------------------------------------ append
 
 def tables(n, hd):
@@ -435,3 +490,118 @@ def test_draw_defaults_and_repeats():
     n = np.ones(300)
     check_draw(x, got, n, 0 * n, n, 0 * n, u)
     assert np.array_equal(got[0], run_draw(x, u=u)[0])
+
+
+# ------------------------------------------------------------------ together
+
+def test_a_server_of_its_own():
+    """The operators as a caller's own program uses them: a pool's pages, QKV
+    rows normed, rotated and appended, attention, an id drawn from each
+    sequence's last row; prompts first, then a fork, then single tokens through
+    one captured step whose arrays change between replays."""
+    H, KH, hd, P, V, n_pages, S = 6, 2, 64, 16, 300, 60, 5
+    g = torch.Generator().manual_seed(31)
+    normal = lambda *s: torch.randn(*s, generator=g).cuda()  # noqa: E731
+    pool = engine.Pool(n_pages, P, S)
+    kv = torch.full((2, n_pages, KH, P, hd), NAN, device="cuda")
+    wq, wk = 1 + 0.2 * normal(hd), 1 + 0.2 * normal(hd)
+    head = 0.3 * normal(V, H * hd)
+    cos, sin = tables(200, hd)
+    pg = engine.pages(kv[0].data_ptr(), kv[1].data_ptr(), n_pages, P, KH, hd)
+    ap = engine.append_cfg(H, cos.data_ptr(), sin.data_ptr(), 200, norm=True, wq=wq.data_ptr(), wk=wk.data_ptr())
+    at = engine.attn_cfg(H)
+    ld, rows = 13, 128
+    dev = dict(start=torch.zeros(S + 1, dtype=torch.int32).cuda(), kv=torch.zeros(S, dtype=torch.int32).cuda(),
+               table=torch.full((S, ld), -1, dtype=torch.int32).cuda(), qkv=torch.zeros(rows, 10 * hd).cuda(),
+               q=torch.zeros(rows, H * hd).cuda(), o=torch.zeros(rows, H * hd).cuda(),
+               u=torch.zeros(S).cuda(), temp=torch.full((S,), 0.8).cuda(),
+               top_k=torch.full((S,), 40, dtype=torch.int32).cuda(), top_p=torch.full((S,), 0.95).cuda(),
+               lg=torch.zeros(S, V).cuda(), ids=torch.zeros(S, dtype=torch.int32).cuda())
+    bt = {m: engine.ragged(dev["start"].data_ptr(), dev["kv"].data_ptr(), dev["table"].data_ptr(), S, m and rows or S,
+                           m or 1, 200, ld) for m in (0, 90)}
+    work = torch.empty(max(engine.paged_attn_work(pg, b, at) for b in bt.values()) + 16, dtype=torch.uint8, device="cuda")
+    history = {s: [] for s in range(S)}  # QKV rows a sequence was given
+
+    def launch(b, last):
+        st = torch.cuda.current_stream().cuda_stream
+        engine.qk_append(pg, b, ap, dev["qkv"].data_ptr(), dev["q"].data_ptr(), st)
+        engine.paged_attn(pg, b, at, dev["q"].data_ptr(), dev["o"].data_ptr(), work.data_ptr(), work.numel(), st)
+        torch.mm(dev["o"][last], head.t(), out=dev["lg"])
+        engine.draw_rows(dev["lg"].data_ptr(), S, V, V, dev["u"].data_ptr(), dev["ids"].data_ptr(),
+                         temp=dev["temp"].data_ptr(), top_k=dev["top_k"].data_ptr(),
+                         top_p=dev["top_p"].data_ptr(), stream=st)
+
+    def put(counts):
+        """New rows for the sequences: the pool's pages, copies, the step's arrays."""
+        new = {s: normal(n, 10 * hd) for s, n in counts.items()}
+        start, copies = [0], []
+        for s in range(S):
+            n = counts.get(s, 0)
+            c = pool.extend(s, n)
+            if c:
+                copies.append(c)
+            t = pool.table(s)
+            dev["table"][s].fill_(-1)
+            dev["table"][s, :len(t)] = torch.from_numpy(t).cuda()
+            if n:
+                dev["qkv"][start[-1]:start[-1] + n] = new[s]
+                history[s] = history[s] + list(new[s])
+            start.append(start[-1] + n)
+        if copies:
+            engine.pages_copy(kv.data_ptr(), 2, kv.stride(0) * 4, n_pages, KH * P * hd * 4,
+                              [a for a, _ in copies], [b for _, b in copies])
+        dev["start"].copy_(torch.tensor(start, dtype=torch.int32))
+        dev["kv"].copy_(torch.tensor([pool.len(s) for s in range(S)], dtype=torch.int32))
+        dev["u"].copy_(torch.rand(S, generator=g))
+        return start
+
+    def check(seqs, at_row):
+        for s in seqs:
+            x = torch.stack(history[s]).double().reshape(-1, 10, hd)
+            n = len(x)
+            nrm = lambda t, w: t / torch.sqrt((t * t).mean(-1, keepdim=True) + 1e-5) * w.double()  # noqa: E731
+            def rot(t):  # noqa: E306
+                c, sn = cos[:n, None].double(), sin[:n, None].double()
+                a, b = t.chunk(2, -1)
+                return torch.cat([a * c + b * sn, b * c - a * sn], -1)
+            q, k, v = rot(nrm(x[:, :H], wq)), rot(nrm(x[:, H:H + KH], wk)), x[:, H + KH:]
+            for h in range(H):
+                p = torch.softmax((k[:, h // 3] @ q[-1, h]) / math.sqrt(hd), 0)
+                want = p @ v[:, h // 3].contiguous()
+                got = dev["o"][at_row[s], h * hd:(h + 1) * hd].double()
+                # (attention's bound with the append's roundings of q, k and v in it)
+                assert (got - want).abs().max() <= 2.0 ** -17 * v.abs().max()
+            r = R.draw_row(dev["lg"][s].cpu().numpy(), float(np.float32(0.8)), 40, float(np.float32(0.95)), 0.0,
+                           float(dev["u"][s]))
+            assert int(dev["ids"][s]) == r[0]
+
+    start = put({0: 50, 1: 7, 2: 1, 3: 33})
+    last = torch.tensor([max(0, start[s + 1] - 1) for s in range(S)], device="cuda")
+    launch(bt[90], last)
+    torch.cuda.synchronize()
+    check(range(4), last.tolist())
+    pool.fork(0, 4, 40)
+    history[4] = history[0][:40]
+    one = torch.arange(S, device="cuda")
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    put({s: 1 for s in range(S)})
+    launch(bt[0], one)  # (eager once, as a caller warms up)
+    torch.cuda.synchronize()
+    check(range(S), list(range(S)))
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        launch(bt[0], one)
+    for _ in range(20):
+        put({s: 1 for s in range(S)})
+        graph.replay()
+        torch.cuda.synchronize()
+        check(range(S), list(range(S)))
+    src, dst = (pool.trim(1), pool.trim(2), pool.compact())[2]
+    assert len(src)
+    engine.pages_copy(kv.data_ptr(), 2, kv.stride(0) * 4, n_pages, KH * P * hd * 4, src, dst)
+    history[1], history[2] = [], []
+    put({0: 1, 1: 1, 2: 1, 3: 1, 4: 1})
+    graph.replay()
+    torch.cuda.synchronize()
+    check(range(S), list(range(S)))
+    pool.close()
