@@ -787,11 +787,12 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
       top = max(top, b[kb]);
     }
     if (top + 31 > wp0 || (p.window > 0 && low <= wp1 - p.window)) {
-      asm volatile("");  // (a branch: most steps are seen whole, and the selects are not few)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {  // (of this lane's keys first + 0 .. 7 and 16 .. 23)
         const int first = b[kb] + 8 * g;
-        const int end = klim - first, from = klo - first, sink = p.sinks - first;
+        int end = klim - first, from = klo - first, sink = p.sinks - first;
+        // (keeps the compares in the branch: most steps are seen whole)
+        asm volatile("" : "+v"(end), "+v"(from), "+v"(sink));
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int x = 16 * (r >> 3) + (r & 7);
