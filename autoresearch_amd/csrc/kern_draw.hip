@@ -126,6 +126,10 @@ struct Row {  // what a row's threads share
   __device__ __forceinline__ place_t place(float v, int i) const {
     return ((place_t)(km - key_of(v)) << ID_BITS) | (uint32_t)i;
   }
+  __device__ __forceinline__ float value(place_t at) const {  // the logit at a place
+    const uint32_t k = km - (uint32_t)(at >> ID_BITS);
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+  }
 };
 
 __device__ __forceinline__ bool drawable(float v) { return v > -INFINITY; }  // (false for NaN)
@@ -164,6 +168,34 @@ __device__ void block_scan2(Shared& s, u64& a, u64& b, u64& all_a, u64& all_b) {
   b = ib - b + (wv ? lane_value(wb, wv - 1) : 0);
   all_a = lane_value(wa, 63);
   all_b = lane_value(wb, 63);
+}
+
+// The n <= LIST places of s.list_at in ascending order, entry tid of them (past
+// n: ~0): a bitonic network on as many wavefronts as they need, whose exchanges
+// across 64 entries and more go through LDS. (k_draw_cut with lists of about
+// 400: 11 us; 24 by comparing the entries with each other.)
+__device__ place_t sort_list(Shared& s, unsigned n) {
+  const int tid = threadIdx.x;
+  place_t v = tid < (int)n ? s.list_at[tid] : ~0ull;
+  int n2 = 64;
+  while (n2 < (int)n) n2 <<= 1;
+#pragma unroll 1
+  for (int k = 2; k <= n2; k <<= 1) {
+#pragma unroll 1
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      place_t o = v;
+      if (j >= 64) {
+        __syncthreads();
+        if (tid < n2) s.list_at[tid] = v;
+        __syncthreads();
+        if (tid < n2) o = s.list_at[tid ^ j];
+      } else if (tid < n2) {
+        o = __shfl_xor(v, j, 64);
+      }
+      v = (v < o) == (((tid & k) == 0) == ((tid & j) == 0)) ? v : o;
+    }
+  }
+  return v;
 }
 
 // For entry tid of the n in the list: how many come before it in the row's order,
@@ -558,9 +590,10 @@ __global__ __launch_bounds__(DT) void k_draw_rows(DrawArgs a) {
 // for the chunks) to one of them. There the two passes that take them, and the
 // maximum's, run on n_slice workgroups a row, in launches of their own, and the
 // cut between them on one.
-// 48 rows of 131073 ids, top-p: 165 us with a workgroup a row, 83 so (the
-// maximum 8, the bins 13, which of them 8, their ids 10, the cut 24, the chunks
-// 18, the draw 5).
+// 48 rows of 131073 ids, top-p: 165 us with a workgroup a row, 71 so (the
+// maximum 8, the bins 13, which of them 8, their ids 10, the cut 11, the chunks
+// 18, the draw 5). Adding up 256 ids in a lane before a wavefront's sum left the
+// chunks at 18: the masses take it, not their sums.
 struct Found {  // of a row's bins
   u64 count_before, mass_before, p_before, all;  // ahead of top_k's bin, of top_p's first; of the row
   int bk, p1, p2;    // top_k's bin, top_p's first and last (BINS: none)
@@ -764,41 +797,37 @@ __global__ __launch_bounds__(DT) void k_draw_cut(SliceArgs p) {
       const float held[PER] = {};
       cut = cut_of<false>(s, row, held, c);
     } else {
-      __syncthreads();  // (tab)
-      int bin = -1;
-      place_t mine = 0;
-      u64 w = 0;
       if (tid < (int)f.n) {
         const int i = p.list[(int64_t)r * LIST + tid];
-        const float v = row.x[i];
-        bin = row.bin_of(v);
-        mine = row.place(v, i);
-        w = row.mass(v);
-        s.list_at[tid] = mine;
+        s.list_at[tid] = row.place(row.x[i], i);
       }
-      u64 all = f.all, rank, mass;
+      if (tid == 0) s.n_list = 0;
+      __syncthreads();
+      const place_t mine = sort_list(s, f.n);
+      int bin = -1;
+      u64 w = 0, all = f.all;
+      if (tid < (int)f.n) {
+        const float v = row.value(mine);
+        bin = row.bin_of(v);
+        w = row.mass(v);
+        if (bin < f.bk && f.bk < BINS) atomicAdd(&s.n_list, 1);
+      }
+      const bool in_k = bin == f.bk, in_p = bin >= f.p1 && bin <= f.p2;
+      u64 mass_k = in_k ? w : 0, mass_p = in_p ? w : 0, all_k, all_p;
+      block_scan2(s, mass_k, mass_p, all_k, all_p);
       if (f.bk < BINS) {  // (of the list, the ids in front of its bin are not counted)
-        if (tid < (int)f.n) s.list_mass[tid] = bin == f.bk ? w : 0;
-        if (tid == 0) s.n_list = 0;
-        __syncthreads();
-        if (tid < (int)f.n && bin < f.bk) atomicAdd(&s.n_list, 1);
-        rank_in_list(s, f.n, rank, mass);
-        if (bin == f.bk && rank - s.n_list == (u64)c.top_k - f.count_before - 1) {
+        if (in_k && tid - s.n_list == (int)((u64)c.top_k - f.count_before) - 1) {
           s.found[0] = mine;
-          s.found[1] = f.mass_before + mass + w;
+          s.found[1] = f.mass_before + mass_k + w;
         }
         __syncthreads();
         cut = s.found[0];
         all = s.found[1];
+        __syncthreads();
       }
       if (c.by_p) {
-        __syncthreads();
-        const bool in = bin >= f.p1 && bin <= f.p2;
-        if (tid < (int)f.n) s.list_mass[tid] = in ? w : 0;
-        __syncthreads();
-        rank_in_list(s, f.n, rank, mass);
         const u64 left = want_of(c.top_p, all) - f.p_before;
-        if (in && mass < left && left <= mass + w) s.found[0] = mine;
+        if (in_p && mass_p < left && left <= mass_p + w) s.found[0] = mine;
         __syncthreads();
         cut = s.found[0] < cut ? s.found[0] : cut;
       }
