@@ -30,8 +30,8 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
              "-Wall", "-Wno-unused-function", "-Wno-unused-result"]
 F_SOURCES = ["fgpt_c.f90", "fgpt_drop_in.f90", "fgpt_util.f90"]
 F_PROGRAMS = ["fgpt_run.f90"]
-# check programs of the drop-in (test code, built next to their sources)
-F_CHECKS = [os.path.join(ROOT, "tests", "fortran", "dropin_checks.f90")]
+# check programs of the binding and the drop-in (test code, built next to their sources)
+F_CHECKS = [os.path.join(ROOT, "tests", "fortran", f) for f in ("dropin_checks.f90", "paged_checks.f90")]
 
 
 def _run(cmd, cwd=None):

@@ -18,7 +18,8 @@
 // the draws of a row with n likely ids.
 //
 // A workgroup a row. Up to 8192 ids the row stays in registers and the time is
-// that of the chain of block-wide steps; past that it is the exponentials'.
+// that of the chain of block-wide steps (one row 15 us, 64 of 8192 ids 16.6);
+// past that it is the exponentials'.
 #include <algorithm>
 
 #include "fgpt_internal.h"

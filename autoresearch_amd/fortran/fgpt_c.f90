@@ -36,12 +36,19 @@ module fgpt_c
     integer(c_int32_t) :: pwin, nblock, byte_space
   end type fg_sample_cfg
 
+  ! Settings of a draw, each the address of n values or null (off); u is required.
+  type, bind(C), public :: fg_draw_cfg
+    type(c_ptr) :: temp = c_null_ptr, top_k = c_null_ptr, top_p = c_null_ptr, &
+        min_p = c_null_ptr, u = c_null_ptr
+  end type fg_draw_cfg
+
   public :: fg_version, fg_last_error, fg_model_create, fg_weights_read, fg_model_load, &
       fg_model_destroy, &
       fg_set_rope, fg_forward, fg_forward_pos, fg_kv_create, fg_kv_destroy, fg_kv_len, fg_kv_set_len, &
       fg_step, fg_step_multi, fg_decode_greedy, fg_sync, fg_eval_bpb, fg_rows_npy, &
       fg_decode_spec, fg_spec_accept, fg_spec_draft, fg_sample, fg_decode_sample, fg_set_option, &
-      fg_error_message
+      fg_paged_create, fg_paged_destroy, fg_paged_len, fg_paged_free, fg_paged_fork, &
+      fg_paged_trim, fg_paged_compact, fg_paged_read, fg_paged_step, fg_error_message
 
   interface
     integer(c_int32_t) function fg_version() bind(C, name="fg_version")
@@ -232,6 +239,68 @@ module fgpt_c
       integer(c_int32_t), value :: n_steps
       integer(c_int32_t), intent(out) :: ids_out(*)
       type(c_ptr), value :: logits_out
+    end function
+
+    integer(c_int32_t) function fg_paged_create(m, n_pages, page_size, max_seq, flags, window, &
+        sinks, out) bind(C, name="fg_paged_create")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: m
+      integer(c_int32_t), value :: n_pages, page_size, max_seq, flags, window, sinks
+      type(c_ptr), intent(out) :: out
+    end function
+
+    integer(c_int32_t) function fg_paged_destroy(pc) bind(C, name="fg_paged_destroy")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+    end function
+
+    integer(c_int32_t) function fg_paged_len(pc, seq, len) bind(C, name="fg_paged_len")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+      integer(c_int32_t), value :: seq
+      integer(c_int32_t), intent(out) :: len
+    end function
+
+    integer(c_int32_t) function fg_paged_free(pc, n_pages) bind(C, name="fg_paged_free")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+      integer(c_int32_t), intent(out) :: n_pages
+    end function
+
+    integer(c_int32_t) function fg_paged_fork(pc, from, to, len) bind(C, name="fg_paged_fork")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+      integer(c_int32_t), value :: from, to, len
+    end function
+
+    integer(c_int32_t) function fg_paged_trim(pc, seq, len) bind(C, name="fg_paged_trim")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+      integer(c_int32_t), value :: seq, len
+    end function
+
+    integer(c_int32_t) function fg_paged_compact(pc, moved) bind(C, name="fg_paged_compact")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+      integer(c_int32_t), intent(out) :: moved
+    end function
+
+    ! k_out, v_out: addresses of fp32 arrays, or null
+    integer(c_int32_t) function fg_paged_read(pc, seq, k_out, v_out) bind(C, name="fg_paged_read")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: pc
+      integer(c_int32_t), value :: seq
+      type(c_ptr), value :: k_out, v_out
+    end function
+
+    ! draw: c_loc of an fg_draw_cfg, or null (argmax); logits, next_ids: addresses, or null
+    integer(c_int32_t) function fg_paged_step(m, pc, n, seqs, counts, ids, draw, logits, next_ids) &
+        bind(C, name="fg_paged_step")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: m, pc
+      integer(c_int32_t), value :: n
+      integer(c_int32_t), intent(in) :: seqs(*), counts(*), ids(*)
+      type(c_ptr), value :: draw, logits, next_ids
     end function
 
     integer(c_int32_t) function fg_sync(m) bind(C, name="fg_sync")
