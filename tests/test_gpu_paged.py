@@ -481,6 +481,35 @@ def test_draw_edges():
     check_draw(x, run_draw(x, *cols[:4], u=cols[4]), *cols)
 
 
+@pytest.mark.parametrize("V", [8193, 30000])
+@pytest.mark.parametrize("n", [1, 2, 64, 65, 128, 129, 400, 511, 512, 513, 2000])
+def test_draw_cut_among_near_equal_ids(n, V):
+    """Rows in slices whose cut lies among n ids of nearly one logit (some of
+    them equal), behind 40 likelier ones: by top_k, by top_p, by both, at the
+    first of them, at the last and between."""
+    rng = np.random.default_rng(n + V)
+    rows = 24
+    x = np.full((rows, V), -7.0, np.float32) - rng.random((rows, V)).astype(np.float32)
+    s = [np.ones(rows, np.float32), np.zeros(rows, np.int32), np.ones(rows, np.float32),
+         np.zeros(rows, np.float32), rng.random(rows).astype(np.float32)]
+    for r in range(rows):
+        ids = rng.permutation(V)
+        x[r, ids[:40]] = -0.2 * rng.random(40)
+        x[r, ids[40:40 + n]] = -1 - np.round(rng.random(n) * 0.01, 3)
+        x[r, ids[-3:]] = np.nan, -np.inf, np.nan
+        s[0][r] = (1.0, 0.6, 1.7)[r % 3]
+        e = np.where(x[r] > -np.inf, np.exp((x[r].astype(np.float64)) / s[0][r]), 0)
+        front, group = e[ids[:40]].sum(), e[ids[40:40 + n]].sum()
+        at = (0.001, 0.999, rng.random())[(r // 3) % 3]
+        if r % 4 != 1:
+            s[1][r] = 40 + max(1, round(at * n))
+        if r % 4 == 1:
+            s[2][r] = (front + at * group) / np.nansum(e)
+        elif r % 4 == 2:
+            s[2][r] = (front + 0.5 * at * group) / (front + at * group)
+    check_draw(x, run_draw(x, *s[:4], u=s[4]), *s)
+
+
 def test_draw_defaults_and_repeats():
     """Every setting absent: one draw from softmax(x); the same call gives the same ids."""
     rng = np.random.default_rng(2)
