@@ -936,9 +936,10 @@ struct Plan {
 // -> 25.5, 2048 (49k) 118 -> 74; bf16, 32 heads on 4, 8 x 8 rows after 1490
 // (6k) 17.4 -> 17.3, 256 after 7744 (128k) 145 -> 54. At 32 rows, 32 sequences
 // of a 2048-key window on 32 heads (17k) 36 -> 42.
-// Parts: as many as fill the CUs once with 16-row tiles (of at least a tile a
-// wavefront; more only add partial results: 64 sequences of ~1000 as one part
-// 44.5, two 49), twice with 128-row ones (mixed chunks and tokens of 9
+// Parts: as many as fill the CUs once with 16-row tiles (more only add partial
+// results: 64 sequences of ~1000 as one part 44.5, two 49), of at least a tile a
+// wavefront (two: one token on 6 fp32 heads after 300 positions 10.5 -> 13.7, on
+// bf16 pages after 1000 9.0 -> 10.3, after 4000 12.8 -> 12.3); twice with 128-row ones (mixed chunks and tokens of 9
 // sequences, 32 heads on 4, one part a CU 78, two 68).
 constexpr int64_t MANY_WORK = 6000;
 Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
