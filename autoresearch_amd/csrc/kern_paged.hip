@@ -192,29 +192,43 @@ __device__ __forceinline__ void split3(const float (&x)[8], bf16x8_t (&t)[3]) {
     t[k] = __builtin_bit_cast(bf16x8_t, u32x4v_t{w[k][0], w[k][1], w[k][2], w[k][3]});
 }
 
-template <bool QF>
-struct Terms {  // of q and of the probabilities
-  static constexpr int N = QF ? 3 : 1;
+// Values as the sum of N bf16 terms: three are exact, one is rounded (2^-8 of the
+// value at most), two are rounded twice (2^-16).
+template <int N>
+struct Terms {
   bf16x8_t t[N];
   __device__ __forceinline__ void set(const float (&x)[8]) {
-    if constexpr (QF) {
+    if constexpr (N == 3) {
       split3(x, t);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) t[0][e] = (__bf16)x[e];
+      for (int e = 0; e < 8; ++e) {
+        t[0][e] = (__bf16)x[e];
+        if constexpr (N == 2) t[1][e] = (__bf16)(x[e] - (float)t[0][e]);
+      }
     }
   }
 };
+// Of q and of the probabilities: fp32 rows three. bf16 rows one of q, exact, and
+// of the probabilities two in k_paged_few, which waits for memory (32 windows of
+// 2048 keys 36.3 us with one, 36.7 with two), one in k_paged_many, which its
+// matrix instructions bound (387 GF of prompts 433 us with one, 597 with two).
+// Error against 64 bits, relative: with one 0.0022, with two 0.0016, which is
+// what rounding the exact result to bf16 gives.
+template <bool QF>
+using QTerms = Terms<QF ? 3 : 1>;
+template <bool QF, bool MANY>
+using PTerms = Terms<QF ? 3 : MANY ? 1 : 2>;
 
 __device__ __forceinline__ f32x4_t mma16(const bf16x8_t& a, const bf16x8_t& b, const f32x4_t& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 // c += a . b over b's terms, smallest first.
-template <bool QF>
-__device__ __forceinline__ f32x4_t mma_terms(const bf16x8_t& a, const Terms<QF>& b, f32x4_t c) {
+template <int N>
+__device__ __forceinline__ f32x4_t mma_terms(const bf16x8_t& a, const Terms<N>& b, f32x4_t c) {
 #pragma unroll
-  for (int i = Terms<QF>::N - 1; i >= 0; --i) c = mma16(a, b.t[i], c);
+  for (int i = N - 1; i >= 0; --i) c = mma16(a, b.t[i], c);
   return c;
 }
 
@@ -268,15 +282,15 @@ struct KvTile<HD, QF, true> {
         o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(at(v[e][i / 4], i % 4), p[e], o[i], 0, 0, 0);
   }
 };
-// bf16 pages: v_mfma_f32_16x16x32_bf16, K and V exact in one term, fp32 q and
-// probabilities in three.
+// bf16 pages: v_mfma_f32_16x16x32_bf16, K and V exact in one term, q and
+// probabilities in QTerms and PTerms.
 template <int HD, bool QF>
 struct KvTile<HD, QF, false> {
   static constexpr int NS = HD / 32, VD = HD / 16;
   typedef uint16_t elem;
   static __device__ __forceinline__ int vdim(int c, int i) { return VD * c + i; }
   typedef uint32_t vrow_t __attribute__((ext_vector_type(VD / 2)));
-  Terms<QF> q[NS];
+  QTerms<QF> q[NS];
   u32x4v_t k[2][NS];
   vrow_t v[8];
   __device__ __forceinline__ void load_q(const void* base, int64_t row, int g) {
@@ -306,7 +320,7 @@ struct KvTile<HD, QF, false> {
     return sc;
   }
   __device__ __forceinline__ void add_values(const float (&p)[8], f32x4_t (&o)[VD]) const {
-    Terms<QF> pt;
+    PTerms<QF, false> pt;
     pt.set(p);
 #pragma unroll
     for (int i = 0; i < VD; ++i) {
@@ -622,13 +636,13 @@ __device__ __forceinline__ float swap_sum(float v) {
   return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
 
-template <int NA, bool QF>
-__device__ __forceinline__ f32x16_t mma32(const bf16x8_t (&a)[NA], const Terms<QF>& b, f32x16_t c) {
+template <int NA, int N>
+__device__ __forceinline__ f32x16_t mma32(const bf16x8_t (&a)[NA], const Terms<N>& b, f32x16_t c) {
 #pragma unroll
   for (int o = 2; o >= 0; --o)
 #pragma unroll
     for (int i = 0; i < NA; ++i)
-      if (o - i >= 0 && o - i < Terms<QF>::N)
+      if (o - i >= 0 && o - i < N)
         c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b.t[o - i], c, 0, 0, 0);
   return c;
 }
@@ -732,7 +746,7 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
   const bool active = w0 < t.rows;
   const int fr = t.r0 + min(w0 + c, t.rows - 1), tok = fr / p.G, h = kvh * p.G + fr % p.G;
   const int klim = t.pos0 + tok + 1, klo = p.window > 0 ? klim - p.window : 0;
-  Terms<QF> q[NS];
+  QTerms<QF> q[NS];
   {
     const int64_t at = (int64_t)(t.row0 + tok) * p.q_ld + h * HD + 8 * g;
 #pragma unroll
@@ -829,7 +843,7 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
     }
   };
   // the probabilities' operands of the four 16-key steps, and their sum
-  auto weigh = [&](const f32x16_t (&sc)[KB], Terms<QF> (&pt)[2 * KB]) __attribute__((always_inline)) {
+  auto weigh = [&](const f32x16_t (&sc)[KB], PTerms<QF, true> (&pt)[2 * KB]) __attribute__((always_inline)) {
 #pragma unroll
     for (int s4 = 0; s4 < 2 * KB; ++s4) {
       float x[8];
@@ -842,7 +856,7 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
     }
   };
   // O^T += V^T P^T from V buffer `to`
-  auto add_values = [&](uint32_t to, const Terms<QF> (&pt)[2 * KB]) __attribute__((always_inline)) {
+  auto add_values = [&](uint32_t to, const PTerms<QF, true> (&pt)[2 * KB]) __attribute__((always_inline)) {
 #pragma unroll
     for (int s4 = 0; s4 < 2 * KB; ++s4)
 #pragma unroll
@@ -879,7 +893,7 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
     f32x16_t sc[KB];
     scores(here, sc);
     settle(st, sc);
-    Terms<QF> pt[2 * KB];
+    PTerms<QF, true> pt[2 * KB];
     weigh(sc, pt);
     add_values(here, pt);
   };

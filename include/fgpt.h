@@ -432,8 +432,10 @@ int32_t fg_qk_append(const fg_pages *pages, const fg_ragged *batch, const fg_app
  * n_kv_head). A row that sees no key gives zeros. q and out are rows of n_head *
  * head_dim values, both fp32 or (with bf16 pages) both bf16; sums, maxima and
  * softmax are fp32. fp32 rows come out as exact as fp32 products give them
- * (operands in three bf16 terms); bf16 ones take one term of each, the
- * probabilities rounded to bf16. Rows that see a position whose table entry is
+ * (operands in three bf16 terms); bf16 ones are within half a bf16 step of that
+ * in launches of few rows, and in those of many take the probabilities rounded
+ * to bf16 (an error of up to 2^-8 of sum_j p_j |v_j|, like the output's own
+ * rounding). Rows that see a position whose table entry is
  * outside [0, n_pages) are NaN, with other rows of the same call and sequence at
  * most. A NaN or infinity in a key or value that no row of the sequence sees
  * changes nothing; one that later tokens of a chunk see may reach its earlier

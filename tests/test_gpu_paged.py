@@ -634,3 +634,21 @@ def test_a_server_of_its_own():
     torch.cuda.synchronize()
     check(range(S), list(range(S)))
     pool.close()
+
+
+# ------------------------------------------------------------------ precision of bf16 rows
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (600, 4)])
+@pytest.mark.parametrize("shape,page", [("gqa5", 64), ("gqa4_64", 16), ("mqa24", 32)])
+def test_few_bf16_rows_lose_the_output_rounding_alone(shape, page, window, sinks):
+    """Single tokens and short chunks: probabilities in two bf16 terms, each off
+    by half a step of what it rounds (2^-16 of a weight in all), so what is left
+    is the output's own rounding (2^-8 of it)."""
+    H, KH, hd = SHAPES[shape]
+    b = R.Batch([(900, 1), (1300, 1), (40, 1), (2500, 1), (700, 1)], H, KH, hd, page, BF16, BF16, seed=41)
+    b.fill(window, sinks)
+    q = b.normal(b.rows, H * hd, dtype=BF16, std=1.5)
+    out, mag, dot = b.attention(q, None, window, sinks)
+    got = run_attn(b, q, window, sinks).double().reshape(out.shape)
+    tol = R.attn_tolerance(out, mag, dot, hd, 2500, False) + 2.0 ** -16 * mag
+    assert ((got - out).abs() <= tol + 2.0 ** -8 * (out.abs() + tol)).all()
