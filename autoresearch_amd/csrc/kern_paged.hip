@@ -39,6 +39,7 @@ struct PagedArgs {
   int n_seq, n_rows, max_q, max_kv, table_ld, n_pages, pshift;
   int H, KH, G;
   int window, sinks;
+  bool one_tile;  // a row tile a sequence at most: tile i is sequence i's
   float cs;       // softmax scale * log2(e)
   int ntile;      // bound on the row tiles of all sequences
   int nsplit;     // key parts of a tile at most
@@ -58,7 +59,8 @@ struct RowTile {
 // Which sequence row tile `id` (of RT flattened rows) belongs to. Tiles are
 // numbered sequence after sequence; with one tile a sequence at most (decoding)
 // the number is the sequence, else the wavefront counts the sequences' tiles,
-// 64 of them a step. False: no such tile.
+// 64 of them a step. False: no such tile (a launch may have more workgroups than
+// the batch has tiles).
 template <int RT>
 __device__ __forceinline__ bool find_tile(const PagedArgs& p, int id, RowTile& t) {
   const int lane = threadIdx.x & 63;
@@ -67,7 +69,8 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& p, int id, RowTile& t
     return a < 0 ? 0 : max(0, min(min(n, p.max_q), p.n_rows - a));
   };
   int first = 0, nq;
-  if (p.max_q * p.G <= RT) {
+  if (p.one_tile) {
+    if (id >= p.n_seq) return false;
     t.seq = id;
     nq = q_of(id);
   } else {
@@ -97,7 +100,7 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& p, int id, RowTile& t
   t.seq = __builtin_amdgcn_readfirstlane(t.seq);
   first = __builtin_amdgcn_readfirstlane(first);
   nq = __builtin_amdgcn_readfirstlane(nq);
-  const int tile = p.max_q * p.G <= RT ? 0 : id - first;
+  const int tile = p.one_tile ? 0 : id - first;
   t.r0 = tile * RT;
   t.rows = min(RT, nq * p.G - t.r0);
   if (t.rows <= 0) return false;
@@ -933,6 +936,7 @@ constexpr int64_t CUS = 256;
 
 struct Plan {
   bool many;
+  bool one_tile;
   int rt;      // rows of a tile
   int ntile, nsplit, cpt;
   int64_t floats;
@@ -959,8 +963,11 @@ constexpr int64_t MANY_WORK = 6000;
 Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
   Plan pl;
   const int64_t G = c.n_head / pg.n_kv_head;
+  // (no sequence has more new tokens than there are rows, whatever the caller's
+  // bound; G of them per row stay far below 2^31)
+  const int64_t max_q = std::min(b.max_q, b.n_rows);
   auto tiles = [&](int64_t rt) {
-    return std::min((b.max_q * G + rt - 1) / rt * b.n_seq, b.n_rows * G / rt + b.n_seq);
+    return std::min((max_q * G + rt - 1) / rt * b.n_seq, b.n_rows * G / rt + b.n_seq);
   };
   auto key_tiles_most = [&](int64_t rt) {
     int64_t keys = b.max_kv;
@@ -968,8 +975,9 @@ Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
       keys = std::min<int64_t>(keys, (int64_t)c.window + rt / G + 1 + c.sinks + 96);
     return (keys + 31) / 32;
   };
-  pl.many = b.max_q * G > 32 && tiles(DR) * pg.n_kv_head * key_tiles_most(DR) > MANY_WORK;
+  pl.many = max_q * G > 32 && tiles(DR) * pg.n_kv_head * key_tiles_most(DR) > MANY_WORK;
   pl.rt = pl.many ? Many<128, true, true>::RT : DR;
+  pl.one_tile = max_q * G <= pl.rt;
   pl.ntile = (int)tiles(pl.rt);
   const int64_t nkt = key_tiles_most(pl.rt), items = (int64_t)pl.ntile * pg.n_kv_head;
   const int64_t want = pl.many ? (2 * CUS + items - 1) / items : CUS / items;
@@ -1037,7 +1045,8 @@ void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, co
   a.table = b.table;
   a.n_seq = b.n_seq;
   a.n_rows = b.n_rows;
-  a.max_q = b.max_q;
+  a.max_q = std::min(b.max_q, b.n_rows);
+  a.one_tile = pl.one_tile;
   a.max_kv = b.max_kv;
   a.table_ld = b.table_ld;
   a.n_pages = pg.n_pages;

@@ -652,3 +652,24 @@ def test_few_bf16_rows_lose_the_output_rounding_alone(shape, page, window, sinks
     got = run_attn(b, q, window, sinks).double().reshape(out.shape)
     tol = R.attn_tolerance(out, mag, dot, hd, 2500, False) + 2.0 ** -16 * mag
     assert ((got - out).abs() <= tol + 2.0 ** -8 * (out.abs() + tol)).all()
+
+
+# ------------------------------------------------------------------ loose bounds
+
+@pytest.mark.parametrize("max_q", [50, 1 << 29, (1 << 31) - 1])
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("shape", ["gqa4_64", "gqa5", "mqa24"])
+@pytest.mark.parametrize("lengths", ["tokens", "chunks", "prompts"])
+def test_bounds_above_the_lengths(lengths, shape, types, max_q):
+    """max_q and max_kv are bounds: loose ones, up to the largest that the type
+    holds, change nothing (16-row and 128-row tiles, one tile a sequence and
+    several)."""
+    H, KH, hd = SHAPES[shape]
+    qt, kt = TYPES[types]
+    b = R.Batch({"tokens": [(700, 1), (40, 1), (0, 0), (1300, 1)], "chunks": [(300, 20), (90, 1), (64, 33)],
+                 "prompts": [(900, 900), (1200, 400), (5, 1), (700, 690)]}[lengths], H, KH, hd, 32, qt, kt, seed=51,
+                pad=6, slack=77)
+    b.max_q = max(b.max_q, max_q)
+    b.fill()
+    q = b.normal(b.rows, H * hd, dtype=qt)
+    check_attn(b, q, run_attn(b, q))

@@ -161,3 +161,14 @@ def test_nothing_to_do_needs_no_device():
     append(bt=batch(n_rows=0))
     copy(src=[], dst=[])
     draw(rows=0)
+
+
+@pytest.mark.parametrize("max_q", [(1 << 31) - 1, 1 << 29, 1 << 20])
+@pytest.mark.parametrize("n_head,n_rows,n_seq", [(8, 40, 1), (16, 4, 4), (16, 4, 3), (16, 32, 1)])
+def test_a_loose_max_q_asks_for_no_more_than_the_rows(max_q, n_head, n_rows, n_seq):
+    """No sequence has more new tokens than there are rows: any larger bound is
+    that one (times the query heads of a key head it would pass 32 bits)."""
+    kw = dict(n_seq=n_seq, n_rows=n_rows, max_kv=20000, table_ld=1250)
+    cfg = engine.attn_cfg(n_head)
+    want = engine.paged_attn_work(pages(), batch(max_q=n_rows, **kw), cfg)
+    assert engine.paged_attn_work(pages(), batch(max_q=max_q, **kw), cfg) == want
