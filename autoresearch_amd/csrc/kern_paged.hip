@@ -970,7 +970,7 @@ Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
     return std::min((max_q * G + rt - 1) / rt * b.n_seq, b.n_rows * G / rt + b.n_seq);
   };
   auto key_tiles_most = [&](int64_t rt) {
-    int64_t keys = b.max_kv;
+    int64_t keys = std::max(1, b.max_kv);  // (a cache of no position still has its rows written)
     if (c.window > 0)  // (a tile's tokens see this many at most, and the tiles at both ends)
       keys = std::min<int64_t>(keys, (int64_t)c.window + rt / G + 1 + c.sinks + 96);
     return (keys + 31) / 32;

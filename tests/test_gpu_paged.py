@@ -673,3 +673,18 @@ def test_bounds_above_the_lengths(lengths, shape, types, max_q):
     b.fill()
     q = b.normal(b.rows, H * hd, dtype=qt)
     check_attn(b, q, run_attn(b, q))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_no_position_at_all(types):
+    """Rows of sequences whose cache is empty (max_kv 0): zeros, and nothing appended."""
+    qt, kt = TYPES[types]
+    b = R.Batch([(0, 3), (0, 0), (0, 40)], 4, 2, 128, 16, qt, kt, seed=52, pad=2)
+    assert b.max_kv == 0
+    got = run_attn(b, b.normal(b.rows, 4 * 128, dtype=qt))
+    assert (got[:43] == 0).all() and (got[43:] == 7.0).all()
+    out = torch.full((b.rows, 4 * 128), 7.0, dtype=qt, device="cuda")
+    qkv = b.normal(b.rows, 8 * 128, dtype=qt)
+    engine.qk_append(pages_of(b), ragged_of(b), engine.append_cfg(4, bf16=qt == BF16), qkv.data_ptr(), out.data_ptr())
+    torch.cuda.synchronize()
+    assert (out == 7.0).all() and torch.isnan(b.k).all() and torch.isnan(b.v).all()

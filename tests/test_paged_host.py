@@ -172,3 +172,11 @@ def test_a_loose_max_q_asks_for_no_more_than_the_rows(max_q, n_head, n_rows, n_s
     cfg = engine.attn_cfg(n_head)
     want = engine.paged_attn_work(pages(), batch(max_q=n_rows, **kw), cfg)
     assert engine.paged_attn_work(pages(), batch(max_q=max_q, **kw), cfg) == want
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(window=8), dict(window=8, sinks=4)])
+def test_a_cache_of_no_position(kw):
+    """max_kv 0: no key to cut into parts."""
+    for n_rows, n_seq in ((1, 1), (4, 2), (5000, 3)):
+        bt = batch(max_kv=0, n_rows=n_rows, n_seq=n_seq, max_q=n_rows)
+        assert engine.paged_attn_work(pages(), bt, engine.attn_cfg(16, **kw)) == 0
