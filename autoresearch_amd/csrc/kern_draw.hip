@@ -371,9 +371,10 @@ struct Settings {
 __device__ __forceinline__ Settings settings_of(const DrawArgs& a, int r) {
   Settings c;
   c.temp = a.c.temp ? a.c.temp[r] : 1.f;
-  c.top_k = a.c.top_k ? a.c.top_k[r] : 0;
-  c.top_p = a.c.top_p ? a.c.top_p[r] : 1.f;
   const float min_p = a.c.min_p ? a.c.min_p[r] : 0.f;
+  // (min_p above 1 keeps one id, also of several equal ones)
+  c.top_k = min_p > 1.f ? 1 : a.c.top_k ? a.c.top_k[r] : 0;
+  c.top_p = a.c.top_p ? a.c.top_p[r] : 1.f;
   c.by_k = c.top_k > 0 && c.top_k < a.V;
   c.by_p = c.top_p < 1.f;
   c.least = min_p > 0.f ? (min_p >= 1.f ? 1ull << 44 : (u64)ceil((double)min_p * 17592186044416.0)) : 0;

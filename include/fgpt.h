@@ -471,7 +471,7 @@ int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t
  * cumulative mass exceeds u times the kept mass. Settings are per row
  * (device arrays, each nullable = off; temp: 1): temp <= 0 takes the first
  * largest id; top_k <= 0, top_p >= 1 and min_p <= 0 are off; a top_p <= 0 or
- * min_p > 1 keeps the largest id alone; u below 0 counts as 0, 1 or more as the last
+ * min_p > 1 keeps the first largest id alone; u below 0 counts as 0, 1 or more as the last
  * mass; NaN settings are off (a NaN u counts as 0). NaN and -inf logits are
  * never drawn; a row of nothing else gives id -1. +inf ones share the
  * mass. probs (nullable): the drawn id's share of the kept mass. Masses are

@@ -688,3 +688,26 @@ def test_no_position_at_all(types):
     engine.qk_append(pages_of(b), ragged_of(b), engine.append_cfg(4, bf16=qt == BF16), qkv.data_ptr(), out.data_ptr())
     torch.cuda.synchronize()
     assert (out == 7.0).all() and torch.isnan(b.k).all() and torch.isnan(b.v).all()
+
+
+# ------------------------------------------------------------------ draws: min_p above 1
+
+@pytest.mark.parametrize("rows,V", [(12, 300), (12, 8192), (12, 30000), (600, 9001)])
+def test_min_p_above_one_keeps_the_first_largest_id(rows, V):
+    """Several ids at the maximum (or, at a large temp, of the same mass as it):
+    min_p 1 leaves them all, above 1 the first of the largest alone."""
+    rng = np.random.default_rng(V)
+    x = rng.normal(0, 1, (rows, V)).astype(np.float32)
+    top = np.stack([np.sort(rng.permutation(V)[:5]) for _ in range(rows)])
+    for r in range(rows):
+        x[r, top[r]] = np.inf if r % 4 == 3 else 9.0
+    n = np.ones(rows, np.float32)
+    u = ((np.arange(rows) % 10) / 10).astype(np.float32)
+    temp = np.where(np.arange(rows) % 3 == 1, 1e30, 1.0).astype(np.float32)
+    for min_p in (1.5, 5.0, np.inf, np.nextafter(np.float32(1), np.float32(2))):
+        for more in ({}, dict(top_k=0 * n + 4, top_p=0.9 * n), dict(top_p=0.99 * n)):
+            ids, probs = run_draw(x, temp=temp, min_p=min_p * n, u=u, **more)
+            assert np.array_equal(ids, top[:, 0]) and (probs == 1).all()
+    ids, probs = run_draw(x, temp=n, min_p=n, u=u)
+    assert np.array_equal(ids, top[np.arange(rows), (u * np.float32(5)).astype(int)])
+    assert np.allclose(probs, 0.2, rtol=2.0 ** -23)
