@@ -2698,16 +2698,18 @@ extern "C" int32_t fg_paged_compact(fg_paged* pc, int32_t* moved) {
   fg_model* m = pc->m;
   GUARD(m);
   try {
-    std::vector<int32_t> src((size_t)pc->n_pages), dst((size_t)pc->n_pages);
-    int32_t n = 0;
-    RCCHK(fg_pool_compact(pc->pool, src.data(), dst.data(), pc->n_pages, &n));
+    PoolMoves mv;
+    pool_plan_moves(pc->pool, &mv);
+    const int32_t n = (int32_t)mv.src.size();
     if (n > 0) {
       hipStream_t s = m->stream;
       timed(m, s, FG_K_OTHER, 0, 4.0 * m->d.L * pc->page_bytes * n, [&] {
-        launch_pages_copy(s, pc->kv, 2 * m->d.L, pc->plane_bytes, pc->page_bytes, src.data(), dst.data(), n);
+        launch_pages_copy(s, pc->kv, 2 * m->d.L, pc->plane_bytes, pc->page_bytes, mv.src.data(), mv.dst.data(), n);
       });
+      // (the sequences name their new pages only once these hold the rows)
       HIPCHK(hipGetLastError());
       HIPCHK(hipStreamSynchronize(s));
+      pool_apply_moves(pc->pool, &mv);
     }
     if (moved) *moved = n;
   } catch (const std::exception& e) {

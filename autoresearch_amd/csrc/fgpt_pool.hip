@@ -236,34 +236,42 @@ extern "C" int32_t fg_pool_slide(fg_pool* p, int32_t seq, int32_t window, int32_
   return FG_OK;
 }
 
+// The pages in use past their own number move to the free ones below it.
+void fgpt::pool_plan_moves(const fg_pool* p, PoolMoves* m) {
+  const int32_t used = p->n_pages - (int32_t)p->free_pages.size();
+  m->to.resize((size_t)p->n_pages);
+  for (int32_t i = 0; i < p->n_pages; ++i) {
+    m->to[i] = i;
+    if (i < used && p->ref[i] == 0) m->dst.push_back(i);
+    if (i >= used && p->ref[i] > 0) m->src.push_back(i);
+  }
+  for (size_t i = 0; i < m->src.size(); ++i) m->to[m->src[i]] = m->dst[i];
+  m->free_pages.reserve((size_t)p->n_pages);  // (room for every page)
+  for (int32_t i = used; i < p->n_pages; ++i) m->free_pages.push_back(i);
+}
+
+void fgpt::pool_apply_moves(fg_pool* p, PoolMoves* m) {
+  for (size_t i = 0; i < m->src.size(); ++i) {
+    p->ref[m->dst[i]] = p->ref[m->src[i]];
+    p->ref[m->src[i]] = 0;
+  }
+  for (fg_pool::Seq& s : p->seqs)
+    for (int32_t& g : s.pages)
+      if (g >= 0) g = m->to[g];
+  p->free_pages.swap(m->free_pages);
+}
+
 extern "C" int32_t fg_pool_compact(fg_pool* p, int32_t* src, int32_t* dst, int32_t cap, int32_t* n) {
   CHECK(p && n, "NULL argument");
   return entry([&] {
-    // the pages in use past their own number move to the free ones below it
-    const int32_t used = p->n_pages - (int32_t)p->free_pages.size();
-    std::vector<int32_t> low, high, to((size_t)p->n_pages);
-    for (int32_t i = 0; i < p->n_pages; ++i) {
-      to[i] = i;
-      if (i < used && p->ref[i] == 0) low.push_back(i);
-      if (i >= used && p->ref[i] > 0) high.push_back(i);
-    }
-    *n = (int32_t)high.size();
+    PoolMoves m;
+    pool_plan_moves(p, &m);
+    *n = (int32_t)m.src.size();
     if (*n == 0) return (int32_t)FG_OK;
     if (!src || !dst || cap < *n) return err(FG_EARG, "%d pages move, room for %d", *n, src && dst ? cap : 0);
-    std::vector<int32_t> free_pages;
-    free_pages.reserve((size_t)p->n_pages);
-    for (int32_t i = used; i < p->n_pages; ++i) free_pages.push_back(i);
-    for (int32_t i = 0; i < *n; ++i) {
-      src[i] = high[i];
-      dst[i] = low[i];
-      to[high[i]] = low[i];
-      p->ref[low[i]] = p->ref[high[i]];
-      p->ref[high[i]] = 0;
-    }
-    for (fg_pool::Seq& s : p->seqs)
-      for (int32_t& g : s.pages)
-        if (g >= 0) g = to[g];
-    p->free_pages.swap(free_pages);
+    std::copy(m.src.begin(), m.src.end(), src);
+    std::copy(m.dst.begin(), m.dst.end(), dst);
+    pool_apply_moves(p, &m);
     return (int32_t)FG_OK;
   });
 }

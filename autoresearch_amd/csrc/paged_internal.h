@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <vector>
+
 #include "../../include/fgpt.h"
 
 namespace fgpt {
@@ -36,6 +38,14 @@ void launch_take_rows(hipStream_t s, const int32_t* rows, int n, const float* x,
 // ---- pages
 // The last page of a pool's sequence (-1: none) and how many sequences hold it.
 int32_t pool_last_page(const fg_pool* p, int32_t seq, int32_t* holders);
+// The moves of a compaction, and their taking effect: between the two the caller
+// copies the pages, or lets the moves go when that fails.
+struct PoolMoves {
+  std::vector<int32_t> src, dst;
+  std::vector<int32_t> to, free_pages;  // each page's new place; the free ones afterwards
+};
+void pool_plan_moves(const fg_pool* p, PoolMoves* m);  // (may throw)
+void pool_apply_moves(fg_pool* p, PoolMoves* m);       // (does not)
 
 // ---- draws
 constexpr int32_t DRAW_MAX_V = 1 << 18;

@@ -537,7 +537,8 @@ int32_t fg_paged_free(const fg_paged *pc, int32_t *n_pages);
 /* fg_pool_fork and fg_pool_trim on the cache's sequences. */
 int32_t fg_paged_fork(fg_paged *pc, int32_t from, int32_t to, int32_t len);
 int32_t fg_paged_trim(fg_paged *pc, int32_t seq, int32_t len);
-/* fg_pool_compact with its copies; *moved (nullable): pages moved. */
+/* fg_pool_compact with its copies; *moved (nullable): pages moved. When a copy
+ * fails the sequences keep the pages they had. */
 int32_t fg_paged_compact(fg_paged *pc, int32_t *moved);
 /* Keys and values of a sequence, fp32 [n_layer][len][n_kv_head * head_dim]
  * (each nullable); zeros where a page was given back. */

@@ -245,3 +245,34 @@ def test_refusals(setup):
     pc.step({0: a[:1], 1: a[:1]})
     assert pc.free == 3
     pc.close()
+
+
+def hip_error_pending():
+    """Leaves an error behind as a failed HIP call of this thread does: the
+    engine's next check after a launch then finds one (the launch itself runs)."""
+    assert engine.load_library().hipSetDevice(1 << 20) != 0
+
+
+def test_a_failed_compaction_moves_nothing(setup):
+    """The sequences name the new pages only after the copies have succeeded."""
+    d, m, ex = setup
+    pc = m.paged(20, 16, 3)
+    a, b = uniform_ids(1, 60, d.vocab), uniform_ids(2, 75, d.vocab)
+    pc.step({0: a}, want_logits=False)
+    pc.step({1: b}, want_logits=False)
+    pc.trim(0)
+    before = pc.read(1)
+    hip_error_pending()
+    with pytest.raises(engine.FgptError) as e:
+        pc.compact()
+    assert e.value.code == -4 and pc.len(1) == 75 and pc.free == 20 - 5
+    for x, y in zip(before, pc.read(1)):
+        assert np.array_equal(x, y)
+    pc.step({2: a[:50]}, want_logits=False)  # (into the pages that the copies wrote to)
+    for x, y in zip(before, pc.read(1)):
+        assert np.array_equal(x, y)
+    pc.trim(2)
+    assert pc.compact() == 4
+    lg, _ = pc.step({1: a[:2]})
+    assert relerr(lg[0], ex.logits(np.concatenate([b, a[:2]]))[0][-1]) < 5e-5
+    pc.close()
