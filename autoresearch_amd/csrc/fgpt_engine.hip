@@ -2525,22 +2525,18 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   RCCHK(grow(m, &pc->work, &pc->work_bytes, wb));
 
   // from here on the sequences have their new tokens' pages
-  std::vector<int32_t> src, dst;
+  std::vector<int32_t> src, dst, who;  // copies of shared last pages, and whose
   src.reserve((size_t)n);
   dst.reserve((size_t)n);
+  who.reserve((size_t)n);
   auto H = [&](int64_t o) { return (int32_t*)(pc->h_meta + o); };
   int done = 0;
   hipStream_t s = m->stream;
-  auto copies = [&] {  // what the shared last pages held, into the sequences' own
-    if (src.empty()) return;
-    timed(m, s, FG_K_OTHER, 0, 4.0 * d.L * pc->page_bytes * src.size(), [&] {
-      launch_pages_copy(s, pc->kv, 2 * d.L, pc->plane_bytes, pc->page_bytes, src.data(), dst.data(),
-                        (int32_t)src.size());
-    });
-  };
-  auto undo = [&](int32_t rc) {  // the new tokens' positions go again
+  // the new tokens' positions go again, and (nothing copied) the copies' places
+  auto undo = [&](int32_t rc, bool copied) {
     (void)hipStreamSynchronize(s);
     for (int i = 0; i < done; ++i) (void)fg_pool_trim(pc->pool, seqs[i], len[i] - counts[i]);
+    for (size_t k = 0; !copied && k < src.size(); ++k) pool_share_again(pc->pool, who[k], src[k]);
     return rc;
   };
   memcpy(H(o_ids), ids, (size_t)rows * 4);
@@ -2548,14 +2544,12 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   for (int i = 0; i < n; ++i) {
     int32_t a = -1, c = -1;
     const int32_t rc = fg_pool_extend(pc->pool, seqs[i], counts[i], &a, &c);
-    if (rc != FG_OK) {
-      copies();
-      return undo(rc);
-    }
+    if (rc != FG_OK) return undo(rc, false);
     ++done;
     if (a >= 0) {
       src.push_back(a);
       dst.push_back(c);
+      who.push_back(seqs[i]);
     }
     H(o_start)[i] = r;
     H(o_one)[i] = i;
@@ -2583,8 +2577,15 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
     dc.min_p = (const float*)put(3, draw->min_p);
     dc.u = (const float*)put(4, draw->u);
   }
+  if (!src.empty()) {  // what the shared last pages held, into the sequences' own
+    timed(m, s, FG_K_OTHER, 0, 4.0 * d.L * pc->page_bytes * src.size(), [&] {
+      launch_pages_copy(s, pc->kv, 2 * d.L, pc->plane_bytes, pc->page_bytes, src.data(), dst.data(),
+                        (int32_t)src.size());
+    });
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return undo(seterr(FG_EHIP, "page copies: %s", hipGetErrorString(e)), false);
+  }
   auto run = [&]() -> int32_t {
-    copies();
     HIPCHK(hipMemcpyAsync(pc->meta, pc->h_meta, (size_t)at, hipMemcpyHostToDevice, s));
     paged_layers(m, pc, s, (int32_t*)(pc->meta + o_ids), b, one, (int32_t*)(pc->meta + o_last), pairs, keys);
     if (next_ids) {
@@ -2602,7 +2603,7 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
     return FG_OK;
   };
   const int32_t rc = run();
-  if (rc != FG_OK) return undo(rc);
+  if (rc != FG_OK) return undo(rc, true);
   if (pc->window > 0)
     for (int i = 0; i < n; ++i) RCCHK(fg_pool_slide(pc->pool, seqs[i], pc->window, pc->sinks));
   return FG_OK;

@@ -91,6 +91,13 @@ int32_t fgpt::pool_last_page(const fg_pool* p, int32_t seq, int32_t* holders) {
   return page;
 }
 
+void fgpt::pool_share_again(fg_pool* p, int32_t seq, int32_t from) {
+  fg_pool::Seq& s = p->seqs[seq];
+  p->give_back(s.pages.back());
+  s.pages.back() = from;
+  ++p->ref[from];
+}
+
 extern "C" int32_t fg_pool_create(int32_t n_pages, int32_t page_size, int32_t max_seq, fg_pool** out) {
   CHECK(out, "out is NULL");
   *out = nullptr;

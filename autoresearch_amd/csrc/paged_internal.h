@@ -38,6 +38,9 @@ void launch_take_rows(hipStream_t s, const int32_t* rows, int n, const float* x,
 // ---- pages
 // The last page of a pool's sequence (-1: none) and how many sequences hold it.
 int32_t pool_last_page(const fg_pool* p, int32_t seq, int32_t* holders);
+// The sequence shares page `from` again, which others hold, in the place of its
+// last one (what fg_pool_extend changed, once its tokens are trimmed).
+void pool_share_again(fg_pool* p, int32_t seq, int32_t from);
 // The moves of a compaction, and their taking effect: between the two the caller
 // copies the pages, or lets the moves go when that fails.
 struct PoolMoves {

@@ -276,3 +276,31 @@ def test_a_failed_compaction_moves_nothing(setup):
     lg, _ = pc.step({1: a[:2]})
     assert relerr(lg[0], ex.logits(np.concatenate([b, a[:2]]))[0][-1]) < 5e-5
     pc.close()
+
+
+def test_a_step_whose_page_copies_fail_changes_nothing(setup):
+    """Forks that go on from one partly filled page share it as before."""
+    d, m, ex = setup
+    pc = m.paged(20, 16, 4)
+    a = uniform_ids(1, 70, d.vocab)
+    pc.step({0: a}, want_logits=False)
+    pc.fork(0, 1, 70)
+    pc.fork(0, 2, 67)
+    before, free = [pc.read(s) for s in range(3)], pc.free
+    for _ in range(2):
+        hip_error_pending()
+        with pytest.raises(engine.FgptError) as e:
+            pc.step({0: a[:2], 1: a[:20], 2: a[:1]})
+        assert e.value.code == -4 and [pc.len(s) for s in range(4)] == [70, 70, 67, 0] and pc.free == free
+    pc.step({3: a[:free * 16]}, want_logits=False)  # (into the pages that were given out and back)
+    for s in range(3):
+        for x, y in zip(before[s], pc.read(s)):
+            assert np.array_equal(x, y)
+    pc.trim(3)
+    lg, _ = pc.step({0: a[:2], 1: a[:20], 2: a[:1]})
+    for s, (n, k) in enumerate(((70, 2), (70, 20), (67, 1))):
+        assert relerr(lg[s], ex.logits(np.concatenate([a[:n], a[:k]]))[0][-1]) < 5e-5
+    for s in range(3):
+        pc.trim(s)
+    assert pc.free == 20
+    pc.close()
