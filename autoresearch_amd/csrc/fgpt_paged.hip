@@ -146,6 +146,36 @@ int32_t check_attn(const fg_pages* pages, const fg_ragged* batch, const fg_attn_
   return FG_OK;
 }
 
+// The pages that a copy list has named, by hash: room for those alone, whatever
+// the pool holds; on the stack up to SMALL pairs.
+class Named {
+ public:
+  static constexpr int32_t SMALL = 64;
+  explicit Named(int32_t n) {  // (may throw)
+    while ((int64_t)1 << bits_ < 4 * (int64_t)n) ++bits_;
+    if (n > SMALL) many_.assign((size_t)1 << bits_, 0);
+    at_ = n > SMALL ? many_.data() : few_;
+  }
+  // 0: not named yet; else how (1 read, 2 written). It is named `how` from now on.
+  int name(int32_t page, int how) {
+    uint64_t& e = slot(page);
+    const int was = (int)(e & 3);
+    e = ((uint64_t)page << 2) | (uint64_t)how;
+    return was;
+  }
+
+ private:
+  uint64_t& slot(int32_t page) {
+    uint64_t i = ((uint64_t)page * 0x9E3779B97F4A7C15ull) >> (64 - bits_);
+    while (at_[i] && (at_[i] >> 2) != (uint64_t)page) i = (i + 1) & (((uint64_t)1 << bits_) - 1);
+    return at_[i];
+  }
+  int bits_ = 4;
+  uint64_t few_[4 * SMALL] = {};  // page << 2 | how; 0: free
+  std::vector<uint64_t> many_;
+  uint64_t* at_;
+};
+
 }  // namespace
 
 // ------------------------------------------------------------ attention
@@ -215,14 +245,13 @@ extern "C" int32_t fg_pages_copy(void* base, int32_t n_planes, int64_t plane_byt
   CHECK(base && src && dst, "NULL argument");
   CHECK(aligned(base), "base is not 16-byte aligned");
   try {
-    std::vector<uint8_t> used((size_t)n_pages, 0);  // 1: read, 2: written
+    CHECK(n <= n_pages, "%d copies among %d pages", n, n_pages);  // (some page would be written twice)
+    Named pages(n);
     for (int32_t i = 0; i < n; ++i) {
       CHECK(src[i] >= 0 && src[i] < n_pages && dst[i] >= 0 && dst[i] < n_pages,
             "copy %d: page %d -> %d outside [0, %d)", i, src[i], dst[i], n_pages);
-      CHECK(!used[dst[i]], "copy %d: page %d is named before", i, dst[i]);
-      used[dst[i]] = 2;
-      CHECK(used[src[i]] != 2, "copy %d: page %d is also written", i, src[i]);
-      used[src[i]] = 1;
+      CHECK(!pages.name(dst[i], 2), "copy %d: page %d is named before", i, dst[i]);
+      CHECK(pages.name(src[i], 1) != 2, "copy %d: page %d is also written", i, src[i]);
     }
   } catch (const std::exception& e) {
     return err(FG_EARG, "page list: %s", e.what());

@@ -458,7 +458,8 @@ int32_t fg_paged_attn(const fg_pages *pages, const fg_ragged *batch, const fg_at
 /* Page src[i] copied to page dst[i] in each of n_planes arrays of n_pages pages
  * (plane_bytes apart; a cache's layers, keys and values), i < n. src and dst
  * are host arrays, read before the call returns; no page may be named twice in
- * dst nor stand in both. page_bytes a multiple of 16. */
+ * dst nor stand in both. page_bytes a multiple of 16. (The check of more than 64
+ * pairs takes some host memory for the time of the call.) */
 int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t n_pages,
                       int64_t page_bytes, const int32_t *src, const int32_t *dst, int32_t n,
                       void *stream);

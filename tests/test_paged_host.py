@@ -1,6 +1,8 @@
 """Refusals of the paged cache's operators, on the CPU: arguments are checked
 before anything asks for a device, and nothing runs without one."""
 import ctypes as C
+import random
+import resource
 
 import pytest
 
@@ -180,3 +182,46 @@ def test_a_cache_of_no_position(kw):
     for n_rows, n_seq in ((1, 1), (4, 2), (5000, 3)):
         bt = batch(max_kv=0, n_rows=n_rows, n_seq=n_seq, max_q=n_rows)
         assert engine.paged_attn_work(pages(), bt, engine.attn_cfg(16, **kw)) == 0
+
+
+def copy_code(src, dst, **kw):
+    with pytest.raises(engine.FgptError) as e:
+        copy(src, dst, **kw)
+    return e.value.code
+
+
+@pytest.mark.skipif(not no_gpu(), reason="a GPU is visible")
+@pytest.mark.parametrize("seed", range(30))
+def test_copy_lists_against_their_definition(seed):
+    """No page twice in dst, none in both; a source may serve several copies."""
+    r = random.Random(seed)
+    for _ in range(40):
+        n = r.choice([1, 2, 15, 63, 64, 65, 300, 1000])
+        n_pages = r.choice([2 * n, 2 * n + 7, 1 << 20, (1 << 31) - 1])
+        pick = r.sample(range(n_pages), 2 * n)
+        src, dst = pick[:n], pick[n:]
+        i, j = r.randrange(n), r.randrange(n)
+        what = r.choice(["good", "shared", "twice", "both"])
+        if what == "shared":
+            src[i] = src[j]
+        elif what == "twice":
+            dst[i] = dst[j]
+        elif what == "both":
+            src[i] = dst[j]
+        good = len(set(dst)) == n and not set(src) & set(dst)
+        assert copy_code(src, dst, planes=1, n_pages=n_pages, page_bytes=16) == (-7 if good else -1), what
+
+
+@pytest.mark.skipif(not no_gpu(), reason="a GPU is visible")
+def test_a_short_copy_list_costs_nothing_of_a_large_pool():
+    """One page of a pool of 2^31 - 1: no memory for each page of it (the check
+    comes to asking for a device under a limit of 256 MB more than now)."""
+    with open("/proc/self/statm") as f:
+        now = int(f.read().split()[0]) * resource.getpagesize()
+    old = resource.getrlimit(resource.RLIMIT_AS)
+    resource.setrlimit(resource.RLIMIT_AS, (now + (256 << 20), old[1]))
+    try:
+        code = copy_code([5], [(1 << 31) - 2], planes=1, n_pages=(1 << 31) - 1, page_bytes=16)
+    finally:
+        resource.setrlimit(resource.RLIMIT_AS, old)
+    assert code == -7
