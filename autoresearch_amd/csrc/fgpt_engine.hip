@@ -2360,13 +2360,33 @@ int32_t grow(fg_model* m, char** p, int64_t* have, int64_t need) {
 
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
+// What a step's attention has to do: (query, key) pairs of all tokens, of the
+// sequences' last ones alone, and the distinct keys that each of the two sees.
+struct Seen {
+  int64_t pairs = 0, last = 0, keys = 0;  // (a last token's pairs are its keys)
+  // Sum over positions p < n of the keys that p sees.
+  static int64_t upto(int64_t n, int64_t window, int64_t sinks) {
+    auto triangle = [](int64_t k) { return k * (k + 1) / 2; };
+    if (window <= 0 || n <= window) return triangle(n);
+    const int64_t past = n - window, s = std::min(past, sinks);  // positions with keys behind their window
+    return triangle(window) + past * window + triangle(s) + (past - s) * sinks;
+  }
+  void add(int64_t len, int64_t count, int64_t window, int64_t sinks) {
+    const int64_t first = len - count;
+    pairs += upto(len, window, sinks) - upto(first, window, sinks);
+    last += upto(len, window, sinks) - upto(len - 1, window, sinks);
+    const int64_t lo = window > 0 ? std::max<int64_t>(0, first - window + 1) : 0;
+    keys += len - lo + std::min(lo, sinks);
+  }
+};
+
 // The pass of fg_paged_step: rows token rows of the batch b (device arrays) at
 // m->ws.ids; logits of the n sequences' last rows to m->ws.logits. Where there
 // are more rows than sequences, the last layer goes on with the last tokens
 // alone from its attention on (batch one: one new token a sequence, whose row is
 // last_rows[i]).
 void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, const fg_ragged& b,
-                  const fg_ragged& one, const int32_t* last_rows, int64_t pairs, int64_t keys) {
+                  const fg_ragged& one, const int32_t* last_rows, const Seen& see) {
   const Dims& d = m->d;
   Work& ws = m->ws;
   int rows = b.n_rows;
@@ -2417,9 +2437,9 @@ void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, 
       out.planes = ws.aos;
       out.plane = prow * d.qd();
     }
-    const double seen = cut ? keys : pairs;
-    timed(m, s, b.max_q > 1 && !cut ? FG_K_ATTN_CHUNK : FG_K_ATTN_DECODE, 4.0 * d.hd * d.H * seen,
-          8.0 * rows * d.qd() + 2 * ekv * keys * d.kvd(), [&] {
+    timed(m, s, b.max_q > 1 && !cut ? FG_K_ATTN_CHUNK : FG_K_ATTN_DECODE,
+          4.0 * d.hd * d.H * (cut ? see.last : see.pairs),
+          8.0 * rows * d.qd() + 2 * ekv * (cut ? see.last : see.keys) * d.kvd(), [&] {
             launch_paged_attn(s, pg, cut ? one : b, at, q, out, (float*)pc->work);
           });
     // x += attn_out Wproj^T; h = relu(rmsnorm(x) Wfc^T)^2; x += h Wproj2^T
@@ -2452,7 +2472,8 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   std::vector<uint8_t> named((size_t)pc->max_seq, 0);
   std::vector<int32_t> len((size_t)n);
   std::map<int32_t, int> shared;  // copies that a shared last page still takes
-  int64_t rows = 0, need = 0, pairs = 0, keys = 0;
+  int64_t rows = 0, need = 0;
+  Seen see;
   int max_q = 0, max_kv = 0;
   for (int i = 0; i < n; ++i) {
     if (seqs[i] < 0 || seqs[i] >= pc->max_seq)
@@ -2474,8 +2495,7 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
     len[i] += counts[i];
     need += pages;
     rows += counts[i];
-    pairs += (int64_t)counts[i] * (len[i] - counts[i]) + (int64_t)counts[i] * (counts[i] + 1) / 2;
-    keys += len[i];
+    see.add(len[i], counts[i], pc->window, pc->sinks);
     max_q = std::max(max_q, counts[i]);
     max_kv = std::max(max_kv, len[i]);
   }
@@ -2587,7 +2607,7 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   }
   auto run = [&]() -> int32_t {
     HIPCHK(hipMemcpyAsync(pc->meta, pc->h_meta, (size_t)at, hipMemcpyHostToDevice, s));
-    paged_layers(m, pc, s, (int32_t*)(pc->meta + o_ids), b, one, (int32_t*)(pc->meta + o_last), pairs, keys);
+    paged_layers(m, pc, s, (int32_t*)(pc->meta + o_ids), b, one, (int32_t*)(pc->meta + o_last), see);
     if (next_ids) {
       timed(m, s, FG_K_OTHER, 0, 4.0 * n * d.V, [&] {
         if (draw)

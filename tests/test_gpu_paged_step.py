@@ -304,3 +304,38 @@ def test_a_step_whose_page_copies_fail_changes_nothing(setup):
         pc.trim(s)
     assert pc.free == 20
     pc.close()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3), (64, 70), (1, 0), (399, 4)])
+@pytest.mark.parametrize("bf16", [False, True], ids=["f32", "bf16"])
+def test_timed_attention_counts_what_its_rows_see(setup, window, sinks, bf16):
+    """fg_timing's operations and bytes of the attention: pairs of a query and a
+    key that it sees, and each visible key and value once."""
+    d, m, _ = setup
+    pc = m.paged(80, 16, 4, bf16=bf16, window=window, sinks=sinks)
+
+    def seen(T, n):
+        p, j = np.arange(T - n, T)[:, None], np.arange(T)[None, :]
+        return (j <= p) & ((j > p - window) | (j < sinks) if window else True)
+
+    lens = {}
+    for counts in ({0: 150, 1: 3, 2: 64}, {0: 1, 1: 1, 2: 1}, {1: 90, 0: 2, 3: 20}):
+        m.timing(True)
+        pc.step({s: uniform_ids(s, n, d.vocab) for s, n in counts.items()}, want_logits=False)
+        got = m.timing_read()
+        m.timing(False)
+        for s, n in counts.items():
+            lens[s] = lens.get(s, 0) + n
+        rows, cut = sum(counts.values()), sum(counts.values()) > len(counts)
+        want = {"attn_chunk": [0, 0.0, 0.0], "attn_decode": [0, 0.0, 0.0]}
+        for layer in range(d.n_layer):
+            last = cut and layer == d.n_layer - 1
+            see = [seen(lens[s], 1 if last else n) for s, n in counts.items()]
+            w = want["attn_chunk" if cut and not last else "attn_decode"]
+            w[0] += 1
+            w[1] += 4.0 * d.head_dim * d.n_head * sum(int(x.sum()) for x in see)
+            w[2] += 8.0 * (len(counts) if last else rows) * d.n_head * d.head_dim \
+                + 2 * (2 if bf16 else 4) * d.n_kv_head * d.head_dim * sum(int(x.any(0).sum()) for x in see)
+        for kind, w in want.items():
+            assert (got[kind][0], got[kind][2], got[kind][3]) == tuple(w), kind
+    pc.close()
