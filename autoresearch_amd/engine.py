@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import weakref
 
 import numpy as np
 
@@ -251,6 +252,7 @@ class Model:
         L = load_library()
         self.d = d
         self._h = _vp()
+        self._caches = weakref.WeakSet()  # its KV and Paged, which must not outlive it
         cd = _cdims(d)
         if weights_dir is not None:
             _check(L.fg_model_load(C.byref(cd), weights_dir.encode(), C.byref(self._h)))
@@ -259,7 +261,10 @@ class Model:
             _check(L.fg_model_create(C.byref(cd), *[_fp(b) for b in bufs], C.byref(self._h)))
 
     def close(self):
+        """Frees the model, its caches first."""
         if self._h:
+            for c in list(self._caches):
+                c.close()
             _LIB.fg_model_destroy(self._h)
             self._h = _vp()
 
@@ -423,11 +428,12 @@ class KV:
         self._h = _vp()
         _check(_LIB.fg_kv_create_ex(m.handle, B, maxT, FG_KV_BF16 if bf16 else 0,
                                     C.byref(self._h)))
+        m._caches.add(self)
 
     def close(self):
-        if self._h:
+        if self._h and self.m.handle:  # (a model collected together with it may be gone)
             _LIB.fg_kv_destroy(self._h)
-            self._h = _vp()
+        self._h = _vp()
 
     def __del__(self):
         try:
@@ -514,11 +520,12 @@ class Paged:
         self._h = _vp()
         _check(_LIB.fg_paged_create(m.handle, n_pages, page_size, max_seq, FG_KV_BF16 if bf16 else 0,
                                     window, sinks, C.byref(self._h)))
+        m._caches.add(self)
 
     def close(self):
-        if self._h:
+        if self._h and self.m.handle:  # (a model collected together with it may be gone)
             _LIB.fg_paged_destroy(self._h)
-            self._h = _vp()
+        self._h = _vp()
 
     def __del__(self):
         try:

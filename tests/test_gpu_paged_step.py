@@ -339,3 +339,20 @@ def test_timed_attention_counts_what_its_rows_see(setup, window, sinks, bf16):
         for kind, w in want.items():
             assert (got[kind][0], got[kind][2], got[kind][3]) == tuple(w), kind
     pc.close()
+
+
+def test_a_model_that_is_closed_first():
+    """Its caches go with it; closing them afterwards, or calling them, is no fault."""
+    m = engine.Model(MHA64, stacks=seeded_weights(MHA64, 5))
+    c, s = rope_tables(MAX, MHA64.head_dim)
+    m.set_rope(c.reshape(-1), s.reshape(-1))
+    pc, kv = m.paged(10, 16, 2), m.kv(1, 64)
+    pc.step({0: [1, 2]})
+    m.close()
+    for call in (lambda: pc.step({0: [3]}), lambda: pc.len(0), pc.compact, lambda: kv.len):
+        with pytest.raises(engine.FgptError) as e:
+            call()
+        assert e.value.code == -1
+    pc.close()
+    kv.close()
+    m.close()
