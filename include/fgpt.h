@@ -438,8 +438,10 @@ int32_t fg_qk_append(const fg_pages *pages, const fg_ragged *batch, const fg_app
  * rounding). Rows that see a position whose table entry is
  * outside [0, n_pages) are NaN, with other rows of the same call and sequence at
  * most. A NaN or infinity in a key or value that no row of the sequence sees
- * changes nothing; one that later tokens of a chunk see may reach its earlier
- * ones. out may be q, with one row distance.
+ * changes nothing. A row that sees one is what the formula gives or NaN, which
+ * of the two by the kernel that the bounds select (a term of zero times an
+ * infinity); where other tokens of the same call and sequence see one, earlier or
+ * (past a window) later ones, a row that does not may be NaN too. out may be q, with one row distance.
  * work: fg_paged_attn_work bytes of device memory (NULL when that is 0),
  * written and read within the call; two calls that may run at once, replays of
  * captured ones included, need one each. */

@@ -711,3 +711,55 @@ def test_min_p_above_one_keeps_the_first_largest_id(rows, V):
     ids, probs = run_draw(x, temp=n, min_p=n, u=u)
     assert np.array_equal(ids, top[np.arange(rows), (u * np.float32(5)).astype(int)])
     assert np.allclose(probs, 0.2, rtol=2.0 ** -23)
+
+
+# ------------------------------------------------------------------ infinities and NaN that are seen
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, NAN], ids=["inf", "-inf", "nan"])
+@pytest.mark.parametrize("where", ["key", "value"])
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("seqs,window", [(((300, 1), (120, 3), (50, 1)), 0), (((700, 500), (400, 300), (90, 20)), 0),
+                                         (((700, 500), (400, 300), (90, 20)), 64)], ids=["few", "many", "many_window"])
+def test_infinities_stay_in_their_sequence(seqs, window, types, where, bad):
+    """One key or value of the second sequence holds it: rows of that sequence
+    are the formula's or NaN (also where they do not see it), other sequences
+    unchanged."""
+    H, KH, hd, dim = 8, 2, 64, 13
+    qt, kt = TYPES[types]
+    b = R.Batch(list(seqs), H, KH, hd, 32, qt, kt, seed=61)
+    b.fill(window, drop_pages=False)
+    q = b.normal(b.rows, H * hd, dtype=qt)
+    clean = run_attn(b, q, window).double().reshape(b.rows, H, hd)
+    exact, mag, dot = b.attention(q, window=window)
+    tol = R.attn_tolerance(exact, mag, dot, hd, 700, qt == BF16)
+    T, n = seqs[1]
+    a = int(b.start_np[1])
+    j = T - (n + 1) // 2  # (the chunk's first half does not see it)
+    (b.k if where == "key" else b.v)[int(b.table_np[1, j // 32]), 0, j % 32, dim] = bad
+    got = run_attn(b, q, window).double().reshape(b.rows, H, hd)
+    mine = torch.zeros(b.rows, dtype=torch.bool, device="cuda")
+    sees = mine.clone()
+    mine[a:a + n] = True
+    sees[a:a + n] = b.visible(1, window, 0)[:, j]
+    assert torch.equal(got[~mine], clean[~mine])
+    assert torch.equal(got[:, H // KH:], clean[:, H // KH:])  # (the other key head's)
+    # (not the same bits: rows of a wavefront move their running maxima together,
+    # and this one's score or NaN moves them; the bound holds for any maxima)
+    assert (((got - exact).abs() <= tol) | torch.isnan(got))[~sees].all()
+    at = got[sees][:, :H // KH]
+    if where == "value":
+        assert (torch.isnan(at[..., dim]) | (at[..., dim] == bad)).all()
+        assert torch.equal(*(t[sees][..., [d for d in range(hd) if d != dim]] for t in (got, clean)))
+        return
+    # a score of -inf leaves the key out, any other one is NaN
+    x = q.double().reshape(b.rows, H, hd)
+    K, V = (torch.nan_to_num(b.history(t, 1)[0], nan=0.0, posinf=0.0, neginf=0.0) for t in (b.k, b.v))
+    see = b.visible(1, window, 0).clone()
+    see[:, j] = False
+    rest = torch.softmax(((x[a:a + n, :H // KH].reshape(-1, hd) @ K.t().contiguous()) / math.sqrt(hd))
+                         .masked_fill(~see.repeat_interleave(H // KH, 0), -math.inf), -1) @ V
+    rest = rest.reshape(n, H // KH, hd)[sees[a:a + n]]
+    out = (x[sees][:, :H // KH, dim] * bad < 0)[..., None]  # (False for NaN)
+    # (as check_attn has it, with sum_j p_j |v_j| and the scores' sizes at their bounds)
+    near = (at - rest).abs() <= (2.0 ** -7 if qt == BF16 else 2.0 ** -12) * V.abs().max()
+    assert (torch.isnan(at) | (out & near)).all()
