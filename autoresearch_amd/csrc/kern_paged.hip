@@ -37,7 +37,7 @@ struct PagedArgs {
   const int32_t* kv_len;
   const int32_t* table;
   int n_seq, n_rows, max_q, max_kv, table_ld, n_pages, pshift;
-  int H, KH, G;
+  int KH, G;
   int window, sinks;
   bool one_tile;  // a row tile a sequence at most: tile i is sequence i's
   float cs;       // softmax scale * log2(e)
@@ -362,8 +362,8 @@ __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.0f
 // from the pages straight to MFMA operands in registers, and meet in LDS.
 // v_mfma_f32_16x16x32_bf16 with S^T = K Q^T: lane 16 g + c then holds query
 // row c's scores of keys 4g .. 4g+3 of both 16-key blocks, which are the 8 K
-// slots of its operand of O^T = V^T P^T. Pages hold 16 rows or a multiple, so
-// a block's page is one scalar load.
+// slots of its operand of O^T = V^T P^T. A block's page comes from the
+// wavefront's list (PageList).
 // Bound by the cache's bytes, every visible key and value being read once: 64
 // tokens over bf16 caches of about 1000 positions, 6 heads of 128, 200 MB, 45 us
 // (4.4 TB/s where a copy reaches 5.1); with rows too few for that by the way
@@ -585,9 +585,10 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
 // ------------------------------------------------------------ many rows
 // For chunks of new tokens: 128 flattened rows a tile, 32 to each of four
 // wavefronts, which all go through the same keys, a 32-key tile a step.
-// v_mfma_f32_32x32x16_bf16 with S^T = K Q^T and O^T = V^T P^T: lane 32 g + c holds query row c of its wavefront. The key rows of a 32-key tile are
-// taken with bits 2 and 3 of their number swapped, so that a lane's scores 8 s ..
-// 8 s + 7 are keys 16 s + 8 g .., which are its K slots of the second product:
+// v_mfma_f32_32x32x16_bf16 with S^T = K Q^T and O^T = V^T P^T: lane 32 g + c
+// holds query row c of its wavefront. The key rows of a 32-key tile are taken
+// with bits 2 and 3 of their number swapped, so that a lane's scores 8 s .. 8 s +
+// 7 are keys 16 s + 8 g .., which are its K slots of the second product:
 // probabilities never leave their registers. V^T's operand is read from the
 // row-major value rows by the LDS's transposing reads (ds_read_b64_tr_b16).
 //
@@ -608,9 +609,8 @@ template <int HD, bool QF, bool KF>
 struct Many {
   static constexpr int RT = 128;  // rows of a tile, 32 a wavefront
   static constexpr int NA = KF ? 3 : 1;
-  static constexpr int KB = 1;        // 32-key tiles a step
-  static constexpr int SK = 32 * KB;
-  static constexpr int ROW = 2 * HD;           // bytes of a K or V row in LDS
+  static constexpr int SK = 32;       // keys a step
+  static constexpr int ROW = 2 * HD;  // bytes of a K or V row in LDS
   static constexpr int PLANE = SK * ROW;
   static constexpr int STAGE = 2 * NA * PLANE;  // K planes, V planes
   static constexpr int LDS = (KF ? 1 : 2) * STAGE;
@@ -661,8 +661,8 @@ __device__ __forceinline__ s16x4_t lds_tr(uint32_t at) {
 template <int HD, bool QF, bool KF>
 __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(PagedArgs p) {
   typedef Many<HD, QF, KF> C;
-  constexpr int NS = HD / 16, ND = HD / 32, NA = C::NA, KB = C::KB, SK = C::SK, ROW = C::ROW,
-                PLANE = C::PLANE, PER = 64 / (2 * KB);  // steps whose blocks a list holds
+  constexpr int NS = HD / 16, ND = HD / 32, NA = C::NA, SK = C::SK, ROW = C::ROW,
+                PLANE = C::PLANE, PER = 32;  // steps whose blocks a list holds
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 5, c = lane & 31;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -673,13 +673,13 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
   const KeyTiles kt = key_tiles(t);
   const int v0 = z * p.cpt, v1 = min(kt.n, v0 + p.cpt);
   if (z > 0 && v0 >= kt.n) return;
-  const int nstep = (v1 - v0 + KB - 1) / KB;
+  const int nstep = v1 - v0;
 
   bool bad = false;
   const int32_t* tab = p.table + (int64_t)t.seq * p.table_ld;
-  // block b of step st is lane 2 KB (st % PER) + b of the step's list
+  // block b of step st is lane 2 (st % PER) + b of the step's list
   auto ask = [&](int st) __attribute__((always_inline)) {
-    return page_ask(p, t, kt, tab, min(v0 + KB * st + lane / 2, v1 - 1), lane & 1);
+    return page_ask(p, t, kt, tab, min(v0 + st + lane / 2, v1 - 1), lane & 1);
   };
   PageList pl = {};  // of the step that is fetched next
   PageAsk next = {};
@@ -700,7 +700,7 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
 #pragma unroll
     for (int q = 0; q < GPP / 4; ++q) {
       const int grp = wv + 4 * q, r = grp * RPG + lane / (ROW / 16), slot = lane % (ROW / 16);
-      const int at = 2 * KB * (st % PER) + grp * RPG / 16;
+      const int at = 2 * (st % PER) + grp * RPG / 16;
       const uint64_t row = (uint64_t)lane_u32(pl.row, at) * HD;
       const int x = page_row(lane_u32(pl.vis, at), r & 15) * HD;
       dma16((const uint16_t*)p.k + row + (x + kslot<HD>(r, slot) * 8), lds0 + to + grp * 1024);
@@ -715,7 +715,8 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int r = i * RPT + tid / CH;
-      const int at = 2 * KB * (st % PER) + __builtin_amdgcn_readfirstlane(r / 16);  // (a wavefront's rows lie in one block)
+      // (a wavefront's rows lie in one block)
+      const int at = 2 * (st % PER) + __builtin_amdgcn_readfirstlane(r / 16);
       const int off = page_row(lane_u32(pl.vis, at), r & 15) * HD + (tid % CH) * 8;
       const uint64_t row = (uint64_t)lane_u32(pl.row, at) * HD;
       const float* kp = (const float*)p.k + row + off;
@@ -788,51 +789,36 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
     for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
 
   // S^T of the step's keys in K buffer `to`
-  auto scores = [&](uint32_t to, f32x16_t (&sc)[KB]) __attribute__((always_inline)) {
+  auto scores = [&](uint32_t to, f32x16_t& sc) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
+    for (int r = 0; r < 16; ++r) sc[r] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[kb][r] = 0.f;
+    for (int s = 0; s < NS; ++s) {
+      bf16x8_t a[NA];
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        bf16x8_t a[NA];
-#pragma unroll
-        for (int k = 0; k < NA; ++k) a[k] = lds_at<bf16x8_t>(ka[s] + to + k * PLANE + kb * 32 * ROW);
-        sc[kb] = mma32(a, q[s], sc[kb]);
-      }
+      for (int k = 0; k < NA; ++k) a[k] = lds_at<bf16x8_t>(ka[s] + to + k * PLANE);
+      sc = mma32(a, q[s], sc);
     }
   };
-  // masks where some row does not see the whole of step st's tiles, and moves
+  // masks where some row does not see the whole of step st's tile, and moves
   // the running maximum (only past a score 2^8 above it, as in k_paged_few)
-  auto settle = [&](int st, f32x16_t (&sc)[KB]) __attribute__((always_inline)) {
-    int b[KB], low = 0x7fffffff, top = 0;  // first keys of the tiles
+  auto settle = [&](int st, f32x16_t& sc) __attribute__((always_inline)) {
+    const int b = tile_base(t, kt, v0 + st);  // the tile's first key
+    if (b + 31 > wp0 || (p.window > 0 && b <= wp1 - p.window)) {
+      const int first = b + 8 * g;  // (this lane's keys are first + 0 .. 7 and 16 .. 23)
+      int end = klim - first, from = klo - first, sink = p.sinks - first;
+      // (keeps the compares in the branch: most steps are seen whole)
+      asm volatile("" : "+v"(end), "+v"(from), "+v"(sink));
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      const int v = v0 + KB * st + kb;
-      b[kb] = v < v1 ? tile_base(t, kt, v) : 0x3fffffff;  // (no such keys: all masked)
-      low = min(low, b[kb]);
-      top = max(top, b[kb]);
-    }
-    if (top + 31 > wp0 || (p.window > 0 && low <= wp1 - p.window)) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {  // (of this lane's keys first + 0 .. 7 and 16 .. 23)
-        const int first = b[kb] + 8 * g;
-        int end = klim - first, from = klo - first, sink = p.sinks - first;
-        // (keeps the compares in the branch: most steps are seen whole)
-        asm volatile("" : "+v"(end), "+v"(from), "+v"(sink));
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int x = 16 * (r >> 3) + (r & 7);
-          const bool seen = x < end && (x >= from || x < sink);
-          sc[kb][r] = seen ? sc[kb][r] : -INFINITY;
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int x = 16 * (r >> 3) + (r & 7);
+        const bool seen = x < end && (x >= from || x < sink);
+        sc[r] = seen ? sc[r] : -INFINITY;
       }
     }
     float mx = -INFINITY;
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[kb][r]);
+    for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[r]);
     mx = swap_max(mx) * p.cs;
     if (__any(mx > m_run + 8.f)) {
       const float m_new = fmaxf(m_run, mx);
@@ -845,33 +831,33 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
       m_run = m_new;
     }
   };
-  // the probabilities' operands of the four 16-key steps, and their sum
-  auto weigh = [&](const f32x16_t (&sc)[KB], PTerms<QF, true> (&pt)[2 * KB]) __attribute__((always_inline)) {
+  // the probabilities' operands of the tile's two 16-key halves, and their sum
+  auto weigh = [&](const f32x16_t& sc, PTerms<QF, true> (&pt)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s4 = 0; s4 < 2 * KB; ++s4) {
+    for (int s = 0; s < 2; ++s) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s4 >> 1][8 * (s4 & 1) + e], p.cs, -m_run));
-      pt[s4].set(x);
+        x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + e], p.cs, -m_run));
+      pt[s].set(x);
 #pragma unroll
       for (int e = 0; e < 8; ++e) l_run += x[e];
     }
   };
   // O^T += V^T P^T from V buffer `to`
-  auto add_values = [&](uint32_t to, const PTerms<QF, true> (&pt)[2 * KB]) __attribute__((always_inline)) {
+  auto add_values = [&](uint32_t to, const PTerms<QF, true> (&pt)[2]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s4 = 0; s4 < 2 * KB; ++s4)
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
         bf16x8_t a[NA];
 #pragma unroll
         for (int k = 0; k < NA; ++k)
           a[k] = __builtin_bit_cast(
-              bf16x8_t, __builtin_shufflevector(lds_tr(va[i] + to + k * PLANE + 16 * s4 * ROW),
-                                                lds_tr(va[i] + to + k * PLANE + (16 * s4 + 4) * ROW), 0, 1, 2,
+              bf16x8_t, __builtin_shufflevector(lds_tr(va[i] + to + k * PLANE + 16 * s * ROW),
+                                                lds_tr(va[i] + to + k * PLANE + (16 * s + 4) * ROW), 0, 1, 2,
                                                 3, 4, 5, 6, 7));
-        o[i] = mma32(a, pt[s4], o[i]);
+        o[i] = mma32(a, pt[s], o[i]);
       }
   };
 
@@ -892,11 +878,11 @@ __global__ __launch_bounds__(256, (Many<HD, QF, KF>::WAVES)) void k_paged_many(P
       stage_sync<0>();  // this step has landed, and nobody reads the other buffer
       if (st + 1 < nstep) fill(st + 1, C::STAGE - here);
     }
-    if (!active || tile_base(t, kt, v0 + KB * st) > wp1) return;  // (behind the wavefront's rows)
-    f32x16_t sc[KB];
+    if (!active || tile_base(t, kt, v0 + st) > wp1) return;  // (behind the wavefront's rows)
+    f32x16_t sc;
     scores(here, sc);
     settle(st, sc);
-    PTerms<QF, true> pt[2 * KB];
+    PTerms<QF, true> pt[2];
     weigh(sc, pt);
     add_values(here, pt);
   };
@@ -946,8 +932,8 @@ struct Plan {
 // alone (lengths may differ under a captured launch).
 //
 // Which kernel: 16-row tiles keep a wavefront a 32-key tile, and read the keys
-// once for each tile; 128-row tiles read them once for eight of those, and
-// have four times the MFMA rate where there are enough of them. The latter take
+// once for each tile; 128-row tiles read and cut them once for eight of those,
+// but keep a workgroup where that has one. The latter take
 // over past 32 rows a sequence from MANY_WORK (16-row tile, 32-key tile) pairs
 // on. us, 16 rows -> 128: fp32 rows and pages, 64 tokens after 936 (768 pairs)
 // 15.0 -> 21.8, 8 x 96 after 1404, 6 heads (13.5k) 90 -> 53, 500 tokens (3k) 18.6
@@ -1051,7 +1037,6 @@ void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, co
   a.table_ld = b.table_ld;
   a.n_pages = pg.n_pages;
   a.pshift = __builtin_ctz(pg.page_size);
-  a.H = c.n_head;
   a.KH = pg.n_kv_head;
   a.G = c.n_head / pg.n_kv_head;
   a.window = c.window;
