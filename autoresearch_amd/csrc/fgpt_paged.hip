@@ -194,6 +194,10 @@ extern "C" int32_t fg_paged_attn(const fg_pages* pages, const fg_ragged* batch,
   if (batch->n_rows == 0 || batch->max_q == 0) return FG_OK;
   CHECK(q && out, "q or out is NULL");
   CHECK(aligned(q) && aligned(out) && aligned(work), "q, out or work is not 16-byte aligned");
+  const int64_t packed = (int64_t)cfg->n_head * pages->head_dim;
+  CHECK(out != q || batch->n_rows == 1 ||
+            (cfg->q_ld ? cfg->q_ld : packed) == (cfg->out_ld ? cfg->out_ld : packed),
+        "out is q with another row distance");
   const int64_t need = 4 * paged_attn_floats(*pages, *batch, *cfg);
   CHECK(need == 0 || (work && work_bytes >= need), "work: %lld bytes needed, %lld given",
         (long long)need, (long long)(work ? work_bytes : 0));
@@ -201,7 +205,7 @@ extern "C" int32_t fg_paged_attn(const fg_pages* pages, const fg_ragged* batch,
   RCCHK(on.enter(stream));
   PagedOut o;
   o.y = out;
-  o.ld = cfg->out_ld ? cfg->out_ld : (int64_t)cfg->n_head * pages->head_dim;
+  o.ld = cfg->out_ld ? cfg->out_ld : packed;
   launch_paged_attn((hipStream_t)stream, *pages, *batch, *cfg, q, o, (float*)work);
   return launched("paged attention");
 }

@@ -225,3 +225,15 @@ def test_a_short_copy_list_costs_nothing_of_a_large_pool():
     finally:
         resource.setrlimit(resource.RLIMIT_AS, old)
     assert code == -7
+
+
+@pytest.mark.parametrize("kw,good", [(dict(), True), (dict(q_ld=256), True), (dict(out_ld=256), True),
+                                     (dict(q_ld=512, out_ld=512), True), (dict(q_ld=512), False),
+                                     (dict(out_ld=260), False), (dict(q_ld=512, out_ld=516), False)])
+@pytest.mark.skipif(not no_gpu(), reason="a GPU is visible")
+def test_attention_in_place_keeps_the_row_distance(kw, good):
+    """With another one, rows would be written over before they are read."""
+    with pytest.raises(engine.FgptError, match="device" if good else "row distance"):
+        attn(q=P, out=P, **kw)
+    with pytest.raises(engine.FgptError, match="device"):  # (one row has no distance)
+        attn(bt=batch(n_rows=1, max_q=1), q=P, out=P, **kw)
