@@ -246,7 +246,7 @@ struct KvTile;
 // of step (j, e) is head dim 16 j + 4 g + e; of the second product, key 4 g + r):
 // exact products without cutting K and V into terms, which costs a wavefront
 // more clocks than these MFMAs take, and registers (one token after 300
-// positions, the cut ones 13.4 us, so 8.3).
+// positions, the cut ones 13.4 us, so 8.4).
 template <int HD, bool QF>
 struct KvTile<HD, QF, true> {
   static constexpr int NJ = HD / 16, VD = HD / 16;
@@ -367,8 +367,8 @@ __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.0f
 // Bound by the cache's bytes, every visible key and value being read once: 64
 // tokens over bf16 caches of about 1000 positions, 6 heads of 128, 200 MB, 45 us
 // (4.4 TB/s where a copy reaches 5.1); with rows too few for that by the way
-// through table, page and products: one token after 300 positions 8.3 us, the
-// merge 2.9.
+// through table, page and products: one token after 300 positions 8.4 us, the
+// merge 3.1.
 constexpr int DR = 16, RWV = 4;
 
 template <int HD>
@@ -598,9 +598,10 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
 // Bound by a step's three chains, which take much the same time: 16 MFMAs, the
 // softmax of 16 scores a lane, and 16 KB of LDS reads a wavefront (64 rows a
 // wavefront would halve those: their scores and outputs do not fit the
-// registers). bf16 prompts, 387 GF: 423 us, 915 TFLOP/s (a library matrix
-// product 1360). fp32 rows and pages take six MFMAs a product: 5.2 GF of mixed
-// chunks 70 us, and 7.5 for the merge.
+// registers). bf16 prompts, 387 GF: 430 us, 900 TFLOP/s (a library matrix
+// product 1360). fp32 rows and pages take six MFMAs a product, on bf16 pages
+// three: one prompt of 2048 tokens on 6 heads of 128, 6.4 GF, 75 and 46 us; 5.2 GF
+// of mixed fp32 chunks 70 us, and 7.5 for the merge.
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -932,19 +933,20 @@ struct Plan {
 // alone (lengths may differ under a captured launch).
 //
 // Which kernel: 16-row tiles keep a wavefront a 32-key tile, and read the keys
-// once for each tile; 128-row tiles read and cut them once for eight of those,
-// but keep a workgroup where that has one. The latter take
-// over past 32 rows a sequence from MANY_WORK (16-row tile, 32-key tile) pairs
-// on. us, 16 rows -> 128: fp32 rows and pages, 64 tokens after 936 (768 pairs)
-// 15.0 -> 21.8, 8 x 96 after 1404, 6 heads (13.5k) 90 -> 53, 500 tokens (3k) 18.6
-// -> 25.5, 2048 (49k) 118 -> 74; bf16, 32 heads on 4, 8 x 8 rows after 1490
-// (6k) 17.4 -> 17.3, 256 after 7744 (128k) 145 -> 54. At 32 rows, 32 sequences
-// of a 2048-key window on 32 heads (17k) 36 -> 42.
-// Parts: as many as fill the CUs once with 16-row tiles (more only add partial
-// results: 64 sequences of ~1000 as one part 44.5, two 49), of at least a tile a
-// wavefront (two: one token on 6 fp32 heads after 300 positions 10.5 -> 13.7, on
-// bf16 pages after 1000 9.0 -> 10.3, after 4000 12.8 -> 12.3); twice with 128-row ones (mixed chunks and tokens of 9
-// sequences, 32 heads on 4, one part a CU 78, two 68).
+// once for each tile; 128-row tiles read them (fp32 ones: cut them) once for eight
+// of those, but keep a whole workgroup where that has one. The latter take over
+// past 32 rows a sequence from MANY_WORK (16-row tile, 32-key tile) pairs on. us,
+// 16 rows -> 128: fp32 rows and pages, 6 heads, 64 tokens after 936 (768 pairs)
+// 14.9 -> 22.2, 8 x 96 after 1404 (13.5k) 90 -> 53, 500 tokens (3k) 18.6 -> 25.7,
+// 2048 (49k) 118 -> 75, on bf16 pages 50 -> 47; bf16 rows, 32 heads on 4, 8 x 8
+// tokens after 1490 (6k) 17.9 -> 17.7, 256 after 7744 (128k) 146 -> 56. At 32
+// rows, 32 sequences of a 2048-key window on 32 heads (17k) 36.5 -> 42.3.
+// Parts: as many as fill the CUs once with 16-row tiles (twice: 500 fp32 tokens
+// 18.6 -> 24.6, those 32 windows 36.5 -> 40.6), of at least a tile a wavefront
+// (two: one token on 6 fp32 heads after 300 positions 10.8 -> 13.9, on bf16 pages
+// after 1000 9.5 -> 10.2, after 4000 13.0 -> 12.1); twice with 128-row ones (once:
+// chunks and tokens of 9 sequences, 10 heads on 2, 92 -> 123, one fp32 prompt of
+// 2048 75 -> 95).
 constexpr int64_t MANY_WORK = 6000;
 Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
   Plan pl;
