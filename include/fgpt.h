@@ -441,7 +441,8 @@ int32_t fg_qk_append(const fg_pages *pages, const fg_ragged *batch, const fg_app
  * changes nothing. A row that sees one is what the formula gives or NaN, which
  * of the two by the kernel that the bounds select (a term of zero times an
  * infinity); where other tokens of the same call and sequence see one, earlier or
- * (past a window) later ones, a row that does not may be NaN too. out may be q, with one row distance.
+ * (past a window) later ones, a row that does not may be NaN too. out may be q,
+ * with one row distance.
  * work: fg_paged_attn_work bytes of device memory (NULL when that is 0),
  * written and read within the call; two calls that may run at once, replays of
  * captured ones included, need one each. */
@@ -474,8 +475,8 @@ int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t
  * cumulative mass exceeds u times the kept mass. Settings are per row
  * (device arrays, each nullable = off; temp: 1): temp <= 0 takes the first
  * largest id; top_k <= 0, top_p >= 1 and min_p <= 0 are off; a top_p <= 0 or
- * min_p > 1 keeps the first largest id alone; u below 0 counts as 0, 1 or more as the last
- * mass; NaN settings are off (a NaN u counts as 0). NaN and -inf logits are
+ * min_p > 1 keeps the first largest id alone; u below 0 counts as 0, 1 or more as
+ * the last mass; NaN settings are off (a NaN u counts as 0). NaN and -inf logits are
  * never drawn; a row of nothing else gives id -1. +inf ones share the
  * mass. probs (nullable): the drawn id's share of the kept mass. Masses are
  * exact sums of 64-bit integers (e_i in steps of 2^-44): ids do not
