@@ -86,16 +86,21 @@ int32_t launched(const char* what) {
   return e == hipSuccess ? FG_OK : err(FG_EHIP, "%s: %s", what, hipGetErrorString(e));
 }
 
-int32_t check_pages(const fg_pages* p) {
-  CHECK(p && p->k && p->v, "pages: NULL argument");
+int32_t check_page(const fg_pages* p) {
   CHECK(p->head_dim == 64 || p->head_dim == 128, "head_dim %d unsupported (64 or 128)", p->head_dim);
   CHECK(p->page_size >= 16 && p->page_size <= 256 && (p->page_size & (p->page_size - 1)) == 0,
         "page_size %d is not a power of two in 16..256", p->page_size);
   CHECK(p->n_pages >= 1 && p->n_kv_head >= 1, "pages: n_pages and n_kv_head must be >= 1");
   CHECK(p->n_kv_head <= 1024, "n_kv_head %d above 1024", p->n_kv_head);
+  CHECK(p->type >= FG_F32 && p->type <= FG_E4M3, "pages: unknown type %d", p->type);
+  return FG_OK;
+}
+
+int32_t check_pages(const fg_pages* p) {
+  CHECK(p && p->k && p->v, "pages: NULL argument");
+  RCCHK(check_page(p));
   CHECK((int64_t)p->n_pages * p->n_kv_head * p->page_size < (int64_t)1 << 32,
         "pages: %d x %d heads x %d rows above 2^32", p->n_pages, p->n_kv_head, p->page_size);
-  CHECK(p->type == FG_F32 || p->type == FG_BF16, "pages: unknown type %d", p->type);
   CHECK(aligned(p->k) && aligned(p->v), "pages are not 16-byte aligned");
   return FG_OK;
 }
@@ -137,7 +142,7 @@ int32_t check_attn(const fg_pages* pages, const fg_ragged* batch, const fg_attn_
   RCCHK(check_batch(batch, pages));
   CHECK(cfg, "cfg is NULL");
   RCCHK(check_heads(cfg->n_head, pages, cfg->type, batch));
-  CHECK(cfg->type == FG_F32 || pages->type == FG_BF16, "bf16 rows need bf16 pages");
+  CHECK(cfg->type == FG_F32 || pages->type != FG_F32, "bf16 rows need bf16 pages or 8-bit ones");
   CHECK(cfg->window >= 0 && cfg->sinks >= 0, "window and sinks must be >= 0");
   CHECK(cfg->window <= (1 << 30) && cfg->sinks <= (1 << 30), "window or sinks above 2^30");
   CHECK(cfg->scale >= 0.f && cfg->scale <= 1e30f, "scale must be finite and >= 0");
@@ -233,6 +238,30 @@ extern "C" int32_t fg_qk_append(const fg_pages* pages, const fg_ragged* batch,
   RCCHK(on.enter(stream));
   launch_qk_append((hipStream_t)stream, *pages, *batch, *cfg, qkv, q_out);
   return launched("append");
+}
+
+// ------------------------------------------------------------ reading back
+extern "C" int32_t fg_page_bytes(const fg_pages* pages, int64_t* bytes) {
+  CHECK(pages && bytes, "NULL argument");
+  RCCHK(check_page(pages));
+  *bytes = (int64_t)pages->n_kv_head * page_head_bytes(*pages);
+  return FG_OK;
+}
+
+extern "C" int32_t fg_pages_read(const fg_pages* pages, const fg_ragged* batch, int32_t type,
+                                 int64_t ld, void* k_out, void* v_out, void* stream) {
+  RCCHK(check_pages(pages));
+  RCCHK(check_batch(batch, pages));
+  CHECK(type == FG_F32 || type == FG_BF16, "unknown row type %d", type);
+  CHECK((int64_t)batch->n_rows * pages->n_kv_head <= 1 << 26, "batch: n_rows %d x %d heads above 2^26",
+        batch->n_rows, pages->n_kv_head);
+  RCCHK(check_ld(ld, (int64_t)pages->n_kv_head * pages->head_dim, type, "ld"));
+  CHECK(aligned(k_out) && aligned(v_out), "k_out or v_out is not 16-byte aligned");
+  if (batch->n_rows == 0 || (!k_out && !v_out)) return FG_OK;
+  OnStream on;
+  RCCHK(on.enter(stream));
+  launch_pages_read((hipStream_t)stream, *pages, *batch, type, ld, k_out, v_out);
+  return launched("reading pages back");
 }
 
 // ------------------------------------------------------------ page copies

@@ -1,9 +1,12 @@
-// kern_pages.hip -- what fills and moves the pages of a paged KV cache:
-// k_qk_append (head norms, rotation, q out, k and v into their slots) and
-// k_pages_copy (include/fgpt.h: fg_qk_append, fg_pages_copy).
+// kern_pages.hip -- what fills, reads and moves the pages of a paged KV cache:
+// k_qk_append (head norms, rotation, q out, k and v into their slots),
+// k_pages_read (tokens' rows back out of their slots) and k_pages_copy
+// (include/fgpt.h: fg_qk_append, fg_pages_read, fg_pages_copy).
 #include <algorithm>
+#include <type_traits>
 
 #include "fgpt_internal.h"
+#include "kern_codes.h"
 #include "kern_common.h"
 #include "paged_internal.h"
 
@@ -79,29 +82,91 @@ __device__ __forceinline__ void store_vals(void* base, int64_t i, const float (&
   }
 }
 
-template <int HD, bool QF, bool KF, int RW>
-__global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
-  typedef RowIO<HD, QF> IO;
-  constexpr int VEC = IO::VEC, LPH = IO::LPH, HPT = 256 / (LPH * RW), HU = 4;  // heads at once
+// Largest of the group's values, likewise.
+template <int N>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  auto dpp = [](uint32_t u, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, decltype(ctrl)::value, 0xF, 0xF, false);
+  };
+  v = max(v, dpp(v, std::integral_constant<int, 0xB1>()));
+  v = max(v, dpp(v, std::integral_constant<int, 0x4E>()));
+  if constexpr (N >= 8) v = max(v, dpp(v, std::integral_constant<int, 0x141>()));
+  if constexpr (N >= 16) v = max(v, dpp(v, std::integral_constant<int, 0x140>()));
+  return v;
+}
+
+// A head's row (this lane's dims of both halves) as 8-bit codes, and its scale:
+// max|x| / top, codes x / scale to the nearest (ties to even). The largest is
+// taken over the values' bits, where infinities and NaN are above every finite
+// one: such a row's scale is NaN.
+template <int KT, int LPH, int VEC>
+__device__ __forceinline__ void store_codes(uint8_t* codes, float* scale, int d, int half,
+                                            const float (&x1)[VEC], const float (&x2)[VEC]) {
+  constexpr float TOP = KT == FG_I8 ? 127.f : 448.f;
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k)
+    m = max(m, max(__float_as_uint(x1[k]) & 0x7FFFFFFFu, __float_as_uint(x2[k]) & 0x7FFFFFFFu));
+  m = group_max<LPH>(m);
+  const bool finite = m < 0x7F800000u;
+  float s = __uint_as_float(m) / TOP;
+  if (!(s >= __FLT_MIN__)) s = 0.f;  // (its inverse would be infinite)
+  const bool live = finite && s > 0.f;  // (else codes of 0, not of -0 or NaN)
+  const float inv = live ? 1.0f / s : 0.f;
+  auto code4 = [&](const float* x) -> uint32_t {
+    float y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = live ? __builtin_amdgcn_fmed3f(x[k] * inv, -TOP, TOP) : 0.f;
+    if constexpr (KT == FG_E4M3) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
+    } else {
+      uint32_t w = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w |= ((uint32_t)(int)__builtin_rintf(y[k]) & 255u) << (8 * k);
+      return w;
+    }
+  };
+  if constexpr (VEC == 8) {
+    *(uint2*)(codes + d) = make_uint2(code4(x1), code4(x1 + 4));
+    *(uint2*)(codes + half + d) = make_uint2(code4(x2), code4(x2 + 4));
+  } else {
+    *(uint32_t*)(codes + d) = code4(x1);
+    *(uint32_t*)(codes + half + d) = code4(x2);
+  }
+  if (d == 0) *scale = finite ? s : NAN;
+}
+
+// The rows r0 .. r0 + RW-1 of a batch, a wavefront each: at[i] = the row's
+// sequence (the number of sequences that end at or before it) and its position;
+// below 0: padding behind the last sequence, or none.
+template <int RW>
+__device__ __forceinline__ void find_rows(const fg_ragged& b, int r0, int (&at)[4][2]) {
   static_assert(RW <= 4, "a wavefront finds a row");
-  __shared__ int at[4][2];  // the rows' sequences and positions
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  const int r0 = blockIdx.x * RW;
   if (wv < RW) {
-    // the row's sequence: the number of sequences that end at or before it
     const int row = r0 + wv;
     int seq = 0;
-    for (int s0 = 0; s0 < a.b.n_seq; s0 += 64) {
-      const bool before = s0 + lane < a.b.n_seq && a.b.q_start[s0 + lane + 1] <= row;
+    for (int s0 = 0; s0 < b.n_seq; s0 += 64) {
+      const bool before = s0 + lane < b.n_seq && b.q_start[s0 + lane + 1] <= row;
       seq += __popcll(__ballot(before));
     }
     if (lane == 0) {
-      const bool real = row < a.b.n_rows && seq < a.b.n_seq;  // (else padding behind the last sequence)
+      const bool real = row < b.n_rows && seq < b.n_seq;
       at[wv][0] = seq;
-      at[wv][1] = real ? a.b.kv_len[seq] - (a.b.q_start[seq + 1] - row) : -1;
+      at[wv][1] = real ? b.kv_len[seq] - (b.q_start[seq + 1] - row) : -1;
     }
   }
   __syncthreads();
+}
+
+template <int HD, bool QF, int KT, int RW>
+__global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
+  typedef RowIO<HD, QF> IO;
+  constexpr int VEC = IO::VEC, LPH = IO::LPH, HPT = 256 / (LPH * RW), HU = 4;  // heads at once
+  __shared__ int at[4][2];  // the rows' sequences and positions
+  const int r0 = blockIdx.x * RW;
+  find_rows<RW>(a.b, r0, at);
   const int slot = threadIdx.x / LPH % RW, seq = at[slot][0], pos = at[slot][1];
   // (a whole group of LPH lanes has one row: the sums stay within it)
   if (pos < 0 || pos >= a.b.max_kv) return;
@@ -191,11 +256,76 @@ __global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
         const bool key = h < H + KH;
         const int kvh = h - H - (key ? 0 : KH);
         void* base = key ? a.pg.k : a.pg.v;
-        const int64_t o = (((int64_t)page * KH + kvh) * P + (pos & (P - 1))) * HD + d;
-        store_vals<VEC, KF>(base, o, x1);
-        store_vals<VEC, KF>(base, o + HD / 2, x2);
+        const int64_t block = (int64_t)page * KH + kvh;
+        const int slot = pos & (P - 1);
+        if constexpr (KT == FG_F32 || KT == FG_BF16) {
+          const int64_t o = (block * P + slot) * HD + d;
+          store_vals<VEC, KT == FG_F32>(base, o, x1);
+          store_vals<VEC, KT == FG_F32>(base, o + HD / 2, x2);
+        } else {
+          uint8_t* b = (uint8_t*)base + block * P * (HD + 4);
+          store_codes<KT, LPH>(b + slot * HD, (float*)(b + P * HD) + slot, d, HD / 2, x1, x2);
+        }
       }
     }
+  }
+}
+
+// ------------------------------------------------------------ reading back
+// A thread takes 8 values of a row of k or v: HD/8 threads a head, RW rows a
+// workgroup as in the append (rows are found the same way). fp32 in, code times
+// scale, one rounding.
+struct ReadArgs {
+  fg_pages pg;
+  fg_ragged b;
+  void* out[2];
+  int64_t ld;
+  int pshift;
+};
+
+template <int HD, int KT, bool OF, int RW>
+__global__ __launch_bounds__(256) void k_pages_read(ReadArgs a) {
+  constexpr int CPH = HD / 8, CPR = 256 / RW;  // 8-value chunks of a head; threads of a row
+  __shared__ int at[4][2];
+  const int r0 = blockIdx.x * RW;
+  find_rows<RW>(a.b, r0, at);
+  const int i = threadIdx.x / CPR, seq = at[i][0], pos = at[i][1];
+  if (pos < 0 || pos >= a.b.max_kv) return;
+  const int64_t row = r0 + i;
+  const int P = 1 << a.pshift, slot = pos & (P - 1), KH = a.pg.n_kv_head;
+  const int page = a.b.table[(int64_t)seq * a.b.table_ld + (pos >> a.pshift)];
+  const bool kept = (uint32_t)page < (uint32_t)a.pg.n_pages;
+  for (int c = threadIdx.x % CPR; c < 2 * KH * CPH; c += CPR) {
+    const int val = c >= KH * CPH, h = c / CPH - val * KH, d = c % CPH * 8;
+    if (!a.out[val]) continue;
+    const void* base = val ? a.pg.v : a.pg.k;
+    const int64_t block = (int64_t)(kept ? page : 0) * KH + h;
+    float x[8];
+    if constexpr (KT == FG_F32 || KT == FG_BF16) {
+      const int64_t o = (block * P + slot) * HD + d;
+      float y[4];
+      if constexpr (KT == FG_F32) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          RowIO<HD, true>::values(RowIO<HD, true>::load(base, o + 4 * u), y);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[4 * u + k] = y[k];
+        }
+      } else {
+        RowIO<HD, false>::values(RowIO<HD, false>::load(base, o), x);
+      }
+    } else {
+      const uint8_t* b = (const uint8_t*)base + block * P * (HD + 4);
+      const uint2 w = *(const uint2*)(b + slot * HD + d);
+      const float s = ((const float*)(b + P * HD))[slot];
+      code_values<KT>(w, x);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= s;
+    }
+    if (!kept)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = NAN;
+    store_vals<8, OF>(a.out[val], row * a.ld + h * HD + d, x);
   }
 }
 
@@ -255,20 +385,42 @@ __global__ __launch_bounds__(256) void k_take_rows(const int32_t* __restrict__ r
   for (int k = threadIdx.x; k < nq; k += 256) qo[to * nq + k] = q[from * nq + k];
 }
 
-template <int HD, bool QF, bool KF>
+template <int HD, bool QF, int KT>
 void append_t(hipStream_t s, const AppendArgs& a) {
   if (a.b.n_rows >= 2048)
-    FG_LAUNCH((k_qk_append<HD, QF, KF, 4>), dim3((unsigned)((a.b.n_rows + 3) / 4)), dim3(256), 0, s, a);
+    FG_LAUNCH((k_qk_append<HD, QF, KT, 4>), dim3((unsigned)((a.b.n_rows + 3) / 4)), dim3(256), 0, s, a);
   else
-    FG_LAUNCH((k_qk_append<HD, QF, KF, 1>), dim3((unsigned)a.b.n_rows), dim3(256), 0, s, a);
+    FG_LAUNCH((k_qk_append<HD, QF, KT, 1>), dim3((unsigned)a.b.n_rows), dim3(256), 0, s, a);
+}
+
+template <int HD, bool QF>
+void append_q(hipStream_t s, const AppendArgs& a) {
+  if (a.pg.type == FG_F32) append_t<HD, QF, FG_F32>(s, a);
+  else if (a.pg.type == FG_BF16) append_t<HD, QF, FG_BF16>(s, a);
+  else if (a.pg.type == FG_I8) append_t<HD, QF, FG_I8>(s, a);
+  else append_t<HD, QF, FG_E4M3>(s, a);
 }
 
 template <int HD>
 void append_hd(hipStream_t s, const AppendArgs& a) {
-  if (a.pg.type == FG_F32 && a.c.type == FG_F32) append_t<HD, true, true>(s, a);
-  else if (a.c.type == FG_F32) append_t<HD, true, false>(s, a);
-  else if (a.pg.type == FG_F32) append_t<HD, false, true>(s, a);
-  else append_t<HD, false, false>(s, a);
+  if (a.c.type == FG_F32) append_q<HD, true>(s, a);
+  else append_q<HD, false>(s, a);
+}
+
+template <int HD, int KT, bool OF>
+void read_t(hipStream_t s, const ReadArgs& a) {
+  if (a.b.n_rows >= 2048)
+    FG_LAUNCH((k_pages_read<HD, KT, OF, 4>), dim3((unsigned)((a.b.n_rows + 3) / 4)), dim3(256), 0, s, a);
+  else
+    FG_LAUNCH((k_pages_read<HD, KT, OF, 1>), dim3((unsigned)a.b.n_rows), dim3(256), 0, s, a);
+}
+
+template <int HD, bool OF>
+void read_k(hipStream_t s, const ReadArgs& a) {
+  if (a.pg.type == FG_F32) read_t<HD, FG_F32, OF>(s, a);
+  else if (a.pg.type == FG_BF16) read_t<HD, FG_BF16, OF>(s, a);
+  else if (a.pg.type == FG_I8) read_t<HD, FG_I8, OF>(s, a);
+  else read_t<HD, FG_E4M3, OF>(s, a);
 }
 
 }  // namespace
@@ -282,6 +434,16 @@ void launch_qk_append(hipStream_t s, const fg_pages& pg, const fg_ragged& b, con
     append_hd<128>(s, a);
   else
     append_hd<64>(s, a);
+}
+
+void launch_pages_read(hipStream_t s, const fg_pages& pg, const fg_ragged& b, int32_t type, int64_t ld,
+                       void* k_out, void* v_out) {
+  const ReadArgs a{pg, b, {k_out, v_out}, ld ? ld : (int64_t)pg.n_kv_head * pg.head_dim,
+                   __builtin_ctz(pg.page_size)};
+  if (pg.head_dim == 128 && type == FG_F32) read_k<128, true>(s, a);
+  else if (pg.head_dim == 128) read_k<128, false>(s, a);
+  else if (type == FG_F32) read_k<64, true>(s, a);
+  else read_k<64, false>(s, a);
 }
 
 void launch_take_rows(hipStream_t s, const int32_t* rows, int n, const float* x, float* xo, int nx,

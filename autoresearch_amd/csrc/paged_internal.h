@@ -11,6 +11,12 @@
 
 namespace fgpt {
 
+// Bytes of one head's part of a page.
+inline int64_t page_head_bytes(const fg_pages& p) {
+  const int64_t row = p.type == FG_F32 ? 4 * p.head_dim : p.type == FG_BF16 ? 2 * p.head_dim : p.head_dim + 4;
+  return row * p.page_size;
+}
+
 // ---- attention
 // Where the attention's output goes: rows of fp32 or bf16, or the split operand
 // planes of the GEMM that follows (tile_at over n_head * head_dim columns).
@@ -25,9 +31,11 @@ int64_t paged_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_attn_
 void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c,
                        const void* q, const PagedOut& out, float* work);
 
-// ---- append and page copies
+// ---- append, reading back and page copies
 void launch_qk_append(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_append_cfg& c,
                       const void* qkv, void* q_out);
+void launch_pages_read(hipStream_t s, const fg_pages& pg, const fg_ragged& b, int32_t type, int64_t ld,
+                       void* k_out, void* v_out);
 void launch_pages_copy(hipStream_t s, void* base, int32_t n_planes, int64_t plane_bytes,
                        int64_t page_bytes, const int32_t* src, const int32_t* dst, int32_t n);
 

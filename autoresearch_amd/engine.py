@@ -37,7 +37,7 @@ EXPORTS = (
     "fg_eval_bpb", "fg_rows_npy", "fg_decode_spec", "fg_spec_accept", "fg_spec_draft",
     "fg_sample", "fg_decode_sample", "fg_set_option", "fg_get_option", "fg_step_dev_noalloc",
     "fg_qk_append", "fg_paged_attn_work", "fg_paged_attn", "fg_pages_copy", "fg_draw_rows_work",
-    "fg_draw_rows",
+    "fg_draw_rows", "fg_page_bytes", "fg_pages_read",
     "fg_pool_create", "fg_pool_destroy", "fg_pool_len", "fg_pool_free", "fg_pool_table",
     "fg_pool_need", "fg_pool_extend", "fg_pool_fork", "fg_pool_trim", "fg_pool_slide",
     "fg_pool_compact",
@@ -88,6 +88,7 @@ class _SampleCfg(C.Structure):
 
 
 FG_F32, FG_BF16 = 0, 1  # value types of the paged operators' rows and pages
+FG_I8, FG_E4M3 = 2, 3  # of pages alone: 8-bit codes with a scale a row
 
 
 class _Pages(C.Structure):
@@ -179,6 +180,8 @@ def load_library(path: str = LIB_PATH):
         "fg_get_option": (i32, [_vp, i32, _i, C.c_char_p, i32]),
         "fg_qk_append": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AppendCfg), _vp,
                                _vp, _vp]),
+        "fg_page_bytes": (i32, [C.POINTER(_Pages), C.POINTER(i64)]),
+        "fg_pages_read": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), i32, i64, _vp, _vp, _vp]),
         "fg_paged_attn_work": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AttnCfg),
                                      C.POINTER(i64)]),
         "fg_paged_attn": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AttnCfg), _vp,
@@ -705,9 +708,19 @@ def spec_draft(ids, p: int, m: int, k: int):
 # descriptors only name the caller's buffers and may be kept with them.
 
 def pages(k: int, v: int, n_pages: int, page_size: int, n_kv_head: int, head_dim: int,
-          bf16: bool = False) -> _Pages:
-    """fg_pages: one layer's keys and values, [n_pages][n_kv_head][page_size][head_dim]."""
-    return _Pages(k, v, n_pages, page_size, n_kv_head, head_dim, FG_BF16 if bf16 else FG_F32)
+          bf16: bool = False, type: int | None = None) -> _Pages:
+    """fg_pages: one layer's keys and values, [n_pages][n_kv_head][page_size][head_dim];
+    type: FG_F32, FG_BF16, FG_I8 or FG_E4M3 (in the place of bf16)."""
+    if type is None:
+        type = FG_BF16 if bf16 else FG_F32
+    return _Pages(k, v, n_pages, page_size, n_kv_head, head_dim, type)
+
+
+def page_bytes(page_size: int, n_kv_head: int, head_dim: int, type: int = FG_F32) -> int:
+    """fg_page_bytes: bytes of one page of keys (or values) of that type."""
+    n = C.c_int64()
+    _check(load_library().fg_page_bytes(_Pages(0, 0, 1, page_size, n_kv_head, head_dim, type), C.byref(n)))
+    return n.value
 
 
 def ragged(q_start: int, kv_len: int, table: int, n_seq: int, n_rows: int, max_q: int, max_kv: int,
@@ -728,6 +741,12 @@ def append_cfg(n_head: int, cos: int = 0, sin: int = 0, rope_n: int = 0, norm: b
 def qk_append(pg: _Pages, batch: _Ragged, cfg: _AppendCfg, qkv: int, q_out: int, stream: int = 0):
     """fg_qk_append: heads normed and rotated, q out, k and v into their slots."""
     _check(load_library().fg_qk_append(pg, batch, cfg, qkv, q_out, stream))
+
+
+def pages_read(pg: _Pages, batch: _Ragged, k_out: int = 0, v_out: int = 0, bf16: bool = False, ld: int = 0,
+               stream: int = 0):
+    """fg_pages_read: the batch's tokens' keys and values as fp32 or bf16 rows."""
+    _check(load_library().fg_pages_read(pg, batch, FG_BF16 if bf16 else FG_F32, ld, k_out, v_out, stream))
 
 
 def attn_cfg(n_head: int, window: int = 0, sinks: int = 0, scale: float = 0.0, bf16: bool = False,

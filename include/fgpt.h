@@ -373,13 +373,20 @@ int32_t fg_model_bytes(const fg_model *m, int64_t *weight_bytes, int64_t *work_b
  *
  * fg_pages: one layer's keys and values, each [n_pages][n_kv_head][page_size]
  * [head_dim] (a head's positions of a page are consecutive rows). head_dim 64
- * or 128; page_size a power of two, 16..256. */
-enum { FG_F32 = 0, FG_BF16 = 1 };
+ * or 128; page_size a power of two, 16..256. Pages of the 8-bit types hold codes
+ * with a scale a row: a head's part of a page is page_size rows of head_dim
+ * codes of a byte each, then page_size fp32 scales, and a value is code * scale.
+ * FG_I8: integers -127..127; FG_E4M3: 8-bit floats of 4 exponent and 3 mantissa
+ * bits, up to 448, no infinities. */
+enum { FG_F32 = 0, FG_BF16 = 1, FG_I8 = 2, FG_E4M3 = 3 };
 typedef struct fg_pages {
   void *k, *v;
   int32_t n_pages, page_size, n_kv_head, head_dim;
-  int32_t type; /* FG_F32 or FG_BF16 */
+  int32_t type; /* of the pages: any of the four */
 } fg_pages;
+/* Bytes of one page of k (or v): an array of n_pages of them, fg_pages_copy's
+ * page_bytes. (k and v may be NULL here.) */
+int32_t fg_page_bytes(const fg_pages *pages, int64_t *bytes);
 
 /* A batch of new tokens: rows q_start[s] .. q_start[s+1]-1 of the row arrays
  * are the last tokens of sequence s, whose cache holds kv_len[s] positions with
@@ -406,7 +413,11 @@ typedef struct fg_ragged {
  * max_kv) the halves (x1, x2) of a q or k head at position p become (x1 c + x2 s, x2 c -
  * x1 s) (rope_4d, src/lib/fortran_rope.f90:25-52). q goes to q_out rows of
  * n_head * head_dim in the type of qkv, k and v to their slots, rounded to the
- * pages' type. All arithmetic is fp32. interleaved: a head's values come in
+ * pages' type; for an 8-bit type, with top its largest code (127, 448), a head's
+ * row gets the scale max|x| / top and the codes x * (1 / scale) rounded to the
+ * nearest (ties to even). A scale below 2^-126 is 0, with codes 0; a row with an
+ * infinity or NaN gets the scale NaN: all its values are NaN. All arithmetic is
+ * fp32. interleaved: a head's values come in
  * pairs (d, d + head_dim/2), as the engine keeps its QKV weights' rows; q_out
  * and the pages are in head order either way. A row at a position below 0 or
  * not below max_kv is left alone; one whose page is not in [0, n_pages)
@@ -425,12 +436,22 @@ typedef struct fg_append_cfg {
 int32_t fg_qk_append(const fg_pages *pages, const fg_ragged *batch, const fg_append_cfg *cfg,
                      const void *qkv, void *q_out, void *stream);
 
+/* The keys and values of the batch's tokens out of their slots: k_out and v_out
+ * (each nullable) are rows of n_kv_head * head_dim values in `type` (FG_F32 or
+ * FG_BF16), ld elements apart (0 = packed), row r those of token row r of the
+ * batch; of an 8-bit page code * scale in fp32, rounded once. A batch whose
+ * q_start counts all of a sequence's positions reads it whole; max_q is not used.
+ * A row at a position below 0 or not below max_kv is left alone; one whose page
+ * is not in [0, n_pages) gets NaN. k_out and v_out must not lie in the pages. */
+int32_t fg_pages_read(const fg_pages *pages, const fg_ragged *batch, int32_t type, int64_t ld,
+                      void *k_out, void *v_out, void *stream);
+
 /* Attention of the batch's new tokens over the paged cache (their own keys and
  * values appended before): out = softmax(scale q.k) v over the keys at
  * positions j <= p of the row's sequence and, with window > 0, only those with
  * j > p - window or j < sinks. Query head h reads key head h / (n_head /
  * n_kv_head). A row that sees no key gives zeros. q and out are rows of n_head *
- * head_dim values, both fp32 or (with bf16 pages) both bf16; sums, maxima and
+ * head_dim values, both fp32 or (unless the pages are fp32) both bf16; sums, maxima and
  * softmax are fp32. fp32 rows come out as exact as fp32 products give them
  * (operands in three bf16 terms); bf16 ones are within half a bf16 step of that
  * in launches of few rows, and in those of many take the probabilities rounded
