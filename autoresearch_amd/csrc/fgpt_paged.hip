@@ -151,6 +151,35 @@ int32_t check_attn(const fg_pages* pages, const fg_ragged* batch, const fg_attn_
   return FG_OK;
 }
 
+int32_t check_prefix(const fg_prefix* f, const fg_ragged* b) {
+  CHECK(f && f->seq_start && f->shared, "prefix: NULL argument");
+  CHECK(f->n_group >= 1 && f->n_group <= b->n_seq, "prefix: n_group %d outside 1..%d sequences", f->n_group, b->n_seq);
+  CHECK(f->max_shared >= 0 && f->max_shared <= b->max_kv, "prefix: max_shared %d outside 0..max_kv %d",
+        f->max_shared, b->max_kv);
+  return FG_OK;
+}
+
+// What both attention calls ask of their rows and workspace.
+int32_t check_rows(const fg_pages* pages, const fg_ragged* batch, const fg_attn_cfg* cfg, const void* q,
+                   const void* out, const void* work, int64_t work_bytes, int64_t need) {
+  CHECK(q && out, "q or out is NULL");
+  CHECK(aligned(q) && aligned(out) && aligned(work), "q, out or work is not 16-byte aligned");
+  const int64_t packed = (int64_t)cfg->n_head * pages->head_dim;
+  CHECK(out != q || batch->n_rows == 1 ||
+            (cfg->q_ld ? cfg->q_ld : packed) == (cfg->out_ld ? cfg->out_ld : packed),
+        "out is q with another row distance");
+  CHECK(need == 0 || (work && work_bytes >= need), "work: %lld bytes needed, %lld given",
+        (long long)need, (long long)(work ? work_bytes : 0));
+  return FG_OK;
+}
+
+PagedOut out_rows(const fg_pages* pages, const fg_attn_cfg* cfg, void* out) {
+  PagedOut o;
+  o.y = out;
+  o.ld = cfg->out_ld ? cfg->out_ld : (int64_t)cfg->n_head * pages->head_dim;
+  return o;
+}
+
 // The pages that a copy list has named, by hash: room for those alone, whatever
 // the pool holds; on the stack up to SMALL pairs.
 class Named {
@@ -197,22 +226,35 @@ extern "C" int32_t fg_paged_attn(const fg_pages* pages, const fg_ragged* batch,
                                  int64_t work_bytes, void* stream) {
   RCCHK(check_attn(pages, batch, cfg));
   if (batch->n_rows == 0 || batch->max_q == 0) return FG_OK;
-  CHECK(q && out, "q or out is NULL");
-  CHECK(aligned(q) && aligned(out) && aligned(work), "q, out or work is not 16-byte aligned");
-  const int64_t packed = (int64_t)cfg->n_head * pages->head_dim;
-  CHECK(out != q || batch->n_rows == 1 ||
-            (cfg->q_ld ? cfg->q_ld : packed) == (cfg->out_ld ? cfg->out_ld : packed),
-        "out is q with another row distance");
-  const int64_t need = 4 * paged_attn_floats(*pages, *batch, *cfg);
-  CHECK(need == 0 || (work && work_bytes >= need), "work: %lld bytes needed, %lld given",
-        (long long)need, (long long)(work ? work_bytes : 0));
+  RCCHK(check_rows(pages, batch, cfg, q, out, work, work_bytes, 4 * paged_attn_floats(*pages, *batch, *cfg)));
   OnStream on;
   RCCHK(on.enter(stream));
-  PagedOut o;
-  o.y = out;
-  o.ld = cfg->out_ld ? cfg->out_ld : packed;
-  launch_paged_attn((hipStream_t)stream, *pages, *batch, *cfg, q, o, (float*)work);
+  launch_paged_attn((hipStream_t)stream, *pages, *batch, *cfg, q, out_rows(pages, cfg, out), (float*)work);
   return launched("paged attention");
+}
+
+// ------------------------------------------------------------ shared prefixes
+extern "C" int32_t fg_prefix_attn_work(const fg_pages* pages, const fg_ragged* batch,
+                                       const fg_prefix* prefix, const fg_attn_cfg* cfg, int64_t* bytes) {
+  CHECK(bytes, "bytes is NULL");
+  RCCHK(check_attn(pages, batch, cfg));
+  RCCHK(check_prefix(prefix, batch));
+  *bytes = batch->n_rows && batch->max_q ? 4 * prefix_attn_floats(*pages, *batch, *prefix, *cfg) : 0;
+  return FG_OK;
+}
+
+extern "C" int32_t fg_prefix_attn(const fg_pages* pages, const fg_ragged* batch, const fg_prefix* prefix,
+                                  const fg_attn_cfg* cfg, const void* q, void* out, void* work,
+                                  int64_t work_bytes, void* stream) {
+  RCCHK(check_attn(pages, batch, cfg));
+  RCCHK(check_prefix(prefix, batch));
+  if (batch->n_rows == 0 || batch->max_q == 0) return FG_OK;
+  RCCHK(check_rows(pages, batch, cfg, q, out, work, work_bytes,
+                   4 * prefix_attn_floats(*pages, *batch, *prefix, *cfg)));
+  OnStream on;
+  RCCHK(on.enter(stream));
+  launch_prefix_attn((hipStream_t)stream, *pages, *batch, *prefix, *cfg, q, out_rows(pages, cfg, out), (float*)work);
+  return launched("prefix attention");
 }
 
 // ------------------------------------------------------------ append

@@ -1029,5 +1029,22 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
   if (!to.whole && g == 0) *(float2*)(to.ml + 2 * r) = make_float2(m_run, l);
 }
 
+// How a launch is cut (kern_paged.hip).
+struct PagedPlan {
+  bool many;
+  bool one_tile;
+  int rt;      // rows of a tile
+  int ntile, nsplit, cpt;
+  int64_t floats;
+};
+// (a constant, not the current device's: a workspace asked for with one device
+// current serves a launch on another)
+constexpr int64_t PAGED_CUS = 256;
+
 }  // namespace paged
+
+paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c);
+paged::PagedArgs paged_args(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, const paged::PagedPlan& pl,
+                            const void* q, const PagedOut& out, float* work);
+
 }  // namespace fgpt

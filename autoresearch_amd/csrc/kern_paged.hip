@@ -108,17 +108,7 @@ __global__ __launch_bounds__(256) void k_paged_merge(PagedArgs p) {
 
 // ------------------------------------------------------------ host side
 
-// (a constant, not the current device's: a workspace asked for with one device
-// current serves a launch on another)
-constexpr int64_t CUS = 256;
-
-struct Plan {
-  bool many;
-  bool one_tile;
-  int rt;      // rows of a tile
-  int ntile, nsplit, cpt;
-  int64_t floats;
-};
+constexpr int64_t CUS = PAGED_CUS;
 
 // The tiles of a launch and the parts its keys are cut into, from the bounds
 // alone (lengths may differ under a captured launch).
@@ -139,8 +129,8 @@ struct Plan {
 // chunks and tokens of 9 sequences, 10 heads on 2, 92 -> 123, one fp32 prompt of
 // 2048 75 -> 95).
 constexpr int64_t MANY_WORK = 6000;
-Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
-  Plan pl;
+PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
+  PagedPlan pl;
   const int64_t G = c.n_head / pg.n_kv_head;
   // (no sequence has more new tokens than there are rows, whatever the caller's
   // bound; G of them per row stay far below 2^31)
@@ -214,9 +204,10 @@ int64_t paged_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_attn_
   return plan_of(pg, b, c).floats;
 }
 
-void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c,
-                       const void* q, const PagedOut& out, float* work) {
-  const Plan pl = plan_of(pg, b, c);
+paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) { return plan_of(pg, b, c); }
+
+paged::PagedArgs paged_args(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, const paged::PagedPlan& pl,
+                            const void* q, const PagedOut& out, float* work) {
   PagedArgs a;
   a.k = pg.k;
   a.v = pg.v;
@@ -243,6 +234,13 @@ void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, co
   a.nsplit = pl.nsplit;
   a.cpt = pl.cpt;
   a.part = work;
+  return a;
+}
+
+void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c,
+                       const void* q, const PagedOut& out, float* work) {
+  const PagedPlan pl = plan_of(pg, b, c);
+  const PagedArgs a = paged_args(pg, b, c, pl, q, out, work);
   if (pg.head_dim == 128)
     launch_hd<128>(s, a, pl.many, c.type == FG_F32, pg.type);
   else

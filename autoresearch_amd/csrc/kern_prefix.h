@@ -1,0 +1,285 @@
+// kern_prefix.h -- attention of a batch whose sequences share the pages of their
+// first positions (fg_prefix_attn of include/fgpt.h): kernels of the loops in
+// kern_paged.h, compiled for the page types in kern_prefix.hip and
+// kern_prefix_codes.hip.
+//
+// Softmax over a union of key sets comes from each set's (maximum, sum, weighted
+// values): the rows of all of a group's sequences, which follow one another,
+// go over the shared keys as if they were one sequence's (a row's position, which
+// windows ask for, is its own), each sequence's rows over its own keys, and a
+// second launch joins the parts. Both kinds of items are in one launch. The shared
+// keys are then read once a group (by each row tile of it), not once a sequence.
+// They end at a multiple of 32, the key tile; what is left is read per sequence.
+#pragma once
+#include "kern_paged.h"
+
+namespace fgpt {
+namespace paged {
+
+struct PrefixArgs {
+  PagedArgs a;  // the sequences' own keys
+  const int32_t* seq_start;
+  const int32_t* shared;
+  int n_group, max_shared;
+  int ptile;   // bound on the row tiles of all groups
+  int psplit;  // key parts of one
+  int pcpt;    // 32-key tiles of a part
+  float* po;   // [psplit][KH][n_rows * G][HD]: parts of the rows over shared keys,
+  float* pml;  // and [..][2]: their maxima and sums
+};
+
+// The shared keys of group g that are read as such.
+__device__ __forceinline__ int shared_keys(const PrefixArgs& x, int g) {
+  return max(0, min(x.shared[g], x.max_shared)) & ~31;
+}
+
+// Shared keys of the group that sequence seq belongs to; 0: none.
+__device__ __forceinline__ int shared_of(const PrefixArgs& x, int seq) {
+  const int lane = threadIdx.x & 63;
+  for (int g0 = 0; g0 < x.n_group; g0 += 64) {
+    const int g = g0 + lane;
+    const bool in = g < x.n_group;
+    const int from = in ? x.seq_start[g] : 0, to = in ? x.seq_start[g + 1] : 0;
+    const int n = in ? shared_keys(x, g) : 0;
+    const uint64_t here = __ballot(in && from <= seq && seq < to);
+    if (here) return __builtin_amdgcn_readlane(n, __builtin_ctzll(here));
+  }
+  return 0;
+}
+
+// A row tile of a group: RowTile of its rows over the shared keys (seq: the
+// group's first sequence, whose table names them; pos0 is not used), and the
+// group's last sequence.
+template <int RT>
+__device__ __forceinline__ bool find_group_tile(const PrefixArgs& x, int id, RowTile& t, int& seq_end) {
+  const PagedArgs& p = x.a;
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int g0 = 0; g0 < x.n_group; g0 += 64) {
+    const int g = g0 + lane;
+    int s0 = 0, s1 = 0, row = 0, rows = 0, keys = 0;
+    if (g < x.n_group) {
+      s0 = max(0, min(x.seq_start[g], p.n_seq));
+      s1 = max(s0, min(x.seq_start[g + 1], p.n_seq));
+      row = p.q_start[s0];
+      keys = shared_keys(x, g);
+      rows = row < 0 || keys == 0 ? 0 : max(0, min(p.q_start[s1], p.n_rows) - row) * p.G;
+    }
+    const int n = (rows + RT - 1) / RT;
+    int sum = n;  // tiles of this step's groups up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += up;
+    }
+    const uint64_t past = __ballot(base + sum > id);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      const int first = base + __builtin_amdgcn_readlane(sum - n, l);
+      t.seq = __builtin_amdgcn_readlane(s0, l);
+      seq_end = __builtin_amdgcn_readlane(s1, l);
+      t.row0 = __builtin_amdgcn_readlane(row, l);
+      t.r0 = (id - first) * RT;
+      t.rows = min(RT, __builtin_amdgcn_readlane(rows, l) - t.r0);
+      t.pos0 = 0;
+      t.kv = t.hi = __builtin_amdgcn_readlane(keys, l);
+      t.lo = t.sa = 0;
+      return true;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return false;
+}
+
+// Position of a row of the group's sequences s0 .. s1-1, the first of whose rows
+// is row0.
+__device__ __forceinline__ int row_position(const PagedArgs& p, int s0, int s1, int row0, int row) {
+  int s = min(s0 + row - row0, s1 - 1);  // (right where every sequence has one new token)
+  if (!__all(p.q_start[s] <= row && row < p.q_start[s + 1])) {
+    s = s0;
+    for (int n = s1 - s0; n > 1;) {  // the last sequence that starts at or before the row
+      const int half = n / 2;
+      if (p.q_start[s + half] <= row) s += half;
+      n -= half;
+    }
+  }
+  return max(0, min(p.kv_len[s], p.max_kv)) - (p.q_start[s + 1] - row);
+}
+
+// A window's first key of the tile's rows: what is before it and behind the
+// sinks, none of them sees.
+__device__ __forceinline__ void see_from(const PagedArgs& p, RowTile& t, int first_pos) {
+  t.lo = max(0, min(first_pos - p.window + 1, t.hi));
+  t.sa = min(p.sinks, t.lo);
+}
+
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v = min(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// Item (group tile, key head, part) over shared keys.
+template <int HD, bool QF, int KT, bool MANY>
+__device__ __forceinline__ void prefix_item(const PrefixArgs& x, uint8_t* lds, int b) {
+  constexpr int RT = MANY ? Many<HD, QF, KT>::RT : DR;
+  const PagedArgs& p = x.a;
+  const int kvh = b % p.KH, rest = b / p.KH;
+  const int id = rest % x.ptile, z = rest / x.ptile;
+  RowTile t;
+  int s1;
+  if (!find_group_tile<RT>(x, id, t, s1)) return;
+  const int lane = threadIdx.x & 63;
+  auto position = [&](int r) __attribute__((always_inline)) {  // of row r of the tile
+    return row_position(p, t.seq, s1, t.row0, t.row0 + (t.r0 + min(r, t.rows - 1)) / p.G);
+  };
+  const int own = MANY ? 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + (lane & 31) : lane & 15;
+  const int pos = position(own);
+  if (p.window > 0) {
+    int first = MANY ? min(position(lane), position(lane + 64)) : pos;
+    see_from(p, t, __builtin_amdgcn_readfirstlane(wave_min(first)));
+  }
+  const KeyTiles kt = key_tiles(t);
+  const int v0 = z * x.pcpt, v1 = max(v0, min(kt.n, v0 + x.pcpt));
+  auto place = [&] {
+    const int64_t row = ((int64_t)z * p.KH + kvh) * ((int64_t)p.n_rows * p.G) + (int64_t)t.row0 * p.G + t.r0;
+    return Place{false, x.po + row * HD, x.pml + row * 2};
+  };
+  if constexpr (MANY) {
+    auto pos_of = [&](int, int& first, int& last) __attribute__((always_inline)) {
+      first = __builtin_amdgcn_readfirstlane(wave_min(pos));
+      last = __builtin_amdgcn_readfirstlane(-wave_min(-pos));
+      return pos;
+    };
+    many_rows<HD, QF, KT>(p, lds, t, kt, kvh, v0, v1, pos_of, place);
+  } else {
+    few_rows<HD, QF, KT>(p, (float*)lds, t, kt, kvh, v0, v1, [&](int) { return pos; }, place);
+  }
+}
+
+// Item (row tile, key head, part) over the sequences' own keys.
+template <int HD, bool QF, int KT, bool MANY>
+__device__ __forceinline__ void own_item(const PrefixArgs& x, uint8_t* lds, int b) {
+  constexpr int RT = MANY ? Many<HD, QF, KT>::RT : DR;
+  const PagedArgs& p = x.a;
+  const int kvh = b % p.KH, rest = b / p.KH;
+  const int id = rest % p.ntile, z = rest / p.ntile;
+  RowTile t;
+  if (!find_tile<RT>(p, id, t)) return;
+  const int from = shared_of(x, t.seq);
+  const KeyTiles kt = key_tiles(t, from);
+  const int v0 = z * p.cpt, v1 = min(kt.n, v0 + p.cpt);
+  if (z > 0 && v0 >= kt.n) return;
+  auto place = [&] {
+    float* P0 = p.part + ((int64_t)(id * p.KH + kvh) * p.nsplit + z) * part_floats<HD>(RT);
+    return Place{from == 0 && kt.n <= p.cpt, P0, P0 + RT * HD};
+  };
+  if constexpr (MANY) {
+    auto pos_of = [&](int tok, int& first, int& last) __attribute__((always_inline)) {
+      const int w0 = 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      first = t.pos0 + (t.r0 + min(w0, t.rows - 1)) / p.G;
+      last = t.pos0 + (t.r0 + min(w0 + 32, t.rows) - 1) / p.G;
+      return t.pos0 + tok;
+    };
+    many_rows<HD, QF, KT>(p, lds, t, kt, kvh, v0, v1, pos_of, place);
+  } else {
+    few_rows<HD, QF, KT>(p, (float*)lds, t, kt, kvh, v0, v1, [&](int tok) { return t.pos0 + tok; }, place);
+  }
+}
+
+// PM, SM: 128-row tiles over the shared keys, over the sequences' own. The shared
+// ones' items come first, being the longer ones.
+template <int HD, bool QF, int KT, bool PM, bool SM>
+__global__ __launch_bounds__(256, 2) void k_prefix(PrefixArgs x) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int shared_items = x.ptile * x.a.KH * x.psplit;
+  if ((int)blockIdx.x < shared_items)
+    prefix_item<HD, QF, KT, PM>(x, lds, blockIdx.x);
+  else
+    own_item<HD, QF, KT, SM>(x, lds, blockIdx.x - shared_items);
+}
+
+// The parts of a row joined: those over shared keys, then its own, in order; a
+// thread per row and four head dims, up to 8 parts in flight.
+template <int HD, bool QF, int RT>
+__global__ __launch_bounds__(256) void k_prefix_merge(PrefixArgs x) {
+  constexpr int PER = 1024 / HD;  // rows a workgroup takes
+  constexpr int64_t PF = part_floats<HD>(RT);
+  const PagedArgs& p = x.a;
+  const int sub = blockIdx.x % (RT / PER), item = blockIdx.x / (RT / PER);
+  const int kvh = item % p.KH, id = item / p.KH;
+  const int r = sub * PER + threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
+  RowTile t;
+  if (!find_tile<RT>(p, id, t)) return;
+  const int from = shared_of(x, t.seq);
+  const KeyTiles kt = key_tiles(t, from);
+  if ((from == 0 && kt.n <= p.cpt) || r >= t.rows) return;  // (written by the attention kernel itself)
+  const int ns = max(1, (kt.n + p.cpt - 1) / p.cpt), np = from ? x.psplit : 0, n = np + ns;
+  const int rr = t.r0 + r;
+  const int64_t NR = (int64_t)p.n_rows * p.G, R = (int64_t)kvh * NR + (int64_t)t.row0 * p.G + rr;
+  const float* P0 = p.part + (int64_t)item * p.nsplit * PF;
+  float m = -FLT_MAX, l = 0.f;
+  float a[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < n; k0 += 8) {
+    float2 s[8];
+    float4 o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int j = k0 + k;
+      if (j >= n) break;
+      const int64_t row = (int64_t)j * p.KH * NR + R;
+      const float* own = P0 + (int64_t)(j - np) * PF;
+      s[k] = *(const float2*)(j < np ? x.pml + row * 2 : own + RT * HD + 2 * r);
+      o[k] = *(const float4*)(j < np ? x.po + row * HD + d : own + r * HD + d);
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = k0 + k < n ? fmaxf(top, s[k].x) : top;
+    const float f = exp2f(m - top);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) a[e] *= f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k0 + k >= n) break;
+      const float w = exp2f(s[k].x - m);
+      l += w * s[k].y;
+      a[0] += w * o[k].x;
+      a[1] += w * o[k].y;
+      a[2] += w * o[k].z;
+      a[3] += w * o[k].w;
+    }
+  }
+  const float inv = inv_sum(l);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] *= inv;
+  store_row4<QF>(p, t.row0 + rr / p.G, (kvh * p.G + rr % p.G) * HD + d, a);
+}
+
+template <int HD, bool QF, int KT, bool PM, bool SM>
+void launch_prefix_t(hipStream_t s, const PrefixArgs& x) {
+  typedef Many<HD, QF, KT> C;
+  constexpr int lds = (PM || SM) && C::LDS > few_lds<HD>() ? C::LDS : few_lds<HD>();
+  constexpr int RT = SM ? C::RT : DR;
+  static std::atomic<uint64_t> lds_set{0};
+  raise_lds_once((const void*)k_prefix<HD, QF, KT, PM, SM>, lds, &lds_set);
+  const int items = (x.ptile * x.psplit + x.a.ntile * x.a.nsplit) * x.a.KH;
+  FG_LAUNCH((k_prefix<HD, QF, KT, PM, SM>), dim3((unsigned)items), dim3(256), lds, s, x);
+  FG_LAUNCH((k_prefix_merge<HD, QF, RT>), dim3((unsigned)(x.a.ntile * x.a.KH * (RT * HD / 1024))), dim3(256), 0,
+            s, x);
+}
+
+template <int HD, bool QF, int KT>
+void launch_prefix_m(hipStream_t s, const PrefixArgs& x, bool pm, bool sm) {
+  if (sm) launch_prefix_t<HD, QF, KT, true, true>(s, x);
+  else if (pm) launch_prefix_t<HD, QF, KT, true, false>(s, x);
+  else launch_prefix_t<HD, QF, KT, false, false>(s, x);
+}
+
+}  // namespace paged
+
+// Page types of kern_prefix_codes.hip (8-bit ones).
+void launch_prefix_codes(hipStream_t s, const paged::PrefixArgs& x, int32_t hd, bool qf, int32_t kt, bool pm, bool sm);
+
+}  // namespace fgpt

@@ -1,0 +1,74 @@
+// kern_prefix.hip -- kern_prefix.h's kernels for fp32 and bf16 pages, and the plan
+// of its launches.
+#include "kern_prefix.h"
+
+namespace fgpt {
+
+namespace {
+
+using namespace paged;
+
+struct Plan {
+  bool pm, sm;
+  int ptile, psplit, pcpt;
+  PagedPlan own;
+  int64_t po, pml, part, floats;  // places in the workspace
+};
+
+Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_prefix& f, const fg_attn_cfg& c) {
+  Plan pl;
+  pl.own = paged_plan(pg, b, c);
+  pl.sm = pl.own.many;
+  const int64_t G = c.n_head / pg.n_kv_head, KH = pg.n_kv_head, NR = b.n_rows * G;
+  const int64_t nkt = f.max_shared / 32;
+  auto tiles = [&](int64_t rt) { return nkt ? NR / rt + std::min<int64_t>(f.n_group, NR) : 0; };
+  // (rows of a group on average: no bound of one is given)
+  pl.pm = pl.sm || (NR / std::max(1, f.n_group) > 32 && tiles(DR) * KH * nkt > 6000);
+  pl.ptile = (int)tiles(pl.pm ? Many<128, true, FG_F32>::RT : DR);
+  const int64_t items = std::max<int64_t>(1, pl.ptile * KH);
+  const int64_t want = ((pl.pm ? 2 : 1) * PAGED_CUS + items - 1) / items;
+  const int64_t ns = std::max<int64_t>(1, std::min(want, (nkt + RWV - 1) / RWV));
+  pl.pcpt = (int)((nkt + ns - 1) / ns + RWV - 1) / RWV * RWV;
+  pl.psplit = pl.pcpt ? (int)((nkt + pl.pcpt - 1) / pl.pcpt) : 0;
+  const int64_t prow = pl.psplit * KH * NR;
+  pl.po = 0;
+  pl.pml = prow * pg.head_dim;
+  pl.part = (pl.pml + 2 * prow + 3) / 4 * 4;
+  pl.floats = pl.part + (int64_t)pl.own.ntile * KH * pl.own.nsplit * pl.own.rt * (pg.head_dim + 2);
+  return pl;
+}
+
+template <int HD>
+void launch_hd(hipStream_t s, const PrefixArgs& x, bool qf, int32_t kt, bool pm, bool sm) {
+  if (kt == FG_F32) launch_prefix_m<HD, true, FG_F32>(s, x, pm, sm);
+  else if (qf) launch_prefix_m<HD, true, FG_BF16>(s, x, pm, sm);
+  else launch_prefix_m<HD, false, FG_BF16>(s, x, pm, sm);
+}
+
+}  // namespace
+
+int64_t prefix_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_prefix& f, const fg_attn_cfg& c) {
+  return plan_of(pg, b, f, c).floats;
+}
+
+void launch_prefix_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_prefix& f,
+                        const fg_attn_cfg& c, const void* q, const PagedOut& out, float* work) {
+  const Plan pl = plan_of(pg, b, f, c);
+  PrefixArgs x;
+  x.a = paged_args(pg, b, c, pl.own, q, out, work + pl.part);
+  x.seq_start = f.seq_start;
+  x.shared = f.shared;
+  x.n_group = f.n_group;
+  x.max_shared = f.max_shared;
+  x.ptile = pl.ptile;
+  x.psplit = pl.psplit;
+  x.pcpt = pl.pcpt;
+  x.po = work + pl.po;
+  x.pml = work + pl.pml;
+  const bool qf = c.type == FG_F32;
+  if (pg.type == FG_I8 || pg.type == FG_E4M3) launch_prefix_codes(s, x, pg.head_dim, qf, pg.type, pl.pm, pl.sm);
+  else if (pg.head_dim == 128) launch_hd<128>(s, x, qf, pg.type, pl.pm, pl.sm);
+  else launch_hd<64>(s, x, qf, pg.type, pl.pm, pl.sm);
+}
+
+}  // namespace fgpt

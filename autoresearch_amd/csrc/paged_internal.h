@@ -31,6 +31,11 @@ int64_t paged_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_attn_
 void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c,
                        const void* q, const PagedOut& out, float* work);
 
+// The same for a batch with shared prefixes.
+int64_t prefix_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_prefix& f, const fg_attn_cfg& c);
+void launch_prefix_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_prefix& f,
+                        const fg_attn_cfg& c, const void* q, const PagedOut& out, float* work);
+
 // ---- append, reading back and page copies
 void launch_qk_append(hipStream_t s, const fg_pages& pg, const fg_ragged& b, const fg_append_cfg& c,
                       const void* qkv, void* q_out);

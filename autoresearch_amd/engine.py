@@ -37,7 +37,8 @@ EXPORTS = (
     "fg_eval_bpb", "fg_rows_npy", "fg_decode_spec", "fg_spec_accept", "fg_spec_draft",
     "fg_sample", "fg_decode_sample", "fg_set_option", "fg_get_option", "fg_step_dev_noalloc",
     "fg_qk_append", "fg_paged_attn_work", "fg_paged_attn", "fg_pages_copy", "fg_draw_rows_work",
-    "fg_draw_rows", "fg_page_bytes", "fg_pages_read",
+    "fg_draw_rows", "fg_page_bytes", "fg_pages_read", "fg_prefix_attn_work",
+    "fg_prefix_attn",
     "fg_pool_create", "fg_pool_destroy", "fg_pool_len", "fg_pool_free", "fg_pool_table",
     "fg_pool_need", "fg_pool_extend", "fg_pool_fork", "fg_pool_trim", "fg_pool_slide",
     "fg_pool_compact",
@@ -116,6 +117,11 @@ class _AttnCfg(C.Structure):
                 ("out_ld", C.c_int64)]
 
 
+class _Prefix(C.Structure):
+    _fields_ = [("n_group", C.c_int32), ("max_shared", C.c_int32), ("seq_start", C.c_void_p),
+                ("shared", C.c_void_p)]
+
+
 class _DrawCfg(C.Structure):
     _fields_ = [("temp", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
                 ("min_p", C.c_void_p), ("u", C.c_void_p)]
@@ -186,6 +192,10 @@ def load_library(path: str = LIB_PATH):
                                      C.POINTER(i64)]),
         "fg_paged_attn": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_AttnCfg), _vp,
                                 _vp, _vp, i64, _vp]),
+        "fg_prefix_attn_work": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_Prefix),
+                                      C.POINTER(_AttnCfg), C.POINTER(i64)]),
+        "fg_prefix_attn": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_Prefix),
+                                 C.POINTER(_AttnCfg), _vp, _vp, _vp, i64, _vp]),
         "fg_pages_copy": (i32, [_vp, i32, i64, i32, i64, _vp, _vp, i32, _vp]),
         "fg_draw_rows_work": (i32, [i32, i32, C.POINTER(i64)]),
         "fg_draw_rows": (i32, [_vp, i32, i32, i64, C.POINTER(_DrawCfg), _vp, _vp, _vp, i64, _vp]),
@@ -766,6 +776,25 @@ def paged_attn(pg: _Pages, batch: _Ragged, cfg: _AttnCfg, q: int, out: int, work
                work_bytes: int = 0, stream: int = 0):
     """fg_paged_attn: the batch's new tokens over their sequences' pages."""
     _check(load_library().fg_paged_attn(pg, batch, cfg, q, out, work, work_bytes, stream))
+
+
+def prefix(seq_start: int, shared: int, n_group: int, max_shared: int) -> _Prefix:
+    """fg_prefix: groups of sequences (device int32 seq_start [n_group+1]) whose first
+    shared[g] positions (device int32 [n_group]) lie in the same pages."""
+    return _Prefix(n_group, max_shared, seq_start, shared)
+
+
+def prefix_attn_work(pg: _Pages, batch: _Ragged, pre: _Prefix, cfg: _AttnCfg) -> int:
+    """Bytes of device memory that prefix_attn needs as its workspace."""
+    n = C.c_int64()
+    _check(load_library().fg_prefix_attn_work(pg, batch, pre, cfg, C.byref(n)))
+    return n.value
+
+
+def prefix_attn(pg: _Pages, batch: _Ragged, pre: _Prefix, cfg: _AttnCfg, q: int, out: int, work: int = 0,
+                work_bytes: int = 0, stream: int = 0):
+    """fg_prefix_attn: paged_attn, the keys that a group's sequences share read once."""
+    _check(load_library().fg_prefix_attn(pg, batch, pre, cfg, q, out, work, work_bytes, stream))
 
 
 def pages_copy(base: int, n_planes: int, plane_bytes: int, n_pages: int, page_bytes: int, src, dst,

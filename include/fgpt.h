@@ -479,6 +479,31 @@ int32_t fg_paged_attn_work(const fg_pages *pages, const fg_ragged *batch, const 
 int32_t fg_paged_attn(const fg_pages *pages, const fg_ragged *batch, const fg_attn_cfg *cfg,
                       const void *q, void *out, void *work, int64_t work_bytes, void *stream);
 
+/* fg_paged_attn for a batch in which groups of sequences share the pages of their
+ * first positions (one instruction and many questions, one prompt and several
+ * answers): the same outputs, up to the order of sums, but the shared keys and
+ * values are read once for all of a group's rows, not once a sequence.
+ * Group g is sequences seq_start[g] .. seq_start[g+1]-1, whose tables name the same
+ * pages for positions 0 .. shared[g]-1 (those that some row sees; read from
+ * the table of the group's first sequence) and whose new tokens all sit at position
+ * shared[g] or later. seq_start[0] is 0 and seq_start does not fall; sequences from
+ * seq_start[n_group] on share nothing, and so does a group with shared[g] 0.
+ * max_shared bounds shared (a larger one counts as max_shared) and is at most
+ * max_kv of the batch; it sizes the launch with the batch's bounds. Shared
+ * positions are taken in whole 32s, what is left is read per sequence. What
+ * fg_paged_attn says of types, masks, NaN, bad pages, out and work holds here, with
+ * "group" for "sequence" where the rows of one can make another's NaN. */
+typedef struct fg_prefix {
+  int32_t n_group, max_shared;
+  const int32_t *seq_start; /* device [n_group + 1] */
+  const int32_t *shared;    /* device [n_group]     */
+} fg_prefix;
+int32_t fg_prefix_attn_work(const fg_pages *pages, const fg_ragged *batch, const fg_prefix *prefix,
+                            const fg_attn_cfg *cfg, int64_t *bytes);
+int32_t fg_prefix_attn(const fg_pages *pages, const fg_ragged *batch, const fg_prefix *prefix,
+                       const fg_attn_cfg *cfg, const void *q, void *out, void *work,
+                       int64_t work_bytes, void *stream);
+
 /* Page src[i] copied to page dst[i] in each of n_planes arrays of n_pages pages
  * (plane_bytes apart; a cache's layers, keys and values), i < n. src and dst
  * are host arrays, read before the call returns; no page may be named twice in
