@@ -24,7 +24,8 @@ FLANG = os.environ.get("FC_AMD", "/opt/rocm/bin/amdflang")
 HIP_SOURCES = ["fgpt_engine.hip", "fgpt_weights.hip", "fgpt_spec.hip", "kern_core.hip",
                "kern_gemm.hip", "kern_rows.hip", "kern_attn.hip", "kern_sample.hip", "kern_fused.hip",
                "kern_fused_gqa.hip", "fgpt_paged.hip", "fgpt_pool.hip", "kern_paged.hip",
-               "kern_pages.hip", "kern_draw.hip", "kern_prefix.hip", "kern_prefix_codes.hip"]
+               "kern_pages.hip", "kern_draw.hip", "kern_prefix.hip", "kern_prefix_codes.hip",
+               "kern_adjust.hip"]
 HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-Wall", "-Wno-unused-function", "-Wno-unused-result"]

@@ -337,6 +337,45 @@ extern "C" int32_t fg_pages_copy(void* base, int32_t n_planes, int64_t plane_byt
   return launched("page copy");
 }
 
+// ------------------------------------------------------------ logits
+namespace {
+
+int32_t check_adjust(const fg_adjust_cfg* c, int32_t rows, int32_t V) {
+  CHECK(c, "cfg is NULL");
+  CHECK(c->n_hist >= 0 && c->n_bias >= 0 && c->n_mask >= 0, "n_hist, n_bias and n_mask must be >= 0");
+  CHECK(c->n_hist <= 1 << 30 && c->n_bias <= 1 << 30, "n_hist or n_bias above 2^30");
+  CHECK(c->n_hist == 0 || (c->hist && c->hist_start), "hist or hist_start is NULL");
+  CHECK(c->n_bias == 0 || (c->bias && c->bias_id && c->bias_start), "bias, bias_id or bias_start is NULL");
+  CHECK(c->n_mask == 0 || c->mask, "mask is NULL");
+  CHECK(c->mask_ld == 0 || (c->mask_ld >= (V + 31) / 32 && c->mask_ld < ((int64_t)1 << 30)),
+        "mask_ld %lld: 0, or %d words and more", (long long)c->mask_ld, (V + 31) / 32);
+  CHECK(c->n_mask == 0 || c->mask_row || c->n_mask >= rows, "%d masks for %d rows, and no mask_row", c->n_mask, rows);
+  return FG_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t fg_adjust_rows(const float* logits, int32_t rows, int32_t V, int64_t ld,
+                                  const fg_adjust_cfg* cfg, float* out, int64_t out_ld, void* stream) {
+  CHECK(rows >= 0, "rows must be >= 0");
+  CHECK(V >= 1 && V <= DRAW_MAX_V, "V %d outside 1..%d", V, DRAW_MAX_V);
+  CHECK(rows <= 1 << 21, "rows %d above 2^21", rows);
+  CHECK(ld >= V && ld < ((int64_t)1 << 40), "ld %lld below V %d", (long long)ld, V);
+  CHECK(out_ld >= V && out_ld < ((int64_t)1 << 40), "out_ld %lld below V %d", (long long)out_ld, V);
+  RCCHK(check_adjust(cfg, rows, V));
+  if (rows == 0) return FG_OK;
+  CHECK(logits && out, "logits or out is NULL");
+  CHECK(out != logits || rows == 1 || ld == out_ld, "out is logits with another row distance");
+  fg_adjust_cfg c = *cfg;  // (lists of nothing are none)
+  if (c.n_hist == 0) c.hist = nullptr;
+  if (c.n_bias == 0) c.bias = nullptr;
+  if (c.n_mask == 0) c.mask = nullptr;
+  OnStream on;
+  RCCHK(on.enter(stream));
+  launch_adjust_rows((hipStream_t)stream, logits, rows, V, ld, c, out, out_ld);
+  return launched("adjusting logits");
+}
+
 // ------------------------------------------------------------ draws
 extern "C" int32_t fg_draw_rows_work(int32_t rows, int32_t V, int64_t* bytes) {
   CHECK(bytes, "bytes is NULL");

@@ -63,6 +63,10 @@ struct PoolMoves {
 void pool_plan_moves(const fg_pool* p, PoolMoves* m);  // (may throw)
 void pool_apply_moves(fg_pool* p, PoolMoves* m);       // (does not)
 
+// ---- logits
+void launch_adjust_rows(hipStream_t s, const float* x, int32_t rows, int32_t V, int64_t ld, const fg_adjust_cfg& c,
+                        float* out, int64_t out_ld);
+
 // ---- draws
 constexpr int32_t DRAW_MAX_V = 1 << 18;
 int64_t draw_work_bytes(int32_t rows, int32_t V);

@@ -38,7 +38,7 @@ EXPORTS = (
     "fg_sample", "fg_decode_sample", "fg_set_option", "fg_get_option", "fg_step_dev_noalloc",
     "fg_qk_append", "fg_paged_attn_work", "fg_paged_attn", "fg_pages_copy", "fg_draw_rows_work",
     "fg_draw_rows", "fg_page_bytes", "fg_pages_read", "fg_prefix_attn_work",
-    "fg_prefix_attn",
+    "fg_prefix_attn", "fg_adjust_rows",
     "fg_pool_create", "fg_pool_destroy", "fg_pool_len", "fg_pool_free", "fg_pool_table",
     "fg_pool_need", "fg_pool_extend", "fg_pool_fork", "fg_pool_trim", "fg_pool_slide",
     "fg_pool_compact",
@@ -122,6 +122,12 @@ class _Prefix(C.Structure):
                 ("shared", C.c_void_p)]
 
 
+class _AdjustCfg(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("hist", "hist_start", "count_from", "rep", "pres", "freq", "bias",
+                                          "bias_id", "bias_start", "mask", "mask_row")] + \
+               [("mask_ld", C.c_int64), ("n_hist", C.c_int32), ("n_bias", C.c_int32), ("n_mask", C.c_int32)]
+
+
 class _DrawCfg(C.Structure):
     _fields_ = [("temp", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p),
                 ("min_p", C.c_void_p), ("u", C.c_void_p)]
@@ -197,6 +203,7 @@ def load_library(path: str = LIB_PATH):
         "fg_prefix_attn": (i32, [C.POINTER(_Pages), C.POINTER(_Ragged), C.POINTER(_Prefix),
                                  C.POINTER(_AttnCfg), _vp, _vp, _vp, i64, _vp]),
         "fg_pages_copy": (i32, [_vp, i32, i64, i32, i64, _vp, _vp, i32, _vp]),
+        "fg_adjust_rows": (i32, [_vp, i32, i32, i64, C.POINTER(_AdjustCfg), _vp, i64, _vp]),
         "fg_draw_rows_work": (i32, [i32, i32, C.POINTER(i64)]),
         "fg_draw_rows": (i32, [_vp, i32, i32, i64, C.POINTER(_DrawCfg), _vp, _vp, _vp, i64, _vp]),
         "fg_pool_create": (i32, [i32, i32, i32, C.POINTER(_vp)]),
@@ -805,6 +812,19 @@ def pages_copy(base: int, n_planes: int, plane_bytes: int, n_pages: int, page_by
         raise ValueError("src and dst must hold one page each per copy")
     _check(load_library().fg_pages_copy(base, n_planes, plane_bytes, n_pages, page_bytes,
                                         src.ctypes.data, dst.ctypes.data, src.size, stream))
+
+
+def adjust_cfg(hist: int = 0, hist_start: int = 0, n_hist: int = 0, count_from: int = 0, rep: int = 0,
+               pres: int = 0, freq: int = 0, bias: int = 0, bias_id: int = 0, bias_start: int = 0,
+               n_bias: int = 0, mask: int = 0, mask_row: int = 0, n_mask: int = 0, mask_ld: int = 0) -> _AdjustCfg:
+    """fg_adjust_cfg: histories and penalties, biases, masks (device arrays, 0 = off)."""
+    return _AdjustCfg(hist, hist_start, count_from, rep, pres, freq, bias, bias_id, bias_start, mask, mask_row,
+                      mask_ld, n_hist, n_bias, n_mask)
+
+
+def adjust_rows(logits: int, rows: int, V: int, ld: int, cfg: _AdjustCfg, out: int, out_ld: int, stream: int = 0):
+    """fg_adjust_rows: penalties, biases and masks on rows of logits (out may be logits)."""
+    _check(load_library().fg_adjust_rows(logits, rows, V, ld, cfg, out, out_ld, stream))
 
 
 def draw_rows_work(rows: int, V: int) -> int:

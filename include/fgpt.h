@@ -513,6 +513,37 @@ int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t
                       int64_t page_bytes, const int32_t *src, const int32_t *dst, int32_t n,
                       void *stream);
 
+/* Logits before a draw: penalties over each row's history, biases, a grammar's mask.
+ * out [rows][out_ld] = x [rows][ld] (fp32, V <= 262144 used; out may be x, with one
+ * row distance), each step where its arrays are given, in fp32:
+ *  1. history: row r's ids are hist[hist_start[r] .. hist_start[r+1]-1]. With n_i
+ *     how often id i is among those from index count_from[r] (of the row's part;
+ *     NULL: 0) on: where n_i > 0, x_i = (x_i - pres) - freq * n_i. Then for every
+ *     id of the whole history, x_i = x_i > 0 ? x_i / rep : x_i * rep. (fg_sample
+ *     takes these two steps in the same order; its rep divides whatever the sign.)
+ *     count_from serves prompts, which rep alone counts, and windows.
+ *  2. bias: x_i += bias[k] for bias_id[k] = i, k in bias_start[r] ..
+ *     bias_start[r+1]-1; several of one id are added up in their order first.
+ *  3. mask: bits, id i of mask m is bit i % 32 of mask[m * mask_ld + i / 32]; 0: x_i =
+ *     -inf, whatever it was. Row r has mask mask_row[r] (NULL: r); one not in
+ *     [0, n_mask) masks nothing. mask_ld in words, 0 = packed.
+ * rep, pres and freq are per row (device, each nullable = off; all off: no history);
+ * a NaN setting and a rep not above 0 are off. Ids outside [0, V) are passed over, parts
+ * of lists outside [0, n_hist) or [0, n_bias) cut off. The results do not depend on
+ * any order of execution. No workspace. */
+typedef struct fg_adjust_cfg {
+  const int32_t *hist, *hist_start, *count_from; /* device [n_hist], [rows + 1], [rows] */
+  const float *rep, *pres, *freq;                /* device [rows] */
+  const float *bias;                             /* device [n_bias] */
+  const int32_t *bias_id, *bias_start;           /* device [n_bias], [rows + 1] */
+  const uint32_t *mask;                          /* device [n_mask][mask_ld] */
+  const int32_t *mask_row;                       /* device [rows] */
+  int64_t mask_ld;
+  int32_t n_hist, n_bias, n_mask;
+} fg_adjust_cfg;
+int32_t fg_adjust_rows(const float *logits, int32_t rows, int32_t V, int64_t ld,
+                       const fg_adjust_cfg *cfg, float *out, int64_t out_ld, void *stream);
+
 /* One id a row of logits [rows][ld] (V <= 262144 used) from given uniform
  * numbers. With e_i = exp((x_i - max x) / temp): of the ids, the top_k largest
  * are kept (ties: the lowest id first); of those, in descending order, each one

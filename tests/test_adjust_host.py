@@ -1,0 +1,40 @@
+"""Refusals of fg_adjust_rows, on the CPU: arguments are checked before anything
+asks for a device."""
+import pytest
+
+from autoresearch_amd import engine
+
+from .test_paged_host import P, no_gpu, refused
+
+
+def adjust(rows=2, V=100, ld=100, out_ld=100, x=P, out=P, **kw):
+    engine.adjust_rows(x, rows, V, ld, engine.adjust_cfg(**kw), out, out_ld)
+
+
+@pytest.mark.parametrize("match,kw", [
+    ("rows", dict(rows=-1)), ("rows", dict(rows=(1 << 21) + 1)), ("V 0", dict(V=0)),
+    ("V", dict(V=(1 << 18) + 1, ld=1 << 20, out_ld=1 << 20)), ("ld", dict(ld=99)), ("out_ld", dict(out_ld=99)),
+    ("NULL", dict(x=0)), ("NULL", dict(out=0)), ("another row distance", dict(out_ld=104)),
+    ("hist or hist_start", dict(n_hist=3, hist=P)), ("hist or hist_start", dict(n_hist=3, hist_start=P)),
+    ("n_hist", dict(n_hist=-1)), ("n_hist", dict(n_hist=(1 << 30) + 1, hist=P, hist_start=P)),
+    ("n_bias", dict(n_bias=-1)), ("bias", dict(n_bias=1, bias=P, bias_id=P)),
+    ("bias", dict(n_bias=1, bias_start=P, bias_id=P)), ("mask is NULL", dict(n_mask=1)),
+    ("n_mask", dict(n_mask=-1)), ("mask_ld", dict(mask=P, n_mask=2, mask_ld=3)),
+    ("mask_ld", dict(mask_ld=-4)), ("1 masks for 2 rows", dict(mask=P, n_mask=1))])
+def test_bad_adjust(match, kw):
+    refused(match, adjust, **kw)
+
+
+def test_no_cfg():
+    assert engine.load_library().fg_adjust_rows(P, 2, 100, 100, None, P, 100, None) == -1
+
+
+def test_nothing_to_do():
+    adjust(rows=0, x=0, out=0)
+
+
+@pytest.mark.skipif(not no_gpu(), reason="a GPU is visible")
+def test_no_device():
+    with pytest.raises(engine.FgptError) as e:
+        adjust()
+    assert e.value.code in (-7, -4)
