@@ -44,16 +44,21 @@ __device__ __forceinline__ float setting(const float* p, int row, float off) {
   return v == v ? v : off;
 }
 
+// Few ids of a slice change: the history's are listed as they are first counted,
+// and new values are made entry by entry, from logits read again, not id by id
+// (a quotient for each of 16 ids a thread took as long as the row itself). They
+// are kept where the counts were, for the thread that writes the id.
 template <int QUADS>
 __global__ __launch_bounds__(AT) void k_adjust(AdjustArgs a) {
 #pragma clang fp contract(off)
-  constexpr int SLICE = 4 * AT * QUADS;
-  __shared__ __attribute__((aligned(16))) uint32_t cnt[SLICE];   // of the history
-  __shared__ __attribute__((aligned(16))) uint32_t nb[SLICE];    // biases of an id
-  __shared__ __attribute__((aligned(16))) float bias[SLICE];     // their sum
-  __shared__ int ids[AT];
+  constexpr int SLICE = 4 * AT * QUADS, HU = 8;  // history ids of a thread in flight
+  __shared__ __attribute__((aligned(16))) uint32_t cnt[SLICE];  // counts, then new values
+  __shared__ uint16_t list[SLICE];                              // ids of the history
+  // bits: ids with a new value; that a bias names; that several do
+  __shared__ uint32_t fresh[SLICE / 32], named[SLICE / 32], again[SLICE / 32];
+  __shared__ int n_list, twice;
+  __shared__ int ids[AT], n_wave[AT / 64];
   __shared__ float vals[AT];
-  __shared__ int twice;  // an id of the slice is named twice
   const int tid = threadIdx.x, row = blockIdx.x / a.slices, lo = blockIdx.x % a.slices * SLICE;
   const fg_adjust_cfg& c = a.c;
   const float* x = a.x + row * a.ld;
@@ -71,12 +76,12 @@ __global__ __launch_bounds__(AT) void k_adjust(AdjustArgs a) {
       for (int e = 0; e < 4; ++e) v[j][e] = i + e < a.V ? x[i + e] : 0.f;
     }
   }
-  uint32_t word[QUADS];
   int mask = -1;
   if (c.mask) {
     mask = c.mask_row ? c.mask_row[row] : row;
     if (mask >= c.n_mask) mask = -1;
   }
+  uint32_t word[QUADS];
 #pragma unroll
   for (int j = 0; j < QUADS; ++j) {
     const int i = lo + 4 * (tid + AT * j);
@@ -86,88 +91,120 @@ __global__ __launch_bounds__(AT) void k_adjust(AdjustArgs a) {
   Part h = {0, 0}, b = {0, 0};
   if (c.hist && (c.rep || c.pres || c.freq)) h = part_of(c.hist_start, row, c.n_hist);
   if (c.bias) b = part_of(c.bias_start, row, c.n_bias);
-  if (h.z > h.a || b.z > b.a) {
-#pragma unroll
-    for (int j = 0; j < QUADS; ++j) {
-      *(u32x4_t*)(cnt + 4 * (tid + AT * j)) = u32x4_t{0, 0, 0, 0};
-      *(u32x4_t*)(nb + 4 * (tid + AT * j)) = u32x4_t{0, 0, 0, 0};
-    }
-    if (tid == 0) twice = 0;
-    __syncthreads();
+  const bool listed = h.z > h.a || b.z > b.a;
+  if (listed) {
     const int end = min(SLICE, a.V - lo);
-    const int from = h.a + (c.count_from ? max(0, min(c.count_from[row], h.z - h.a)) : 0);
-    for (int k = h.a + tid; k < h.z; k += 4 * AT) {
-      int id[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) id[u] = k + u * AT < h.z ? c.hist[k + u * AT] : -1;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t s = (uint32_t)id[u] - (uint32_t)lo;
-        if (id[u] < 0 || s >= (uint32_t)end) continue;
-        if (k + u * AT >= from) atomicAdd(cnt + s, 1u);
-        else atomicOr(cnt + s, SEEN);
-      }
-    }
-    for (int k = b.a + tid; k < b.z; k += AT) {
-      const int id = c.bias_id[k];
+    // the place of an id in the slice, or SLICE
+    auto place = [&](int id) {
       const uint32_t s = (uint32_t)id - (uint32_t)lo;
-      if (id >= 0 && s < (uint32_t)end && atomicAdd(nb + s, 1u)) twice = 1;
-    }
-    __syncthreads();
-    if (b.z > b.a) {
-      if (!twice) {
-        for (int k = b.a + tid; k < b.z; k += AT) {
-          const int id = c.bias_id[k];
-          const uint32_t s = (uint32_t)id - (uint32_t)lo;
-          if (id >= 0 && s < (uint32_t)end) bias[s] = c.bias[k];
-        }
-      } else {
-        // the list in order, AT entries at a time: the first entry of an id in them
-        // adds up the id's, so that sums do not depend on who comes first
+      return id >= 0 && s < (uint32_t)end ? (int)s : SLICE;
+    };
+    auto bit = [](const uint32_t* set, int s) { return (set[s / 32] >> (s % 32)) & 1; };
+    auto put = [](uint32_t* set, int s) { return (atomicOr(set + s / 32, 1u << (s % 32)) >> (s % 32)) & 1; };
+    int id[HU];
+    auto load = [&](int k) {
 #pragma unroll
-        for (int j = 0; j < QUADS; ++j) *(f32x4_t*)(bias + 4 * (tid + AT * j)) = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        for (int k0 = b.a; k0 < b.z; k0 += AT) {
-          const int k = k0 + tid, id = k < b.z ? c.bias_id[k] : -1;
-          __syncthreads();
-          ids[tid] = id;
-          vals[tid] = k < b.z ? c.bias[k] : 0.f;
-          __syncthreads();
-          const uint32_t s = (uint32_t)id - (uint32_t)lo;
-          if (id < 0 || s >= (uint32_t)end) continue;
-          bool first = true;
-          float sum = bias[s];
-          if (nb[s] == 1) {
-            sum = vals[tid];
-          } else {
-            for (int u = 0; u < tid; ++u) first &= ids[u] != id;
-            for (int u = tid; first && u < AT; ++u)
-              if (ids[u] == id) sum += vals[u];
-          }
-          if (first) bias[s] = sum;
-        }
-      }
-      __syncthreads();
-    }
+      for (int u = 0; u < HU; ++u) id[u] = k + u * AT < h.z ? c.hist[k + u * AT] : -1;
+    };
+    load(h.a + tid);
+    // this thread's entry of the bias list's first AT
+    const int id0 = b.a + tid < b.z ? c.bias_id[b.a + tid] : -1;
+    const float bias0 = b.a + tid < b.z ? c.bias[b.a + tid] : 0.f;
+    const int from = h.a + (c.count_from ? max(0, min(c.count_from[row], h.z - h.a)) : 0);
     const float rep0 = setting(c.rep, row, 1.f), pres = setting(c.pres, row, 0.f), freq = setting(c.freq, row, 0.f);
     const float rep = rep0 > 0.f ? rep0 : 1.f;
 #pragma unroll
-    for (int j = 0; j < QUADS; ++j) {
-      const u32x4_t n = *(const u32x4_t*)(cnt + 4 * (tid + AT * j)), m = *(const u32x4_t*)(nb + 4 * (tid + AT * j));
+    for (int j = 0; j < QUADS; ++j) *(u32x4_t*)(cnt + 4 * (tid + AT * j)) = u32x4_t{0, 0, 0, 0};
+    if (tid < SLICE / 32) fresh[tid] = named[tid] = again[tid] = 0;
+    if (tid == 0) n_list = twice = 0;
+    lds_barrier();
+
+    for (int k = h.a + tid; h.z > h.a;) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n[e]) {
-          const uint32_t times = n[e] & ~SEEN;
-          float y = v[j][e];
-          if (times) y = (y - pres) - freq * (float)times;
-          v[j][e] = y > 0.f ? y / rep : y * rep;
+      for (int u = 0; u < HU; ++u) {
+        const int s = place(id[u]);
+        if (s == SLICE) continue;
+        const uint32_t was = k + u * AT >= from ? atomicAdd(cnt + s, 1u) : atomicOr(cnt + s, SEEN);
+        if (was == 0) list[atomicAdd(&n_list, 1)] = (uint16_t)s;
+      }
+      k += HU * AT;
+      if (k >= h.z) break;
+      load(k);
+    }
+    auto name = [&](int i) {
+      const int s = place(i);
+      if (s < SLICE && put(named, s)) {
+        put(again, s);
+        twice = 1;
+      }
+    };
+    name(id0);
+    for (int k = b.a + tid + AT; k < b.z; k += AT) name(c.bias_id[k]);
+    lds_barrier();
+
+    for (int i = tid; i < n_list; i += AT) {
+      const int s = list[i];
+      const uint32_t times = cnt[s] & ~SEEN;
+      float y = x[lo + s];
+      if (times) y = (y - pres) - freq * (float)times;
+      y = y > 0.f ? y / rep : y * rep;
+      cnt[s] = __float_as_uint(y);
+      put(fresh, s);
+    }
+    if (b.z > b.a) {
+      lds_barrier();
+      auto add = [&](int s, float y) {
+        const float was = bit(fresh, s) ? __uint_as_float(cnt[s]) : x[lo + s];
+        cnt[s] = __float_as_uint(was + y);
+        put(fresh, s);
+      };
+      const int s0 = place(id0);
+      if (s0 < SLICE && !bit(again, s0)) add(s0, bias0);
+      for (int k = b.a + tid + AT; k < b.z; k += AT) {
+        const int s = place(c.bias_id[k]);
+        if (s < SLICE && !bit(again, s)) add(s, c.bias[k]);
+      }
+      // ids that several entries name: these entries in order, AT of the list at a
+      // time; the first entry of an id among them adds all of the id's
+      for (int k0 = b.a; twice && k0 < b.z; k0 += AT) {
+        const int k = k0 + tid, mine = k < b.z ? c.bias_id[k] : -1, s = place(mine);
+        const bool one = s < SLICE && bit(again, s);
+        const uint64_t all = __ballot(one);
+        __syncthreads();  // (the last AT entries' are used)
+        if ((tid & 63) == 0) n_wave[tid >> 6] = __popcll(all);
+        __syncthreads();
+        int at = __popcll(all & ((1ull << (tid & 63)) - 1)), n = 0;
+#pragma unroll
+        for (int w = 0; w < AT / 64; ++w) {
+          if (w < tid >> 6) at += n_wave[w];
+          n += n_wave[w];
         }
-        if (m[e]) v[j][e] += bias[4 * (tid + AT * j) + e];
+        if (one) {
+          ids[at] = mine;
+          vals[at] = c.bias[k];
+        }
+        __syncthreads();
+        if (tid >= n) continue;
+        const int it = ids[tid];
+        bool first = true;
+        for (int u = 0; u < tid; ++u) first &= ids[u] != it;
+        for (int u = tid; first && u < n; ++u)
+          if (ids[u] == it) add(place(it), vals[u]);
       }
     }
+    lds_barrier();
   }
 #pragma unroll
   for (int j = 0; j < QUADS; ++j) {
-    const int i = lo + 4 * (tid + AT * j);
+    const int t = 4 * (tid + AT * j), i = lo + t;
+    if (listed) {
+      const uint32_t has = fresh[t / 32] >> (t % 32);
+      if (has & 15) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((has >> e) & 1) v[j][e] = __uint_as_float(cnt[t + e]);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (!((word[j] >> e) & 1)) v[j][e] = -INFINITY;

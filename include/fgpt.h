@@ -523,7 +523,7 @@ int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t
  *     takes these two steps in the same order; its rep divides whatever the sign.)
  *     count_from serves prompts, which rep alone counts, and windows.
  *  2. bias: x_i += bias[k] for bias_id[k] = i, k in bias_start[r] ..
- *     bias_start[r+1]-1; several of one id are added up in their order first.
+ *     bias_start[r+1]-1; several of one id are added one after another.
  *  3. mask: bits, id i of mask m is bit i % 32 of mask[m * mask_ld + i / 32]; 0: x_i =
  *     -inf, whatever it was. Row r has mask mask_row[r] (NULL: r); one not in
  *     [0, n_mask) masks nothing. mask_ld in words, 0 = packed.

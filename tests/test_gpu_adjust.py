@@ -32,12 +32,9 @@ def reference(x, hist=None, count_from=None, rep=None, pres=None, freq=None, bia
                 ids = np.unique(h)
                 y[ids] = np.where(y[ids] > 0, y[ids] / t, y[ids] * t)
             if bias is not None:
-                sums = {}
                 for i, v in bias[r]:
                     if 0 <= i < V:
-                        sums[i] = real(v) if i not in sums else real(sums[i] + real(v))
-                for i, v in sums.items():
-                    y[i] = y[i] + v
+                        y[i] = y[i] + real(v)
         if mask is not None:
             m = r if mask_row is None else int(mask_row[r])
             if 0 <= m < len(mask):
@@ -152,7 +149,7 @@ def test_odd_settings():
 @pytest.mark.parametrize("rows", [2, 300])
 def test_biases_named_often(V, rows):
     """Ids named twice, in one piece of the list and far apart, and a thousand times:
-    their sums are those in the list's order, whoever runs first."""
+    they are added in the list's order, whoever runs first."""
     rng = np.random.default_rng(6)
     x = rng.normal(0, 3, (rows, V)).astype(F)
     bias = []
