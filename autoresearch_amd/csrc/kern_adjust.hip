@@ -224,9 +224,9 @@ void launch_adjust_rows(hipStream_t s, const float* x, int32_t rows, int32_t V, 
                         float* out, int64_t out_ld) {
   AdjustArgs a{x, out, V, 0, ld, out_ld, c};
   if (!a.c.mask_ld) a.c.mask_ld = (V + 31) / 32;
-  a.slices = (V + 4095) / 4096;
+  a.slices = (V + 2047) / 2048;
   if ((int64_t)rows * a.slices >= 512) {
-    FG_LAUNCH((k_adjust<4>), dim3((unsigned)(rows * a.slices)), dim3(AT), 0, s, a);
+    FG_LAUNCH((k_adjust<2>), dim3((unsigned)(rows * a.slices)), dim3(AT), 0, s, a);
   } else {
     a.slices = (V + 1023) / 1024;
     FG_LAUNCH((k_adjust<1>), dim3((unsigned)(rows * a.slices)), dim3(AT), 0, s, a);

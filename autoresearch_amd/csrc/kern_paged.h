@@ -455,6 +455,22 @@ __device__ __forceinline__ void store_row4(const PagedArgs& p, int64_t row, int 
   }
 }
 
+// Largest over the lanes c, 16 + c, 32 + c, 48 + c, in each of them.
+__device__ __forceinline__ float quad_max(float v) {
+  uint32_t u = bits(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  u = bits(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+  const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Least over the 16 lanes of a row.
+__device__ __forceinline__ int rows_min(int v) {
+  v = min(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));
+  v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));
+  v = min(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));
+  return min(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));
+}
+
 // Sum of a row's weights -> the factor of its output (no visible key: 0).
 __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
@@ -502,6 +518,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs& p, float* xo, const Ro
   const int fr = t.r0 + min(c, t.rows - 1), tok = fr / p.G, h = kvh * p.G + fr % p.G;
   const int pos = pos_of(tok);
   const int klim = pos + 1, klo = p.window > 0 ? pos - p.window + 1 : 0;
+  // the rows' least klim and largest klo: tiles between them need no mask
+  const int whole_lim = __builtin_amdgcn_readfirstlane(rows_min(klim)),
+            whole_from = __builtin_amdgcn_readfirstlane(-rows_min(-klo));
 
   Tile kv;
   bool bad = false;
@@ -559,16 +578,20 @@ __device__ __forceinline__ void few_rows(const PagedArgs& p, float* xo, const Ro
     }
     f32x4_t sc[2] = {kv.scores(0), kv.scores(1)};
     if (more) load_k(it + 1);
+    if (b + 32 > whole_lim || (p.window > 0 && b < whole_from)) {  // (else every row sees every key)
+      int end = klim - b, from = klo - b, sink = p.sinks - b;
+      asm volatile("" : "+v"(end), "+v"(from), "+v"(sink));  // (keeps the compares in the branch)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int x = 16 * (e >> 2) + 4 * g + (e & 3);
+        const bool seen = x < end && (x >= from || x < sink);
+        sc[e >> 2][e & 3] = seen ? sc[e >> 2][e & 3] : -INFINITY;
+      }
+    }
     float mx = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int j = b + 16 * (e >> 2) + 4 * g + (e & 3);
-      const bool seen = j < klim && (j >= klo || j < p.sinks);
-      sc[e >> 2][e & 3] = seen ? sc[e >> 2][e & 3] : -INFINITY;
-      mx = fmaxf(mx, sc[e >> 2][e & 3]);
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.cs;
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, sc[e >> 2][e & 3]);
+    mx = quad_max(mx) * p.cs;
     // the running maximum moves only when a score passes it by 2^8, so that
     // most tiles leave O as it is; probabilities stay below 2^8
     if (__any(mx > m_run + 8.f)) {
@@ -1043,7 +1066,8 @@ constexpr int64_t PAGED_CUS = 256;
 
 }  // namespace paged
 
-paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c);
+// (may_many: 128-row tiles are allowed)
+paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many);
 paged::PagedArgs paged_args(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, const paged::PagedPlan& pl,
                             const void* q, const PagedOut& out, float* work);
 

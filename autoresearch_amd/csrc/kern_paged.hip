@@ -129,7 +129,7 @@ constexpr int64_t CUS = PAGED_CUS;
 // chunks and tokens of 9 sequences, 10 heads on 2, 92 -> 123, one fp32 prompt of
 // 2048 75 -> 95).
 constexpr int64_t MANY_WORK = 6000;
-PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) {
+PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many = true) {
   PagedPlan pl;
   const int64_t G = c.n_head / pg.n_kv_head;
   // (no sequence has more new tokens than there are rows, whatever the caller's
@@ -144,7 +144,7 @@ PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) 
       keys = std::min<int64_t>(keys, (int64_t)c.window + rt / G + 1 + c.sinks + 96);
     return (keys + 31) / 32;
   };
-  pl.many = max_q * G > 32 && tiles(DR) * pg.n_kv_head * key_tiles_most(DR) > MANY_WORK;
+  pl.many = may_many && max_q * G > 32 && tiles(DR) * pg.n_kv_head * key_tiles_most(DR) > MANY_WORK;
   pl.rt = pl.many ? Many<128, true, FG_F32>::RT : DR;
   pl.one_tile = max_q * G <= pl.rt;
   pl.ntile = (int)tiles(pl.rt);
@@ -204,7 +204,9 @@ int64_t paged_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_attn_
   return plan_of(pg, b, c).floats;
 }
 
-paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c) { return plan_of(pg, b, c); }
+paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many) {
+  return plan_of(pg, b, c, may_many);
+}
 
 paged::PagedArgs paged_args(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, const paged::PagedPlan& pl,
                             const void* q, const PagedOut& out, float* work) {

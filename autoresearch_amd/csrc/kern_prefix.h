@@ -6,7 +6,7 @@
 // Softmax over a union of key sets comes from each set's (maximum, sum, weighted
 // values): the rows of all of a group's sequences, which follow one another,
 // go over the shared keys as if they were one sequence's (a row's position, which
-// windows ask for, is its own), each sequence's rows over its own keys, and a
+// only windows ask for, is its own), each sequence's rows over its own keys, and a
 // second launch joins the parts. Both kinds of items are in one launch. The shared
 // keys are then read once a group (by each row tile of it), not once a sequence.
 // They end at a multiple of 32, the key tile; what is left is read per sequence.
@@ -33,18 +33,32 @@ __device__ __forceinline__ int shared_keys(const PrefixArgs& x, int g) {
   return max(0, min(x.shared[g], x.max_shared)) & ~31;
 }
 
-// Shared keys of the group that sequence seq belongs to; 0: none.
-__device__ __forceinline__ int shared_of(const PrefixArgs& x, int seq) {
-  const int lane = threadIdx.x & 63;
-  for (int g0 = 0; g0 < x.n_group; g0 += 64) {
-    const int g = g0 + lane;
-    const bool in = g < x.n_group;
-    const int from = in ? x.seq_start[g] : 0, to = in ? x.seq_start[g + 1] : 0;
-    const int n = in ? shared_keys(x, g) : 0;
-    const uint64_t here = __ballot(in && from <= seq && seq < to);
-    if (here) return __builtin_amdgcn_readlane(n, __builtin_ctzll(here));
+// Groups g0 .. g0+63, one a lane: their sequences and shared keys.
+struct Groups {
+  int from, to, keys;
+};
+__device__ __forceinline__ Groups groups_at(const PrefixArgs& x, int g0) {
+  const int g = g0 + (threadIdx.x & 63);
+  Groups r = {0, 0, 0};
+  if (g < x.n_group) r = {x.seq_start[g], x.seq_start[g + 1], shared_keys(x, g)};
+  return r;
+}
+// The keys of a row tile's sequence that its rows have over the group's tiles: the
+// group's shared ones, 0 where it has none or a new token sits among them (its
+// rows then read all of their keys themselves). first: groups_at(x, 0), asked for
+// early.
+__device__ __forceinline__ int shared_of(const PrefixArgs& x, const Groups& first, const RowTile& t) {
+  Groups r = first;
+  for (int g0 = 0;;) {
+    const uint64_t here = __ballot(r.from <= t.seq && t.seq < r.to);
+    if (here) {
+      const int n = __builtin_amdgcn_readlane(r.keys, __builtin_ctzll(here));
+      return t.pos0 >= n ? n : 0;
+    }
+    g0 += 64;
+    if (g0 >= x.n_group) return 0;
+    r = groups_at(x, g0);
   }
-  return 0;
 }
 
 // A row tile of a group: RowTile of its rows over the shared keys (seq: the
@@ -91,6 +105,8 @@ __device__ __forceinline__ bool find_group_tile(const PrefixArgs& x, int id, Row
   return false;
 }
 
+constexpr int AFTER = 1 << 30;  // a position behind every key
+
 // Position of a row of the group's sequences s0 .. s1-1, the first of whose rows
 // is row0.
 __device__ __forceinline__ int row_position(const PagedArgs& p, int s0, int s1, int row0, int row) {
@@ -133,10 +149,12 @@ __device__ __forceinline__ void prefix_item(const PrefixArgs& x, uint8_t* lds, i
   auto position = [&](int r) __attribute__((always_inline)) {  // of row r of the tile
     return row_position(p, t.seq, s1, t.row0, t.row0 + (t.r0 + min(r, t.rows - 1)) / p.G);
   };
-  const int own = MANY ? 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + (lane & 31) : lane & 15;
-  const int pos = position(own);
+  int pos = AFTER;  // (where the shared keys end: only windows ask for more)
   if (p.window > 0) {
-    int first = MANY ? min(position(lane), position(lane + 64)) : pos;
+    const int own = MANY ? 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) + (lane & 31) : lane & 15;
+    auto behind = [](int at, int keys) { return at >= keys ? at : AFTER; };  // (others' rows are not used)
+    pos = behind(position(own), t.kv);
+    const int first = MANY ? min(behind(position(lane), t.kv), behind(position(lane + 64), t.kv)) : pos;
     see_from(p, t, __builtin_amdgcn_readfirstlane(wave_min(first)));
   }
   const KeyTiles kt = key_tiles(t);
@@ -164,9 +182,10 @@ __device__ __forceinline__ void own_item(const PrefixArgs& x, uint8_t* lds, int 
   const PagedArgs& p = x.a;
   const int kvh = b % p.KH, rest = b / p.KH;
   const int id = rest % p.ntile, z = rest / p.ntile;
+  const Groups groups = groups_at(x, 0);
   RowTile t;
   if (!find_tile<RT>(p, id, t)) return;
-  const int from = shared_of(x, t.seq);
+  const int from = shared_of(x, groups, t);
   const KeyTiles kt = key_tiles(t, from);
   const int v0 = z * p.cpt, v1 = min(kt.n, v0 + p.cpt);
   if (z > 0 && v0 >= kt.n) return;
@@ -209,9 +228,10 @@ __global__ __launch_bounds__(256) void k_prefix_merge(PrefixArgs x) {
   const int sub = blockIdx.x % (RT / PER), item = blockIdx.x / (RT / PER);
   const int kvh = item % p.KH, id = item / p.KH;
   const int r = sub * PER + threadIdx.x / (HD / 4), d = 4 * (threadIdx.x % (HD / 4));
+  const Groups groups = groups_at(x, 0);
   RowTile t;
   if (!find_tile<RT>(p, id, t)) return;
-  const int from = shared_of(x, t.seq);
+  const int from = shared_of(x, groups, t);
   const KeyTiles kt = key_tiles(t, from);
   if ((from == 0 && kt.n <= p.cpt) || r >= t.rows) return;  // (written by the attention kernel itself)
   const int ns = max(1, (kt.n + p.cpt - 1) / p.cpt), np = from ? x.psplit : 0, n = np + ns;

@@ -485,8 +485,8 @@ int32_t fg_paged_attn(const fg_pages *pages, const fg_ragged *batch, const fg_at
  * values are read once for all of a group's rows, not once a sequence.
  * Group g is sequences seq_start[g] .. seq_start[g+1]-1, whose tables name the same
  * pages for positions 0 .. shared[g]-1 (those that some row sees; read from
- * the table of the group's first sequence) and whose new tokens all sit at position
- * shared[g] or later. seq_start[0] is 0 and seq_start does not fall; sequences from
+ * the table of the group's first sequence). A sequence with a new token at a
+ * position below shared[g] reads all of its keys itself. seq_start[0] is 0 and seq_start does not fall; sequences from
  * seq_start[n_group] on share nothing, and so does a group with shared[g] 0.
  * max_shared bounds shared (a larger one counts as max_shared) and is at most
  * max_kv of the batch; it sizes the launch with the batch's bounds. Shared

@@ -262,3 +262,14 @@ def test_far_pages():
     b.table_np = (b.table_np + far).astype(np.int32)
     b.table = b.put(b.table_np)
     assert torch.equal(run(b, q), want)
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 3)])
+@pytest.mark.parametrize("types", ["f32", "bf16_i8"])
+def test_tokens_among_the_shared(types, window, sinks):
+    """Sequences with a new token below shared[g] read all of their keys themselves;
+    the others of their group are as they were."""
+    g = [(512, [(1, 1), (10, 30), (3, 500), (200, 2)]), (512, [(5, 511), (7, 1)])]
+    b = make(g, "gqa5", 16, types, window, sinks, seed=11)
+    q = normal_q(b)
+    check(b, q, run(b, q, window, sinks), window, sinks)
