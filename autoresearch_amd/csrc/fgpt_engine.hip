@@ -2320,8 +2320,9 @@ struct fg_paged {
   fg_model* m = nullptr;
   fg_pool* pool = nullptr;
   int n_pages = 0, page_size = 0, max_seq = 0, window = 0, sinks = 0;
-  bool kv16 = false;
-  char* kv = nullptr;         // [2 (k, v)][L][n_pages][KH][page_size][hd]
+  int type = FG_F32;          // of the pages
+  bool prefix = false;        // FG_KV_PREFIX
+  char* kv = nullptr;         // [2 (k, v)][L][n_pages] pages
   int64_t plane_bytes = 0, page_bytes = 0;
   float* last = nullptr;      // [max_seq][D], then [max_seq][H*hd]: last tokens' rows
   char* meta = nullptr;       // a step's ids, lengths, tables and settings
@@ -2342,8 +2343,35 @@ fg_pages paged_layer(const fg_paged* pc, int l) {
   p.page_size = pc->page_size;
   p.n_kv_head = d.KH;
   p.head_dim = d.hd;
-  p.type = pc->kv16 ? FG_BF16 : FG_F32;
+  p.type = pc->type;
   return p;
+}
+
+// Bytes of a cached value, its share of a scale included.
+double paged_value_bytes(const fg_paged* pc) {
+  const fg_pages p = paged_layer(pc, 0);
+  return (double)page_head_bytes(p) / ((double)p.page_size * p.head_dim);
+}
+
+// Value e of a head's slot in a page's bytes, as fp32.
+float paged_value(const fg_paged* pc, const char* page, int h, int slot, int e) {
+  const int hd = pc->m->d.hd;
+  const size_t at = ((size_t)h * pc->page_size + slot) * hd + e;
+  float v;
+  if (pc->type == FG_F32) return ((const float*)page)[at];
+  if (pc->type == FG_BF16) {
+    const uint32_t u = (uint32_t)((const uint16_t*)page)[at] << 16;
+    memcpy(&v, &u, 4);
+    return v;
+  }
+  const char* head = page + h * page_head_bytes(paged_layer(pc, 0));
+  float scale;
+  memcpy(&scale, head + (size_t)pc->page_size * hd + 4 * slot, 4);
+  const uint8_t c = (uint8_t)head[(size_t)slot * hd + e];
+  if (pc->type == FG_I8) return (float)(int8_t)c * scale;
+  const int x = c >> 3 & 15, f = c & 7;  // e4m3: 2^(x - 7) (1 + f / 8), f 2^-9 at x = 0; 0x7F is NaN
+  v = (c & 127) == 127 ? NAN : x ? ldexpf((float)(8 + f), x - 10) : ldexpf((float)f, -9);
+  return (c & 128 ? -v : v) * scale;
 }
 
 // *p of at least `need` bytes; what it held is lost.
@@ -2364,6 +2392,7 @@ int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 // sequences' last ones alone, and the distinct keys that each of the two sees.
 struct Seen {
   int64_t pairs = 0, last = 0, keys = 0;  // (a last token's pairs are its keys)
+  int64_t again = 0;                      // of the keys: seen by several sequences, read once
   // Sum over positions p < n of the keys that p sees.
   static int64_t upto(int64_t n, int64_t window, int64_t sinks) {
     auto triangle = [](int64_t k) { return k * (k + 1) / 2; };
@@ -2385,8 +2414,9 @@ struct Seen {
 // are more rows than sequences, the last layer goes on with the last tokens
 // alone from its attention on (batch one: one new token a sequence, whose row is
 // last_rows[i]).
+// prefix (nullable): sequences that share pages, in the same numbers for both.
 void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, const fg_ragged& b,
-                  const fg_ragged& one, const int32_t* last_rows, const Seen& see) {
+                  const fg_ragged& one, const fg_prefix* prefix, const int32_t* last_rows, const Seen& see) {
   const Dims& d = m->d;
   Work& ws = m->ws;
   int rows = b.n_rows;
@@ -2396,7 +2426,7 @@ void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, 
   float* x = ws.x;
   const float* q = ws.q;
   auto W = [&](const bf16_t* p) { return gm ? m->wt + (p - m->w.base) : p; };
-  const double ekv = pc->kv16 ? 2 : 4;
+  const double ekv = paged_value_bytes(pc);
   timed(m, s, FG_K_OTHER, 0, (double)rows * d.D * (gm ? 10 : 6), [&] {
     launch_embed_norm(s, d, m->w.wte, ids, rows, x, gm ? ws.xs : nullptr, prow * d.D,
                       gm ? ws.ssq : nullptr);
@@ -2439,8 +2469,9 @@ void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, 
     }
     timed(m, s, b.max_q > 1 && !cut ? FG_K_ATTN_CHUNK : FG_K_ATTN_DECODE,
           4.0 * d.hd * d.H * (cut ? see.last : see.pairs),
-          8.0 * rows * d.qd() + 2 * ekv * (cut ? see.last : see.keys) * d.kvd(), [&] {
-            launch_paged_attn(s, pg, cut ? one : b, at, q, out, (float*)pc->work);
+          8.0 * rows * d.qd() + 2 * ekv * ((cut ? see.last : see.keys) - see.again) * d.kvd(), [&] {
+            if (prefix) launch_prefix_attn(s, pg, cut ? one : b, *prefix, at, q, out, (float*)pc->work);
+            else launch_paged_attn(s, pg, cut ? one : b, at, q, out, (float*)pc->work);
           });
     // x += attn_out Wproj^T; h = relu(rmsnorm(x) Wfc^T)^2; x += h Wproj2^T
     a.x = ws.ao; a.xs = ws.aos; a.xs_plane = prow * d.qd(); a.ssq_n = 0;
@@ -2465,12 +2496,57 @@ void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, 
   linear(m, s, GV_STORE, a, nullptr, gm);
 }
 
+// Keys that groups have to save over all sequences before a step takes fg_prefix_attn.
+constexpr int64_t PREFIX_SAVED = 2048;
+
+// Neighbours of a step's sequences that share their first pages, as groups: a
+// sequence joins the group before it where that leaves at least as many keys read
+// once. starts and shared are fg_prefix's; false: too few to make up for the launch
+// that joins the parts.
+bool shared_groups(const fg_paged* pc, int n, const int32_t* seqs, const std::vector<int32_t>& before,
+                   std::vector<int32_t>* starts, std::vector<int32_t>* shared, int64_t* again) {
+  std::vector<std::vector<int32_t>> table((size_t)n);
+  for (int i = 0; i < n; ++i) {  // the pages that the new tokens do not touch
+    int32_t held = 0;
+    (void)fg_pool_table(pc->pool, seqs[i], nullptr, 0, &held);
+    table[i].resize((size_t)held);
+    (void)fg_pool_table(pc->pool, seqs[i], table[i].data(), held, &held);
+    table[i].resize((size_t)(before[i] / pc->page_size));
+  }
+  int64_t saved = 0;
+  int64_t common = 0, members = 0;  // of the last group: pages, sequences
+  for (int i = 0; i < n; ++i) {
+    int64_t k = 0;
+    if (members > 0) {
+      const std::vector<int32_t>&a = table[i - 1], &b = table[i];
+      const int64_t most = std::min<int64_t>({common, (int64_t)a.size(), (int64_t)b.size()});
+      while (k < most && a[k] == b[k]) ++k;
+    }
+    if (members > 0 && k > 0 && members * k >= (members - 1) * common) {
+      common = k;
+      ++members;
+      shared->back() = (int32_t)(k * pc->page_size);
+    } else {
+      saved += std::max<int64_t>(0, members - 1) * common * pc->page_size;
+      starts->push_back(i);
+      common = (int64_t)table[i].size();
+      members = 1;
+      shared->push_back(0);
+    }
+  }
+  saved += std::max<int64_t>(0, members - 1) * common * pc->page_size;
+  starts->push_back(n);
+  *again = pc->window ? 0 : saved;  // (what windows leave of it is not counted)
+  return saved >= PREFIX_SAVED;
+}
+
 int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const int32_t* counts,
-                   const int32_t* ids, const fg_draw_cfg* draw, float* logits, int32_t* next_ids) {
+                   const int32_t* ids, const fg_adjust_cfg* adjust, const fg_draw_cfg* draw, float* logits,
+                   int32_t* next_ids) {
   const Dims& d = m->d;
   // what the batch needs, before anything changes
   std::vector<uint8_t> named((size_t)pc->max_seq, 0);
-  std::vector<int32_t> len((size_t)n);
+  std::vector<int32_t> len((size_t)n), before((size_t)n);
   std::map<int32_t, int> shared;  // copies that a shared last page still takes
   int64_t rows = 0, need = 0;
   Seen see;
@@ -2492,6 +2568,7 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
       auto it = shared.emplace(page, holders - 1).first;
       if (it->second-- <= 0) --pages;
     }
+    before[i] = len[i];
     len[i] += counts[i];
     need += pages;
     rows += counts[i];
@@ -2518,6 +2595,42 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   const int64_t o_ids = place(rows * 4), o_start = place((n + 1) * 4ll), o_one = place((n + 1) * 4ll),
                 o_len = place(n * 4ll), o_last = place(n * 4ll), o_table = place((int64_t)n * ld * 4);
   const int64_t o_set = place(5 * up16(n * 4ll));
+  std::vector<int32_t> groups, group_keys;  // fg_prefix's arrays
+  int64_t again = 0;
+  const bool sharing = pc->prefix && n > 1 && shared_groups(pc, n, seqs, before, &groups, &group_keys, &again);
+  if (sharing) see.again = again;
+  const int64_t o_groups = place(sharing ? (int64_t)groups.size() * 4 : 0),
+                o_shared = place(sharing ? (int64_t)group_keys.size() * 4 : 0);
+  // the adjustments' arrays: their places, and the host's
+  struct Array {
+    int64_t at;
+    const void* host;
+    int64_t bytes;
+  };
+  std::vector<Array> arrays;
+  auto array = [&](const void* host, int64_t bytes) -> const char* {
+    if (!host || bytes == 0) return nullptr;
+    arrays.push_back({place(bytes), host, bytes});
+    return (const char*)arrays.back().at;  // (made an address when the buffer is there)
+  };
+  fg_adjust_cfg ac = {};
+  const bool adjusts = adjust && next_ids;
+  if (adjusts) {
+    ac = *adjust;
+    ac.mask_ld = adjust->mask_ld ? adjust->mask_ld : (d.V + 31) / 32;
+    const int64_t col = n * 4ll, starts_bytes = col + 4;
+    ac.hist = (const int32_t*)array(adjust->n_hist ? adjust->hist : nullptr, adjust->n_hist * 4ll);
+    ac.hist_start = (const int32_t*)array(adjust->n_hist ? adjust->hist_start : nullptr, starts_bytes);
+    ac.count_from = (const int32_t*)array(adjust->count_from, col);
+    ac.rep = (const float*)array(adjust->rep, col);
+    ac.pres = (const float*)array(adjust->pres, col);
+    ac.freq = (const float*)array(adjust->freq, col);
+    ac.bias = (const float*)array(adjust->n_bias ? adjust->bias : nullptr, adjust->n_bias * 4ll);
+    ac.bias_id = (const int32_t*)array(adjust->n_bias ? adjust->bias_id : nullptr, adjust->n_bias * 4ll);
+    ac.bias_start = (const int32_t*)array(adjust->n_bias ? adjust->bias_start : nullptr, starts_bytes);
+    ac.mask = (const uint32_t*)array(adjust->n_mask ? adjust->mask : nullptr, adjust->n_mask * ac.mask_ld * 4);
+    ac.mask_row = (const int32_t*)array(adjust->n_mask ? adjust->mask_row : nullptr, col);
+  }
   if (at > pc->meta_bytes) {
     if (pc->h_meta) HIPCHK(hipHostFree(pc->h_meta));
     pc->h_meta = nullptr;
@@ -2541,6 +2654,15 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   const fg_attn_cfg cfg = {d.H, FG_F32, pc->window, pc->sinks, 0.f, 0, 0};
   int64_t wb = 4 * std::max(paged_attn_floats(paged_layer(pc, 0), b, cfg),
                             paged_attn_floats(paged_layer(pc, 0), one, cfg));
+  fg_prefix prefix = {};
+  if (sharing) {
+    prefix.n_group = (int32_t)group_keys.size();
+    prefix.max_shared = *std::max_element(group_keys.begin(), group_keys.end());
+    prefix.seq_start = (const int32_t*)(pc->meta + o_groups);
+    prefix.shared = (const int32_t*)(pc->meta + o_shared);
+    wb = std::max(4 * prefix_attn_floats(paged_layer(pc, 0), b, prefix, cfg),
+                  4 * prefix_attn_floats(paged_layer(pc, 0), one, prefix, cfg));
+  }
   wb = std::max(wb, draw_work_bytes(n, d.V));
   RCCHK(grow(m, &pc->work, &pc->work_bytes, wb));
 
@@ -2583,7 +2705,21 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   }
   H(o_start)[n] = r;
   H(o_one)[n] = n;
+  if (sharing) {
+    std::copy(groups.begin(), groups.end(), H(o_groups));
+    std::copy(group_keys.begin(), group_keys.end(), H(o_shared));
+  }
+  for (const Array& a : arrays) memcpy(pc->h_meta + a.at, a.host, (size_t)a.bytes);
+  auto place_of = [&](auto*& p) {
+    if (p) p = (std::remove_reference_t<decltype(p)>)(pc->meta + (int64_t)p);
+  };
+  place_of(ac.hist), place_of(ac.hist_start), place_of(ac.count_from), place_of(ac.rep), place_of(ac.pres);
+  place_of(ac.freq), place_of(ac.bias), place_of(ac.bias_id), place_of(ac.bias_start), place_of(ac.mask);
+  place_of(ac.mask_row);
   fg_draw_cfg dc = {};
+  const std::vector<float> zeros(adjusts && !draw ? (size_t)n : 0, 0.f);
+  const fg_draw_cfg largest = {zeros.data(), nullptr, nullptr, nullptr, zeros.data()};
+  if (adjusts && !draw) draw = &largest;  // (the argmax, or -1 where a mask leaves nothing)
   if (draw) {
     const int64_t col = up16(n * 4ll);
     auto put = [&](int k, const void* p) -> const void* {
@@ -2607,7 +2743,15 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
   }
   auto run = [&]() -> int32_t {
     HIPCHK(hipMemcpyAsync(pc->meta, pc->h_meta, (size_t)at, hipMemcpyHostToDevice, s));
-    paged_layers(m, pc, s, (int32_t*)(pc->meta + o_ids), b, one, (int32_t*)(pc->meta + o_last), see);
+    paged_layers(m, pc, s, (int32_t*)(pc->meta + o_ids), b, one, sharing ? &prefix : nullptr,
+                 (int32_t*)(pc->meta + o_last), see);
+    if (adjusts) {
+      // (the caller's logits are the model's own)
+      if (logits) RCCHK(copy_out(m, logits, m->ws.logits, (size_t)n * d.V * 4, s));
+      timed(m, s, FG_K_OTHER, 0, 8.0 * n * d.V, [&] {
+        launch_adjust_rows(s, m->ws.logits, n, d.V, d.V, ac, m->ws.logits, d.V);
+      });
+    }
     if (next_ids) {
       timed(m, s, FG_K_OTHER, 0, 4.0 * n * d.V, [&] {
         if (draw)
@@ -2618,7 +2762,7 @@ int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const 
     }
     HIPCHK(hipGetLastError());
     if (next_ids) HIPCHK(hipMemcpyAsync(next_ids, m->ws.amax, (size_t)n * 4, hipMemcpyDeviceToHost, s));
-    if (logits) RCCHK(copy_out(m, logits, m->ws.logits, (size_t)n * d.V * 4, s));
+    if (logits && !adjusts) RCCHK(copy_out(m, logits, m->ws.logits, (size_t)n * d.V * 4, s));
     HIPCHK(hipStreamSynchronize(s));
     return FG_OK;
   };
@@ -2635,7 +2779,10 @@ extern "C" int32_t fg_paged_create(fg_model* m, int32_t n_pages, int32_t page_si
                                    int32_t flags, int32_t window, int32_t sinks, fg_paged** out) {
   if (!m || !out) return seterr(FG_EARG, "NULL argument");
   *out = nullptr;
-  if (flags & ~FG_KV_BF16) return seterr(FG_EARG, "unknown cache flags 0x%x", flags);
+  constexpr int32_t TYPES = FG_KV_BF16 | FG_KV_I8 | FG_KV_E4M3;
+  if (flags & ~(TYPES | FG_KV_PREFIX)) return seterr(FG_EARG, "unknown cache flags 0x%x", flags);
+  const int32_t type = flags & TYPES;
+  if (type & (type - 1)) return seterr(FG_EARG, "cache flags 0x%x name more than one type", flags);
   if (window < 0 || sinks < 0 || window > (1 << 30) || sinks > (1 << 30))
     return seterr(FG_EARG, "window and sinks must be in 0..2^30");
   // (the attention numbers a layer's rows with 32 bits)
@@ -2657,8 +2804,9 @@ extern "C" int32_t fg_paged_create(fg_model* m, int32_t n_pages, int32_t page_si
   pc->max_seq = max_seq;
   pc->window = window;
   pc->sinks = sinks;
-  pc->kv16 = (flags & FG_KV_BF16) != 0;
-  pc->page_bytes = (int64_t)d.kvd() * page_size * (pc->kv16 ? 2 : 4);
+  pc->type = type == FG_KV_BF16 ? FG_BF16 : type == FG_KV_I8 ? FG_I8 : type == FG_KV_E4M3 ? FG_E4M3 : FG_F32;
+  pc->prefix = (flags & FG_KV_PREFIX) != 0;
+  pc->page_bytes = d.KH * page_head_bytes(paged_layer(pc, 0));
   pc->plane_bytes = n_pages * pc->page_bytes;
   const size_t bytes = (size_t)(2 * d.L * pc->plane_bytes);
   const size_t last = (size_t)max_seq * (d.D + d.qd()) * 4;
@@ -2762,14 +2910,7 @@ extern "C" int32_t fg_paged_read(fg_paged* pc, int32_t seq, float* k_out, float*
           for (int h = 0; h < d.KH; ++h)
             for (int p = i * pc->page_size; p < std::min<int>(len, (i + 1) * pc->page_size); ++p)
               for (int e = 0; e < d.hd; ++e) {
-                const size_t at = ((size_t)h * pc->page_size + p % pc->page_size) * d.hd + e;
-                float v = 0.f;
-                if (pages[i] >= 0 && pc->kv16) {
-                  const uint32_t u = (uint32_t)((const uint16_t*)page.data())[at] << 16;
-                  memcpy(&v, &u, 4);
-                } else if (pages[i] >= 0) {
-                  v = ((const float*)page.data())[at];
-                }
+                const float v = pages[i] >= 0 ? paged_value(pc, page.data(), h, p % pc->page_size, e) : 0.f;
                 outs[t][((size_t)l * len + p) * d.kvd() + h * d.hd + e] = v;
               }
         }
@@ -2779,17 +2920,38 @@ extern "C" int32_t fg_paged_read(fg_paged* pc, int32_t seq, float* k_out, float*
   return FG_OK;
 }
 
-extern "C" int32_t fg_paged_step(fg_model* m, fg_paged* pc, int32_t n, const int32_t* seqs,
-                                 const int32_t* counts, const int32_t* ids, const fg_draw_cfg* draw,
-                                 float* logits, int32_t* next_ids) {
+namespace {
+
+int32_t paged_step(fg_model* m, fg_paged* pc, int32_t n, const int32_t* seqs, const int32_t* counts,
+                   const int32_t* ids, const fg_adjust_cfg* adjust, const fg_draw_cfg* draw, float* logits,
+                   int32_t* next_ids) {
   if (!m || !pc || pc->m != m || !seqs || !counts || !ids) return seterr(FG_EARG, "bad argument");
   if (n < 1) return seterr(FG_EARG, "n must be >= 1");
   if (draw && (!draw->u || !next_ids)) return seterr(FG_EARG, "a draw needs u and next_ids");
-  if (draw && m->d.V > DRAW_MAX_V) return seterr(FG_EARG, "draws up to %d ids", DRAW_MAX_V);
+  if ((draw || adjust) && m->d.V > DRAW_MAX_V) return seterr(FG_EARG, "draws up to %d ids", DRAW_MAX_V);
+  if (adjust) {
+    if (!next_ids) return seterr(FG_EARG, "adjusted logits are drawn from: next_ids is NULL");
+    RCCHK(check_adjust(adjust, n, m->d.V));
+  }
   GUARD(m);
   try {
-    return paged_pass(m, pc, n, seqs, counts, ids, draw, logits, next_ids);
+    return paged_pass(m, pc, n, seqs, counts, ids, adjust, draw, logits, next_ids);
   } catch (const std::exception& e) {
     return seterr(FG_EARG, "paged step: %s", e.what());
   }
+}
+
+}  // namespace
+
+extern "C" int32_t fg_paged_step(fg_model* m, fg_paged* pc, int32_t n, const int32_t* seqs,
+                                 const int32_t* counts, const int32_t* ids, const fg_draw_cfg* draw,
+                                 float* logits, int32_t* next_ids) {
+  return paged_step(m, pc, n, seqs, counts, ids, nullptr, draw, logits, next_ids);
+}
+
+extern "C" int32_t fg_paged_step_adjust(fg_model* m, fg_paged* pc, int32_t n, const int32_t* seqs,
+                                        const int32_t* counts, const int32_t* ids,
+                                        const fg_adjust_cfg* adjust, const fg_draw_cfg* draw,
+                                        float* logits, int32_t* next_ids) {
+  return paged_step(m, pc, n, seqs, counts, ids, adjust, draw, logits, next_ids);
 }

@@ -338,9 +338,7 @@ extern "C" int32_t fg_pages_copy(void* base, int32_t n_planes, int64_t plane_byt
 }
 
 // ------------------------------------------------------------ logits
-namespace {
-
-int32_t check_adjust(const fg_adjust_cfg* c, int32_t rows, int32_t V) {
+int32_t fgpt::check_adjust(const fg_adjust_cfg* c, int32_t rows, int32_t V) {
   CHECK(c, "cfg is NULL");
   CHECK(c->n_hist >= 0 && c->n_bias >= 0 && c->n_mask >= 0, "n_hist, n_bias and n_mask must be >= 0");
   CHECK(c->n_hist <= 1 << 30 && c->n_bias <= 1 << 30, "n_hist or n_bias above 2^30");
@@ -352,8 +350,6 @@ int32_t check_adjust(const fg_adjust_cfg* c, int32_t rows, int32_t V) {
   CHECK(c->n_mask == 0 || c->mask_row || c->n_mask >= rows, "%d masks for %d rows, and no mask_row", c->n_mask, rows);
   return FG_OK;
 }
-
-}  // namespace
 
 extern "C" int32_t fg_adjust_rows(const float* logits, int32_t rows, int32_t V, int64_t ld,
                                   const fg_adjust_cfg* cfg, float* out, int64_t out_ld, void* stream) {

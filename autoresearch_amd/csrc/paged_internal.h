@@ -64,6 +64,8 @@ void pool_plan_moves(const fg_pool* p, PoolMoves* m);  // (may throw)
 void pool_apply_moves(fg_pool* p, PoolMoves* m);       // (does not)
 
 // ---- logits
+// (FG_EARG where cfg is not one for `rows` rows of V logits)
+int32_t check_adjust(const fg_adjust_cfg* c, int32_t rows, int32_t V);
 void launch_adjust_rows(hipStream_t s, const float* x, int32_t rows, int32_t V, int64_t ld, const fg_adjust_cfg& c,
                         float* out, int64_t out_ld);
 

@@ -43,7 +43,7 @@ EXPORTS = (
     "fg_pool_need", "fg_pool_extend", "fg_pool_fork", "fg_pool_trim", "fg_pool_slide",
     "fg_pool_compact",
     "fg_paged_create", "fg_paged_destroy", "fg_paged_len", "fg_paged_free", "fg_paged_fork",
-    "fg_paged_trim", "fg_paged_compact", "fg_paged_read", "fg_paged_step",
+    "fg_paged_trim", "fg_paged_compact", "fg_paged_read", "fg_paged_step", "fg_paged_step_adjust",
 )
 
 KERNEL_KINDS = {0: "gemm", 1: "gemv", 2: "attn_chunk", 3: "attn_decode", 4: "other",
@@ -54,6 +54,7 @@ FG_OPT_SAMPLED_IN_LOOP = 3
 
 
 FG_KV_BF16 = 1  # fg_kv_create_ex flag: bf16 K/V cache
+FG_KV_I8, FG_KV_E4M3, FG_KV_PREFIX = 2, 4, 8  # of fg_paged_create: 8-bit pages, shared pages read once
 
 
 class FgptError(RuntimeError):
@@ -226,6 +227,8 @@ def load_library(path: str = LIB_PATH):
         "fg_paged_compact": (i32, [_vp, _i]),
         "fg_paged_read": (i32, [_vp, i32, _f, _f]),
         "fg_paged_step": (i32, [_vp, _vp, i32, _i, _i, _i, C.POINTER(_DrawCfg), _f, _i]),
+        "fg_paged_step_adjust": (i32, [_vp, _vp, i32, _i, _i, _i, C.POINTER(_AdjustCfg),
+                                       C.POINTER(_DrawCfg), _f, _i]),
         "fg_timing_read": (i32, [_vp, i32, C.POINTER(i64), C.POINTER(C.c_double),
                                  C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     }
@@ -435,8 +438,8 @@ class Model:
         return KV(self, B, maxT, bf16)
 
     def paged(self, n_pages: int, page_size: int = 64, max_seq: int = 64, bf16: bool = False,
-              window: int = 0, sinks: int = 0) -> "Paged":
-        return Paged(self, n_pages, page_size, max_seq, bf16, window, sinks)
+              window: int = 0, sinks: int = 0, type: int | None = None, prefix: bool = False) -> "Paged":
+        return Paged(self, n_pages, page_size, max_seq, bf16, window, sinks, type, prefix)
 
 
 class KV:
@@ -535,10 +538,16 @@ class Paged:
     (numbered 0..max_seq-1, empty until a step names them)."""
 
     def __init__(self, m: Model, n_pages: int, page_size: int = 64, max_seq: int = 64,
-                 bf16: bool = False, window: int = 0, sinks: int = 0):
+                 bf16: bool = False, window: int = 0, sinks: int = 0, type: int | None = None,
+                 prefix: bool = False):
+        """type: of the pages (FG_F32, FG_BF16, FG_I8, FG_E4M3), in the place of bf16.
+        prefix: steps read pages that neighbours among their sequences share once."""
         self.m, self.n_pages, self.page_size, self.max_seq = m, n_pages, page_size, max_seq
         self._h = _vp()
-        _check(_LIB.fg_paged_create(m.handle, n_pages, page_size, max_seq, FG_KV_BF16 if bf16 else 0,
+        if type is None:
+            type = FG_BF16 if bf16 else FG_F32
+        flags = {FG_F32: 0, FG_BF16: FG_KV_BF16, FG_I8: FG_KV_I8, FG_E4M3: FG_KV_E4M3}[type]
+        _check(_LIB.fg_paged_create(m.handle, n_pages, page_size, max_seq, flags | (FG_KV_PREFIX if prefix else 0),
                                     window, sinks, C.byref(self._h)))
         m._caches.add(self)
 
@@ -588,11 +597,15 @@ class Paged:
         return k, v
 
     def step(self, batch: dict, want_logits: bool = True, u=None, temp=None, top_k=None, top_p=None,
-             min_p=None):
+             min_p=None, history=None, count_from=None, rep=None, pres=None, freq=None, bias=None, allowed=None):
         """fg_paged_step over {sequence: its new ids}: (logits [n, V] or None,
         next ids [n]) of each sequence's last token, in the dict's order. With u
         (a uniform number a sequence) the ids are drawn under the given
-        settings (a value a sequence, or one for all), else they are the argmax."""
+        settings (a value a sequence, or one for all), else they are the argmax.
+        What fg_adjust_rows does before (fg_paged_step_adjust), a value or list a
+        sequence: history (ids; count_from: where presence and frequency begin) with
+        rep, pres and freq; bias ((id, value) pairs, or a dict); allowed (a truth value
+        an id, or None)."""
         seqs = _i32(list(batch))
         parts = [_i32(v).reshape(-1) for v in batch.values()]
         n = seqs.size
@@ -609,11 +622,57 @@ class Paged:
                             col(min_p, np.float32), col(u, np.float32))
         elif any(a is not None for a in (temp, top_k, top_p, min_p)):
             raise ValueError("settings of a draw without u")
+        adjust = self._adjust(n, keep, history, count_from, rep, pres, freq, bias, allowed)
         lg = np.empty((n, self.m.d.vocab), np.float32) if want_logits else None
         nxt = np.empty(n, np.int32)
-        _check(_LIB.fg_paged_step(self.m.handle, self._h, n, _ip(seqs), _ip(counts), _ip(ids), draw,
-                                  _fp(lg), _ip(nxt)))
+        _check(_LIB.fg_paged_step_adjust(self.m.handle, self._h, n, _ip(seqs), _ip(counts), _ip(ids), adjust, draw,
+                                         _fp(lg), _ip(nxt)))
         return lg, nxt
+
+    def _adjust(self, n, keep, history, count_from, rep, pres, freq, bias, allowed):
+        """A step's fg_adjust_cfg of host arrays (kept in `keep`), None where nothing is given."""
+        if all(a is None for a in (history, bias, allowed)):
+            if any(a is not None for a in (count_from, rep, pres, freq)):
+                raise ValueError("penalties without a history")
+            return None
+
+        def ptr(a, t):
+            keep.append(np.ascontiguousarray(a, t))
+            return keep[-1].ctypes.data
+
+        def col(a, t):
+            return 0 if a is None else ptr(np.broadcast_to(np.asarray(a, t), (n,)), t)
+
+        def starts(parts):
+            if len(parts) != n:
+                raise ValueError("a list for each sequence is wanted")
+            return ptr(np.concatenate([[0], np.cumsum([len(p) for p in parts])]), np.int32)
+
+        c = adjust_cfg(count_from=col(count_from, np.int32), rep=col(rep, np.float32), pres=col(pres, np.float32),
+                       freq=col(freq, np.float32))
+        if history is not None:
+            parts = [_i32(h).reshape(-1) for h in history]
+            flat = np.concatenate(parts) if n else _i32([])
+            c.hist_start, c.hist, c.n_hist = starts(parts), ptr(flat, np.int32), flat.size
+        if bias is not None:
+            parts = [list(b.items() if isinstance(b, dict) else b or ()) for b in bias]
+            flat = [p for b in parts for p in b]
+            c.bias_start, c.n_bias = starts(parts), len(flat)
+            c.bias_id, c.bias = ptr([i for i, _ in flat], np.int32), ptr([v for _, v in flat], np.float32)
+        if allowed is not None:
+            V = self.m.d.vocab
+            rows, masks = [], []
+            for a in allowed:
+                rows.append(len(masks) if a is not None else -1)
+                if a is not None:
+                    bits = np.zeros((V + 31) // 32 * 32, bool)
+                    bits[:V] = np.asarray(a, bool).reshape(V)
+                    masks.append(np.packbits(bits, bitorder="little"))
+            if len(rows) != n:
+                raise ValueError("a mask, or None, for each sequence is wanted")
+            if masks:
+                c.mask, c.mask_row, c.n_mask = ptr(np.stack(masks), np.uint8), ptr(rows, np.int32), len(masks)
+        return c
 
 
 class Pool:

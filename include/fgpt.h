@@ -151,6 +151,8 @@ int32_t fg_kv_create(fg_model *m, int32_t B, int32_t maxT, fg_kv **out);
  * the reference (whose cache is fp32); fg_kv_create is flags = 0. The B=1
  * persistent decode loop runs on fp32 caches only. */
 enum { FG_KV_BF16 = 1 };
+/* Further flags of fg_paged_create. */
+enum { FG_KV_I8 = 2, FG_KV_E4M3 = 4, FG_KV_PREFIX = 8 };
 int32_t fg_kv_create_ex(fg_model *m, int32_t B, int32_t maxT, int32_t flags, fg_kv **out);
 int32_t fg_kv_destroy(fg_kv *kv);
 /* cache_len in/out of gpt_step: the number of filled positions. set_len
@@ -605,8 +607,11 @@ int32_t fg_pool_slide(fg_pool *pool, int32_t seq, int32_t window, int32_t sinks)
 int32_t fg_pool_compact(fg_pool *pool, int32_t *src, int32_t *dst, int32_t cap, int32_t *n);
 
 /* A model's paged KV cache: up to max_seq sequences of their own lengths in
- * n_pages pages of page_size positions for every layer, fp32 or (FG_KV_BF16)
- * bf16. window > 0: each token sees the last `window` positions and the first
+ * n_pages pages of page_size positions for every layer, fp32 or, by one of the
+ * flags FG_KV_BF16, FG_KV_I8 and FG_KV_E4M3, of that type. With FG_KV_PREFIX a
+ * step reads pages that neighbours among its sequences share (fg_paged_fork) once
+ * for all of them (fg_prefix_attn); its results are then those of the step
+ * without it up to the order of sums. window > 0: each token sees the last `window` positions and the first
  * `sinks`, and pages behind both are given back after each step. The model must
  * outlive it; its calls count as the model's (FG_EBUSY). */
 typedef struct fg_paged fg_paged;
@@ -633,6 +638,14 @@ int32_t fg_paged_read(fg_paged *pc, int32_t seq, float *k_out, float *v_out);
 int32_t fg_paged_step(fg_model *m, fg_paged *pc, int32_t n, const int32_t *seqs,
                       const int32_t *counts, const int32_t *ids, const fg_draw_cfg *draw,
                       float *logits, int32_t *next_ids);
+/* The same, the ids drawn from logits that fg_adjust_rows has changed: adjust is
+ * an fg_adjust_cfg of host arrays for n rows (NULL: fg_paged_step). Without draw
+ * next_ids are the argmax of those, or -1 where a mask leaves nothing. logits are
+ * the model's own. */
+int32_t fg_paged_step_adjust(fg_model *m, fg_paged *pc, int32_t n, const int32_t *seqs,
+                             const int32_t *counts, const int32_t *ids,
+                             const fg_adjust_cfg *adjust, const fg_draw_cfg *draw, float *logits,
+                             int32_t *next_ids);
 
 #ifdef __cplusplus
 }
