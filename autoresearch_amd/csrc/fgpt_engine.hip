@@ -2496,8 +2496,14 @@ void paged_layers(fg_model* m, fg_paged* pc, hipStream_t s, const int32_t* ids, 
   linear(m, s, GV_STORE, a, nullptr, gm);
 }
 
-// Keys that groups have to save over all sequences before a step takes fg_prefix_attn.
-constexpr int64_t PREFIX_SAVED = 2048;
+// Bytes of a layer that groups have to save before a step takes fg_prefix_attn, whose
+// second launch and look-ups cost 1 to 1.6 us. us a call, each sequence alone ->
+// shared, 6 heads of 128 with their own keys: fp32 pages, 9 MB saved 10.6 -> 11.6, 22
+// MB 10.7 -> 11.7, 23 MB of 16 sequences 13.5 -> 12.0, 47 MB 16.7 -> 12.1, 790 MB 110 ->
+// 29; bf16, 23 MB 10.7 -> 10.3, 396 MB 43.5 -> 19; e4m3, 12 MB 10.7 -> 10.1, 204 MB
+// 38.6 -> 17.6. 10 heads on 2: fp32, 31 MB 13.7 -> 12.9; bf16, 33 MB 11.0 -> 11.8, 132 MB
+// 19.0 -> 14.4.
+constexpr int64_t PREFIX_SAVED = 16 << 20;
 
 // Neighbours of a step's sequences that share their first pages, as groups: a
 // sequence joins the group before it where that leaves at least as many keys read
@@ -2537,7 +2543,7 @@ bool shared_groups(const fg_paged* pc, int n, const int32_t* seqs, const std::ve
   saved += std::max<int64_t>(0, members - 1) * common * pc->page_size;
   starts->push_back(n);
   *again = pc->window ? 0 : saved;  // (what windows leave of it is not counted)
-  return saved >= PREFIX_SAVED;
+  return saved * 2 * pc->m->d.kvd() * paged_value_bytes(pc) >= PREFIX_SAVED;
 }
 
 int32_t paged_pass(fg_model* m, fg_paged* pc, int n, const int32_t* seqs, const int32_t* counts,

@@ -610,8 +610,8 @@ int32_t fg_pool_compact(fg_pool *pool, int32_t *src, int32_t *dst, int32_t cap, 
  * n_pages pages of page_size positions for every layer, fp32 or, by one of the
  * flags FG_KV_BF16, FG_KV_I8 and FG_KV_E4M3, of that type. With FG_KV_PREFIX a
  * step reads pages that neighbours among its sequences share (fg_paged_fork) once
- * for all of them (fg_prefix_attn); its results are then those of the step
- * without it up to the order of sums. window > 0: each token sees the last `window` positions and the first
+ * for all of them (fg_prefix_attn) where that saves enough (16 MiB a layer); its
+ * results are then those of the step without it up to the order of sums. window > 0: each token sees the last `window` positions and the first
  * `sinks`, and pages behind both are given back after each step. The model must
  * outlive it; its calls count as the model's (FG_EBUSY). */
 typedef struct fg_paged fg_paged;

@@ -120,35 +120,49 @@ def test_ragged_passes_in_8_bits(setup, kind, window, sinks):
     pc.close()
 
 
+def taken(m, pc, f, saved):
+    """f()'s answer; whether its step read the shared keys once (its bytes say so)."""
+    m.timing(True)
+    out = f()
+    got = m.timing_read()
+    m.timing(False)
+    return out, saved and got["attn_decode"][3] + got["attn_chunk"][3] < saved
+
+
 @pytest.mark.parametrize("type,window,sinks", [(engine.FG_F32, 0, 0), (engine.FG_F32, 200, 5), (engine.FG_BF16, 0, 0),
                                                (engine.FG_E4M3, 0, 0)])
 def test_shared_prefixes(setup, type, window, sinks):
-    """Forks of two prompts, beside others, tokens and chunks: each sequence's logits
-    are its own model's, and near those of a cache that reads every sequence alone."""
+    """Many forks of two prompts, beside others, tokens and chunks: each sequence's
+    logits are near those of a cache that reads every sequence alone, and a sample of
+    them are the float64 model's."""
     d, m, ex = setup
     ex = exact_of(ex, "e4m3" if type == engine.FG_E4M3 else None)
     bar = {engine.FG_F32: 5e-5, engine.FG_BF16: 2e-3, engine.FG_E4M3: BARS["e4m3"]}[type]
-    pcs = [m.paged(160, 16, 24, type=type, window=window, sinks=sinks, prefix=p) for p in (True, False)]
+    pcs = [m.paged(900, 16, 256, type=type, window=window, sinks=sinks, prefix=p) for p in (True, False)]
     prompts = [uniform_ids(7, 300, d.vocab), uniform_ids(8, 260, d.vocab), uniform_ids(9, 50, d.vocab)]
-    text = {}
+    B = 190  # the second prompt's first
     for pc in pcs:
-        pc.step({0: prompts[0], 12: prompts[1], 23: prompts[2]}, want_logits=False)
-        for s in range(1, 12):
+        pc.step({0: prompts[0], B: prompts[1], 255: prompts[2]}, want_logits=False)
+        for s in range(1, B):
             pc.fork(0, s, 300 - (s % 4) if not window else 300)
-        for s in range(13, 20):
-            pc.fork(12, s)
-    text = {s: prompts[0][:pcs[0].len(s)] for s in range(12)} | {s: prompts[1] for s in range(12, 20)}
-    text[23] = prompts[2]
+        for s in range(B + 1, 250):
+            pc.fork(B, s)
+    text = {s: prompts[0][:pcs[0].len(s)] for s in range(B)} | {s: prompts[1] for s in range(B, 250)}
+    text[255] = prompts[2]
     for k in range(3):
-        new = {s: uniform_ids(100 * k + s, 1 if k < 2 else 1 + s % 4, d.vocab) for s in text}
+        new = {s: uniform_ids(1000 * k + s, 1 if k < 2 else 1 + s % 4, d.vocab) for s in text}
         if k == 1:  # another order, a sequence left out
-            new = {s: new[s] for s in (23, 5, 4, 3, 2, 1, 0, 11, 10, 9, 8, 7, 19, 18, 17, 16, 15, 14, 13, 12)}
-        lgs = [pc.step(new)[0] for pc in pcs]
-        assert relerr(*lgs) < 2 * bar
+            new = {s: new[s] for s in [255, *range(B - 1, 5, -1), *range(0, 5), *range(249, B - 1, -1)]}
+        row = {engine.FG_F32: 4.0, engine.FG_BF16: 2.0, engine.FG_E4M3: (d.head_dim + 4) / d.head_dim}[type]
+        alone = 2 * row * d.n_kv_head * d.head_dim * d.n_layer * sum(len(text[s]) for s in new)
+        (lg, _), once = taken(m, pcs[0], lambda: pcs[0].step(new), 0 if window else 0.5 * alone)
+        assert window or once
+        lg2, _ = pcs[1].step(new)
+        assert relerr(lg, lg2) < 2 * bar
         for i, s in enumerate(new):
             text[s] = np.concatenate([text[s], new[s]])
-            want, _ = ex.logits(text[s], window, sinks)
-            for lg in lgs:
+            if s % 25 == 0 or s in (255, 249, B - 1):
+                want, _ = ex.logits(text[s], window, sinks)
                 assert relerr(lg[i], want[-1]) < bar, (k, s, relerr(lg[i], want[-1]))
     for pc in pcs:
         pc.close()
@@ -210,39 +224,43 @@ def test_steps_that_adjust(setup):
 def test_a_served_run(setup, kind):
     """All of it as a server has it: an 8-bit cache, forks of one prompt that draw
     under penalties and a mask, ends and new forks among them, a compaction. Every
-    step's logits are the float64 model's on the sequence's own ids, and its ids the
-    definition's on those logits."""
+    step's ids are the definition's on its logits, and a sample of the sequences'
+    logits the float64 model's on their own ids."""
     d, m, ex = setup
     ex = exact_of(ex, kind)
-    pc = m.paged(120, 16, 12, type=Q.TYPES[kind], prefix=True)
+    pc = m.paged(600, 16, 256, type=Q.TYPES[kind], prefix=True)
     prompt = uniform_ids(3, 320, d.vocab)
     pc.step({0: prompt}, want_logits=False)
     rng = np.random.default_rng(6)
-    text = {s: list(prompt) for s in range(10)}
-    for s in range(1, 10):
+    text = {s: list(prompt) for s in range(250)}
+    for s in range(1, 250):
         pc.fork(0, s)
     banned = rng.random(d.vocab) < 0.3
-    last = {s: 5 + s for s in range(10)}
+    last = {s: 5 + s for s in range(250)}
     for k in range(6):
         if k == 3:
-            for s in (1, 4, 5):
+            for s in (1, 4, 5, 130):
                 pc.trim(s)
                 del text[s], last[s]
             pc.compact()
-            pc.fork(0, 11, 320)
-            text[11], last[11] = list(prompt), 9
+            pc.fork(0, 251, 320)
+            text[251], last[251] = list(prompt), 9
         new = {s: [last[s]] for s in text}
         for s in new:
             text[s] += new[s]
         u = rng.random(len(new)).astype(np.float32)
-        lg, ids = pc.step(new, u=u, temp=0.9, top_p=0.95, history=list(text.values()), count_from=320, pres=0.5,
-                          freq=0.1, rep=1.1, allowed=[~banned] * len(new))
+        alone = 2 * (d.head_dim + 4) * d.n_kv_head * d.n_layer * sum(len(t) for t in text.values())
+        (lg, ids), once = taken(m, pc, lambda: pc.step(
+            new, u=u, temp=0.9, top_p=0.95, history=list(text.values()), count_from=320, pres=0.5, freq=0.1, rep=1.1,
+            allowed=[~banned] * len(new)), 0.5 * alone)
+        assert once
         mask = np.packbits(~banned, bitorder="little").view(np.uint32)[None]
         full = lambda v: np.full(len(new), v, np.float32)  # noqa: E731
         adj = TA.reference(lg, hist=[np.asarray(t) for t in text.values()], count_from=np.full(len(new), 320),
                            rep=full(1.1), pres=full(0.5), freq=full(0.1), mask=mask, mask_row=np.zeros(len(new), int))
         for i, s in enumerate(new):
-            assert relerr(lg[i], ex.logits(np.asarray(text[s]))[0][-1]) < BARS[kind], (k, s)
+            if s % 40 == 0 or s in (251, 6):
+                assert relerr(lg[i], ex.logits(np.asarray(text[s]))[0][-1]) < BARS[kind], (k, s)
             assert ids[i] == R.draw_row(adj[i], float(np.float32(0.9)), 0, float(np.float32(0.95)), 0.0, float(u[i]))[0]
             assert not banned[ids[i]]
             last[s] = int(ids[i])
