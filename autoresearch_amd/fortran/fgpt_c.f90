@@ -14,6 +14,10 @@ module fgpt_c
       FG_EBUSY = -8, FG_EARCH = -9, FG_ERANGE = -10
   integer(c_int32_t), parameter, public :: FG_OPT_FUSED_DECODE = 1, FG_OPT_FORWARD_F16 = 2
 
+  ! flags of fg_paged_create: one of the types, and shared pages read once
+  integer(c_int32_t), parameter, public :: FG_KV_BF16 = 1, FG_KV_I8 = 2, FG_KV_E4M3 = 4, &
+      FG_KV_PREFIX = 8
+
   type, bind(C), public :: fg_dims
     integer(c_int32_t) :: n_layer, d_model, n_head, n_kv_head, head_dim, vocab_size
     real(c_float) :: eps
@@ -42,13 +46,23 @@ module fgpt_c
         min_p = c_null_ptr, u = c_null_ptr
   end type fg_draw_cfg
 
+  ! What happens to logits before a draw: addresses of arrays, or null (off).
+  type, bind(C), public :: fg_adjust_cfg
+    type(c_ptr) :: hist = c_null_ptr, hist_start = c_null_ptr, count_from = c_null_ptr, &
+        rep = c_null_ptr, pres = c_null_ptr, freq = c_null_ptr, bias = c_null_ptr, &
+        bias_id = c_null_ptr, bias_start = c_null_ptr, mask = c_null_ptr, mask_row = c_null_ptr
+    integer(c_int64_t) :: mask_ld = 0
+    integer(c_int32_t) :: n_hist = 0, n_bias = 0, n_mask = 0
+  end type fg_adjust_cfg
+
   public :: fg_version, fg_last_error, fg_model_create, fg_weights_read, fg_model_load, &
       fg_model_destroy, &
       fg_set_rope, fg_forward, fg_forward_pos, fg_kv_create, fg_kv_destroy, fg_kv_len, fg_kv_set_len, &
       fg_step, fg_step_multi, fg_decode_greedy, fg_sync, fg_eval_bpb, fg_rows_npy, &
       fg_decode_spec, fg_spec_accept, fg_spec_draft, fg_sample, fg_decode_sample, fg_set_option, &
       fg_paged_create, fg_paged_destroy, fg_paged_len, fg_paged_free, fg_paged_fork, &
-      fg_paged_trim, fg_paged_compact, fg_paged_read, fg_paged_step, fg_error_message
+      fg_paged_trim, fg_paged_compact, fg_paged_read, fg_paged_step, fg_paged_step_adjust, &
+      fg_error_message
 
   interface
     integer(c_int32_t) function fg_version() bind(C, name="fg_version")
@@ -301,6 +315,16 @@ module fgpt_c
       integer(c_int32_t), value :: n
       integer(c_int32_t), intent(in) :: seqs(*), counts(*), ids(*)
       type(c_ptr), value :: draw, logits, next_ids
+    end function
+
+    ! adjust: c_loc of an fg_adjust_cfg of host arrays, or null; the rest as above
+    integer(c_int32_t) function fg_paged_step_adjust(m, pc, n, seqs, counts, ids, adjust, draw, &
+        logits, next_ids) bind(C, name="fg_paged_step_adjust")
+      import :: c_int32_t, c_ptr
+      type(c_ptr), value :: m, pc
+      integer(c_int32_t), value :: n
+      integer(c_int32_t), intent(in) :: seqs(*), counts(*), ids(*)
+      type(c_ptr), value :: adjust, draw, logits, next_ids
     end function
 
     integer(c_int32_t) function fg_sync(m) bind(C, name="fg_sync")
