@@ -694,7 +694,11 @@ struct Many {
   static constexpr int PLANE = SK * ROW;
   static constexpr int STAGE = 2 * NA * PLANE;  // K planes, V planes
   static constexpr int SCALES = 4 * 2 * SK;  // bytes of a stage's scales
-  static constexpr int LDS = (KF ? 1 : 2) * STAGE + (CODES ? 2 * SCALES : 0);
+  // buffers; 8-bit pages: a barrier every NB / 2 steps. bf16 rows on e4m3 pages, 397 GF of
+  // prompts, two 554 us, four 531; fp32 rows of 128 dims, where registers spill, 1022 and 1046
+  static constexpr int NB = KF ? 1 : !CODES || (QF && HD == 128) ? 2 : 4;
+  static constexpr int AHEAD = NB / 2;  // steps that codes are put into LDS ahead
+  static constexpr int LDS = NB * STAGE + (CODES ? NB * SCALES : 0);
   static constexpr int WAVES = QF || CODES ? 2 : 3;  // a SIMD
 };
 
@@ -823,13 +827,13 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
     }
   };
 
-  // 8-bit: this thread's CPT codes of a K and a V row and their scales, loaded two
-  // steps ahead, made bf16 ones a step ahead
+  // 8-bit: this thread's CPT codes of a K and a V row and their scales, made bf16 ones in
+  // LDS AHEAD steps ahead, loaded a step before that
   constexpr int CPT = HD / 8;
   typedef uint32_t codes_t __attribute__((ext_vector_type(CPT / 4)));
   codes_t code[2];
   float scale[2];
-  float* const scales = (float*)(lds + 2 * C::STAGE);  // [buffer][K, V][SK]
+  float* const scales = (float*)(lds + C::NB * C::STAGE);  // [buffer][K, V][SK]
   auto fetch_codes = [&](int st) __attribute__((always_inline)) {
     turn(st);
     const int r = tid / 8;
@@ -845,7 +849,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
   auto put_codes = [&](int st) __attribute__((always_inline)) {
     if constexpr (CODES) {
       const int r = tid / 8;
-      uint8_t* to = lds + (st & 1) * C::STAGE + r * ROW;
+      uint8_t* to = lds + (st % C::NB) * C::STAGE + r * ROW;
 #pragma unroll
       for (int kvi = 0; kvi < 2; ++kvi) {
 #pragma unroll
@@ -854,7 +858,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
           const int slot = kvi ? vslot<HD>(r, chunk) : kslot<HD>(r, chunk);
           *(bf16x8_t*)(to + kvi * PLANE + slot * 16) = codes_bf16<KT>(code[kvi][2 * i], code[kvi][2 * i + 1]);
         }
-        if (tid % 8 == 0) scales[(st & 1) * 2 * SK + kvi * SK + r] = scale[kvi];
+        if (tid % 8 == 0) scales[(st % C::NB) * 2 * SK + kvi * SK + r] = scale[kvi];
       }
     }
   };
@@ -917,7 +921,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
   auto settle = [&](int st, f32x16_t& sc) __attribute__((always_inline)) {
     const int b = tile_base(t, kt, v0 + st);  // the tile's first key
     if constexpr (CODES) {
-      const float* ks = scales + (st & 1) * 2 * SK + 8 * g;
+      const float* ks = scales + (st % C::NB) * 2 * SK + 8 * g;
 #pragma unroll
       for (int r = 0; r < 16; r += 4) {
         const f32x4_t x = *(const f32x4_t*)(ks + 16 * (r >> 3) + (r & 7));
@@ -963,7 +967,7 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
 #pragma unroll
       for (int e = 0; e < 8; ++e) l_run += x[e];
       if constexpr (CODES) {
-        const float* vs = scales + ((st & 1) * 2 + 1) * SK + 16 * s + 8 * g;
+        const float* vs = scales + ((st % C::NB) * 2 + 1) * SK + 16 * s + 8 * g;
 #pragma unroll
         for (int e = 0; e < 8; e += 4) {
           const f32x4_t y = *(const f32x4_t*)(vs + e);
@@ -1000,6 +1004,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
     if constexpr (CODES) {
       put_codes(0);
       if (nstep > 1) fetch_codes(1);
+      if (C::AHEAD > 1 && nstep > 1) {
+        put_codes(1);
+        if (nstep > 2) fetch_codes(2);
+      }
     }
   }
   auto step = [&](auto buf, int st) __attribute__((always_inline)) {
@@ -1010,9 +1018,10 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
       __syncthreads();
       if (st + 1 < nstep) fetch(st + 1);
     } else if constexpr (CODES) {
-      lds_barrier();  // this step's rows are there, and nobody reads the other buffer
-      if (st + 1 < nstep) put_codes(st + 1);
-      if (st + 2 < nstep) fetch_codes(st + 2);
+      // (the next AHEAD steps are there, and nobody reads the buffers of those after them)
+      if constexpr (decltype(buf)::value % C::AHEAD == 0) lds_barrier();
+      if (st + C::AHEAD < nstep) put_codes(st + C::AHEAD);
+      if (st + C::AHEAD + 1 < nstep) fetch_codes(st + C::AHEAD + 1);
     } else {
       stage_sync<0>();  // this step has landed, and nobody reads the other buffer
       if (st + 1 < nstep) fill(st + 1, C::STAGE - here);
@@ -1025,9 +1034,13 @@ __device__ __forceinline__ void many_rows(const PagedArgs& p, uint8_t* lds, cons
     weigh(st, sc, pt);
     add_values(here, pt);
   };
-  for (int st = 0; st < nstep; st += 2) {
+  for (int st = 0; st < nstep; st += C::NB < 2 ? 2 : C::NB) {
     step(std::integral_constant<int, 0>(), st);
-    if (st + 1 < nstep) step(std::integral_constant<int, KF ? 0 : 1>(), st + 1);
+    if (st + 1 < nstep) step(std::integral_constant<int, C::NB < 2 ? 0 : 1>(), st + 1);
+    if constexpr (C::NB > 2) {
+      if (st + 2 < nstep) step(std::integral_constant<int, 2>(), st + 2);
+      if (st + 3 < nstep) step(std::integral_constant<int, 3>(), st + 3);
+    }
   }
   if (!active) return;
 
