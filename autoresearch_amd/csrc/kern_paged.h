@@ -66,21 +66,28 @@ struct RowTile {
 template <int RT>
 __device__ __forceinline__ bool find_tile(const PagedArgs& p, int id, RowTile& t) {
   const int lane = threadIdx.x & 63;
-  auto q_of = [&](int s) {  // new tokens of sequence s, kept inside the arrays
-    const int a = p.q_start[s], n = p.q_start[s + 1] - a;
-    return a < 0 ? 0 : max(0, min(min(n, p.max_q), p.n_rows - a));
+  auto tokens = [&](int a, int z) {  // of a sequence's rows a .. z-1 those inside the arrays and bounds
+    return a < 0 ? 0 : max(0, min(min(z - a, p.max_q), p.n_rows - a));
   };
-  int first = 0, nq;
+  // the sequence's rows and length, asked for together: a second round trip would
+  // cost a decoding kernel a tenth of its time
+  int first = 0, a, z, kv;
   if (p.one_tile) {
     if (id >= p.n_seq) return false;
     t.seq = id;
-    nq = q_of(id);
+    a = p.q_start[id];
+    z = p.q_start[id + 1];
+    kv = p.kv_len[id];
   } else {
     int base = 0;
     t.seq = -1;
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
       const int s = s0 + lane;
-      const int n = s < p.n_seq ? (q_of(s) * p.G + RT - 1) / RT : 0;
+      const bool in = s < p.n_seq;
+      a = in ? p.q_start[s] : 0;
+      z = in ? p.q_start[s + 1] : 0;
+      kv = in ? p.kv_len[s] : 0;
+      const int n = in ? (tokens(a, z) * p.G + RT - 1) / RT : 0;
       int sum = n;  // tiles of this step's sequences up to this one
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -91,25 +98,29 @@ __device__ __forceinline__ bool find_tile(const PagedArgs& p, int id, RowTile& t
       if (past) {
         const int l = __builtin_ctzll(past);
         t.seq = s0 + l;
-        first = base + __shfl(sum - n, l, 64);
+        first = base + __builtin_amdgcn_readlane(sum - n, l);
+        a = __builtin_amdgcn_readlane(a, l);
+        z = __builtin_amdgcn_readlane(z, l);
+        kv = __builtin_amdgcn_readlane(kv, l);
         break;
       }
-      base += __shfl(sum, 63, 64);
+      base += __builtin_amdgcn_readlane(sum, 63);
     }
     if (t.seq < 0) return false;
-    nq = q_of(t.seq);
   }
+  // (said to be uniform, or the compiler keeps masks and places per lane)
   t.seq = __builtin_amdgcn_readfirstlane(t.seq);
   first = __builtin_amdgcn_readfirstlane(first);
-  nq = __builtin_amdgcn_readfirstlane(nq);
+  a = __builtin_amdgcn_readfirstlane(a);
+  z = __builtin_amdgcn_readfirstlane(z);
+  kv = __builtin_amdgcn_readfirstlane(kv);
   const int tile = p.one_tile ? 0 : id - first;
   t.r0 = tile * RT;
-  t.rows = min(RT, nq * p.G - t.r0);
+  t.rows = min(RT, tokens(a, z) * p.G - t.r0);
   if (t.rows <= 0) return false;
-  // (said to be uniform, or the compiler keeps masks and places per lane)
-  t.row0 = __builtin_amdgcn_readfirstlane(p.q_start[t.seq]);
-  t.kv = __builtin_amdgcn_readfirstlane(max(0, min(p.kv_len[t.seq], p.max_kv)));
-  t.pos0 = t.kv - (__builtin_amdgcn_readfirstlane(p.q_start[t.seq + 1]) - t.row0);
+  t.row0 = a;
+  t.kv = max(0, min(kv, p.max_kv));
+  t.pos0 = t.kv - (z - a);
   const int pf = t.pos0 + t.r0 / p.G, pl = t.pos0 + (t.r0 + t.rows - 1) / p.G;
   t.hi = max(0, min(pl + 1, t.kv));
   t.lo = p.window > 0 ? max(0, min(pf - p.window + 1, t.hi)) : 0;

@@ -424,7 +424,8 @@ typedef struct fg_ragged {
  * and the pages are in head order either way. A row at a position below 0 or
  * not below max_kv is left alone; one whose page is not in [0, n_pages)
  * gets its q, and its k and v go nowhere. Two rows on one slot (a page that two
- * sequences share) leave either's values. */
+ * sequences share) leave either's values (in 8-bit pages the codes of one with the
+ * scale of the other, maybe). */
 typedef struct fg_append_cfg {
   int32_t n_head;
   int32_t type;        /* of qkv and q_out: FG_F32 or FG_BF16 */
