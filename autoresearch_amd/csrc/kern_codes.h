@@ -9,25 +9,17 @@ namespace fgpt {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
-// Eight codes in order as fp32. Both kinds are exact in bf16 too: integers up to
+// Four codes in order as fp32. Both kinds are exact in bf16 too: integers up to
 // 127, and three bits behind a leading one.
 template <int KT>
-__device__ __forceinline__ void code_values(const uint2& w, float (&x)[8]) {
+__device__ __forceinline__ void code_values(uint32_t w, float* x) {
   static_assert(KT == FG_I8 || KT == FG_E4M3, "an 8-bit type");
+  if constexpr (KT == FG_E4M3) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    x[0] = lo[0], x[1] = lo[1], x[2] = hi[0], x[3] = hi[1];
+  } else {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int u = (int)(i ? w.y : w.x);
-    if constexpr (KT == FG_E4M3) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const auto v = k ? __builtin_amdgcn_cvt_pk_f32_fp8(u, true) : __builtin_amdgcn_cvt_pk_f32_fp8(u, false);
-        x[4 * i + 2 * k] = v[0];
-        x[4 * i + 2 * k + 1] = v[1];
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) x[4 * i + k] = (float)(int8_t)(u >> (8 * k));
-    }
+    for (int k = 0; k < 4; ++k) x[k] = (float)(int8_t)(w >> (8 * k));
   }
 }
 

@@ -19,13 +19,18 @@ typedef uint32_t u32x4v_t __attribute__((ext_vector_type(4)));
 // A thread keeps to one token row and LPH-th of a head: VEC dims of the head's
 // first half and the same of its second, so that a rotation pair lies in one
 // lane, every access is a 16-byte one and its cos and sin are read once; it goes
-// through the row's heads, HU of them in flight at a time. The mean square of a
+// through the row's heads, HU of them in flight at a time. Five, since the rows of
+// 40 heads of 128 in bf16 and of 18 in fp32 then take one round (12k rows of the
+// former, 62 us with four, 59 with five, 61 with six). The mean square of a
 // head is a sum over its LPH lanes. A workgroup takes RW rows: four from 2048
 // rows on, where the head weights that a thread reads serve more heads (12k
-// rows of 40 bf16 heads of 128 with weights, 271 MB: 118 us with one row, 62 with
+// rows of 40 bf16 heads of 128 with weights, 271 MB: 118 us with one row, 59 with
 // four; 11k of 24 heads of 64 without 25, 15), one below that (1024 rows of the
 // former shape 7.0 us, with four rows 8.6).
-// Bound by bytes: the row once in, once out.
+// Bound by bytes: the row once in, once out. Into 8-bit pages a head's lanes find its
+// largest value and write 8 codes each, and one the scale: 10k rows of 32 bf16 heads on
+// 4, 203 MB, 49 us (4.2 TB/s). q is stored in the ordinary way: past the caches' order of
+// use it takes 43, but the attention that reads it next 6 more.
 struct AppendArgs {
   fg_pages pg;
   fg_ragged b;
@@ -62,6 +67,21 @@ __device__ __forceinline__ float group_sum(float v) {
   if constexpr (N >= 8) v += dpp_f<0x141>(v);
   if constexpr (N >= 16) v += dpp_f<0x140>(v);
   return v;
+}
+
+template <int VEC, bool F>
+__device__ __forceinline__ void load_vals(const void* base, int64_t i, float (&v)[VEC]) {
+#pragma unroll
+  for (int k = 0; k < VEC; k += 4) {
+    if constexpr (F) {
+      const float4 x = *(const float4*)((const float*)base + i + k);
+      v[k] = x.x, v[k + 1] = x.y, v[k + 2] = x.z, v[k + 3] = x.w;
+    } else {
+      const uint2 x = *(const uint2*)((const uint16_t*)base + i + k);
+      v[k] = __uint_as_float(x.x << 16), v[k + 1] = __uint_as_float(x.x & 0xFFFF0000u);
+      v[k + 2] = __uint_as_float(x.y << 16), v[k + 3] = __uint_as_float(x.y & 0xFFFF0000u);
+    }
+  }
 }
 
 template <int VEC, bool F>
@@ -163,7 +183,7 @@ __device__ __forceinline__ void find_rows(const fg_ragged& b, int r0, int (&at)[
 template <int HD, bool QF, int KT, int RW>
 __global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
   typedef RowIO<HD, QF> IO;
-  constexpr int VEC = IO::VEC, LPH = IO::LPH, HPT = 256 / (LPH * RW), HU = 4;  // heads at once
+  constexpr int VEC = IO::VEC, LPH = IO::LPH, HPT = 256 / (LPH * RW), HU = 5;  // heads at once
   __shared__ int at[4][2];  // the rows' sequences and positions
   const int r0 = blockIdx.x * RW;
   find_rows<RW>(a.b, r0, at);
@@ -272,9 +292,11 @@ __global__ __launch_bounds__(256) void k_qk_append(AppendArgs a) {
 }
 
 // ------------------------------------------------------------ reading back
-// A thread takes 8 values of a row of k or v: HD/8 threads a head, RW rows a
-// workgroup as in the append (rows are found the same way). fp32 in, code times
-// scale, one rounding.
+// A thread takes as many values of a row of k or v as a 16-byte store holds, so that
+// a wavefront's stores are whole lines; rows are found as in the append, RW of them a
+// workgroup. fp32 in, code times scale, one rounding. The rows go out past the
+// caches' order of use (stores marked nontemporal): 12 sequences of 3000 to 9000
+// positions, e4m3 to bf16, 256 MB, 40 us, with ordinary stores 61.
 struct ReadArgs {
   fg_pages pg;
   fg_ragged b;
@@ -285,7 +307,8 @@ struct ReadArgs {
 
 template <int HD, int KT, bool OF, int RW>
 __global__ __launch_bounds__(256) void k_pages_read(ReadArgs a) {
-  constexpr int CPH = HD / 8, CPR = 256 / RW;  // 8-value chunks of a head; threads of a row
+  constexpr int VPT = OF ? 4 : 8;                 // values a thread
+  constexpr int CPH = HD / VPT, CPR = 256 / RW;   // chunks of a head; threads of a row
   __shared__ int at[4][2];
   const int r0 = blockIdx.x * RW;
   find_rows<RW>(a.b, r0, at);
@@ -296,36 +319,38 @@ __global__ __launch_bounds__(256) void k_pages_read(ReadArgs a) {
   const int page = a.b.table[(int64_t)seq * a.b.table_ld + (pos >> a.pshift)];
   const bool kept = (uint32_t)page < (uint32_t)a.pg.n_pages;
   for (int c = threadIdx.x % CPR; c < 2 * KH * CPH; c += CPR) {
-    const int val = c >= KH * CPH, h = c / CPH - val * KH, d = c % CPH * 8;
+    const int val = c >= KH * CPH, h = c / CPH - val * KH, d = c % CPH * VPT;
     if (!a.out[val]) continue;
     const void* base = val ? a.pg.v : a.pg.k;
     const int64_t block = (int64_t)(kept ? page : 0) * KH + h;
-    float x[8];
+    float x[VPT];
     if constexpr (KT == FG_F32 || KT == FG_BF16) {
-      const int64_t o = (block * P + slot) * HD + d;
-      float y[4];
-      if constexpr (KT == FG_F32) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          RowIO<HD, true>::values(RowIO<HD, true>::load(base, o + 4 * u), y);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) x[4 * u + k] = y[k];
-        }
-      } else {
-        RowIO<HD, false>::values(RowIO<HD, false>::load(base, o), x);
-      }
+      load_vals<VPT, KT == FG_F32>(base, (block * P + slot) * HD + d, x);
     } else {
       const uint8_t* b = (const uint8_t*)base + block * P * (HD + 4);
-      const uint2 w = *(const uint2*)(b + slot * HD + d);
       const float s = ((const float*)(b + P * HD))[slot];
-      code_values<KT>(w, x);
+      uint32_t w[VPT / 4];
+      if constexpr (VPT == 8) {
+        const uint2 u = *(const uint2*)(b + slot * HD + d);
+        w[0] = u.x;
+        w[1] = u.y;
+      } else {
+        w[0] = *(const uint32_t*)(b + slot * HD + d);
+      }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] *= s;
+      for (int k = 0; k < VPT / 4; ++k) code_values<KT>(w[k], x + 4 * k);
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) x[k] *= s;
     }
     if (!kept)
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = NAN;
-    store_vals<8, OF>(a.out[val], row * a.ld + h * HD + d, x);
+      for (int k = 0; k < VPT; ++k) x[k] = NAN;
+    u32x4v_t w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      w[k] = OF ? __float_as_uint(x[k])
+                : (uint32_t)f32_to_bf16_rne(x[2 * k % VPT]) | ((uint32_t)f32_to_bf16_rne(x[(2 * k + 1) % VPT]) << 16);
+    __builtin_nontemporal_store(w, (u32x4v_t*)((char*)a.out[val] + (row * a.ld + h * HD + d) * (OF ? 4 : 2)));
   }
 }
 
