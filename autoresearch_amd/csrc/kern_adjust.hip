@@ -5,6 +5,9 @@
 // LDS (integers: the order of the atomics does not matter), goes through its logits
 // once and writes them once. Each slice reads the whole history, which is short
 // beside the row and comes from the L2.
+// Bound by a slice's round trips one after another (starts, history, counts, new
+// values), then by bytes: 48 rows of 131073 ids, histories of up to 4000, 300 biases,
+// masks, 51 MB, 16.7 us (9 without lists). One row of 8192 ids takes 4.2.
 #include "fgpt_internal.h"
 #include "kern_common.h"
 #include "paged_internal.h"
@@ -224,6 +227,8 @@ void launch_adjust_rows(hipStream_t s, const float* x, int32_t rows, int32_t V, 
                         float* out, int64_t out_ld) {
   AdjustArgs a{x, out, V, 0, ld, out_ld, c};
   if (!a.c.mask_ld) a.c.mask_ld = (V + 31) / 32;
+  // slices of 2048 ids, or 1024 where those are too few to fill the CUs twice (the rows
+  // above with 4096: 18.5 us)
   a.slices = (V + 2047) / 2048;
   if ((int64_t)rows * a.slices >= 512) {
     FG_LAUNCH((k_adjust<2>), dim3((unsigned)(rows * a.slices)), dim3(AT), 0, s, a);
