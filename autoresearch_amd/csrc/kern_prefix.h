@@ -14,7 +14,7 @@
 // Few rows: bound by the way through groups, lengths, tables and pages, then by the
 // instructions of a tile. 64 tokens behind 3900 shared positions, 10 heads on 2, bf16
 // pages, fp32 rows: 19 us and 4 for the join (26 MB: 5 us at a copy's rate; each
-// sequence alone 34). Four tokens behind 512, 6 heads, fp32 pages: 9 and 4. Many rows:
+// sequence alone 30.5). Four tokens behind 512, 6 heads, fp32 pages: 9 and 4. Many rows:
 // by the loop of many_rows; 240 tokens in three groups behind up to 6000 positions, 32
 // heads on 4, e4m3 pages, 19 GF: 55 and 9.
 #pragma once

@@ -32,7 +32,12 @@ Plan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_prefix& f, const f
   pl.pm = pl.sm || (NR / std::max(1, f.n_group) > 32 && tiles(DR) * KH * nkt > 6000);
   pl.ptile = (int)tiles(pl.pm ? Many<128, true, FG_F32>::RT : DR);
   const int64_t items = std::max<int64_t>(1, pl.ptile * KH);
-  const int64_t want = ((pl.pm ? 2 : 1) * PAGED_CUS + items - 1) / items;
+  // 128-row tiles: two items a CU once each has enough keys to pay for its start and its
+  // share of the join. us, one -> two, by the 32-key tiles of them all: 1500 (10 heads on
+  // 2, fp32 rows on bf16 pages) 28.8 -> 32.3, 4464 (bf16 rows on e4m3 pages, three groups)
+  // 36.6 -> 41.5, 9000 (bf16) 48.6 -> 50.9, 10000 (fp32 rows) 70.5 -> 64.9, 13000 (e4m3)
+  // 72.4 -> 69.3, 13464 65.9 -> 58.2, 18000 131.6 -> 105.8.
+  const int64_t want = ((pl.pm && items * nkt > 9216 ? 2 : 1) * PAGED_CUS + items - 1) / items;
   const int64_t ns = std::max<int64_t>(1, std::min(want, (nkt + RWV - 1) / RWV));
   pl.pcpt = (int)((nkt + ns - 1) / ns + RWV - 1) / RWV * RWV;
   pl.psplit = pl.pcpt ? (int)((nkt + pl.pcpt - 1) / pl.pcpt) : 0;
