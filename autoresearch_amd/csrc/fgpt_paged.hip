@@ -356,6 +356,8 @@ extern "C" int32_t fg_adjust_rows(const float* logits, int32_t rows, int32_t V, 
   CHECK(rows >= 0, "rows must be >= 0");
   CHECK(V >= 1 && V <= DRAW_MAX_V, "V %d outside 1..%d", V, DRAW_MAX_V);
   CHECK(rows <= 1 << 21, "rows %d above 2^21", rows);
+  // (launches of fewer than 2^32 threads, which take up to 8 ids)
+  CHECK((int64_t)rows * ((V + 2047) / 2048) < 1 << 24, "rows %d x V %d: 2^24 slices of 2048 ids or more", rows, V);
   CHECK(ld >= V && ld < ((int64_t)1 << 40), "ld %lld below V %d", (long long)ld, V);
   CHECK(out_ld >= V && out_ld < ((int64_t)1 << 40), "out_ld %lld below V %d", (long long)out_ld, V);
   RCCHK(check_adjust(cfg, rows, V));

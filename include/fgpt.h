@@ -489,8 +489,9 @@ int32_t fg_paged_attn(const fg_pages *pages, const fg_ragged *batch, const fg_at
  * Group g is sequences seq_start[g] .. seq_start[g+1]-1, whose tables name the same
  * pages for positions 0 .. shared[g]-1 (those that some row sees; read from
  * the table of the group's first sequence). A sequence with a new token at a
- * position below shared[g] reads all of its keys itself. seq_start[0] is 0 and seq_start does not fall; sequences from
- * seq_start[n_group] on share nothing, and so does a group with shared[g] 0.
+ * position below shared[g] reads all of its keys itself. seq_start[0] is 0 and
+ * seq_start does not fall; sequences from seq_start[n_group] on share nothing, and
+ * so does a group with shared[g] 0.
  * max_shared bounds shared (a larger one counts as max_shared) and is at most
  * max_kv of the batch; it sizes the launch with the batch's bounds. Shared
  * positions are taken in whole 32s, what is left is read per sequence. What
@@ -533,7 +534,8 @@ int32_t fg_pages_copy(void *base, int32_t n_planes, int64_t plane_bytes, int32_t
  * rep, pres and freq are per row (device, each nullable = off; all off: no history);
  * a NaN setting and a rep not above 0 are off. Ids outside [0, V) are passed over, parts
  * of lists outside [0, n_hist) or [0, n_bias) cut off. The results do not depend on
- * any order of execution. No workspace. */
+ * any order of execution. No workspace. rows <= 2^21, and rows * ceil(V / 2048)
+ * below 2^24. */
 typedef struct fg_adjust_cfg {
   const int32_t *hist, *hist_start, *count_from; /* device [n_hist], [rows + 1], [rows] */
   const float *rep, *pres, *freq;                /* device [rows] */

@@ -25,6 +25,13 @@ def test_bad_adjust(match, kw):
     refused(match, adjust, **kw)
 
 
+def test_more_than_a_launch_holds():
+    """A row is taken in slices of 2048 ids; fewer than 2^24 of them."""
+    V = 1 << 18
+    refused("slices", adjust, rows=1 << 17, V=V, ld=V, out_ld=V)
+    refused("slices", adjust, rows=1 << 21, V=2049 * 8, ld=V, out_ld=V)
+
+
 def test_no_cfg():
     assert engine.load_library().fg_adjust_rows(P, 2, 100, 100, None, P, 100, None) == -1
 
