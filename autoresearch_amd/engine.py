@@ -546,7 +546,9 @@ class Paged:
         self._h = _vp()
         if type is None:
             type = FG_BF16 if bf16 else FG_F32
-        flags = {FG_F32: 0, FG_BF16: FG_KV_BF16, FG_I8: FG_KV_I8, FG_E4M3: FG_KV_E4M3}[type]
+        flags = {FG_F32: 0, FG_BF16: FG_KV_BF16, FG_I8: FG_KV_I8, FG_E4M3: FG_KV_E4M3}.get(type)
+        if flags is None:
+            raise ValueError(f"unknown page type {type}")
         _check(_LIB.fg_paged_create(m.handle, n_pages, page_size, max_seq, flags | (FG_KV_PREFIX if prefix else 0),
                                     window, sinks, C.byref(self._h)))
         m._caches.add(self)
@@ -631,9 +633,9 @@ class Paged:
 
     def _adjust(self, n, keep, history, count_from, rep, pres, freq, bias, allowed):
         """A step's fg_adjust_cfg of host arrays (kept in `keep`), None where nothing is given."""
+        if history is None and any(a is not None for a in (count_from, rep, pres, freq)):
+            raise ValueError("penalties without a history")
         if all(a is None for a in (history, bias, allowed)):
-            if any(a is not None for a in (count_from, rep, pres, freq)):
-                raise ValueError("penalties without a history")
             return None
 
         def ptr(a, t):

@@ -45,3 +45,28 @@ def test_no_device():
     with pytest.raises(engine.FgptError) as e:
         adjust()
     assert e.value.code in (-7, -4)
+
+
+def step_cfg(**kw):
+    """The lists of a Paged.step of two sequences as fg_adjust_cfg."""
+    given = dict.fromkeys(("history", "count_from", "rep", "pres", "freq", "bias", "allowed")) | kw
+    return engine.Paged._adjust(None, 2, [], *given.values())
+
+
+@pytest.mark.parametrize("what", ["count_from", "rep", "pres", "freq"])
+def test_penalties_need_a_history(what):
+    assert step_cfg() is None
+    for other in ({}, {"bias": [{}, {3: 1.0}]}):
+        with pytest.raises(ValueError, match="without a history"):
+            step_cfg(**{what: 1}, **other)
+
+
+def test_lists_for_each_sequence():
+    for kw in ({"history": [[1]]}, {"bias": [{}]}):
+        with pytest.raises(ValueError, match="for each sequence"):
+            step_cfg(**kw)
+
+
+def test_unknown_page_type():
+    with pytest.raises(ValueError, match="page type"):
+        engine.Paged(None, 4, type=7)
