@@ -347,6 +347,7 @@ int32_t fgpt::check_adjust(const fg_adjust_cfg* c, int32_t rows, int32_t V) {
   CHECK(c->n_mask == 0 || c->mask, "mask is NULL");
   CHECK(c->mask_ld == 0 || (c->mask_ld >= (V + 31) / 32 && c->mask_ld < ((int64_t)1 << 30)),
         "mask_ld %lld: 0, or %d words and more", (long long)c->mask_ld, (V + 31) / 32);
+  CHECK(c->n_mask * (c->mask_ld ? c->mask_ld : (V + 31) / 32) < (int64_t)1 << 40, "masks of 2^40 words or more");
   CHECK(c->n_mask == 0 || c->mask_row || c->n_mask >= rows, "%d masks for %d rows, and no mask_row", c->n_mask, rows);
   return FG_OK;
 }

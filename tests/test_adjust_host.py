@@ -20,7 +20,8 @@ def adjust(rows=2, V=100, ld=100, out_ld=100, x=P, out=P, **kw):
     ("n_bias", dict(n_bias=-1)), ("bias", dict(n_bias=1, bias=P, bias_id=P)),
     ("bias", dict(n_bias=1, bias_start=P, bias_id=P)), ("mask is NULL", dict(n_mask=1)),
     ("n_mask", dict(n_mask=-1)), ("mask_ld", dict(mask=P, n_mask=2, mask_ld=3)),
-    ("mask_ld", dict(mask_ld=-4)), ("1 masks for 2 rows", dict(mask=P, n_mask=1))])
+    ("mask_ld", dict(mask_ld=-4)), ("2\\^40 words", dict(mask=P, n_mask=1 << 30, mask_ld=1 << 29)),
+    ("1 masks for 2 rows", dict(mask=P, n_mask=1))])
 def test_bad_adjust(match, kw):
     refused(match, adjust, **kw)
 
