@@ -2521,6 +2521,9 @@ bool shared_groups(const fg_paged* pc, int n, const int32_t* seqs, const std::ve
   }
   int64_t saved = 0;
   int64_t common = 0, members = 0;  // of the last group: pages, sequences
+  auto held = [&](const std::vector<int32_t>& t) {  // (pages behind a window are none)
+    return std::count_if(t.begin(), t.begin() + common, [](int32_t p) { return p >= 0; }) * (int64_t)pc->page_size;
+  };
   for (int i = 0; i < n; ++i) {
     int64_t k = 0;
     if (members > 0) {
@@ -2533,16 +2536,16 @@ bool shared_groups(const fg_paged* pc, int n, const int32_t* seqs, const std::ve
       ++members;
       shared->back() = (int32_t)(k * pc->page_size);
     } else {
-      saved += std::max<int64_t>(0, members - 1) * common * pc->page_size;
+      if (members > 1) saved += (members - 1) * held(table[i - 1]);
       starts->push_back(i);
       common = (int64_t)table[i].size();
       members = 1;
       shared->push_back(0);
     }
   }
-  saved += std::max<int64_t>(0, members - 1) * common * pc->page_size;
+  if (members > 1) saved += (members - 1) * held(table[n - 1]);
   starts->push_back(n);
-  *again = pc->window ? 0 : saved;  // (what windows leave of it is not counted)
+  *again = pc->window ? 0 : saved;  // (a window may end inside of a page)
   return saved * 2 * pc->m->d.kvd() * paged_value_bytes(pc) >= PREFIX_SAVED;
 }
 
