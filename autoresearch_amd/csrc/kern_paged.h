@@ -1099,7 +1099,7 @@ constexpr int64_t PAGED_CUS = 256;
 
 }  // namespace paged
 
-// (may_many: 128-row tiles are allowed)
+// (of a launch whose parts a second one joins anyway; may_many: 128-row tiles are allowed)
 paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many);
 paged::PagedArgs paged_args(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, const paged::PagedPlan& pl,
                             const void* q, const PagedOut& out, float* work);

@@ -128,8 +128,15 @@ constexpr int64_t CUS = PAGED_CUS;
 // after 1000 9.5 -> 10.2, after 4000 13.0 -> 12.1); twice with 128-row ones (once:
 // chunks and tokens of 9 sequences, 10 heads on 2, 92 -> 123, one fp32 prompt of
 // 2048 75 -> 95).
+// 8-bit pages, up to three tiles a wavefront: one part, as the launch that joins them
+// costs the host more than they save on the GPU. us a call, in a captured graph and
+// from the host, 6 heads, parts -> one: int8, 200 positions 7.7 -> 7.2 and 13.6 -> 10.5,
+// 300 7.9 -> 8.9 and 13.7 -> 10.9, 16 sequences of 300 9.8 -> 9.2; e4m3, 300 7.4 -> 7.7
+// and 13.5 -> 10.5; four tiles (int8, 400) 13.5 -> 11.0 from the host, 500 8.0 -> 10.6 in
+// a graph.
 constexpr int64_t MANY_WORK = 6000;
-PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many = true) {
+PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many = true,
+                  bool joins = false) {
   PagedPlan pl;
   const int64_t G = c.n_head / pg.n_kv_head;
   // (no sequence has more new tokens than there are rows, whatever the caller's
@@ -150,7 +157,8 @@ PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, 
   pl.ntile = (int)tiles(pl.rt);
   const int64_t nkt = key_tiles_most(pl.rt), items = (int64_t)pl.ntile * pg.n_kv_head;
   const int64_t want = pl.many ? (2 * CUS + items - 1) / items : CUS / items;
-  const int64_t ns = std::max<int64_t>(1, std::min(want, (nkt + RWV - 1) / RWV));
+  const bool few_codes = (pg.type == FG_I8 || pg.type == FG_E4M3) && !pl.many && !joins && nkt <= 3 * RWV;
+  const int64_t ns = few_codes ? 1 : std::max<int64_t>(1, std::min(want, (nkt + RWV - 1) / RWV));
   pl.cpt = (int)((nkt + ns - 1) / ns + RWV - 1) / RWV * RWV;
   pl.nsplit = (int)std::max<int64_t>(1, (nkt + pl.cpt - 1) / pl.cpt);
   pl.floats = pl.nsplit > 1 ? items * pl.nsplit * pl.rt * (pg.head_dim + 2) : 0;
@@ -205,7 +213,7 @@ int64_t paged_attn_floats(const fg_pages& pg, const fg_ragged& b, const fg_attn_
 }
 
 paged::PagedPlan paged_plan(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many) {
-  return plan_of(pg, b, c, may_many);
+  return plan_of(pg, b, c, may_many, true);
 }
 
 paged::PagedArgs paged_args(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, const paged::PagedPlan& pl,
