@@ -490,7 +490,7 @@ __device__ __forceinline__ int rows_min(int v) {
 __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.0f / l; }
 
 // ------------------------------------------------------------ few rows
-// 16 flattened rows a tile, for decoding and short chunks: a workgroup's RWV
+// 16 flattened rows a tile, for decoding and short chunks: a workgroup's RWV (or WV)
 // wavefronts take every RWV-th 32-key tile of the item's part, keys and values
 // from the pages straight to MFMA operands in registers, and meet in LDS.
 // v_mfma_f32_16x16x32_bf16 with S^T = K Q^T: lane 16 g + c then holds query
@@ -503,10 +503,10 @@ __device__ __forceinline__ float inv_sum(float l) { return l == 0.f ? 0.f : 1.0f
 // through table, page and products: one token after 300 positions 8.4 us, the
 // merge 3.1. A tile that every row sees whole is not masked (a fifth of its
 // vector instructions).
-constexpr int DR = 16, RWV = 4;
+constexpr int DR = 16, RWV = 4, LWV = 8;
 
-template <int HD>
-constexpr int few_lds() { return RWV * DR * (HD + 4) * 4; }
+template <int HD, int WV = RWV>
+constexpr int few_lds() { return WV * DR * (HD + 4) * 4; }
 template <int HD>
 constexpr int64_t part_floats(int rows) { return (int64_t)rows * (HD + 2); }
 
@@ -519,14 +519,14 @@ struct Place {
 
 // Rows t of key head kvh against key tiles v0 .. v1-1. pos(tok): position of the
 // sequence's (or group's) new token tok; place(): see Place.
-template <int HD, bool QF, int KT, class Pos, class Put>
+template <int HD, bool QF, int KT, int WV = RWV, class Pos, class Put>
 __device__ __forceinline__ void few_rows(const PagedArgs& p, float* xo, const RowTile& t, const KeyTiles& kt,
                                          int kvh, int v0, int v1, Pos&& pos_of, Put&& place) {
   typedef KvTile<HD, QF, KT> Tile;
   typedef typename Tile::elem E;
   constexpr int VD = Tile::VD, OST = HD + 4;
   constexpr bool CODES = KT == FG_I8 || KT == FG_E4M3;
-  __shared__ float ml[RWV][DR][2];  // (xo: [RWV][DR][OST])
+  __shared__ float ml[WV][DR][2];  // (xo: [WV][DR][OST])
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
 
@@ -541,9 +541,9 @@ __device__ __forceinline__ void few_rows(const PagedArgs& p, float* xo, const Ro
   Tile kv;
   bool bad = false;
   const int32_t* tab = p.table + (int64_t)t.seq * p.table_ld;
-  const int vw = v0 + wv;  // this wavefront's tiles: vw, vw + RWV, ..
+  const int vw = v0 + wv;  // this wavefront's tiles: vw, vw + WV, ..
   auto ask = [&](int it) {
-    return page_ask(p, t, kt, tab, min(vw + RWV * (it + lane / 2), v1 - 1), lane & 1);
+    return page_ask(p, t, kt, tab, min(vw + WV * (it + lane / 2), v1 - 1), lane & 1);
   };
   PageList pl = {};
   PageAsk next = {};
@@ -585,8 +585,8 @@ __device__ __forceinline__ void few_rows(const PagedArgs& p, float* xo, const Ro
   for (int i = 0; i < VD; ++i) o[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   float m_run = -FLT_MAX, l_run = 0.f;  // log2 domain; l_run: this lane's keys
 
-  for (int it = 0, v = vw; v < v1; ++it, v += RWV) {
-    const bool more = v + RWV < v1;
+  for (int it = 0, v = vw; v < v1; ++it, v += WV) {
+    const bool more = v + WV < v1;
     const int b = tile_base(t, kt, v);
     if (more && (it & 31) == 31) {
       pl = page_place(p, t, kvh, next, bad);
@@ -647,14 +647,14 @@ __device__ __forceinline__ void few_rows(const PagedArgs& p, float* xo, const Ro
   __syncthreads();
   const Place to = place();
   // a thread per row and four head dims, the wavefronts' sums in their order
-  for (int w = tid; w < t.rows * (HD / 4); w += 64 * RWV) {
+  for (int w = tid; w < t.rows * (HD / 4); w += 64 * WV) {
     const int r = w / (HD / 4), d = 4 * (w % (HD / 4));
     float m = -FLT_MAX, l = 0.f;
 #pragma unroll
-    for (int k = 0; k < RWV; ++k) m = fmaxf(m, ml[k][r][0]);
+    for (int k = 0; k < WV; ++k) m = fmaxf(m, ml[k][r][0]);
     float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < RWV; ++k) {
+    for (int k = 0; k < WV; ++k) {
       const float f = exp2f(ml[k][r][0] - m);
       const float4 x = *(const float4*)(xo + (k * DR + r) * OST + d);
       l += f * ml[k][r][1];
@@ -1090,6 +1090,7 @@ struct PagedPlan {
   bool many;
   bool one_tile;
   int rt;      // rows of a tile
+  bool wide;   // LWV wavefronts a workgroup of 16-row tiles
   int ntile, nsplit, cpt;
   int64_t floats;
 };

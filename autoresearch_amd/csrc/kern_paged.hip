@@ -10,8 +10,8 @@ namespace {
 using namespace paged;
 
 // Item (tile id, key head, part z) of a launch.
-template <int HD, bool QF, int KT>
-__global__ __launch_bounds__(64 * RWV, 2) void k_paged_few(PagedArgs p) {
+template <int HD, bool QF, int KT, int WV = RWV>
+__global__ __launch_bounds__(64 * WV, 2) void k_paged_few(PagedArgs p) {
   extern __shared__ __attribute__((aligned(16))) float xo[];
   const int kvh = blockIdx.x % p.KH, rest = blockIdx.x / p.KH;
   const int id = rest % p.ntile, z = rest / p.ntile;
@@ -20,7 +20,7 @@ __global__ __launch_bounds__(64 * RWV, 2) void k_paged_few(PagedArgs p) {
   const KeyTiles kt = key_tiles(t);
   const int v0 = z * p.cpt, v1 = min(kt.n, v0 + p.cpt);
   if (z > 0 && v0 >= kt.n) return;
-  few_rows<HD, QF, KT>(p, xo, t, kt, kvh, v0, v1, [&](int tok) { return t.pos0 + tok; }, [&] {
+  few_rows<HD, QF, KT, WV>(p, xo, t, kt, kvh, v0, v1, [&](int tok) { return t.pos0 + tok; }, [&] {
     float* P0 = p.part + ((int64_t)(id * p.KH + kvh) * p.nsplit + z) * part_floats<HD>(DR);
     return Place{kt.n <= p.cpt, P0, P0 + DR * HD};
   });
@@ -128,12 +128,15 @@ constexpr int64_t CUS = PAGED_CUS;
 // after 1000 9.5 -> 10.2, after 4000 13.0 -> 12.1); twice with 128-row ones (once:
 // chunks and tokens of 9 sequences, 10 heads on 2, 92 -> 123, one fp32 prompt of
 // 2048 75 -> 95).
-// 8-bit pages, up to three tiles a wavefront: one part, as the launch that joins them
-// costs the host more than they save on the GPU. us a call, in a captured graph and
-// from the host, 6 heads, parts -> one: int8, 200 positions 7.7 -> 7.2 and 13.6 -> 10.5,
-// 300 7.9 -> 8.9 and 13.7 -> 10.9, 16 sequences of 300 9.8 -> 9.2; e4m3, 300 7.4 -> 7.7
-// and 13.5 -> 10.5; four tiles (int8, 400) 13.5 -> 11.0 from the host, 500 8.0 -> 10.6 in
-// a graph.
+// 8-bit pages, up to two key tiles for each of LWV = 8 wavefronts: one part, without the
+// launch that joins (4 wavefronts where those have one tile each, or workgroups are many).
+// us a call, in a captured graph and from the host, 6 heads of 128, fp32 rows, parts -> one:
+// int8, 200 positions 7.7 -> 7.0 and 13.6 -> 10.4, 300 7.9 -> 7.8 and 13.5 -> 10.4 (of 4
+// wavefronts 8.9 and 10.9), 500 8.0 -> 9.5 and 13.2 -> 10.4, 16 sequences of 300 9.8 -> 8.0,
+// of 500 10.4 -> 10.3; e4m3, 300 7.4 -> 7.1, 500 7.6 -> 8.5; int8, 100, 4 wavefronts 5.5, 8
+// 5.7. Three tiles a wavefront (700): 8.2 -> 11.8 and 13.5 -> 12.4. A model's step of depth
+// 12, one sequence of 300, which the host's launches bound: 35 to 60 us less.
+// (16 wavefronts: their registers spill.)
 constexpr int64_t MANY_WORK = 6000;
 PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, bool may_many = true,
                   bool joins = false) {
@@ -157,7 +160,8 @@ PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, 
   pl.ntile = (int)tiles(pl.rt);
   const int64_t nkt = key_tiles_most(pl.rt), items = (int64_t)pl.ntile * pg.n_kv_head;
   const int64_t want = pl.many ? (2 * CUS + items - 1) / items : CUS / items;
-  const bool few_codes = (pg.type == FG_I8 || pg.type == FG_E4M3) && !pl.many && !joins && nkt <= 3 * RWV;
+  const bool few_codes = (pg.type == FG_I8 || pg.type == FG_E4M3) && !pl.many && !joins && nkt <= 2 * LWV;
+  pl.wide = few_codes && nkt > RWV && items <= CUS;
   const int64_t ns = few_codes ? 1 : std::max<int64_t>(1, std::min(want, (nkt + RWV - 1) / RWV));
   pl.cpt = (int)((nkt + ns - 1) / ns + RWV - 1) / RWV * RWV;
   pl.nsplit = (int)std::max<int64_t>(1, (nkt + pl.cpt - 1) / pl.cpt);
@@ -165,12 +169,12 @@ PagedPlan plan_of(const fg_pages& pg, const fg_ragged& b, const fg_attn_cfg& c, 
   return pl;
 }
 
-template <int HD, bool QF, int KT>
+template <int HD, bool QF, int KT, int WV = RWV>
 void launch_few(hipStream_t s, const PagedArgs& a) {
-  constexpr int lds = few_lds<HD>();
+  constexpr int lds = few_lds<HD, WV>();
   static std::atomic<uint64_t> lds_set{0};
-  raise_lds_once((const void*)k_paged_few<HD, QF, KT>, lds, &lds_set);
-  FG_LAUNCH((k_paged_few<HD, QF, KT>), dim3((unsigned)(a.ntile * a.KH * a.nsplit)), dim3(64 * RWV),
+  raise_lds_once((const void*)k_paged_few<HD, QF, KT, WV>, lds, &lds_set);
+  FG_LAUNCH((k_paged_few<HD, QF, KT, WV>), dim3((unsigned)(a.ntile * a.KH * a.nsplit)), dim3(64 * WV),
             lds, s, a);
   if (a.nsplit > 1)
     FG_LAUNCH((k_paged_merge<HD, QF, DR>), dim3((unsigned)(a.ntile * a.KH * (DR * HD / 1024))),
@@ -190,20 +194,22 @@ void launch_many(hipStream_t s, const PagedArgs& a) {
 }
 
 template <int HD, bool QF, int KT>
-void launch_t(hipStream_t s, const PagedArgs& a, bool many) {
-  if (many) launch_many<HD, QF, KT>(s, a);
+void launch_t(hipStream_t s, const PagedArgs& a, const PagedPlan& pl) {
+  if constexpr (Many<HD, QF, KT>::CODES)
+    if (pl.wide) return launch_few<HD, QF, KT, LWV>(s, a);
+  if (pl.many) launch_many<HD, QF, KT>(s, a);
   else launch_few<HD, QF, KT>(s, a);
 }
 
 template <int HD>
-void launch_hd(hipStream_t s, const PagedArgs& a, bool many, bool qf, int32_t kt) {
-  if (kt == FG_F32) launch_t<HD, true, FG_F32>(s, a, many);
-  else if (kt == FG_BF16 && qf) launch_t<HD, true, FG_BF16>(s, a, many);
-  else if (kt == FG_BF16) launch_t<HD, false, FG_BF16>(s, a, many);
-  else if (kt == FG_I8 && qf) launch_t<HD, true, FG_I8>(s, a, many);
-  else if (kt == FG_I8) launch_t<HD, false, FG_I8>(s, a, many);
-  else if (qf) launch_t<HD, true, FG_E4M3>(s, a, many);
-  else launch_t<HD, false, FG_E4M3>(s, a, many);
+void launch_hd(hipStream_t s, const PagedArgs& a, const PagedPlan& pl, bool qf, int32_t kt) {
+  if (kt == FG_F32) launch_t<HD, true, FG_F32>(s, a, pl);
+  else if (kt == FG_BF16 && qf) launch_t<HD, true, FG_BF16>(s, a, pl);
+  else if (kt == FG_BF16) launch_t<HD, false, FG_BF16>(s, a, pl);
+  else if (kt == FG_I8 && qf) launch_t<HD, true, FG_I8>(s, a, pl);
+  else if (kt == FG_I8) launch_t<HD, false, FG_I8>(s, a, pl);
+  else if (qf) launch_t<HD, true, FG_E4M3>(s, a, pl);
+  else launch_t<HD, false, FG_E4M3>(s, a, pl);
 }
 
 }  // namespace
@@ -252,9 +258,9 @@ void launch_paged_attn(hipStream_t s, const fg_pages& pg, const fg_ragged& b, co
   const PagedPlan pl = plan_of(pg, b, c);
   const PagedArgs a = paged_args(pg, b, c, pl, q, out, work);
   if (pg.head_dim == 128)
-    launch_hd<128>(s, a, pl.many, c.type == FG_F32, pg.type);
+    launch_hd<128>(s, a, pl, c.type == FG_F32, pg.type);
   else
-    launch_hd<64>(s, a, pl.many, c.type == FG_F32, pg.type);
+    launch_hd<64>(s, a, pl, c.type == FG_F32, pg.type);
 }
 
 }  // namespace fgpt

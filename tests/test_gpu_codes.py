@@ -275,15 +275,15 @@ def test_attention(shape, page, kind, rows, lengths):
 @pytest.mark.parametrize("rows", sorted(ROWS))
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("shape", ["mha128", "gqa4_64"])
-@pytest.mark.parametrize("T", [127, 128, 129, 255, 257, 383, 384, 385, 417])
+@pytest.mark.parametrize("T", [127, 128, 129, 255, 257, 385, 511, 512, 513, 545])
 def test_where_parts_begin(T, shape, kind, rows):
-    """Up to 384 positions at most, three key tiles a wavefront, one part takes them."""
+    """Up to 512 positions at most, two key tiles for each of eight wavefronts, one part takes them."""
     H, KH, hd = SHAPES[shape]
     b = Q.Batch([(T, 1), (1, 1), (T // 2, 2), (0, 0)], H, KH, hd, 16, ROWS[rows], kind=kind, seed=24)
     b.fill()
     q = b.normal(b.rows, H * hd, dtype=ROWS[rows])
     at = engine.attn_cfg(H, bf16=rows == "bf16")
-    assert (engine.paged_attn_work(b.pages(), b.ragged(), at) == 0) == (T <= 384)
+    assert (engine.paged_attn_work(b.pages(), b.ragged(), at) == 0) == (T <= 512)
     check_attn(b, q, run_attn(b, q))
 
 
